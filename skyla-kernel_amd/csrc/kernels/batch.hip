@@ -1,0 +1,531 @@
+// The operators of a served batch, gfx950: rows of many sequences over a paged KV cache, and
+// what is done to their logits before a token is chosen.
+//
+// Contract (bindings, push words; every grid is [1, rows, 1], and the runtime chooses the launch):
+//   kv_append              [W, A, C, KV, KV8]   24 words  spec [K_Q8, V_Q8, head_dim]
+//   attention_paged        [A, C, KV, KV8, KVS] 19 words  spec [N_REP, K_Q8, V_Q8, head_dim]
+//   attention_paged_merge  [A, C]               10 words  spec [head_dim]
+//   logits_adjust          [A, C]               12 words
+// Bindings as in attention.hip.  Heads are 128 wide.
+//
+// Rows: ctl[2] of them are live (the others are left as they were).  Row r has four words at
+// rows_off + 4 r: {seq, len, share, 0}.  Its token is at position len - 1 of sequence seq and
+// attends to the positions below len; a row of len 0 has no token: it appends nothing and
+// attends to nothing (its output is zeros).  Position p of sequence s lies in slot
+// table[s * table_stride + p / page] * page + p % page of the pool, whose rows are laid out as a
+// contiguous cache's (attention.hip: slot for pos).
+// Shared positions: ctl[3] = P of them, in the pages of sequence ctl[4].  A row with share != 0
+// and len >= P takes the positions below P from there; its own pages serve those from P on (all
+// of them otherwise).
+// Words that name no page or sequence reach no memory outside the pool: a row of such a sequence
+// counts as one of len 0, a length past the table's ends there, keys and values of such a page
+// are not stored, and a read of it goes to the pool's last page.
+#include "common.h"
+
+namespace {
+
+constexpr uint32_t HD = 128;         // head width
+constexpr uint32_t PART = HD + 2;    // one partial: m, l, acc[128]
+constexpr uint32_t TILE = 64;        // positions a wave takes at a time
+constexpr float F16_MAX = 65504.0f;
+
+struct AppendPush {
+  uint32_t q_off, k_off, v_off, o_off, qn_off, kn_off, rope_off;
+  float eps, mscale;
+  uint32_t n_head, n_kv, q_stride, kv_stride, o_stride, kc_off, vc_off, ks_off, vs_off, rows_off, table_off,
+      table_stride, n_seq, n_pages, page_log2;
+};
+struct PagedPush {
+  uint32_t q_off, q_stride, o_off, o_stride, part_off, kc_off, vc_off, ks_off, vs_off, n_kv;
+  float scale;
+  uint32_t n_shared, n_own, rows_off, table_off, table_stride, n_seq, n_pages, page_log2;
+};
+struct PagedMergePush {
+  uint32_t part_off, o_off, o_stride, n_head, n_shared, n_own, rows_off, table_stride, n_seq, page_log2;
+};
+struct LogitsPush {
+  uint32_t x_off, y_off, x_stride, y_stride, n_vocab, ctrl_off, hist_off, hist_stride, bias_off, bias_stride, mask_off,
+      mask_stride;
+};
+
+SK_DEV float wave_max(float v) {
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, 64));
+  return v;
+}
+
+// What a row attends to: [0, shared) from the shared pass and [start, len) of its own pages.
+struct Range {
+  uint32_t seq, len, start;
+  bool member;
+};
+// Shared positions, as the kernels take them: none without slots for their partials or a
+// sequence that holds them.
+SK_DEV uint32_t shared_positions(const uint32_t *ctl, uint32_t n_shared, uint32_t n_seq, uint32_t table_stride,
+                                 uint32_t page_log2) {
+  if (n_shared == 0 || ctl[4] >= n_seq) return 0;
+  const uint64_t cap = (uint64_t)table_stride << page_log2;
+  return ctl[3] < cap ? ctl[3] : (uint32_t)cap;
+}
+SK_DEV Range row_range(const uint32_t *ctl, uint32_t rows_off, uint32_t row, uint32_t shared, uint32_t n_seq,
+                       uint32_t table_stride, uint32_t page_log2) {
+  const uint4 w = *(const uint4 *)(ctl + rows_off + 4 * row);
+  const uint64_t cap = (uint64_t)table_stride << page_log2;
+  Range r;
+  r.seq = w.x < n_seq ? w.x : 0;
+  r.len = w.x < n_seq ? (w.y < cap ? w.y : (uint32_t)cap) : 0;
+  r.member = shared != 0 && w.z != 0 && r.len >= shared;
+  r.start = r.member ? shared : 0;
+  return r;
+}
+
+// A run of positions [lo, hi) in tiles of TILE from a multiple of 16 at or below lo, cut into at
+// most n parts of whole tiles.
+struct Split {
+  uint32_t base, tiles, per;
+};
+SK_DEV Split split_of(uint32_t lo, uint32_t hi, uint32_t n) {
+  Split s;
+  s.base = lo & ~15u;
+  s.tiles = hi > lo ? (hi - s.base + TILE - 1) / TILE : 0;
+  s.per = s.tiles ? (s.tiles + n - 1) / n : 1;
+  return s;
+}
+SK_DEV uint32_t live_parts(const Split &s) { return (s.tiles + s.per - 1) / s.per; }
+
+// Elements t and t + 64 of one head's cache row, held as attention.hip holds them but for one
+// thing: an f16 past the type's largest value is stored as that value, so that the cache has no
+// infinity (its products with the f16 parts of a query or a weight would be NaN).
+template <int Q8>
+SK_DEV void store_row(f16 *kv, int8_t *kv8, uint32_t cache, uint32_t scales, uint32_t kv_dim, uint32_t slot,
+                      uint32_t head, uint32_t t, float y0, float y1) {
+  auto fit = [](float v) { return v > F16_MAX ? F16_MAX : v < -F16_MAX ? -F16_MAX : v; };  // keeps NaN
+  const uint32_t dst = cache + slot * kv_dim + head * HD;
+  if constexpr (!Q8) {
+    kv[dst + t] = (f16)fit(y0);
+    kv[dst + t + 64] = (f16)fit(y1);
+  } else {
+    float m0 = fabsf(y0), m1 = fabsf(y1);  // blocks: the lower and upper 32 lanes
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) {
+      m0 = fmaxf(m0, __shfl_xor(m0, d, 64));
+      m1 = fmaxf(m1, __shfl_xor(m1, d, 64));
+    }
+    const float s0 = m0 / 127.0f, s1 = m1 / 127.0f;
+    kv8[dst + t] = (int8_t)(s0 > 0.0f ? __builtin_rintf(y0 / s0) : 0.0f);
+    kv8[dst + t + 64] = (int8_t)(s1 > 0.0f ? __builtin_rintf(y1 / s1) : 0.0f);
+    if ((t & 31) == 0) {
+      const uint32_t sd = scales + slot * (kv_dim / 32) + head * 4 + t / 32;
+      kv[sd] = (f16)fit(s0);
+      kv[sd + 2] = (f16)fit(s1);
+    }
+  }
+}
+
+// One wave per (head, row): lane t holds the pair (t, t + 64) that the rotation turns.  The
+// angle (len - 1) f_t is formed in 64 bits as revolutions and reduced there: an f32 product is off
+// by 2^-24 of an angle of 1e5, 3e-3 of a radian.
+template <int K8, int V8>
+SK_DEV void append_body(const float *w, float *a, const uint32_t *ctl, f16 *kv, int8_t *kv8, const AppendPush &p) {
+#pragma clang fp contract(off)
+  const uint32_t row = blockIdx.y, t = threadIdx.x & 63, h = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= ctl[2] || h >= p.n_head + 2 * p.n_kv) return;
+  const Range r = row_range(ctl, p.rows_off, row, 0, p.n_seq, p.table_stride, p.page_log2);
+  if (r.len == 0) return;
+  const uint32_t pos = r.len - 1;
+  const uint32_t page = ctl[p.table_off + r.seq * p.table_stride + (pos >> p.page_log2)];
+  const uint32_t slot = (page << p.page_log2) + (pos & ((1u << p.page_log2) - 1));
+  const uint32_t kv_dim = p.n_kv * HD;
+  if (h >= p.n_head + p.n_kv) {  // a value head: kept as it is
+    const uint32_t vh = h - p.n_head - p.n_kv, src = p.v_off + row * p.kv_stride + vh * HD;
+    if (page < p.n_pages) store_row<V8>(kv, kv8, p.vc_off, p.vs_off, kv_dim, slot, vh, t, a[src + t], a[src + t + 64]);
+    return;
+  }
+  const bool is_q = h < p.n_head;
+  const uint32_t head = is_q ? h : h - p.n_head;
+  const float *x = a + (is_q ? p.q_off + row * p.q_stride : p.k_off + row * p.kv_stride) + head * HD;
+  const float *nw = w + (is_q ? p.qn_off : p.kn_off);
+  const float x0 = x[t], x1 = x[t + 64];
+  const float rms = 1.0f / sqrtf(group_sum<64>(x0 * x0 + x1 * x1) / (float)HD + p.eps);
+  const float n0 = x0 * rms * nw[t], n1 = x1 * rms * nw[t + 64];
+  const double turns = (double)pos * (double)w[p.rope_off + t] * 0.15915494309189533577;  // 1 / (2 pi)
+  float s, c;
+  sincospif((float)(2.0 * (turns - __builtin_rint(turns))), &s, &c);
+  c *= p.mscale;
+  s *= p.mscale;
+  const float y0 = n0 * c - n1 * s, y1 = n0 * s + n1 * c;
+  if (is_q) {
+    float *o = a + p.o_off + row * p.o_stride + head * HD;
+    o[t] = y0;
+    o[t + 64] = y1;
+  } else if (page < p.n_pages) {
+    store_row<K8>(kv, kv8, p.kc_off, p.ks_off, kv_dim, slot, head, t, y0, y1);
+  }
+}
+
+// The state of 16 query rows (row c = lane % 16) over the positions seen so far: m the largest
+// score (in powers of two), l the sum of e = 2^(score - m), o[d] the sums of e v for the dims
+// 8 (4 g + r) + d (g = lane / 16), times 2^15 and, with 8-bit values, 2^(7 - ve).
+struct Rows16 {
+  f16x8 qh[4], ql[4];  // the query row's dims 8 g + 32 k + [0, 8) times 2^sh, in two f16 parts
+  int sh;
+  float m, l;
+  f32x4 o[8];
+  int ve;  // 8-bit values: the exponent of the largest scale so far of the dims this lane holds (block g)
+};
+
+// The query row at `q` (this lane's row), scaled to scores in powers of two.
+SK_DEV void load_query(Rows16 &s, const float *q, float scale, uint32_t g) {
+  float v[4][8], big = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    const float4 u0 = *(const float4 *)(q + 8 * g + 32 * k), u1 = *(const float4 *)(q + 8 * g + 32 * k + 4);
+    const float u[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      v[k][e] = u[e] * (scale * 1.44269504088896340736f);
+      big = fmaxf(big, fabsf(v[k][e]));
+    }
+  }
+  big = fmaxf(big, __shfl_xor(big, 16, 64));
+  big = fmaxf(big, __shfl_xor(big, 32, 64));
+  s.sh = big > 0.0f && big < INFINITY ? 11 - __builtin_amdgcn_frexp_expf(big) : 0;
+#pragma unroll
+  for (int k = 0; k < 4; k++)
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const float x = ldexpf(v[k][e], s.sh);
+      s.qh[k][e] = (f16)x;
+      s.ql[k][e] = (f16)(x - (float)s.qh[k][e]);
+    }
+  s.m = -INFINITY;
+  s.l = 0.0f;
+  s.ve = -200;
+#pragma unroll
+  for (int d = 0; d < 8; d++) s.o[d] = {0.0f, 0.0f, 0.0f, 0.0f};
+}
+
+// One tile of positions into the state: group t of 16 starts at pool slot slot[t], positions
+// [lo, hi) of the tile are live.  Loads of the others go to live positions of the tile, and their
+// scores are -inf, so what lies there reaches nothing.
+template <int K8, int V8>
+SK_DEV void tile_step(Rows16 &s, const f16 *kv, const int8_t *kv8, const PagedPush &p, uint32_t kvh,
+                      const uint32_t (&slot)[4], uint32_t lo, uint32_t hi) {
+  const uint32_t lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, kv_dim = p.n_kv * HD;
+  // the pool row of position i of group t, moved to a live one
+  auto at = [&](uint32_t t, uint32_t i) {
+    const uint32_t pos = min(max(16 * t + i, lo), hi - 1), tt = pos >> 4;
+    const uint32_t first = tt == 0 ? slot[0] : tt == 1 ? slot[1] : tt == 2 ? slot[2] : slot[3];
+    return first + (pos & 15);
+  };
+  uint4 kr[4][4];
+#pragma unroll
+  for (uint32_t t = 0; t < 4; t++) {
+    const uint32_t src = p.kc_off + at(t, c) * kv_dim + kvh * HD + 8 * g;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      if constexpr (K8) {
+        const uint2 r = *(const uint2 *)(kv8 + src + 32 * k);
+        kr[t][k] = make_uint4(r.x, r.y, 0u, 0u);
+      } else {
+        kr[t][k] = *(const uint4 *)(kv + src + 32 * k);
+      }
+    }
+  }
+  f16x4 ks[4][4];
+  if constexpr (K8)
+#pragma unroll
+    for (uint32_t t = 0; t < 4; t++)
+#pragma unroll
+      for (uint32_t r = 0; r < 4; r++)
+        ks[t][r] = *(const f16x4 *)(kv + p.ks_off + at(t, 4 * g + r) * (kv_dim / 32) + kvh * 4);
+  uint4 vr[2][8];
+  f16 vs[2][8];
+#pragma unroll
+  for (uint32_t u = 0; u < 2; u++)
+#pragma unroll
+    for (uint32_t e = 0; e < 8; e++) {
+      const uint32_t row = at(2 * u + (e >> 2), 4 * g + (e & 3)), src = p.vc_off + row * kv_dim + kvh * HD + 8 * c;
+      if constexpr (V8) {
+        const uint2 r = *(const uint2 *)(kv8 + src);
+        vr[u][e] = make_uint4(r.x, r.y, 0u, 0u);
+        vs[u][e] = kv[p.vs_off + row * (kv_dim / 32) + kvh * 4 + (c >> 2)];
+      } else {
+        vr[u][e] = *(const uint4 *)(kv + src);
+      }
+    }
+  // two bytes picked by sel as an f16 pair: 1024 + (byte ^ 0x80), minus 1152
+  auto widen = [](uint32_t x1, uint32_t x0, uint32_t sel) {
+    const f16x2 off = {(f16)1152.0f, (f16)1152.0f};
+    return as_u32(as_f16x2((__builtin_amdgcn_perm(x1, x0, sel) ^ 0x00800080u) | 0x64006400u) - off);
+  };
+  // scores: lane holds row c's at positions 16 t + 4 g + r
+  float sc[4][4], m = s.m;
+#pragma unroll
+  for (uint32_t t = 0; t < 4; t++) {
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      if constexpr (K8) {
+        const uint32_t x = kr[t][k].x, y = kr[t][k].y;
+        const f16x8 b = __builtin_bit_cast(f16x8, make_uint4(widen(x, x, 0x0c010c00u), widen(x, x, 0x0c030c02u),
+                                                             widen(y, y, 0x0c010c00u), widen(y, y, 0x0c030c02u)));
+        f32x4 part = {0.0f, 0.0f, 0.0f, 0.0f};
+        part = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, s.ql[k], part, 0, 0, 0);
+        part = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, s.qh[k], part, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 4; r++) acc[r] = __builtin_fmaf((float)ks[t][r][k], part[r], acc[r]);
+      } else {
+        const f16x8 b = __builtin_bit_cast(f16x8, kr[t][k]);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, s.ql[k], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, s.qh[k], acc, 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (uint32_t r = 0; r < 4; r++) {
+      const uint32_t pos = 16 * t + 4 * g + r;
+      sc[t][r] = pos >= lo && pos < hi ? ldexpf(acc[r], -s.sh) : -INFINITY;
+      m = fmaxf(m, sc[t][r]);
+    }
+  }
+  m = fmaxf(m, __shfl_xor(m, 16, 64));
+  m = fmaxf(m, __shfl_xor(m, 32, 64));
+  const float mu = m > -INFINITY ? m : 0.0f;  // scores of -inf alone: every e is 0
+  float down = __builtin_amdgcn_exp2f(s.m - mu);  // 0 for the first tile
+  s.m = m;
+  float l = 0.0f;
+  f16x8 ph[2], pl[2];  // e 2^15 in two parts: 22 bits from e = 2^-18 on, 2^-40 of the largest below
+#pragma unroll
+  for (uint32_t t = 0; t < 4; t++)
+#pragma unroll
+    for (uint32_t r = 0; r < 4; r++) {
+      const float e = __builtin_amdgcn_exp2f(sc[t][r] - mu), x = e * 32768.0f;
+      l += e;
+      const uint32_t i = 4 * (t & 1) + r;
+      ph[t >> 1][i] = (f16)x;
+      pl[t >> 1][i] = (f16)(x - (float)ph[t >> 1][i]);
+    }
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  s.l = __builtin_fmaf(s.l, down, l);
+  if constexpr (V8) {  // the scales of a block, largest first: to [64, 128), and the sums with them
+    float top = 0.0f;
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf((float)vs[u][e]));
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const int mine = __shfl(s.ve, (int)(16 * (c >> 2)), 64);  // this lane's values' block is c / 4
+    const int ve = top > 0.0f ? max(mine, __builtin_amdgcn_frexp_expf(top)) : mine;
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) vs[u][e] = (f16)ldexpf((float)vs[u][e], 7 - ve);
+    const int next = __shfl(ve, (int)(4 * g), 64);
+    down = ldexpf(down, s.ve - next);
+    s.ve = next;
+  }
+#pragma unroll
+  for (int d = 0; d < 8; d++) s.o[d] *= down;
+  auto word = [](const uint4 &u, int i) { return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w; };
+#pragma unroll
+  for (int d = 0; d < 8; d++) {
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      f16x8 vh, vl;
+      if constexpr (V8) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const uint32_t sel = 0x0c040c00u + (d & 3) * 0x00010001u;
+          const f16x2 v = as_f16x2(widen(word(vr[u][e + 1], d >> 2), word(vr[u][e], d >> 2), sel));
+          const f16x2 sv = {vs[u][e], vs[u][e + 1]};
+          const f16x2 hi = v * sv, rest = __builtin_elementwise_fma(v, sv, -hi);
+          vh[e] = hi.x, vh[e + 1] = hi.y;
+          vl[e] = rest.x, vl[e + 1] = rest.y;
+        }
+        s.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[u], s.o[d], 0, 0, 0);
+      } else {
+        const uint32_t sel = d & 1 ? 0x07060302u : 0x05040100u;
+        uint32_t x[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          x[e] = __builtin_amdgcn_perm(word(vr[u][2 * e + 1], d >> 1), word(vr[u][2 * e], d >> 1), sel);
+        vh = __builtin_bit_cast(f16x8, make_uint4(x[0], x[1], x[2], x[3]));
+      }
+      s.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl[u], s.o[d], 0, 0, 0);
+      s.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[u], s.o[d], 0, 0, 0);
+    }
+  }
+}
+
+// One wave per (key head, part of a run of positions, 16 query rows): the shared run with 16 of
+// all rows' heads, or one row's own run with its N_REP heads.
+template <int N_REP, int K8, int V8>
+SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_t *kv8, const PagedPush &p,
+                       uint32_t n_grid) {
+  const uint32_t lane = threadIdx.x, c = lane & 15, g = lane >> 4, kvh = blockIdx.y, work = blockIdx.x;
+  const uint32_t n_rows = min(ctl[2], n_grid), slots = p.n_shared + p.n_own;
+  const uint32_t shared = shared_positions(ctl, p.n_shared, p.n_seq, p.table_stride, p.page_log2);
+  const uint32_t tiles16 = (n_grid * N_REP + 15) / 16;
+  uint32_t row, head, lo, hi, part, seq;
+  bool live;
+  Split sp;
+  if (work < tiles16 * p.n_shared) {  // the shared run
+    const uint32_t i = work / p.n_shared * 16 + c;
+    part = work % p.n_shared;
+    row = i / N_REP;
+    head = i % N_REP;
+    live = row < n_rows && row_range(ctl, p.rows_off, row, shared, p.n_seq, p.table_stride, p.page_log2).member;
+    if (!__any(live)) return;
+    if (row >= n_rows) row = n_rows - 1;
+    lo = 0, hi = shared, seq = ctl[4];
+    sp = split_of(lo, hi, p.n_shared);
+  } else {
+    const uint32_t i = work - tiles16 * p.n_shared;
+    row = i / p.n_own;
+    part = i % p.n_own;
+    if (row >= n_rows) return;
+    head = c % N_REP;
+    live = c < N_REP;
+    const Range r = row_range(ctl, p.rows_off, row, shared, p.n_seq, p.table_stride, p.page_log2);
+    lo = r.start, hi = r.len, seq = r.seq;
+    sp = split_of(lo, hi, p.n_own);
+  }
+  const uint32_t first = part * sp.per, last = min(first + sp.per, sp.tiles);
+  if (first >= last) return;
+  if (work >= tiles16 * p.n_shared) part += p.n_shared;
+  Rows16 s;
+  load_query(s, a + p.q_off + row * p.q_stride + (kvh * N_REP + head) * HD, p.scale, g);
+  const uint32_t *table = ctl + p.table_off + seq * p.table_stride;
+  for (uint32_t tile = first; tile < last; tile++) {
+    const uint32_t begin = sp.base + tile * TILE;
+    uint32_t slot[4];
+#pragma unroll
+    for (uint32_t t = 0; t < 4; t++) {
+      const uint32_t pos = min(begin + 16 * t, (hi - 1) & ~15u);
+      const uint32_t page = min(table[pos >> p.page_log2], p.n_pages - 1);
+      slot[t] = (page << p.page_log2) + (pos & ((1u << p.page_log2) - 1));
+    }
+    tile_step<K8, V8>(s, kv, kv8, p, kvh, slot, max(lo, begin) - begin, min(hi - begin, TILE));
+  }
+  if (!live) return;
+  float *out = a + p.part_off + ((row * p.n_kv * N_REP + kvh * N_REP + head) * slots + part) * PART;
+  const int back = V8 ? s.ve - 22 : -15;
+#pragma unroll
+  for (int r = 0; r < 4; r++)
+#pragma unroll
+    for (int d = 0; d < 8; d += 2)
+      *(float2 *)(out + 2 + 8 * (4 * g + r) + d) = make_float2(ldexpf(s.o[d][r], back), ldexpf(s.o[d + 1][r], back));
+  if (g == 0) *(float2 *)out = make_float2(s.m, s.l);
+}
+
+}  // namespace
+
+#define APPEND(K8, V8)                                                                                 \
+  extern "C" __global__ __launch_bounds__(256) void kv_append__##K8##_##V8##_128(                      \
+      const float *w, float *a, const uint32_t *ctl, f16 *kv, int8_t *kv8, AppendPush p) {              \
+    append_body<K8, V8>(w, a, ctl, kv, kv8, p);                                                         \
+  }
+APPEND(0, 0)
+APPEND(0, 1)
+APPEND(1, 1)
+
+#define PAGED(R, K8, V8)                                                                               \
+  extern "C" __global__ __launch_bounds__(64) void attention_paged__##R##_##K8##_##V8##_128(            \
+      float *a, const uint32_t *ctl, const f16 *kv, const int8_t *kv8, const f16 *kvs, PagedPush p,     \
+      uint32_t n_grid) {                                                                               \
+    (void)kvs;                                                                                         \
+    paged_body<R, K8, V8>(a, ctl, kv, kv8, p, n_grid);                                                 \
+  }
+#define PAGED_REP(K8, V8) PAGED(1, K8, V8) PAGED(2, K8, V8) PAGED(4, K8, V8) PAGED(8, K8, V8)
+PAGED_REP(0, 0)
+PAGED_REP(0, 1)
+PAGED_REP(1, 1)
+
+// o = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s over a row's live partials, one wave per
+// (head, row), lane t dims 2 t and 2 t + 1.
+extern "C" __global__ __launch_bounds__(256) void attention_paged_merge__128(float *a, const uint32_t *ctl,
+                                                                             PagedMergePush p) {
+  const uint32_t lane = threadIdx.x & 63, h = blockIdx.x * 4 + (threadIdx.x >> 6), row = blockIdx.y;
+  if (row >= ctl[2] || h >= p.n_head) return;
+  const uint32_t shared = shared_positions(ctl, p.n_shared, p.n_seq, p.table_stride, p.page_log2);
+  const Range r = row_range(ctl, p.rows_off, row, shared, p.n_seq, p.table_stride, p.page_log2);
+  const uint32_t ns = r.member ? live_parts(split_of(0, shared, p.n_shared)) : 0;
+  const uint32_t no = live_parts(split_of(r.start, r.len, p.n_own)), n = ns + no;
+  const float *part = a + p.part_off + (row * p.n_head + h) * (p.n_shared + p.n_own) * PART;
+  // live partial i
+  auto at = [&](uint32_t i) { return part + (i < ns ? i : p.n_shared + i - ns) * PART; };
+  float big = -INFINITY;
+  for (uint32_t i = lane; i < n; i += 64) big = fmaxf(big, at(i)[0]);
+  big = wave_max(big);
+  float l = 0.0f, ox = 0.0f, oy = 0.0f;
+  for (uint32_t i = 0; i < n; i++) {
+    const float *s = at(i);
+    const float w = __builtin_amdgcn_exp2f(s[0] - big);
+    const float2 v = *(const float2 *)(s + 2 + 2 * lane);
+    l = __builtin_fmaf(w, s[1], l);
+    ox = __builtin_fmaf(w, v.x, ox);
+    oy = __builtin_fmaf(w, v.y, oy);
+  }
+  *(float2 *)(a + p.o_off + row * p.o_stride + h * HD + 2 * lane) =
+      n ? make_float2(ox / l, oy / l) : make_float2(0.0f, 0.0f);
+}
+
+// logits_adjust: y = adjust(x) for every token of a row's vocabulary.  Row r has eight words at
+// ctrl_off + 8 r: {history length, prompt length, biases, mask (0: none), repetition, frequency,
+// presence, 0} (the last three floats); its history is token ids, the prompt's first, its biases
+// pairs (id, f32), its mask one bit a token (1: allowed).  With c the token's count past the prompt:
+//   in the history   x / repetition where x > 0, x repetition elsewhere
+//   c > 0            - (frequency c + presence)
+//   biased           + the last bias of its id
+//   not allowed      -inf
+// Ids past the vocabulary count for nothing.  Lengths are cut to the strides.
+//
+// A workgroup takes VT tokens of a row: it counts the history's tokens among them in LDS (integer
+// counts, so any order gives the same), then passes over the logits once.
+constexpr uint32_t VT = 4096;
+extern "C" __global__ __launch_bounds__(256) void logits_adjust(float *a, const uint32_t *ctl, LogitsPush p) {
+#pragma clang fp contract(off)
+  __shared__ uint32_t count[VT];  // uses past the prompt; bit 31: in the prompt
+  __shared__ uint32_t entry[VT];  // 1 + the place of the token's last bias
+  const uint32_t row = blockIdx.y, t = threadIdx.x, base = blockIdx.x * VT, n = min(VT, p.n_vocab - base);
+  if (row >= ctl[2]) return;
+  const uint32_t *c = ctl + p.ctrl_off + 8 * row;
+  const float rho = __builtin_bit_cast(float, c[4]), freq = __builtin_bit_cast(float, c[5]),
+              pres = __builtin_bit_cast(float, c[6]);
+  const uint32_t n_hist = rho != 1.0f || freq != 0.0f || pres != 0.0f ? min(c[0], p.hist_stride) : 0;
+  const uint32_t n_prompt = c[1], n_bias = min(c[2], p.bias_stride / 2);
+  const uint32_t *hist = ctl + p.hist_off + row * p.hist_stride, *bias = ctl + p.bias_off + row * p.bias_stride;
+  const bool masked = c[3] != 0 && p.mask_stride != 0;
+  for (uint32_t i = t; i < VT; i += 256) {
+    count[i] = 0;
+    entry[i] = 0;
+  }
+  __syncthreads();
+  for (uint32_t i = t; i < n_hist; i += 256) {
+    const uint32_t id = hist[i] - base;
+    if (id < n) {
+      if (i < n_prompt)
+        atomicOr(&count[id], 0x80000000u);
+      else
+        atomicAdd(&count[id], 1u);
+    }
+  }
+  for (uint32_t i = t; i < n_bias; i += 256) {
+    const uint32_t id = bias[2 * i] - base;
+    if (id < n) atomicMax(&entry[id], i + 1);
+  }
+  __syncthreads();
+  const float *x = a + p.x_off + row * p.x_stride + base;
+  float *y = a + p.y_off + row * p.y_stride + base;
+  for (uint32_t i = t; i < n; i += 256) {
+    float v = x[i];
+    const uint32_t k = count[i], made = k & 0x7fffffffu;
+    if (k) v = v > 0.0f ? v / rho : v * rho;
+    if (made) v -= freq * (float)made + pres;
+    if (entry[i]) v += __builtin_bit_cast(float, bias[2 * (entry[i] - 1) + 1]);
+    if (masked && !((ctl[p.mask_off + row * p.mask_stride + (base + i) / 32] >> ((base + i) & 31)) & 1)) v = -INFINITY;
+    y[i] = v;
+  }
+}

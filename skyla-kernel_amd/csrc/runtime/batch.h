@@ -1,0 +1,199 @@
+// Host side of the batch operators (kernels/batch.hip): the checks of their push words against
+// the buffers they are bound to, and the launch a dispatch of theirs becomes.  Plain C++, no HIP.
+#pragma once
+
+#include <cstdarg>
+#include <cstdint>
+#include <cstdio>
+#include <cstring>
+#include <string>
+#include <vector>
+
+namespace batch {
+
+enum Op { kNone, kAppend, kAttend, kMerge, kLogits };
+
+inline Op op_of(const char *name) {
+  if (std::strcmp(name, "kv_append") == 0) return kAppend;
+  if (std::strcmp(name, "attention_paged") == 0) return kAttend;
+  if (std::strcmp(name, "attention_paged_merge") == 0) return kMerge;
+  if (std::strcmp(name, "logits_adjust") == 0) return kLogits;
+  return kNone;
+}
+
+constexpr uint32_t kHead = 128, kPart = kHead + 2;
+constexpr uint32_t kMaxSlots = 1024;      // partials of a row and head
+constexpr uint32_t kMaxGrid = 65535;      // rows of a dispatch
+constexpr uint32_t kMaxWork = 1u << 22;   // workgroups of an attention launch for each key head
+constexpr uint32_t kLogitsTile = 4096;    // tokens of a logits workgroup (batch.hip VT)
+
+// [off, off + stride (rows - 1) + width) in elements
+struct Region {
+  const char *what;
+  uint64_t off, stride, width, rows;
+  uint64_t end() const { return rows ? off + stride * (rows - 1) + width : off; }
+  bool meets(const Region &o) const { return rows && o.rows && off < o.end() && o.off < end(); }
+};
+
+class Check {
+ public:
+  std::string error;
+  void fail(const char *fmt, ...) {
+    if (!error.empty()) return;
+    char buf[256];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    error = buf;
+  }
+  void need(bool ok, const char *what) {
+    if (!ok) fail("%s", what);
+  }
+  // r lies in a binding of `elements`, its rows apart from each other, offset and stride multiples of `align`
+  void holds(const Region &r, uint64_t elements, uint32_t align) {
+    if (!r.rows) return;
+    if (r.off % align || (r.rows > 1 && r.stride % align)) fail("%s: offset or stride not a multiple of %u", r.what, align);
+    if (r.rows > 1 && r.stride < r.width) fail("%s: stride %llu below the row's %llu", r.what,
+                                               (unsigned long long)r.stride, (unsigned long long)r.width);
+    if (r.end() > elements)
+      fail("%s ends at %llu, past the binding's %llu", r.what, (unsigned long long)r.end(), (unsigned long long)elements);
+  }
+  void apart(const Region &a, const Region &b) {
+    if (a.meets(b)) fail("%s and %s overlap", a.what, b.what);
+  }
+};
+
+// the page table's words and the words of the rows
+inline void check_pages(Check &c, const Region &rows, const Region &table, uint64_t words, uint32_t page_log2,
+                        uint32_t n_pages) {
+  c.need(page_log2 >= 4 && page_log2 <= 12, "pages hold 16 to 4096 positions");
+  c.need(n_pages >= 1, "the pool has no pages");
+  c.holds(rows, words, 4);
+  c.holds(table, words, 1);
+}
+
+// a pool's keys and values and the scales of its 8-bit halves: in their bindings, apart from each other
+inline void check_pool(Check &c, bool k8, bool v8, const uint32_t off[4], uint64_t slots, uint64_t kv_dim,
+                       uint64_t kv_bytes, uint64_t kv8_bytes) {
+  const Region half[2] = {{"the pool's keys", off[0], 0, slots * kv_dim, 1}, {"the pool's values", off[1], 0, slots * kv_dim, 1}};
+  std::vector<Region> bytes;
+  for (int i = 0; i < 2; i++) {
+    const bool q8 = i ? v8 : k8;
+    const uint64_t size = q8 ? 1 : 2;
+    c.holds(half[i], q8 ? kv8_bytes : kv_bytes / 2, 8);
+    bytes.push_back({half[i].what, half[i].off * size, 0, half[i].width * size, 1});
+    if (q8) {
+      const Region s{i ? "the values' scales" : "the keys' scales", off[2 + i], 0, slots * (kv_dim / 32), 1};
+      c.holds(s, kv_bytes / 2, 4);
+      bytes.push_back({s.what, s.off * 2, 0, s.width * 2, 1});
+    }
+  }
+  for (size_t i = 0; i < bytes.size(); i++)
+    for (size_t j = 0; j < i; j++) c.apart(bytes[j], bytes[i]);
+}
+
+// "" or why a dispatch of `op` (spec, push words, grid, bytes of the bound buffers) is refused.
+inline std::string refusal(Op op, const uint32_t *spec, const uint32_t *w, const uint32_t *groups,
+                           const uint64_t *bytes) {
+  Check c;
+  const uint64_t rows = groups[1];
+  c.need(groups[0] == 1 && groups[2] == 1, "the grid is [1, rows, 1]");
+  if (rows > kMaxGrid) c.fail("%llu rows: at most %u", (unsigned long long)rows, kMaxGrid);
+  if (!c.error.empty() || rows == 0) return c.error;
+  if (op == kAppend) {
+    const uint64_t a = bytes[1] / 4, n_head = w[9], n_kv = w[10], kv_dim = n_kv * kHead;
+    c.need(n_head >= 1 && n_head <= 1024 && n_kv >= 1 && n_kv <= 1024, "1 to 1024 heads");
+    if (!c.error.empty()) return c.error;
+    const Region q{"q", w[0], w[11], n_head * kHead, rows}, k{"k", w[1], w[12], kv_dim, rows},
+        v{"v", w[2], w[12], kv_dim, rows}, o{"the rotated q", w[3], w[13], n_head * kHead, rows};
+    const Region words{"the rows' words", w[18], 4, 4, rows}, table{"the page table", w[19], 0, (uint64_t)w[21] * w[20], 1};
+    check_pages(c, words, table, bytes[2] / 4, w[23], w[22]);
+    c.need(w[20] >= 1 && w[21] >= 1, "the page table is empty");
+    if (!c.error.empty()) return c.error;
+    const uint64_t slots = (uint64_t)w[22] << w[23];
+    for (const Region *r : {&q, &k, &v, &o}) c.holds(*r, a, 1);
+    for (uint32_t i : {4u, 5u}) c.holds({"a norm's weights", w[i], 0, kHead, 1}, bytes[0] / 4, 1);
+    c.holds({"the rotation's frequencies", w[6], 0, kHead / 2, 1}, bytes[0] / 4, 1);
+    check_pool(c, spec[0], spec[1], w + 14, slots, kv_dim, bytes[3], bytes[4]);
+    // in place, or apart: another wave may still read what this one writes
+    if (!(o.off == q.off && (o.stride == q.stride || rows == 1))) c.apart(o, q);
+    c.apart(o, k);
+    c.apart(o, v);
+    c.apart(o, words);
+    c.apart(o, table);
+  } else if (op == kAttend) {
+    const uint64_t a = bytes[0] / 4, n_kv = w[9], kv_dim = n_kv * kHead, n_head = n_kv * spec[0];
+    const uint64_t parts = (uint64_t)w[11] + w[12];
+    c.need(n_kv >= 1 && n_kv <= 1024, "1 to 1024 key heads");
+    c.need(w[12] >= 1 && parts <= kMaxSlots, "a row's own positions take 1 part or more, all of them at most 1024");
+    if (!c.error.empty()) return c.error;
+    const Region q{"q", w[0], w[1], n_head * kHead, rows}, o{"the output", w[2], w[3], n_head * kHead, rows};
+    const Region part{"the partials", w[4], 0, rows * n_head * parts * kPart, 1};
+    const Region words{"the rows' words", w[13], 4, 4, rows}, table{"the page table", w[14], 0, (uint64_t)w[16] * w[15], 1};
+    check_pages(c, words, table, bytes[1] / 4, w[18], w[17]);
+    c.need(w[15] >= 1 && w[16] >= 1, "the page table is empty");
+    if (!c.error.empty()) return c.error;
+    const uint64_t slots = (uint64_t)w[17] << w[18];
+    c.holds(q, a, 4);
+    c.holds(o, a, 2);
+    c.holds(part, a, 2);
+    check_pool(c, spec[1], spec[2], w + 5, slots, kv_dim, bytes[2], bytes[3]);
+    for (const Region *r : {&q, &o, &words, &table}) c.apart(part, *r);
+    c.apart(o, words);
+    c.apart(o, table);
+    if ((rows * spec[0] + 15) / 16 * w[11] + rows * w[12] > kMaxWork)
+      c.fail("%llu rows in %llu parts: too many workgroups", (unsigned long long)rows, (unsigned long long)parts);
+  } else if (op == kMerge) {
+    const uint64_t a = bytes[0] / 4, n_head = w[3], parts = (uint64_t)w[4] + w[5];
+    c.need(n_head >= 1 && n_head <= 8192, "1 to 8192 heads");
+    c.need(w[5] >= 1 && parts <= kMaxSlots, "a row's own positions take 1 part or more, all of them at most 1024");
+    c.need(w[9] >= 4 && w[9] <= 12, "pages hold 16 to 4096 positions");
+    if (!c.error.empty()) return c.error;
+    const Region part{"the partials", w[0], 0, rows * n_head * parts * kPart, 1},
+        o{"the output", w[1], w[2], n_head * kHead, rows}, words{"the rows' words", w[6], 4, 4, rows};
+    c.holds(part, a, 2);
+    c.holds(o, a, 2);
+    c.holds(words, bytes[1] / 4, 4);
+    c.apart(o, part);
+    c.apart(o, words);
+  } else if (op == kLogits) {
+    const uint64_t a = bytes[0] / 4, u = bytes[1] / 4, v = w[4];
+    c.need(v >= 1, "an empty vocabulary");
+    const Region x{"the logits", w[0], w[2], v, rows}, y{"the adjusted logits", w[1], w[3], v, rows};
+    const Region ctrl{"the rows' words", w[5], 8, 8, rows}, hist{"the histories", w[6], w[7], w[7], w[7] ? rows : 0},
+        bias{"the biases", w[8], w[9], w[9], w[9] ? rows : 0}, mask{"the masks", w[10], w[11], w[11], w[11] ? rows : 0};
+    c.holds(x, a, 4);
+    c.holds(y, a, 4);
+    c.holds(ctrl, u, 4);
+    c.holds(hist, u, 4);
+    c.holds(bias, u, 2);
+    c.holds(mask, u, 1);
+    if (w[11] && w[11] < (v + 31) / 32) c.fail("a mask of %u words for %llu tokens", w[11], (unsigned long long)v);
+    if (!(y.off == x.off && (y.stride == x.stride || rows == 1))) c.apart(y, x);
+    for (const Region *r : {&ctrl, &hist, &bias, &mask}) c.apart(y, *r);
+  }
+  return c.error;
+}
+
+// The launch of a dispatch: its grid and trailing by-value words.
+inline void shape(Op op, const uint32_t *spec, const uint32_t *w, uint32_t rows, uint32_t groups[3],
+                  std::vector<uint32_t> &extra) {
+  groups[2] = 1;
+  if (op == kAppend) {
+    groups[0] = (w[9] + 2 * w[10] + 3) / 4;  // one wave a head
+    groups[1] = rows;
+  } else if (op == kAttend) {
+    groups[0] = (rows * spec[0] + 15) / 16 * w[11] + rows * w[12];
+    groups[1] = w[9];
+    extra = {rows};
+  } else if (op == kMerge) {
+    groups[0] = (w[3] + 3) / 4;
+    groups[1] = rows;
+  } else {
+    groups[0] = (w[4] + kLogitsTile - 1) / kLogitsTile;
+    groups[1] = rows;
+  }
+}
+
+}  // namespace batch

@@ -16,4 +16,5 @@ EMBED(skyla_co_matmul_ring, "matmul_ring.hsaco")
 EMBED(skyla_co_moe, "moe.hsaco")
 EMBED(skyla_co_util, "util.hsaco")
 EMBED(skyla_co_attention, "attention.hsaco")
+EMBED(skyla_co_batch, "batch.hsaco")
     .section .note.GNU-stack,"",@progbits

@@ -8,8 +8,8 @@
 //     hipModuleGetFunction, and launches it with hipModuleLaunchKernel.
 //   * A recording is a launch list.  Replaying it launches one HIP graph (built once by
 //     capturing the list on the context stream), so a decode step costs one submission
-//     instead of one per kernel; a profiled recording replays eagerly with a HIP event
-//     after every mark.
+//     instead of one per kernel; a list of few launches replays as those launches; a profiled
+//     recording replays eagerly with a HIP event after every mark.
 //   * Dispatches the engine records with no barrier between them are independent.  Runs of
 //     such dispatches of one matvec pipeline (q/k/v, gate/up, an expert's gate/up) become
 //     one launch over their combined rows: each kernel launch on MI355X carries ~1.7 us of
@@ -29,6 +29,8 @@
 #include <string>
 #include <vector>
 
+#include "batch.h"
+
 // Code objects embedded by embed.S.
 extern "C" const unsigned char skyla_co_matvec[], skyla_co_matvec_end[];
 extern "C" const unsigned char skyla_co_matmul[], skyla_co_matmul_end[];
@@ -36,6 +38,7 @@ extern "C" const unsigned char skyla_co_matmul_ring[], skyla_co_matmul_ring_end[
 extern "C" const unsigned char skyla_co_moe[], skyla_co_moe_end[];
 extern "C" const unsigned char skyla_co_util[], skyla_co_util_end[];
 extern "C" const unsigned char skyla_co_attention[], skyla_co_attention_end[];
+extern "C" const unsigned char skyla_co_batch[], skyla_co_batch_end[];
 
 namespace {
 
@@ -61,6 +64,10 @@ int fail(int code, const char *fmt, ...) {
 constexpr uint64_t kMaxBuffer = 4ull << 30;  // keeps u32 element offsets valid
 constexpr uint32_t kMaxMarks = 2048;          // skyla-vk/src/record.rs:6
 constexpr uint64_t kMaxPinned = 1ull << 30;   // host mirrors pinned up to this size
+// Recordings of at most this many launches replay as direct launches: a graph's submission costs
+// a fixed 30 us of host time, a launch of its own 3 (us a replay of small kernels, graph / direct:
+// 1 launch 29.8 / 12.0, 2 30.2 / 15.2, 4 30.5 / 20.3, 6 32 / 25.4, 8 32.4 / 48, 12 38.9 / 64).
+constexpr uint32_t kDirectLaunches = 6;
 
 // Tactics: every choice the runtime makes between kernel forms that compute the same
 // values, in one table.  The defaults are the forms measured fastest on MI355X; the
@@ -104,7 +111,8 @@ const Tactic kTactics[] = {
     {"merge_join", "1", "the f16 row prepass of the matmul after a batched attention merge runs in the merge's launch "
                         "(0: a launch of its own)"},
     {"attn_rows", "1", "attention of several tokens on the matrix cores, 16 query rows a wave (0: a workgroup per token)"},
-    {"nograph", "0", "1: recordings replay as direct launches instead of one HIP graph (kernel traces)"},
+    {"nograph", "", "recordings replay as direct launches (1: all, for kernel traces; 0: none) instead of one HIP graph; "
+                    "by default those of at most kDirectLaunches launches"},
 };
 
 // The value of tactic `key`: the last `key=value` entry of SKYLA_HIP_TACTIC, else the
@@ -186,6 +194,11 @@ const KernelInfo kKernels[] = {
     {"rope_table", 3, 3, 0, 0, -1, false, false, 64},         // a decode step's rope pairs
     {"take_last", 2, 4, 0, 0, -1, false, false},
     {"embed", 4, 8, 1, 1, -1, false, false},  // token rows from the HBM token_embd (util.hip)
+    // a served batch (kernels/batch.hip): grids of [1, rows, 1]
+    {"kv_append", 5, 24, 3, 3, -1, false, false},
+    {"attention_paged", 5, 19, 4, 4, -1, false, false, 64},
+    {"attention_paged_merge", 2, 10, 1, 1, -1, false, false},
+    {"logits_adjust", 2, 12, 0, 0, -1, false, false},
 };
 
 const KernelInfo *find_kernel(const char *name) {
@@ -306,7 +319,10 @@ struct skyla_hip_pipeline {
   hipFunction_t moe_fn = nullptr;        // MoE decode forms (fuse_moe), Q4_K experts: the gate/up pair,
   hipFunction_t moe_fn3 = nullptr;       // the down projection with moe_combine,
   hipFunction_t moe_fn4 = nullptr;       // and the gate/up pair that routes for itself
+  batch::Op batch = batch::kNone;        // a batch operator, its spec words
+  std::vector<uint32_t> spec;
   std::vector<std::vector<void *>> sets;
+  std::vector<std::vector<uint64_t>> set_bytes;  // sizes of the bound buffers
 };
 
 namespace {
@@ -327,6 +343,8 @@ struct Command {
   uint32_t tok_per_wg = 0, tok_per_wg_y = 0, tok_per_wg_z = 0, tok_threads = 0;
   std::string name;                 // the pipeline's shader name
   hipFunction_t moe_fn = nullptr, moe_fn3 = nullptr, moe_fn4 = nullptr;
+  batch::Op batch = batch::kNone;
+  std::vector<uint32_t> spec;       // of a batch operator
   uint32_t groups[3] = {0, 0, 0};
   std::vector<void *> bufs;
   std::vector<uint32_t> push;
@@ -410,6 +428,10 @@ Launch pack(const Command *const *run, uint32_t n) {
   if (!a.segmented) {
     for (int i = 0; i < 3; i++) l.groups[i] = a.groups[i];
     l.args = a.push;
+    if (a.batch) {
+      batch::shape(a.batch, a.spec.data(), a.push.data(), a.groups[1], l.groups, l.extra);
+      return l;
+    }
     if (a.tok_fn && a.tok_per_wg_z) {
       if (attention_rows_fit(a)) {
         l.fn = a.tok_fn;
@@ -1174,10 +1196,22 @@ Command dispatch_command(const skyla_hip_pipeline *p, const std::vector<void *> 
   c.moe_fn = p->moe_fn;
   c.moe_fn3 = p->moe_fn3;
   c.moe_fn4 = p->moe_fn4;
+  c.batch = p->batch;
+  c.spec = p->spec;
   for (int i = 0; i < 3; i++) c.groups[i] = groups[i];
   c.bufs = bufs;
   c.push.assign(push, push + n_push);
   return c;
+}
+
+// A batch operator's push words and grid against the buffers of its set: "" or the reason it
+// is refused.  The other kernels' words are the caller's to get right, as in the reference.
+int check_batch(const skyla_hip_pipeline *p, uint32_t set, const uint32_t *groups, const uint32_t *push,
+                const char *what) {
+  if (!p->batch) return SKYLA_HIP_OK;
+  const std::string why = batch::refusal(p->batch, p->spec.data(), push, groups, p->set_bytes[set].data());
+  if (why.empty()) return SKYLA_HIP_OK;
+  return fail(SKYLA_HIP_E_ARG, "%s: %s: %s", what, p->symbol.c_str(), why.c_str());
 }
 
 hipFunction_t find_function(skyla_hip_context *ctx, const std::string &sym) {
@@ -1452,7 +1486,7 @@ int skyla_hip_context_new(int device, skyla_hip_context **out) {
   ctx->warp = (uint32_t)prop.warpSize;
   HIP_TRY(hipStreamCreateWithFlags(&ctx->stream, hipStreamNonBlocking));
   const unsigned char *images[] = {skyla_co_matvec, skyla_co_matmul, skyla_co_matmul_ring, skyla_co_moe,
-                                   skyla_co_util, skyla_co_attention};
+                                   skyla_co_util, skyla_co_attention, skyla_co_batch};
   for (const unsigned char *img : images) {
     hipModule_t m = nullptr;
     hipError_t le = hipModuleLoadData(&m, img);
@@ -1508,6 +1542,7 @@ int skyla_hip_context_new(int device, skyla_hip_context **out) {
       if (all) ctx->ring[t][acc] = ring;
     }
   if (prop.multiProcessorCount > 0) ctx->n_cu = (uint32_t)prop.multiProcessorCount;
+  (void)hipGetLastError();  // the lookups above miss in every module but one: not the caller's error
   *out = ctx.release();
   return SKYLA_HIP_OK;
 }
@@ -1670,6 +1705,9 @@ int skyla_hip_pipeline_new(skyla_hip_context *ctx, const char *name, uint32_t n_
   p->threads = threads;
   p->segmented = k->segmented;
   p->sets.assign(n_sets, std::vector<void *>(n_buffers, nullptr));
+  p->set_bytes.assign(n_sets, std::vector<uint64_t>(n_buffers, 0));
+  p->batch = batch::op_of(name);
+  p->spec.assign(spec, spec + n_spec);
   HIP_TRY(hipSetDevice(ctx->device));
   for (hipModule_t m : ctx->modules) {
     hipFunction_t fn = nullptr;
@@ -1784,7 +1822,10 @@ int skyla_hip_pipeline_bind(skyla_hip_pipeline *p, uint32_t set, skyla_hip_buffe
     if (bufs[i]->ctx != p->ctx)
       return fail(SKYLA_HIP_E_ARG, "pipeline_bind: binding %u belongs to another context", i);
   }
-  for (uint32_t i = 0; i < n; i++) p->sets[set][i] = bufs[i]->dev;
+  for (uint32_t i = 0; i < n; i++) {
+    p->sets[set][i] = bufs[i]->dev;
+    p->set_bytes[set][i] = bufs[i]->size;
+  }
   return SKYLA_HIP_OK;
 }
 
@@ -1831,6 +1872,7 @@ int skyla_hip_record_dispatch(skyla_hip_recorder *r, const skyla_hip_pipeline *p
     if (!b)
       return record_fail(r, fail(SKYLA_HIP_E_STATE, "record_dispatch: %s set %u is not bound",
                                  p->symbol.c_str(), set));
+  if (int s = check_batch(p, set, groups, push, "record_dispatch")) return record_fail(r, s);
   Command c = dispatch_command(p, p->sets[set], groups, push, n_push);
   if (groups[0] && groups[1] && groups[2]) r->cmds.push_back(std::move(c));
   return SKYLA_HIP_OK;
@@ -1881,9 +1923,11 @@ int skyla_hip_record_end(skyla_hip_recorder *r, skyla_hip_recording **out) {
   rec->mark_ns.assign(rec->labels.size(), 0.0);
   HIP_TRY(hipSetDevice(rec->ctx->device));
   if (int s = bind_workspace(rec->launches, &rec->workspace)) return s;
-  // the nograph tactic 1: replay the launch list as direct launches (kernel traces of the
-  // exact launches a graph would hold, fused forms included)
-  if (!rec->profile && skyla_hip_recording_len(rec.get()) > 0 && tactic("nograph") != "1") {
+  // short lists, and all with the nograph tactic 1 (kernel traces of the exact launches a graph
+  // would hold, fused forms included), replay as direct launches
+  const std::string nograph = tactic("nograph");
+  const bool direct = nograph.empty() ? skyla_hip_recording_launches(rec.get()) <= kDirectLaunches : nograph == "1";
+  if (!rec->profile && skyla_hip_recording_len(rec.get()) > 0 && !direct) {
     // One graph for the whole recording, captured from the launch list on the stream.
     skyla_hip_context *ctx = rec->ctx;
     HIP_TRY(hipSetDevice(ctx->device));
@@ -2025,13 +2069,14 @@ int skyla_hip_marks(skyla_hip_context *ctx, const skyla_hip_recording *rec, cons
 int skyla_hip_time_dispatch(skyla_hip_context *ctx, const skyla_hip_pipeline *p,
                             const uint32_t groups[3], const uint32_t *push, uint32_t n_push,
                             uint32_t reps, double *ns_out) {
-  if (!ctx || !p || !groups || !ns_out || reps == 0)
+  if (!ctx || !p || !groups || !ns_out || reps == 0 || (n_push && !push))
     return fail(SKYLA_HIP_E_ARG, "time_dispatch: bad argument");
   if (n_push != p->push_words)
     return fail(SKYLA_HIP_E_ARG, "time_dispatch: %s takes %u push words, got %u",
                 p->symbol.c_str(), p->push_words, n_push);
   for (void *b : p->sets[0])
     if (!b) return fail(SKYLA_HIP_E_STATE, "time_dispatch: %s is not bound", p->symbol.c_str());
+  if (int s = check_batch(p, 0, groups, push, "time_dispatch")) return s;
   HIP_TRY(hipSetDevice(ctx->device));
   const Command c = dispatch_command(p, p->sets[0], groups, push, n_push);
   const Command *one[1] = {&c};
@@ -2072,6 +2117,7 @@ int skyla_hip_dispatch_noalloc(skyla_hip_context *ctx, const skyla_hip_pipeline 
                 p->push_words, n_push);
   for (void *b : p->sets[0])
     if (!b) return fail(SKYLA_HIP_E_STATE, "dispatch_noalloc: %s is not bound", p->symbol.c_str());
+  if (int s = check_batch(p, 0, groups, push, "dispatch_noalloc")) return s;
   if (!ctx->scratch || !ctx->fill_u32) return fail(SKYLA_HIP_E_STATE, "dispatch_noalloc: no scratch on this context");
   HIP_TRY(hipSetDevice(ctx->device));
   const Command c = dispatch_command(p, p->sets[0], groups, push, n_push);
