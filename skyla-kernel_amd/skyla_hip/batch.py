@@ -8,6 +8,7 @@ what a server of many needs beside it, over the same weights, arena rows and C-A
                   attention_paged (attention of rows over their pages, a leading run of positions
                   that many rows share read once for all of them)
   LogitsKernels   logits_adjust (penalties for repeated tokens, biases, grammar masks)
+  BatchEngine     sequences of one model: open, fork, prefill, step, close
 
 The operators read the batch's rows from four words each, {sequence, length, share, 0}: the
 row's token is at position length - 1, a row of length 0 has none.  Their push words are in
@@ -159,3 +160,359 @@ class LogitsKernels:
 
     def free(self) -> None:
         self._adjust.free()
+
+
+# ---- sequences of one model ----------------------------------------------------------------
+@dataclasses.dataclass
+class Controls:
+    """What acts on a sequence's logits (logits_adjust): a repetition penalty over all its tokens
+    (1: none), frequency and presence penalties over its generated ones, biases by token id, and
+    the tokens allowed (a truth value each; None: all)."""
+    repetition: float = 1.0
+    frequency: float = 0.0
+    presence: float = 0.0
+    bias: dict = dataclasses.field(default_factory=dict)
+    allowed: np.ndarray | None = None
+
+    @property
+    def counts(self) -> bool:
+        return self.repetition != 1.0 or self.frequency != 0.0 or self.presence != 0.0
+
+
+class _Sequence:
+    def __init__(self, pages=(), tokens=(), n_prompt=0, controls=None):
+        self.pages, self.tokens = list(pages), list(tokens)
+        self.n_prompt, self.controls = n_prompt, controls or Controls()
+
+
+class _BatchGraph(E.Graph):
+    """A layer's dispatches with the batch's cache in place of the contiguous one."""
+
+    def __init__(self, r: Recorder, eng: "BatchEngine", batched: bool, rows: int, parts: tuple[int, int]):
+        super().__init__(r, eng.kernels, eng.arena, eng.c, batched)
+        self.eng, self.rows, self.parts = eng, rows, parts
+
+    def qk_rope(self, l: int, q_norm: int, k_norm: int, rope: int) -> None:
+        a = self.a
+        q = (a.q, a.s_q)
+        self.eng.batch.append(self.r, l, self.eng.at, q, (a.k, a.s_kv), a.v, q, q_norm, k_norm, rope, self.rows,
+                              self.c.rope_mscale)
+        self.stage("kv append")
+
+    def attend(self, l: int) -> None:
+        a = self.a
+        self.eng.batch.attend(self.r, l, self.eng.at, (a.q, a.s_q), (a.attn, a.s_attn), self.rows, self.parts)
+        self.stage("attention")
+
+
+class BatchEngine:
+    """Up to BATCH sequences of one model, decoded together.  A sequence is a number from open() or
+    fork(); extend() puts tokens into its cache, step() takes a token of each of several sequences
+    and returns the logits after them, with their controls applied; close() gives its pages back.
+
+    A forked sequence shares the whole pages of the one it came from (the rest of the last page is
+    copied), and a step reads the pages that its sequences share once for all of them.  A
+    sequence's row in the batch is its number: sequences that a step leaves out are idle rows."""
+
+    MAX_BIASES = 512
+
+    def __init__(self, ctx: Context, model: dict, c: E.Config, max_ctx: int, n_pages: int, page: int = 64,
+                 precision: E.KvPrecision = E.KvPrecision.F16_KEYS_Q8_VALUES, max_seq: int = E.BATCH):
+        if not 1 <= max_seq <= E.BATCH:
+            raise ValueError(f"{max_seq} sequences: a batch holds 1 to {E.BATCH}")
+        if max_ctx < 1:
+            raise ValueError(f"max_ctx {max_ctx}")
+        self.ctx, self.c, self.max_ctx, self.max_seq = ctx, c, max_ctx, max_seq
+        self.paged = Paged(precision, page, n_pages, max_seq, -(-max_ctx // page), c.n_head_kv * c.head_dim)
+        if self.paged.bytes() > ctx.max_buffer():
+            raise ValueError(f"a layer's pool of {n_pages} pages needs {self.paged.bytes() >> 20} MiB, above the "
+                             "allocation cap")
+        self.rep = c.n_head // c.n_head_kv
+        self.s_vocab, self.s_mask = E._next64(c.n_vocab), -(-c.n_vocab // 32)
+        self.s_hist = -(-max_ctx // 4) * 4
+        part = max(part_size(r, c.n_head, self._parts(r, shared, own)) for r in self._buckets(E.BATCH)
+                   for shared in [0, *self._buckets(max_ctx)] for own in self._buckets(max_ctx))
+        self.weights = E.load_weights(ctx, model, c)
+        a = self.arena = E.Arena(ctx, c, extra={
+            "rows": 4 * E.BATCH, "table": max_seq * self.paged.seq_pages, "part": part,
+            "logits": self.s_vocab * max_seq, "controls": 8 * max_seq, "history": self.s_hist * max_seq,
+            "bias": 2 * self.MAX_BIASES * max_seq, "mask": self.s_mask * max_seq})
+        x = a.extra
+        self.pools = [ctx.alloc_host(self.paged.bytes()) for _ in range(c.n_layer)]
+        self.at = BatchRegions(rows=x["rows"], table=x["table"], part=x["part"])
+        self.logits_at = LogitsRegions(x["controls"], x["history"], self.s_hist, x["bias"], 2 * self.MAX_BIASES,
+                                       x["mask"], self.s_mask)
+        self.kernels = E.Kernels(ctx, self.weights.buffers, a.buffer, kv=self.pools[0], c=c, precision=precision,
+                                 embd_dtype=self.weights.embd.dtype)
+        self.batch = BatchKernels(ctx, self.weights.buffers[0], a.buffer, self.pools, c, self.paged)
+        self.logits = LogitsKernels(ctx, a.buffer)
+        self.recordings = {}
+        self.free_pages = list(range(n_pages - 1, -1, -1))
+        self.uses = np.zeros(n_pages, np.int64)  # sequences that hold a page
+        self.sequences: dict[int, _Sequence] = {}
+
+    # ---- sequences ----
+    def open(self) -> int:
+        return self._add(_Sequence())
+
+    def _add(self, s: _Sequence) -> int:
+        n = next((i for i in range(self.max_seq) if i not in self.sequences), None)
+        if n is None:
+            raise ValueError(f"all {self.max_seq} sequences are open")
+        self.sequences[n] = s
+        self._upload_controls(n)
+        return n
+
+    def _get(self, seq: int) -> _Sequence:
+        if seq not in self.sequences:
+            raise ValueError(f"no open sequence {seq}")
+        return self.sequences[seq]
+
+    def length(self, seq: int) -> int:
+        """Positions in a sequence's cache."""
+        return len(self._get(seq).tokens)
+
+    def fork(self, seq: int) -> int:
+        """A new sequence that goes on from where `seq` is, with its controls."""
+        s, page = self._get(seq), self.paged.page
+        whole, rest = divmod(len(s.tokens), page)
+        if len(self.sequences) == self.max_seq:
+            raise ValueError(f"all {self.max_seq} sequences are open")
+        own = self._take(1 if rest else 0)
+        self.uses[s.pages[:whole]] += 1
+        if rest:
+            self._copy_page(s.pages[whole], own[0], rest)
+        n = self._add(_Sequence(s.pages[:whole] + own, s.tokens, s.n_prompt, s.controls))
+        self._upload_table(n)
+        return n
+
+    def close(self, seq: int) -> None:
+        self._give(self._get(seq).pages)
+        del self.sequences[seq]
+
+    def control(self, seq: int, controls: Controls) -> None:
+        """Sets what acts on a sequence's logits from its next step on."""
+        s = self._get(seq)
+        values = [controls.repetition, controls.frequency, controls.presence, *controls.bias.values()]
+        if not controls.repetition > 0 or any(np.isnan(v) for v in values) or not np.isfinite(values[:3]).all():
+            raise ValueError("a repetition penalty above 0, finite penalties, biases that are numbers")
+        if len(controls.bias) > self.MAX_BIASES or any(not 0 <= int(t) < self.c.n_vocab for t in controls.bias):
+            raise ValueError(f"at most {self.MAX_BIASES} biases, of tokens of the vocabulary")
+        if controls.allowed is not None and np.shape(controls.allowed) != (self.c.n_vocab,):
+            raise ValueError(f"allowed: a truth value for each of {self.c.n_vocab} tokens")
+        s.controls = controls
+        self._upload_controls(seq)
+
+    # ---- pages ----
+    def _take(self, n: int) -> list[int]:
+        if n > len(self.free_pages):
+            raise ValueError(f"{n} pages needed, {len(self.free_pages)} free")
+        got = [self.free_pages.pop() for _ in range(n)]
+        self.uses[got] += 1
+        return got
+
+    def _give(self, pages: Sequence[int]) -> None:
+        for p in pages:
+            self.uses[p] -= 1
+            if self.uses[p] == 0:
+                self.free_pages.append(p)
+
+    def _copy_page(self, src: int, dst: int, n: int) -> None:
+        lay, page, dim = self.paged.layout, self.paged.page, self.c.n_head_kv * self.c.head_dim
+        pr = lay.precision
+        for kv in self.pools:
+            for off, scales, q8 in ((lay.keys(0), lay.key_scales(0), pr.keys_q8),
+                                    (lay.values(0), lay.value_scales(0), pr.values_q8)):
+                size = 1 if q8 else 2
+                at = lambda p: (off + p * page * dim) * size  # noqa: E731
+                kv.copy_from(at(dst), kv, at(src), n * dim * size)
+                if q8:
+                    at = lambda p: (scales + p * page * (dim // 32)) * 2  # noqa: E731
+                    kv.copy_from(at(dst), kv, at(src), n * (dim // 32) * 2)
+
+    def _room(self, need: dict[int, int]) -> None:
+        """Pages for sequences to grow by need[seq] positions: all of them or none."""
+        page, new = self.paged.page, {}
+        for seq, n in need.items():
+            s = self._get(seq)
+            if len(s.tokens) + n > self.max_ctx:
+                raise ValueError(f"sequence {seq}: context full ({self.max_ctx} tokens)")
+            new[seq] = -(-(len(s.tokens) + n) // page) - len(s.pages)
+        if sum(new.values()) > len(self.free_pages):
+            raise ValueError(f"{sum(new.values())} pages needed, {len(self.free_pages)} free")
+        for seq, n in new.items():
+            if n:
+                self._get(seq).pages += self._take(n)
+                self._upload_table(seq)
+
+    # ---- words ----
+    def _upload_table(self, seq: int) -> None:
+        a, pages = self.arena, self._get(seq).pages
+        off = self.at.table + seq * self.paged.seq_pages
+        a.u32()[off: off + len(pages)] = pages
+        if pages:
+            a.buffer.upload(off * 4, len(pages) * 4)
+
+    def _upload_history(self, seq: int, first: int = 0) -> None:
+        a, tokens = self.arena, self._get(seq).tokens
+        off = self.logits_at.history + seq * self.s_hist
+        if len(tokens) > first:
+            a.u32()[off + first: off + len(tokens)] = tokens[first:]
+            a.buffer.upload((off + first) * 4, (len(tokens) - first) * 4)
+
+    def _upload_controls(self, seq: int) -> None:
+        a, k = self.arena, self._get(seq).controls
+        u, f = a.u32(), a.f32()
+        bias = self.logits_at.bias + 2 * self.MAX_BIASES * seq
+        n = len(k.bias)
+        if n:
+            u[bias: bias + 2 * n: 2] = list(k.bias)
+            f[bias + 1: bias + 2 * n: 2] = list(k.bias.values())
+            a.buffer.upload(bias * 4, n * 8)
+        if k.allowed is not None:
+            mask = self.logits_at.mask + self.s_mask * seq
+            bits = np.zeros(32 * self.s_mask, bool)
+            bits[: self.c.n_vocab] = k.allowed
+            u[mask: mask + self.s_mask] = np.packbits(bits, bitorder="little").view("<u4")
+            a.buffer.upload(mask * 4, self.s_mask * 4)
+        if k.counts:
+            self._upload_history(seq)
+
+    def _words(self, live: int, rows: np.ndarray, tokens: Sequence[int], shared: int, leader: int) -> None:
+        a = self.arena
+        u, n = a.u32(), len(rows)
+        u[a.tokens: a.tokens + n] = tokens
+        u[self.at.rows: self.at.rows + 4 * n] = rows.ravel()
+        u[0], u[1], u[2], u[3], u[4] = int(tokens[0]), 0, live, shared, leader
+        a.buffer.upload(0, 64 * 4)
+        a.buffer.upload(a.tokens * 4, n * 4)
+        a.buffer.upload(self.at.rows * 4, n * 16)
+
+    def _check(self, tokens) -> list[int]:
+        tokens = [int(t) for t in tokens]
+        if any(not 0 <= t < self.c.n_vocab for t in tokens):
+            raise ValueError("token outside the vocabulary")
+        return tokens
+
+    # ---- recordings ----
+    @staticmethod
+    def _buckets(most: int) -> list[int]:
+        out = [1]
+        while out[-1] < most:
+            out.append(min(2 * out[-1], most))
+        return out
+
+    def _parts(self, rows: int, shared: int, own: int) -> tuple[int, int]:
+        return splits(rows, self.c.n_head_kv, self.rep, shared, own)
+
+    def _recording(self, rows: int, shared: int, own: int, head: bool):
+        """The recording for up to `rows` rows over `shared` shared and `own` positions of their own,
+        with the output head and the logits' controls or without (extend)."""
+        up = lambda n, most: next(b for b in self._buckets(most) if b >= n)  # noqa: E731
+        rows = up(rows, E.BATCH)
+        parts = self._parts(rows, up(shared, self.max_ctx) if shared else 0, up(own, self.max_ctx))
+        key = rows, parts, head
+        if key not in self.recordings:
+            self.recordings[key] = self.ctx.record(False, lambda r: self._record(r, rows, parts, head))
+        return self.recordings[key]
+
+    def _record(self, r: Recorder, rows: int, parts: tuple[int, int], head: bool) -> None:
+        a, w, c, batched = self.arena, self.weights, self.c, rows > 1
+        g = _BatchGraph(r, self, batched, rows, parts)
+        g.embed(w.embd)
+        for l, lw in enumerate(w.layers):
+            g.layer(l, lw, w.rope)
+        if head:
+            g.rmsnorm(a.x, w.out_norm, a.n, rows)
+            g.stage("rmsnorm")
+            y = (a.extra["logits"], self.s_vocab)
+            g.matvec(w.output, (a.n, a.s_embd), y, False, batched)
+            g.stage("matvec output")
+            self.logits.adjust(r, self.logits_at, y, y, c.n_vocab, min(rows, self.max_seq))
+        r.host_barrier()
+
+    # ---- decoding ----
+    def extend(self, seq: int, tokens) -> None:
+        """Puts tokens into a sequence's cache, as its prompt: BATCH of them at a time."""
+        s, tokens = self._get(seq), self._check(tokens)
+        self._room({seq: len(tokens)})
+        for i in range(0, len(tokens), E.BATCH):
+            chunk, pos = tokens[i: i + E.BATCH], len(s.tokens)
+            n = len(chunk)
+            rows = np.zeros((n, 4), np.uint32)
+            rows[:, 0], rows[:, 1], rows[:, 2] = seq, pos + 1 + np.arange(n), pos
+            self._words(n, rows, chunk, pos, seq)
+            self.ctx.replay(self._recording(n, pos, n, False))
+            s.tokens += chunk
+        s.n_prompt = len(s.tokens)
+        if s.controls.counts:
+            self._upload_history(seq, len(s.tokens) - len(tokens))
+
+    def shared_run(self, seqs) -> tuple[int, list[int]]:
+        """The positions that sequences of a step read once for all: (how many, whose).  Of the
+        sequences that begin with the same page the largest group's common whole pages."""
+        groups = {}
+        for q in seqs:
+            pages = self._get(q).pages
+            if pages:
+                groups.setdefault(pages[0], []).append(q)
+        members = max(groups.values(), key=len, default=[])
+        if len(members) < 2:
+            return 0, []
+        lists = [self._get(q).pages for q in members]
+        n = 0
+        while all(len(p) > n and p[n] == lists[0][n] for p in lists):
+            n += 1
+        return n * self.paged.page, members
+
+    def step(self, tokens: dict, prompt=()) -> np.ndarray:
+        """One token of each of several sequences ({sequence: token}): the logits after them, a row
+        each in the order given.  `prompt`: sequences whose token is their prompt's last (the
+        others' count as generated)."""
+        if not tokens:
+            raise ValueError("step needs a token of at least one sequence")
+        values, seqs = self._check(tokens.values()), list(tokens)
+        if any(q not in tokens for q in prompt):
+            raise ValueError("prompt: sequences of this step")
+        self._room({q: 1 for q in seqs})
+        live = max(seqs) + 1
+        shared, members = self.shared_run(seqs)
+        rows, ids, own = np.zeros((live, 4), np.uint32), np.zeros(live, np.uint32), 1
+        for q, t in zip(seqs, values):
+            s = self._get(q)
+            s.tokens.append(t)
+            if q in prompt:
+                s.n_prompt = len(s.tokens)
+            n, take = len(s.tokens), shared if q in members and len(s.tokens) >= shared else 0
+            rows[q], ids[q], own = (q, n, take, 0), t, max(own, n - take)
+            if s.controls.counts:
+                self._upload_history(q, n - 1)
+        self._words(live, rows, ids, shared, members[0] if members else 0)
+        self._control_words(live)
+        self.ctx.replay(self._recording(live, shared, own, True))
+        a, v = self.arena, self.c.n_vocab
+        out = np.empty((len(seqs), v), np.float32)
+        for i, q in enumerate(seqs):
+            off = a.extra["logits"] + q * self.s_vocab
+            a.buffer.download(off * 4, v * 4)
+            out[i] = a.f32()[off: off + v]
+        return out
+
+    def _control_words(self, live: int) -> None:
+        a, off = self.arena, self.logits_at.controls
+        u, f = a.u32(), a.f32()
+        for q in range(live):
+            s, o = self.sequences.get(q), off + 8 * q
+            k = s.controls if s else Controls()
+            u[o: o + 4] = (len(s.tokens), s.n_prompt, len(k.bias), k.allowed is not None) if s else 0
+            f[o + 4: o + 7] = k.repetition, k.frequency, k.presence
+        a.buffer.upload(off * 4, live * 32)
+
+    def free(self) -> None:
+        for rec in self.recordings.values():
+            rec.free()
+        self.recordings = {}
+        self.batch.free()
+        self.logits.free()
+        for b in [*self.weights.buffers, *self.pools, self.arena.buffer]:
+            b.free()

@@ -494,7 +494,9 @@ class Arena:
     chunk, which the embed kernel gathers rows for (the reference dequantises them on the
     host into x, engine.rs:100-117), and the MoE tile map moe_sort writes before its table."""
 
-    def __init__(self, ctx: Context, c: Config, max_ctx: int = 64, precision: KvPrecision | None = None):
+    def __init__(self, ctx: Context, c: Config, max_ctx: int = 64, precision: KvPrecision | None = None,
+                 extra: dict | None = None):
+        """`extra`: regions more (name -> words), their offsets in self.extra."""
         self.size = 64
         n_split = -(-max_ctx // ATTENTION_CHUNK)
         if n_split > MAX_SPLITS:
@@ -548,6 +550,7 @@ class Arena:
         # and FFN norms, then the output norm (filled by Engine from the weight tables)
         self.s_norm, self.n_layer = _next64(c.n_embd), c.n_layer
         self.norms = single(self.s_norm * (2 * c.n_layer + 1)) if c.n_layer else None
+        self.extra = {name: single(words) for name, words in (extra or {}).items()}
         self.buffer = ctx.alloc_host(self.size * 4)
         self.n_split = n_split
         self.max_ctx = max_ctx
