@@ -359,44 +359,15 @@ SK_DEV void tile_step(Rows16 &s, const f16 *kv, const int8_t *kv8, const PagedPu
   }
 }
 
-// One wave per (key head, part of a run of positions, 16 query rows): the shared run with 16 of
-// all rows' heads, or one row's own run with its N_REP heads.
-template <int N_REP, int K8, int V8>
-SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_t *kv8, const PagedPush &p,
-                       uint32_t n_grid) {
-  const uint32_t lane = threadIdx.x, c = lane & 15, g = lane >> 4, kvh = blockIdx.y, work = blockIdx.x;
-  const uint32_t n_rows = min(ctl[2], n_grid), slots = p.n_shared + p.n_own;
-  const uint32_t shared = shared_positions(ctl, p.n_shared, p.n_seq, p.table_stride, p.page_log2);
-  const uint32_t tiles16 = (n_grid * N_REP + 15) / 16;
-  uint32_t row, head, lo, hi, part, seq;
-  bool live;
-  Split sp;
-  if (work < tiles16 * p.n_shared) {  // the shared run
-    const uint32_t i = work / p.n_shared * 16 + c;
-    part = work % p.n_shared;
-    row = i / N_REP;
-    head = i % N_REP;
-    live = row < n_rows && row_range(ctl, p.rows_off, row, shared, p.n_seq, p.table_stride, p.page_log2).member;
-    if (!__any(live)) return;
-    if (row >= n_rows) row = n_rows - 1;
-    lo = 0, hi = shared, seq = ctl[4];
-    sp = split_of(lo, hi, p.n_shared);
-  } else {
-    const uint32_t i = work - tiles16 * p.n_shared;
-    row = i / p.n_own;
-    part = i % p.n_own;
-    if (row >= n_rows) return;
-    head = c % N_REP;
-    live = c < N_REP;
-    const Range r = row_range(ctl, p.rows_off, row, shared, p.n_seq, p.table_stride, p.page_log2);
-    lo = r.start, hi = r.len, seq = r.seq;
-    sp = split_of(lo, hi, p.n_own);
-  }
-  const uint32_t first = part * sp.per, last = min(first + sp.per, sp.tiles);
-  if (first >= last) return;
-  if (work >= tiles16 * p.n_shared) part += p.n_shared;
+// A run of positions through one wave for 16 query rows, and their partial.  `live`: the lane's
+// row is written.
+template <int K8, int V8>
+SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t *kv8, const PagedPush &p, uint32_t kvh,
+                     const float *q, float *out, bool live, uint32_t seq, uint32_t lo, uint32_t hi, const Split &sp,
+                     uint32_t first, uint32_t last) {
+  const uint32_t g = (threadIdx.x & 63) >> 4;
   Rows16 s;
-  load_query(s, a + p.q_off + row * p.q_stride + (kvh * N_REP + head) * HD, p.scale, g);
+  load_query(s, q, p.scale, g);
   const uint32_t *table = ctl + p.table_off + seq * p.table_stride;
   for (uint32_t tile = first; tile < last; tile++) {
     const uint32_t begin = sp.base + tile * TILE;
@@ -410,7 +381,6 @@ SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_
     tile_step<K8, V8>(s, kv, kv8, p, kvh, slot, max(lo, begin) - begin, min(hi - begin, TILE));
   }
   if (!live) return;
-  float *out = a + p.part_off + ((row * p.n_kv * N_REP + kvh * N_REP + head) * slots + part) * PART;
   const int back = V8 ? s.ve - 22 : -15;
 #pragma unroll
   for (int r = 0; r < 4; r++)
@@ -418,6 +388,342 @@ SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_
     for (int d = 0; d < 8; d += 2)
       *(float2 *)(out + 2 + 8 * (4 * g + r) + d) = make_float2(ldexpf(s.o[d][r], back), ldexpf(s.o[d + 1][r], back));
   if (g == 0) *(float2 *)out = make_float2(s.m, s.l);
+}
+
+// The shared run for WIDE = 128 query rows a workgroup, 32 a wave: what 16 rows a wave read from
+// L2 again and again passes through LDS once for all four waves.  A step takes STEP = 32
+// positions: waves 0 and 1 stage the next step's values (transposed on the way, 4 positions by 8
+// dims a thread), 2 and 3 its keys, in the order the matrix instructions read them:
+//   S^T = K Q^T   v_mfma_f32_32x32x16_f16, A = keys (row: position lane % 32, dims 16 k + 8 h +
+//                 [0, 8), h = lane / 32), B = the query rows' two f16 parts, held in registers
+//   O^T = V^T P^T B = this lane's own e: element e of k-step s is position 16 s + 8 (e / 4) + 4 h +
+//                 e % 4, as S^T leaves them; A = values of those positions, row: dim 32 d + lane % 32
+// An LDS fragment is 64 pieces of 16 bytes, lane l's at place l ^ (a constant of the fragment, and
+// for values l / 16 % 2), so that a row of the cache, whose pieces go to 16 fragments, is written
+// to 16 banks' groups.
+// The largest score is followed loosely: sums are scaled down only where a score passes the
+// reference by 2^8 (e is held times 2^7, so that it stays in f16's range), which after the first
+// steps is rare.  8-bit values are held as two f16 parts of q s 2^(7 - ve), ve the exponent of the
+// part's largest scale of the 32 dims, found first.
+constexpr uint32_t WIDE = 128, STEP = 32;
+template <int K8, int V8>
+struct WideStage {  // one step's keys and values
+  uint4 k[8][64];                 // [k-step]
+  uint4 v[V8 ? 2 : 1][2][4][64];  // [part][k-step][dims / 32]
+  float ks[K8 ? 4 : 1][K8 ? STEP : 1];  // 8-bit keys: [dims / 32][position]
+};
+template <int K8, int V8>
+SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t *kv8, const PagedPush &p, uint32_t rep,
+                     uint32_t kvh, uint32_t tile, uint32_t part, uint32_t shared, uint32_t n_rows) {
+  __shared__ WideStage<K8, V8> stage[2];
+  __shared__ float tops[V8 ? 4 : 1][4];
+  const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63, col = lane & 31, h = lane >> 5;
+  const uint32_t kv_dim = p.n_kv * HD;
+  const Split sp = split_of(0, shared, p.n_shared);
+  const uint32_t begin = part * sp.per * TILE, end = min(begin + sp.per * TILE, shared);
+  if (begin >= end) return;
+  const uint32_t i = tile * WIDE + wave * 32 + col;
+  uint32_t row = i / rep;
+  const uint32_t head = i % rep;
+  const bool live =
+      row < n_rows && row_range(ctl, p.rows_off, row, shared, p.n_seq, p.table_stride, p.page_log2).member;
+  if (!__syncthreads_or(live)) return;
+  row = min(row, n_rows - 1);
+  const uint32_t *table = ctl + p.table_off + ctl[4] * p.table_stride;
+  auto slot_of = [&](uint32_t pos) {
+    const uint32_t page = min(table[pos >> p.page_log2], p.n_pages - 1);
+    return (page << p.page_log2) + (pos & ((1u << p.page_log2) - 1));
+  };
+
+  // this wave's query rows
+  f16x8 qh[8], ql[8];
+  float inv;
+  {
+    const float *q = a + p.q_off + row * p.q_stride + (kvh * rep + head) * HD + 8 * h;
+    float u[8][8], big = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const float4 x = *(const float4 *)(q + 16 * k), y = *(const float4 *)(q + 16 * k + 4);
+      const float w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        u[k][e] = w[e] * (p.scale * 1.44269504088896340736f);
+        big = fmaxf(big, fabsf(u[k][e]));
+      }
+    }
+    big = fmaxf(big, __shfl_xor(big, 32, 64));
+    const int sh = big > 0.0f && big < INFINITY ? 11 - __builtin_amdgcn_frexp_expf(big) : 0;
+    inv = ldexpf(1.0f, -sh);
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float x = ldexpf(u[k][e], sh);
+        qh[k][e] = (f16)x;
+        ql[k][e] = (f16)(x - (float)qh[k][e]);
+      }
+  }
+
+  int ve[4] = {0, 0, 0, 0};
+  if constexpr (V8) {
+    float top[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t pos = begin + t; pos < end; pos += 256) {
+      const f16x4 s = *(const f16x4 *)(kv + p.vs_off + slot_of(pos) * (kv_dim / 32) + kvh * 4);
+#pragma unroll
+      for (int b = 0; b < 4; b++) top[b] = fmaxf(top[b], fabsf((float)s[b]));
+    }
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+      top[b] = wave_max(top[b]);
+      if (lane == 0) tops[wave][b] = top[b];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+      const float m = fmaxf(fmaxf(tops[0][b], tops[1][b]), fmaxf(tops[2][b], tops[3][b]));
+      ve[b] = m > 0.0f && m < INFINITY ? __builtin_amdgcn_frexp_expf(m) : 0;
+    }
+  }
+
+  // staging: dims 8 dg + [0, 8) of positions 4 pg + [0, 4)
+  const uint32_t dg = t & 15, pg = (t >> 4) & 7;
+  const bool keys = t >= 128;
+  uint4 ld[4];
+  f16 ls[4];
+  uint32_t next;  // the pool row of this thread's first position, a step ahead of the loads
+  auto look = [&](uint32_t at) { next = slot_of(min(at + 4 * pg, end - 1)); };
+  auto load = [&](uint32_t at) {
+    const uint32_t first = min(at + 4 * pg, end - 1), room = end - 1 - first;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++) {
+      const uint32_t r = next + min(j, room);
+      if (keys) {
+        const uint32_t src = p.kc_off + r * kv_dim + kvh * HD + 8 * dg;
+        if constexpr (K8) {
+          const uint2 x = *(const uint2 *)(kv8 + src);
+          ld[j] = make_uint4(x.x, x.y, 0u, 0u);
+          ls[j] = kv[p.ks_off + r * (kv_dim / 32) + kvh * 4 + (dg >> 2)];
+        } else {
+          ld[j] = *(const uint4 *)(kv + src);
+        }
+      } else {
+        const uint32_t src = p.vc_off + r * kv_dim + kvh * HD + 8 * dg;
+        if constexpr (V8) {
+          const uint2 x = *(const uint2 *)(kv8 + src);
+          ld[j] = make_uint4(x.x, x.y, 0u, 0u);
+          ls[j] = kv[p.vs_off + r * (kv_dim / 32) + kvh * 4 + (dg >> 2)];
+        } else {
+          ld[j] = *(const uint4 *)(kv + src);
+        }
+      }
+    }
+  };
+  auto widen = [](uint32_t x1, uint32_t x0, uint32_t sel) {
+    const f16x2 off = {(f16)1152.0f, (f16)1152.0f};
+    return as_f16x2((__builtin_amdgcn_perm(x1, x0, sel) ^ 0x00800080u) | 0x64006400u) - off;
+  };
+  auto word = [](const uint4 &u, int n) { return n == 0 ? u.x : n == 1 ? u.y : n == 2 ? u.z : u.w; };
+  int vmine = ve[0];
+  if constexpr (V8) vmine = dg >> 2 == 0 ? ve[0] : dg >> 2 == 1 ? ve[1] : dg >> 2 == 2 ? ve[2] : ve[3];
+  auto put = [&](WideStage<K8, V8> &s) {
+    if (keys) {
+      const uint32_t ks = dg >> 1, hh = dg & 1, sw = ks | (hh << 3);
+#pragma unroll
+      for (uint32_t j = 0; j < 4; j++) {
+        uint4 x = ld[j];
+        if constexpr (K8) {
+          x = make_uint4(as_u32(widen(ld[j].x, ld[j].x, 0x0c010c00u)), as_u32(widen(ld[j].x, ld[j].x, 0x0c030c02u)),
+                         as_u32(widen(ld[j].y, ld[j].y, 0x0c010c00u)), as_u32(widen(ld[j].y, ld[j].y, 0x0c030c02u)));
+          if ((dg & 3) == 0) s.ks[dg >> 2][4 * pg + j] = (float)ls[j];
+        }
+        s.k[ks][(hh * 32 + 4 * pg + j) ^ sw] = x;
+      }
+    } else {
+      const uint32_t dt = dg >> 2, ks = pg >> 2, hh = pg & 1, half = (pg >> 1) & 1;
+      const uint32_t sw = dt | ((dg >> 1 & 1) << 2);
+      f16x2 s01, s23;
+      if constexpr (V8) {
+        s01 = f16x2{(f16)ldexpf((float)ls[0], 7 - vmine), (f16)ldexpf((float)ls[1], 7 - vmine)};
+        s23 = f16x2{(f16)ldexpf((float)ls[2], 7 - vmine), (f16)ldexpf((float)ls[3], 7 - vmine)};
+      }
+#pragma unroll
+      for (uint32_t e = 0; e < 8; e++) {
+        const uint32_t at = (hh * 32 + 8 * (dg & 3) + e) ^ sw;
+        if constexpr (V8) {
+          const uint32_t sel = 0x0c040c00u + (e & 3) * 0x00010001u;
+          const f16x2 v01 = widen(word(ld[1], e >> 2), word(ld[0], e >> 2), sel);
+          const f16x2 v23 = widen(word(ld[3], e >> 2), word(ld[2], e >> 2), sel);
+          const f16x2 h01 = v01 * s01, h23 = v23 * s23;
+          ((uint2 *)&s.v[0][ks][dt][at])[half] = make_uint2(as_u32(h01), as_u32(h23));
+          ((uint2 *)&s.v[V8 ? 1 : 0][ks][dt][at])[half] =
+              make_uint2(as_u32(__builtin_elementwise_fma(v01, s01, -h01)), as_u32(__builtin_elementwise_fma(v23, s23, -h23)));
+        } else {
+          const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+          ((uint2 *)&s.v[0][ks][dt][at])[half] =
+              make_uint2(__builtin_amdgcn_perm(word(ld[1], e >> 1), word(ld[0], e >> 1), sel),
+                         __builtin_amdgcn_perm(word(ld[3], e >> 1), word(ld[2], e >> 1), sel));
+        }
+      }
+    }
+  };
+
+  f32x16 o[4];
+#pragma unroll
+  for (int d = 0; d < 4; d++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
+  float m = -INFINITY, l = 0.0f;
+  look(begin);
+  load(begin);
+  look(min(begin + STEP, end - 1));
+  put(stage[0]);
+  uint32_t buf = 0;
+  for (uint32_t at = begin; at < end; at += STEP, buf ^= 1) {
+    __syncthreads();  // this step is staged, and the other stage read
+    const bool more = at + STEP < end;
+    if (more) {
+      load(at + STEP);
+      look(min(at + 2 * STEP, end - 1));
+    }
+    const WideStage<K8, V8> &s = stage[buf];
+    f32x16 sc;
+#pragma unroll
+    for (int r = 0; r < 16; r++) sc[r] = 0.0f;
+    auto key = [&](uint32_t k) { return __builtin_bit_cast(f16x8, s.k[k][lane ^ (k | (h << 3))]); };
+    if constexpr (K8) {
+#pragma unroll
+      for (uint32_t b = 0; b < 4; b++) {
+        f32x16 x;
+#pragma unroll
+        for (int r = 0; r < 16; r++) x[r] = 0.0f;
+#pragma unroll
+        for (uint32_t k = 2 * b; k < 2 * b + 2; k++) {
+          const f16x8 w = key(k);
+          x = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, ql[k], x, 0, 0, 0);
+          x = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, qh[k], x, 0, 0, 0);
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) {
+          const float4 f = *(const float4 *)&s.ks[b][8 * j + 4 * h];
+          sc[4 * j] = __builtin_fmaf(f.x, x[4 * j], sc[4 * j]);
+          sc[4 * j + 1] = __builtin_fmaf(f.y, x[4 * j + 1], sc[4 * j + 1]);
+          sc[4 * j + 2] = __builtin_fmaf(f.z, x[4 * j + 2], sc[4 * j + 2]);
+          sc[4 * j + 3] = __builtin_fmaf(f.w, x[4 * j + 3], sc[4 * j + 3]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (uint32_t k = 0; k < 8; k++) {
+        const f16x8 w = key(k);
+        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, ql[k], sc, 0, 0, 0);
+        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, qh[k], sc, 0, 0, 0);
+      }
+    }
+    if (at + STEP > end) {  // the run's last positions
+#pragma unroll
+      for (uint32_t r = 0; r < 16; r++)
+        if (at + 8 * (r >> 2) + 4 * h + (r & 3) >= end) sc[r] = -INFINITY;
+    }
+    float mt = sc[0];
+#pragma unroll
+    for (int r = 1; r < 16; r++) mt = fmaxf(mt, sc[r]);
+    mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * inv;
+    if (__any(mt > m + 8.0f)) {
+      const float mn = mt > m + 8.0f ? mt : m;
+      const float down = mn > -INFINITY ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
+      m = mn;
+      l *= down;
+#pragma unroll
+      for (int d = 0; d < 4; d++) o[d] *= down;
+    }
+    const float c = 7.0f - (m > -INFINITY ? m : 0.0f);
+    f16x8 ph[2], pl[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k + e], inv, c));
+        l += x;
+        ph[k][e] = (f16)x;
+        pl[k][e] = (f16)(x - (float)ph[k][e]);
+      }
+#pragma unroll
+    for (uint32_t k = 0; k < 2; k++)
+#pragma unroll
+      for (uint32_t d = 0; d < 4; d++) {
+        const uint32_t from = lane ^ (d | ((lane >> 4 & 1) << 2));
+        const f16x8 vh = __builtin_bit_cast(f16x8, s.v[0][k][d][from]);
+        if constexpr (V8) {
+          const f16x8 vl = __builtin_bit_cast(f16x8, s.v[V8 ? 1 : 0][k][d][from]);
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[k], o[d], 0, 0, 0);
+        }
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[k], o[d], 0, 0, 0);
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[k], o[d], 0, 0, 0);
+      }
+    if (more) put(stage[buf ^ 1]);
+  }
+  l += __shfl_xor(l, 32, 64);
+  if (!live) return;
+  float *out = a + p.part_off + ((row * p.n_kv * rep + kvh * rep + head) * (p.n_shared + p.n_own) + part) * PART;
+#pragma unroll
+  for (int d = 0; d < 4; d++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const float f = ldexpf(1.0f, V8 ? ve[d] - 14 : -7);
+      float *to = out + 2 + 32 * d + 8 * j + 4 * h;
+      *(float2 *)to = make_float2(o[d][4 * j] * f, o[d][4 * j + 1] * f);
+      *(float2 *)(to + 2) = make_float2(o[d][4 * j + 2] * f, o[d][4 * j + 3] * f);
+    }
+  if (h == 0) *(float2 *)out = make_float2(m, l * 0.0078125f);
+}
+
+// Workgroups of four waves: first those of the shared run (`wide`: wide_run, the row tiles of a
+// key head's part 8 workgroups apart, so on one XCD and its L2; otherwise a wave for 16 rows of a
+// part), then a wave for each (row, part of its own run, key head).
+template <int N_REP, int K8, int V8>
+SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_t *kv8, const PagedPush &p,
+                       uint32_t n_grid, uint32_t wide) {
+  const uint32_t lane = threadIdx.x & 63, c = lane & 15;
+  const uint32_t n_rows = min(ctl[2], n_grid), slots = p.n_shared + p.n_own, groups = p.n_kv * p.n_shared;
+  const uint32_t shared = shared_positions(ctl, p.n_shared, p.n_seq, p.table_stride, p.page_log2);
+  uint32_t w = blockIdx.x;
+  if (n_rows == 0) return;
+  if (wide) {
+    const uint32_t tiles = (n_grid * N_REP + WIDE - 1) / WIDE, n = (groups + 7) / 8 * 8 * tiles;
+    if (w < n) {
+      const uint32_t g = w / (8 * tiles) * 8 + w % 8;
+      if (g < groups && shared) wide_run<K8, V8>(a, ctl, kv, kv8, p, N_REP, g % p.n_kv, w / 8 % tiles, g / p.n_kv, shared, n_rows);
+      return;
+    }
+    w -= n;
+  }
+  w = 4 * w + (threadIdx.x >> 6);
+  if (!wide) {
+    const uint32_t tiles = (n_grid * N_REP + 15) / 16, n = groups * tiles;
+    if (w < n) {
+      const uint32_t kvh = w % p.n_kv, part = w / p.n_kv % p.n_shared, i = w / groups * 16 + c;
+      const uint32_t row = min(i / N_REP, n_rows - 1), head = i % N_REP;
+      const bool live = i / N_REP < n_rows &&
+                        row_range(ctl, p.rows_off, row, shared, p.n_seq, p.table_stride, p.page_log2).member;
+      const Split sp = split_of(0, shared, p.n_shared);
+      const uint32_t first = part * sp.per, last = min(first + sp.per, sp.tiles);
+      if (!__any(live) || first >= last) return;
+      wave_run<K8, V8>(a, ctl, kv, kv8, p, kvh, a + p.q_off + row * p.q_stride + (kvh * N_REP + head) * HD,
+                       a + p.part_off + ((row * p.n_kv * N_REP + kvh * N_REP + head) * slots + part) * PART, live, ctl[4],
+                       0, shared, sp, first, last);
+      return;
+    }
+    w -= n;
+  }
+  const uint32_t kvh = w % p.n_kv, part = w / p.n_kv % p.n_own, row = w / (p.n_kv * p.n_own), head = c % N_REP;
+  if (row >= n_rows) return;
+  const Range r = row_range(ctl, p.rows_off, row, shared, p.n_seq, p.table_stride, p.page_log2);
+  const Split sp = split_of(r.start, r.len, p.n_own);
+  const uint32_t first = part * sp.per, last = min(first + sp.per, sp.tiles);
+  if (first >= last) return;
+  wave_run<K8, V8>(a, ctl, kv, kv8, p, kvh, a + p.q_off + row * p.q_stride + (kvh * N_REP + head) * HD,
+                   a + p.part_off + ((row * p.n_kv * N_REP + kvh * N_REP + head) * slots + p.n_shared + part) * PART,
+                   c < N_REP, r.seq, r.start, r.len, sp, first, last);
 }
 
 }  // namespace
@@ -432,23 +738,24 @@ APPEND(0, 1)
 APPEND(1, 1)
 
 #define PAGED(R, K8, V8)                                                                               \
-  extern "C" __global__ __launch_bounds__(64) void attention_paged__##R##_##K8##_##V8##_128(            \
-      float *a, const uint32_t *ctl, const f16 *kv, const int8_t *kv8, const f16 *kvs, PagedPush p,     \
-      uint32_t n_grid) {                                                                               \
+  extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))                  \
+  void attention_paged__##R##_##K8##_##V8##_128(float *a, const uint32_t *ctl, const f16 *kv,           \
+                                                const int8_t *kv8, const f16 *kvs, PagedPush p,         \
+                                                uint32_t n_grid, uint32_t wide) {                       \
     (void)kvs;                                                                                         \
-    paged_body<R, K8, V8>(a, ctl, kv, kv8, p, n_grid);                                                 \
+    paged_body<R, K8, V8>(a, ctl, kv, kv8, p, n_grid, wide);                                           \
   }
 #define PAGED_REP(K8, V8) PAGED(1, K8, V8) PAGED(2, K8, V8) PAGED(4, K8, V8) PAGED(8, K8, V8)
 PAGED_REP(0, 0)
 PAGED_REP(0, 1)
 PAGED_REP(1, 1)
 
-// o = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s over a row's live partials, one wave per
-// (head, row), lane t dims 2 t and 2 t + 1.
-extern "C" __global__ __launch_bounds__(256) void attention_paged_merge__128(float *a, const uint32_t *ctl,
-                                                                             PagedMergePush p) {
-  const uint32_t lane = threadIdx.x & 63, h = blockIdx.x * 4 + (threadIdx.x >> 6), row = blockIdx.y;
-  if (row >= ctl[2] || h >= p.n_head) return;
+// o = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s over a row's live partials, W waves of a
+// (head, row), lane t dims 2 t and 2 t + 1, wave w the partials w + W i, the waves' sums added in
+// order.
+template <uint32_t W>
+SK_DEV void paged_merge(float *a, const uint32_t *ctl, const PagedMergePush &p, uint32_t h, uint32_t row, uint32_t wave,
+                        uint32_t lane) {
   const uint32_t shared = shared_positions(ctl, p.n_shared, p.n_seq, p.table_stride, p.page_log2);
   const Range r = row_range(ctl, p.rows_off, row, shared, p.n_seq, p.table_stride, p.page_log2);
   const uint32_t ns = r.member ? live_parts(split_of(0, shared, p.n_shared)) : 0;
@@ -459,17 +766,51 @@ extern "C" __global__ __launch_bounds__(256) void attention_paged_merge__128(flo
   float big = -INFINITY;
   for (uint32_t i = lane; i < n; i += 64) big = fmaxf(big, at(i)[0]);
   big = wave_max(big);
+  big = big > -INFINITY ? big : 0.0f;
   float l = 0.0f, ox = 0.0f, oy = 0.0f;
-  for (uint32_t i = 0; i < n; i++) {
-    const float *s = at(i);
-    const float w = __builtin_amdgcn_exp2f(s[0] - big);
-    const float2 v = *(const float2 *)(s + 2 + 2 * lane);
-    l = __builtin_fmaf(w, s[1], l);
-    ox = __builtin_fmaf(w, v.x, ox);
-    oy = __builtin_fmaf(w, v.y, oy);
+  constexpr uint32_t U = 8;  // partials in flight
+  for (uint32_t i0 = wave; i0 < n; i0 += U * W) {
+    float2 ml[U], v[U];
+#pragma unroll
+    for (uint32_t k = 0; k < U; k++) {
+      const float *s = at(min(i0 + k * W, n - 1));
+      ml[k] = *(const float2 *)s;
+      v[k] = *(const float2 *)(s + 2 + 2 * lane);
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < U; k++) {
+      const float w = i0 + k * W < n ? __builtin_amdgcn_exp2f(ml[k].x - big) : 0.0f;
+      l = __builtin_fmaf(w, ml[k].y, l);
+      ox = __builtin_fmaf(w, v[k].x, ox);
+      oy = __builtin_fmaf(w, v[k].y, oy);
+    }
+  }
+  if constexpr (W > 1) {
+    __shared__ float3 sum[W][64];
+    sum[wave][lane] = make_float3(l, ox, oy);
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (uint32_t w = 1; w < W; w++) {
+      l += sum[w][lane].x;
+      ox += sum[w][lane].y;
+      oy += sum[w][lane].z;
+    }
   }
   *(float2 *)(a + p.o_off + row * p.o_stride + h * HD + 2 * lane) =
       n ? make_float2(ox / l, oy / l) : make_float2(0.0f, 0.0f);
+}
+// a wave a head, four heads a workgroup
+extern "C" __global__ __launch_bounds__(256) void attention_paged_merge__128(float *a, const uint32_t *ctl,
+                                                                             PagedMergePush p) {
+  const uint32_t h = blockIdx.x * 4 + (threadIdx.x >> 6), row = blockIdx.y;
+  if (row < ctl[2] && h < p.n_head) paged_merge<1>(a, ctl, p, h, row, 0, threadIdx.x & 63);
+}
+// eight waves a head
+extern "C" __global__ __launch_bounds__(512) void attention_paged_merge_8__128(float *a, const uint32_t *ctl,
+                                                                               PagedMergePush p) {
+  const uint32_t h = blockIdx.x, row = blockIdx.y;
+  if (row < ctl[2]) paged_merge<8>(a, ctl, p, h, row, threadIdx.x >> 6, threadIdx.x & 63);
 }
 
 // logits_adjust: y = adjust(x) for every token of a row's vocabulary.  Row r has eight words at
@@ -482,13 +823,14 @@ extern "C" __global__ __launch_bounds__(256) void attention_paged_merge__128(flo
 //   not allowed      -inf
 // Ids past the vocabulary count for nothing.  Lengths are cut to the strides.
 //
-// A workgroup takes VT tokens of a row: it counts the history's tokens among them in LDS (integer
-// counts, so any order gives the same), then passes over the logits once.
-constexpr uint32_t VT = 4096;
-extern "C" __global__ __launch_bounds__(256) void logits_adjust(float *a, const uint32_t *ctl, LogitsPush p) {
+// A workgroup of T threads takes 16 T tokens of a row: it loads its logits, counts the history's
+// tokens among them in LDS meanwhile (integer counts, so any order gives the same), and writes the
+// row's part once.  Its biases come last, each by the thread whose entry is the last of its id.
+template <uint32_t T>
+SK_DEV void logits_body(float *a, const uint32_t *ctl, const LogitsPush &p) {
 #pragma clang fp contract(off)
+  constexpr uint32_t VT = 16 * T;
   __shared__ uint32_t count[VT];  // uses past the prompt; bit 31: in the prompt
-  __shared__ uint32_t entry[VT];  // 1 + the place of the token's last bias
   const uint32_t row = blockIdx.y, t = threadIdx.x, base = blockIdx.x * VT, n = min(VT, p.n_vocab - base);
   if (row >= ctl[2]) return;
   const uint32_t *c = ctl + p.ctrl_off + 8 * row;
@@ -497,35 +839,95 @@ extern "C" __global__ __launch_bounds__(256) void logits_adjust(float *a, const 
   const uint32_t n_hist = rho != 1.0f || freq != 0.0f || pres != 0.0f ? min(c[0], p.hist_stride) : 0;
   const uint32_t n_prompt = c[1], n_bias = min(c[2], p.bias_stride / 2);
   const uint32_t *hist = ctl + p.hist_off + row * p.hist_stride, *bias = ctl + p.bias_off + row * p.bias_stride;
+  const uint32_t *mask = ctl + p.mask_off + row * p.mask_stride;
   const bool masked = c[3] != 0 && p.mask_stride != 0;
-  for (uint32_t i = t; i < VT; i += 256) {
-    count[i] = 0;
-    entry[i] = 0;
-  }
-  __syncthreads();
-  for (uint32_t i = t; i < n_hist; i += 256) {
-    const uint32_t id = hist[i] - base;
-    if (id < n) {
-      if (i < n_prompt)
-        atomicOr(&count[id], 0x80000000u);
-      else
-        atomicAdd(&count[id], 1u);
-    }
-  }
-  for (uint32_t i = t; i < n_bias; i += 256) {
-    const uint32_t id = bias[2 * i] - base;
-    if (id < n) atomicMax(&entry[id], i + 1);
-  }
-  __syncthreads();
   const float *x = a + p.x_off + row * p.x_stride + base;
   float *y = a + p.y_off + row * p.y_stride + base;
-  for (uint32_t i = t; i < n; i += 256) {
-    float v = x[i];
-    const uint32_t k = count[i], made = k & 0x7fffffffu;
-    if (k) v = v > 0.0f ? v / rho : v * rho;
-    if (made) v -= freq * (float)made + pres;
-    if (entry[i]) v += __builtin_bit_cast(float, bias[2 * (entry[i] - 1) + 1]);
-    if (masked && !((ctl[p.mask_off + row * p.mask_stride + (base + i) / 32] >> ((base + i) & 31)) & 1)) v = -INFINITY;
-    y[i] = v;
+  // tokens 4 (t + T k) + [0, 4): offset and stride are multiples of 4, so a last float4 that
+  // passes n stays in its row's stride or is read one by one
+  float4 v[4];
+  uint32_t bits[4];
+#pragma unroll
+  for (uint32_t k = 0; k < 4; k++) {
+    const uint32_t i = 4 * (t + T * k);
+    v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    bits[k] = 15;
+    if (i + 4 <= n) {
+      v[k] = *(const float4 *)(x + i);
+    } else if (i < n) {
+      v[k].x = x[i];
+      if (i + 1 < n) v[k].y = x[i + 1];
+      if (i + 2 < n) v[k].z = x[i + 2];
+    }
+    if (masked && i < n) bits[k] = (mask[(base + i) / 32] >> ((base + i) & 31)) & 15;
+  }
+  if (n_hist) {
+#pragma unroll
+    for (uint32_t k = 0; k < 4; k++) *(uint4 *)&count[4 * (t + T * k)] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    auto use = [&](uint32_t i, uint32_t id) {
+      id -= base;
+      if (id < n) {
+        if (i < n_prompt)
+          atomicOr(&count[id], 0x80000000u);
+        else
+          atomicAdd(&count[id], 1u);
+      }
+    };
+    const uint32_t whole = n_hist & ~3u;
+    for (uint32_t i = 4 * t; i < whole; i += 4 * T) {
+      const uint4 h = *(const uint4 *)(hist + i);
+      use(i, h.x);
+      use(i + 1, h.y);
+      use(i + 2, h.z);
+      use(i + 3, h.w);
+    }
+    if (whole + t < n_hist) use(whole + t, hist[whole + t]);
+    __syncthreads();
+  }
+#pragma unroll
+  for (uint32_t k = 0; k < 4; k++) {
+    const uint32_t i = 4 * (t + T * k);
+    const uint4 u = n_hist ? *(const uint4 *)&count[i] : make_uint4(0, 0, 0, 0);
+    float w[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+    const uint32_t uses[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const uint32_t made = uses[j] & 0x7fffffffu;
+      if (uses[j]) w[j] = w[j] > 0.0f ? w[j] / rho : w[j] * rho;
+      if (made) w[j] -= freq * (float)made + pres;
+      if (!((bits[k] >> j) & 1)) w[j] = -INFINITY;
+    }
+    if (i + 4 <= n) {
+      *(float4 *)(y + i) = make_float4(w[0], w[1], w[2], w[3]);
+    } else if (i < n) {
+      y[i] = w[0];
+      if (i + 1 < n) y[i + 1] = w[1];
+      if (i + 2 < n) y[i + 2] = w[2];
+    }
+  }
+  if (n_bias == 0) return;
+  // the counts are read: their words now hold 1 + the place of a token's last bias
+  __syncthreads();
+  for (uint32_t i = t; i < n_bias; i += T) {
+    const uint32_t id = bias[2 * i] - base;
+    if (id < n) count[id] = 0;
+  }
+  __syncthreads();
+  for (uint32_t i = t; i < n_bias; i += T) {
+    const uint32_t id = bias[2 * i] - base;
+    if (id < n) atomicMax(&count[id], i + 1);
+  }
+  __syncthreads();  // and this workgroup's y is written
+  for (uint32_t i = t; i < n_bias; i += T) {
+    const uint32_t at = bias[2 * i], id = at - base;
+    if (id < n && count[id] == i + 1 && (!masked || ((mask[at / 32] >> (at & 31)) & 1)))
+      y[id] += __builtin_bit_cast(float, bias[2 * i + 1]);
   }
 }
+#define LOGITS(T)                                                                                        \
+  extern "C" __global__ __launch_bounds__(T) void logits_adjust_##T(float *a, const uint32_t *ctl, LogitsPush p) { \
+    logits_body<T>(a, ctl, p);                                                                           \
+  }
+LOGITS(256)
+LOGITS(1024)

@@ -2,6 +2,7 @@
 // the buffers they are bound to, and the launch a dispatch of theirs becomes.  Plain C++, no HIP.
 #pragma once
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -24,8 +25,10 @@ inline Op op_of(const char *name) {
 constexpr uint32_t kHead = 128, kPart = kHead + 2;
 constexpr uint32_t kMaxSlots = 1024;      // partials of a row and head
 constexpr uint32_t kMaxGrid = 65535;      // rows of a dispatch
-constexpr uint32_t kMaxWork = 1u << 22;   // workgroups of an attention launch for each key head
-constexpr uint32_t kLogitsTile = 4096;    // tokens of a logits workgroup (batch.hip VT)
+constexpr uint32_t kMergeParts = 16;      // partials above which eight waves merge a head
+constexpr uint32_t kLogitsWide = 512;     // workgroups of 4096 tokens from which a logits launch takes 16384 each
+constexpr uint32_t kNarrow = 32;          // query rows of a key head up to which the shared run takes waves of 16
+constexpr uint32_t kMaxWork = 1u << 24;   // waves of an attention launch
 
 // [off, off + stride (rows - 1) + width) in elements
 struct Region {
@@ -142,7 +145,7 @@ inline std::string refusal(Op op, const uint32_t *spec, const uint32_t *w, const
     for (const Region *r : {&q, &o, &words, &table}) c.apart(part, *r);
     c.apart(o, words);
     c.apart(o, table);
-    if ((rows * spec[0] + 15) / 16 * w[11] + rows * w[12] > kMaxWork)
+    if (n_kv * ((rows * spec[0] + 15) / 16 * w[11] + rows * w[12]) > kMaxWork)
       c.fail("%llu rows in %llu parts: too many workgroups", (unsigned long long)rows, (unsigned long long)parts);
   } else if (op == kMerge) {
     const uint64_t a = bytes[0] / 4, n_head = w[3], parts = (uint64_t)w[4] + w[5];
@@ -176,24 +179,41 @@ inline std::string refusal(Op op, const uint32_t *spec, const uint32_t *w, const
   return c.error;
 }
 
-// The launch of a dispatch: its grid and trailing by-value words.
-inline void shape(Op op, const uint32_t *spec, const uint32_t *w, uint32_t rows, uint32_t groups[3],
-                  std::vector<uint32_t> &extra) {
-  groups[2] = 1;
+// The launch of a dispatch: its grid, threads, form (0: the pipeline's own kernel, 1: the other
+// one, other_form) and trailing by-value words.
+struct Shape {
+  uint32_t groups[3] = {1, 1, 1}, threads = 256, form = 0;
+  std::vector<uint32_t> extra;
+};
+inline std::string other_form(Op op, const std::string &symbol) {
+  if (op == kLogits) return "logits_adjust_1024";
+  if (op == kMerge) return "attention_paged_merge_8__128";
+  return symbol;
+}
+inline Shape shape(Op op, const uint32_t *spec, const uint32_t *w, uint32_t rows) {
+  Shape s;
+  s.groups[1] = rows;
   if (op == kAppend) {
-    groups[0] = (w[9] + 2 * w[10] + 3) / 4;  // one wave a head
-    groups[1] = rows;
+    s.groups[0] = (w[9] + 2 * w[10] + 3) / 4;  // one wave a head
   } else if (op == kAttend) {
-    groups[0] = (rows * spec[0] + 15) / 16 * w[11] + rows * w[12];
-    groups[1] = w[9];
-    extra = {rows};
+    const uint32_t q = rows * spec[0], groups = w[9] * w[11], own = rows * w[9] * w[12];
+    const bool wide = w[11] && q > kNarrow;
+    if (wide)
+      s.groups[0] = (groups + 7) / 8 * 8 * ((q + 127) / 128) + (own + 3) / 4;
+    else
+      s.groups[0] = (groups * ((q + 15) / 16) + own + 3) / 4;
+    s.groups[1] = 1;
+    s.extra = {rows, wide};
   } else if (op == kMerge) {
-    groups[0] = (w[3] + 3) / 4;
-    groups[1] = rows;
+    s.form = w[4] + w[5] > kMergeParts;
+    s.groups[0] = s.form ? w[3] : (w[3] + 3) / 4;
+    s.threads = s.form ? 512 : 256;
   } else {
-    groups[0] = (w[4] + kLogitsTile - 1) / kLogitsTile;
-    groups[1] = rows;
+    s.form = (uint64_t)rows * ((w[4] + 4095) / 4096) >= kLogitsWide;
+    s.threads = s.form ? 1024 : 256;
+    s.groups[0] = (w[4] + 16 * s.threads - 1) / (16 * s.threads);
   }
+  return s;
 }
 
 }  // namespace batch

@@ -196,7 +196,7 @@ const KernelInfo kKernels[] = {
     {"embed", 4, 8, 1, 1, -1, false, false},  // token rows from the HBM token_embd (util.hip)
     // a served batch (kernels/batch.hip): grids of [1, rows, 1]
     {"kv_append", 5, 24, 3, 3, -1, false, false},
-    {"attention_paged", 5, 19, 4, 4, -1, false, false, 64},
+    {"attention_paged", 5, 19, 4, 4, -1, false, false},
     {"attention_paged_merge", 2, 10, 1, 1, -1, false, false},
     {"logits_adjust", 2, 12, 0, 0, -1, false, false},
 };
@@ -321,6 +321,7 @@ struct skyla_hip_pipeline {
   hipFunction_t moe_fn4 = nullptr;       // and the gate/up pair that routes for itself
   batch::Op batch = batch::kNone;        // a batch operator, its spec words
   std::vector<uint32_t> spec;
+  hipFunction_t batch_fn = nullptr;      // and its other form (batch::shape)
   std::vector<std::vector<void *>> sets;
   std::vector<std::vector<uint64_t>> set_bytes;  // sizes of the bound buffers
 };
@@ -345,6 +346,7 @@ struct Command {
   hipFunction_t moe_fn = nullptr, moe_fn3 = nullptr, moe_fn4 = nullptr;
   batch::Op batch = batch::kNone;
   std::vector<uint32_t> spec;       // of a batch operator
+  hipFunction_t batch_fn = nullptr;  // and its other form
   uint32_t groups[3] = {0, 0, 0};
   std::vector<void *> bufs;
   std::vector<uint32_t> push;
@@ -429,7 +431,11 @@ Launch pack(const Command *const *run, uint32_t n) {
     for (int i = 0; i < 3; i++) l.groups[i] = a.groups[i];
     l.args = a.push;
     if (a.batch) {
-      batch::shape(a.batch, a.spec.data(), a.push.data(), a.groups[1], l.groups, l.extra);
+      const batch::Shape s = batch::shape(a.batch, a.spec.data(), a.push.data(), a.groups[1]);
+      std::copy(s.groups, s.groups + 3, l.groups);
+      l.threads = s.threads;
+      l.extra = s.extra;
+      if (s.form) l.fn = a.batch_fn;
       return l;
     }
     if (a.tok_fn && a.tok_per_wg_z) {
@@ -1198,6 +1204,7 @@ Command dispatch_command(const skyla_hip_pipeline *p, const std::vector<void *> 
   c.moe_fn4 = p->moe_fn4;
   c.batch = p->batch;
   c.spec = p->spec;
+  c.batch_fn = p->batch_fn;
   for (int i = 0; i < 3; i++) c.groups[i] = groups[i];
   c.bufs = bufs;
   c.push.assign(push, push + n_push);
@@ -1215,12 +1222,13 @@ int check_batch(const skyla_hip_pipeline *p, uint32_t set, const uint32_t *group
 }
 
 hipFunction_t find_function(skyla_hip_context *ctx, const std::string &sym) {
+  hipFunction_t fn = nullptr;
   for (hipModule_t m : ctx->modules) {
-    hipFunction_t fn = nullptr;
-    if (hipModuleGetFunction(&fn, m, sym.c_str()) == hipSuccess && fn) return fn;
+    if (hipModuleGetFunction(&fn, m, sym.c_str()) == hipSuccess && fn) break;
+    fn = nullptr;
   }
   (void)hipGetLastError();  // lookups that missed leave a sticky error behind
-  return nullptr;
+  return fn;
 }
 
 // Variant choice for matvec launches, from sweeps on MI355X.  Dense rows (Qwen3-8B decode
@@ -1692,6 +1700,7 @@ int skyla_hip_pipeline_new(skyla_hip_context *ctx, const char *name, uint32_t n_
   if (std::strcmp(name, "matmul") == 0 && n_spec == 4 && spec[3] == 0) n_key = 3;
   std::string sym = name;
   for (uint32_t i = 0; i < n_key; i++) sym += (i ? "_" : "__") + std::to_string(spec[i]);
+  if (std::strcmp(name, "logits_adjust") == 0) sym += "_256";  // its workgroup; a launch may take the other
   uint32_t threads = k->threads;
   if (k->threads_from_spec >= 0)
     threads = k->waves ? 64 * spec[k->threads_from_spec] : spec[k->threads_from_spec];
@@ -1719,6 +1728,10 @@ int skyla_hip_pipeline_new(skyla_hip_context *ctx, const char *name, uint32_t n_
   (void)hipGetLastError();  // lookups that missed leave a sticky error behind
   if (!p->fn)
     return fail(SKYLA_HIP_E_NO_KERNEL, "no gfx950 kernel %s for this spec", sym.c_str());
+  if (p->batch) {
+    p->batch_fn = find_function(ctx, batch::other_form(p->batch, sym));
+    if (!p->batch_fn) return fail(SKYLA_HIP_E_NO_KERNEL, "no gfx950 kernel %s", batch::other_form(p->batch, sym).c_str());
+  }
   p->retile = make_retile(ctx, name, spec, n_spec);
   p->name = name;
   // MoE decode forms (fuse_moe): Q4_K expert matvecs whose launches the variant rule puts

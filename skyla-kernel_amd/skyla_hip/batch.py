@@ -24,6 +24,7 @@ import numpy as np
 from . import engine as E
 from .abi import Buffer, Context, Recorder
 
+NARROW = 32             # query rows of a key head up to which the shared run takes waves of 16 (runtime/batch.h)
 MAX_PARTS = 1024        # partials of a row and head (runtime/batch.h)
 PAGE_SIZES = tuple(16 << i for i in range(9))  # 16 to 4096 positions
 CTL_ROWS, CTL_SHARED, CTL_LEADER = 2, 3, 4     # control words: live rows, shared positions, their sequence
@@ -76,11 +77,17 @@ def splits(rows: int, n_kv: int, rep: int, shared: int, own: int) -> tuple[int, 
     """Parts that a batch's attention cuts the shared run and each row's own run into, for
     `shared` shared positions and at most `own` of a row's own: enough workgroups to fill the
     GPU, each with some tiles of 64 positions."""
-    def parts(positions: int, groups: int, most: int) -> int:
+    def parts(positions: int, groups: int, want: int, most: int) -> int:
         tiles = -(-positions // 64)
-        return max(1, min(tiles, -(-2048 // max(1, groups)), most))
-    n_shared = parts(shared, n_kv * -(-rows * rep // 16), 128) if shared > 0 else 0
-    return n_shared, parts(own, n_kv * rows, 512)
+        return max(1, min(tiles, -(-want // groups), most))
+    q = rows * rep
+    if shared == 0:
+        n_shared = 0
+    elif q > NARROW:  # workgroups of 128 query rows: two a compute unit
+        n_shared = parts(shared, n_kv * -(-q // 128), 512, 128)
+    else:             # waves of 16
+        n_shared = parts(shared, n_kv * -(-q // 16), 2048, 128)
+    return n_shared, parts(own, n_kv * rows, 2048, 64)
 
 
 def part_size(rows: int, n_head: int, parts: tuple[int, int]) -> int:

@@ -22,9 +22,9 @@ extern "C" int refuse(const char *name, const uint32_t *spec, const uint32_t *w,
   return !s.empty();
 }
 extern "C" int shape(const char *name, const uint32_t *spec, const uint32_t *w, uint32_t rows, uint32_t *groups) {
-  std::vector<uint32_t> extra;
-  batch::shape(batch::op_of(name), spec, w, rows, groups, extra);
-  return (int)extra.size();
+  const batch::Shape s = batch::shape(batch::op_of(name), spec, w, rows);
+  std::copy(s.groups, s.groups + 3, groups);
+  return (int)s.threads;
 }
 """
 
@@ -129,8 +129,9 @@ def test_unknown_names_and_launches(host):
     for rows in (1, 7, 128, 2048):
         host.shape(b"kv_append", u32([0, 1, 128]), u32(_append()), rows, g)
         assert g[0] * g[1] >= 1 and g[2] == 1
-        host.shape(b"logits_adjust", u32([0]), u32(_logits()), rows, g)
-        assert g[1] == rows and g[2] == 1
+        for v in (1, 1000, 4097, 151936):
+            t = host.shape(b"logits_adjust", u32([0]), u32(_logits(v=v)), rows, g)
+            assert g[1] == rows and g[2] == 1 and g[0] == -(-v // (16 * t))
 
 
 def test_pages_and_parts():
