@@ -20,7 +20,7 @@
 // Words that name no page or sequence reach no memory outside the pool: a row of such a sequence
 // counts as one of len 0, a length past the table's ends there, keys and values of such a page
 // are not stored, and a read of it goes to the pool's last page.
-#include "common.h"
+#include "matmul_common.h"
 
 namespace {
 
@@ -391,33 +391,48 @@ SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
 }
 
 // The shared run for WIDE = 128 query rows a workgroup, 32 a wave: what 16 rows a wave read from
-// L2 again and again passes through LDS once for all four waves.  A step takes STEP = 32
-// positions: waves 0 and 1 stage the next step's values (transposed on the way, 4 positions by 8
-// dims a thread), 2 and 3 its keys, in the order the matrix instructions read them:
+// L2 again and again passes through LDS once for all four waves, STEP = 32 positions at a time:
 //   S^T = K Q^T   v_mfma_f32_32x32x16_f16, A = keys (row: position lane % 32, dims 16 k + 8 h +
 //                 [0, 8), h = lane / 32), B = the query rows' two f16 parts, held in registers
 //   O^T = V^T P^T B = this lane's own e: element e of k-step s is position 16 s + 8 (e / 4) + 4 h +
 //                 e % 4, as S^T leaves them; A = values of those positions, row: dim 32 d + lane % 32
-// An LDS fragment is 64 pieces of 16 bytes, lane l's at place l ^ (a constant of the fragment, and
-// for values l / 16 % 2), so that a row of the cache, whose pieces go to 16 fragments, is written
-// to 16 banks' groups.
+// The cache's rows are loaded straight into LDS, into rings of DEPTH steps, each wave loading
+// positions 8 w to 8 w + 7 of a step with four loads (so a wait for all but 4 (DEPTH - 2) loads
+// leaves that many steps in flight).  f16 rows: 16 pieces of 16 bytes at places piece ^ (position %
+// 16) for keys, so that 16 rows' like pieces lie in 16 bank groups, and piece ^ 4 (position % 4)
+// for values, which are read transposed (ds_read_b64_tr_b16: of 16 lanes, lanes 4 j to 4 j + 3 read
+// 16 dims of position j, and lane i receives dim i of the four).  8-bit rows are converted to f16
+// in LDS a step before they are read: keys as they are, values into fragments of 64 pieces, lane
+// l's at place l ^ (d | (l / 16 % 2) 4), so that a row's dims go to 16 bank groups.
+// With f16 keys a step multiplies the next step's scores while it makes this one's e, so that the
+// matrix pipe and the vector ALU work side by side in one wave; reads from LDS run two products
+// ahead.  (8-bit keys' block sums leave no registers for a second step's scores.)
 // The largest score is followed loosely: sums are scaled down only where a score passes the
 // reference by 2^8 (e is held times 2^7, so that it stays in f16's range), which after the first
 // steps is rare.  8-bit values are held as two f16 parts of q s 2^(7 - ve), ve the exponent of the
 // part's largest scale of the 32 dims, found first.
 constexpr uint32_t WIDE = 128, STEP = 32;
+template <int Q8>
+struct RawRows {
+  uint4 x[STEP][Q8 ? 8 : 16];
+  uint2 s[Q8 ? STEP : 1];  // the four blocks' scales
+};
 template <int K8, int V8>
-struct WideStage {  // one step's keys and values
-  uint4 k[8][64];                 // [k-step]
-  uint4 v[V8 ? 2 : 1][2][4][64];  // [part][k-step][dims / 32]
-  float ks[K8 ? 4 : 1][K8 ? STEP : 1];  // 8-bit keys: [dims / 32][position]
+struct WideStage {  // at most half of the 160 KB: two workgroups a compute unit
+  static constexpr int DEPTH = V8 ? 3 : 4;
+  RawRows<K8> k[DEPTH];
+  RawRows<V8> v[DEPTH];
+  uint4 kh[K8 ? 2 : 1][K8 ? STEP : 1][16];        // converted keys,
+  float ks[K8 ? 2 : 1][4][K8 ? STEP : 4];         // their scales: [step][dims / 32][position]
+  uint4 vh[V8 ? 2 : 1][V8 ? 2 : 1][2][4][V8 ? 64 : 1];  // and values: [step][part][k-step][dims / 32]
 };
 template <int K8, int V8>
 SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t *kv8, const PagedPush &p, uint32_t rep,
                      uint32_t kvh, uint32_t tile, uint32_t part, uint32_t shared, uint32_t n_rows) {
-  __shared__ WideStage<K8, V8> stage[2];
+  __shared__ __attribute__((aligned(1024))) WideStage<K8, V8> st;
   __shared__ float tops[V8 ? 4 : 1][4];
-  const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63, col = lane & 31, h = lane >> 5;
+  const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, col = lane & 31,
+                 h = lane >> 5;
   const uint32_t kv_dim = p.n_kv * HD;
   const Split sp = split_of(0, shared, p.n_shared);
   const uint32_t begin = part * sp.per * TILE, end = min(begin + sp.per * TILE, shared);
@@ -485,126 +500,124 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
     }
   }
 
-  // staging: dims 8 dg + [0, 8) of positions 4 pg + [0, 4)
-  const uint32_t dg = t & 15, pg = (t >> 4) & 7;
-  const bool keys = t >= 128;
-  uint4 ld[4];
-  f16 ls[4];
-  uint32_t next;  // the pool row of this thread's first position, a step ahead of the loads
-  auto look = [&](uint32_t at) { next = slot_of(min(at + 4 * pg, end - 1)); };
-  auto load = [&](uint32_t at) {
-    const uint32_t first = min(at + 4 * pg, end - 1), room = end - 1 - first;
+  // Staging.  Positions past the end are read as the last one.  The page table is read through
+  // the scalar cache: a vector load's wait would be one for the rows in flight, too.
+  constexpr int DEPTH = WideStage<K8, V8>::DEPTH;
+  typedef const __attribute__((address_space(4))) uint32_t ConstWord;
+  ConstWord *pages = (ConstWord *)(uintptr_t)table;
+  const uint32_t n_at = 8 * wave;  // the wave's first position of a step
+  struct Rows {
+    uint32_t first, room;  // that position's pool row, and how many live positions follow it
+  };
+  auto look = [&](uint32_t step) {
+    const uint32_t pos = min(begin + step * STEP + n_at, end - 1);
+    const uint32_t page = min(pages[pos >> p.page_log2], p.n_pages - 1);
+    return Rows{(page << p.page_log2) + (pos & ((1u << p.page_log2) - 1)), end - 1 - pos};
+  };
+  const uint64_t pool = (uint64_t)(p.n_pages << p.page_log2) * kv_dim;
+  const u32x4 kres = K8 ? dl_res(kv8 + p.kc_off, pool) : dl_res(kv + p.kc_off, 2 * pool);
+  const u32x4 vres = V8 ? dl_res(kv8 + p.vc_off, pool) : dl_res(kv + p.vc_off, 2 * pool);
+  const u32x4 ksres = dl_res(kv + p.ks_off, pool / 16), vsres = dl_res(kv + p.vs_off, pool / 16);
+  // two loads: the wave's rows in 16 bits, or in 8 and their scales
+  auto load_f16 = [&](RawRows<0> &to, const u32x4 &res, const Rows &at, bool is_v) {
 #pragma unroll
-    for (uint32_t j = 0; j < 4; j++) {
-      const uint32_t r = next + min(j, room);
-      if (keys) {
-        const uint32_t src = p.kc_off + r * kv_dim + kvh * HD + 8 * dg;
-        if constexpr (K8) {
-          const uint2 x = *(const uint2 *)(kv8 + src);
-          ld[j] = make_uint4(x.x, x.y, 0u, 0u);
-          ls[j] = kv[p.ks_off + r * (kv_dim / 32) + kvh * 4 + (dg >> 2)];
-        } else {
-          ld[j] = *(const uint4 *)(kv + src);
-        }
-      } else {
-        const uint32_t src = p.vc_off + r * kv_dim + kvh * HD + 8 * dg;
-        if constexpr (V8) {
-          const uint2 x = *(const uint2 *)(kv8 + src);
-          ld[j] = make_uint4(x.x, x.y, 0u, 0u);
-          ls[j] = kv[p.vs_off + r * (kv_dim / 32) + kvh * 4 + (dg >> 2)];
-        } else {
-          ld[j] = *(const uint4 *)(kv + src);
-        }
-      }
+    for (uint32_t j = 0; j < 2; j++) {
+      const uint32_t n = 4 * j + (lane >> 4), piece = (lane & 15) ^ (is_v ? (n & 3) << 2 : (n_at + n) & 15);
+      dl_load16(res, lds_addr(&to.x[n_at + 4 * j][0]), (min(n, at.room) * kv_dim + 8 * piece) * 2,
+                (at.first * kv_dim + kvh * HD) * 2);
     }
   };
+  auto load_q8 = [&](RawRows<1> &to, const u32x4 &res, const u32x4 &sres, const Rows &at) {
+    dl_load16(res, lds_addr(&to.x[n_at][0]), min(lane >> 3, at.room) * kv_dim + 16 * (lane & 7),
+              at.first * kv_dim + kvh * HD);
+    const uint32_t base = __builtin_amdgcn_readfirstlane(at.first * (kv_dim / 16) + kvh * 8);
+    if (lane < 16)
+      dl_load4(sres, lds_addr(&to.s[n_at]), min(lane >> 1, at.room) * (kv_dim / 16) + 4 * (lane & 1), base);
+  };
+  auto load_keys = [&](uint32_t step, const Rows &at) {
+    if constexpr (K8)
+      load_q8(st.k[step % DEPTH], kres, ksres, at);
+    else
+      load_f16(st.k[step % DEPTH], kres, at, false);
+  };
+  auto load_values = [&](uint32_t step, const Rows &at) {
+    if constexpr (V8)
+      load_q8(st.v[step % DEPTH], vres, vsres, at);
+    else
+      load_f16(st.v[step % DEPTH], vres, at, true);
+  };
+
+  // 8-bit rows to f16: dims 8 dg + [0, 8) of positions 2 pr and 2 pr + 1
+  const uint32_t dg = t & 15, pr = t >> 4;
   auto widen = [](uint32_t x1, uint32_t x0, uint32_t sel) {
     const f16x2 off = {(f16)1152.0f, (f16)1152.0f};
     return as_f16x2((__builtin_amdgcn_perm(x1, x0, sel) ^ 0x00800080u) | 0x64006400u) - off;
   };
-  auto word = [](const uint4 &u, int n) { return n == 0 ? u.x : n == 1 ? u.y : n == 2 ? u.z : u.w; };
   int vmine = ve[0];
   if constexpr (V8) vmine = dg >> 2 == 0 ? ve[0] : dg >> 2 == 1 ? ve[1] : dg >> 2 == 2 ? ve[2] : ve[3];
-  auto put = [&](WideStage<K8, V8> &s) {
-    if (keys) {
-      const uint32_t ks = dg >> 1, hh = dg & 1, sw = ks | (hh << 3);
+  constexpr bool AHEAD = !K8;
+  auto convert_keys = [&](uint32_t step) {
+    if constexpr (K8) {
 #pragma unroll
-      for (uint32_t j = 0; j < 4; j++) {
-        uint4 x = ld[j];
-        if constexpr (K8) {
-          x = make_uint4(as_u32(widen(ld[j].x, ld[j].x, 0x0c010c00u)), as_u32(widen(ld[j].x, ld[j].x, 0x0c030c02u)),
-                         as_u32(widen(ld[j].y, ld[j].y, 0x0c010c00u)), as_u32(widen(ld[j].y, ld[j].y, 0x0c030c02u)));
-          if ((dg & 3) == 0) s.ks[dg >> 2][4 * pg + j] = (float)ls[j];
-        }
-        s.k[ks][(hh * 32 + 4 * pg + j) ^ sw] = x;
+      for (uint32_t j = 0; j < 2; j++) {
+        const uint32_t pos = 2 * pr + j;
+        const uint2 x = ((const uint2 *)st.k[step % DEPTH].x[pos])[dg];
+        st.kh[step & 1][pos][dg ^ (pos & 15)] =
+            make_uint4(as_u32(widen(x.x, x.x, 0x0c010c00u)), as_u32(widen(x.x, x.x, 0x0c030c02u)),
+                       as_u32(widen(x.y, x.y, 0x0c010c00u)), as_u32(widen(x.y, x.y, 0x0c030c02u)));
       }
-    } else {
-      const uint32_t dt = dg >> 2, ks = pg >> 2, hh = pg & 1, half = (pg >> 1) & 1;
+      if (t < 4 * STEP) st.ks[step & 1][t & 3][t >> 2] = (float)((const f16 *)st.k[step % DEPTH].s)[t];
+    }
+  };
+  auto convert_values = [&](uint32_t step) {
+    if constexpr (V8) {
+      const RawRows<1> &from = st.v[step % DEPTH];
+      const uint32_t dt = dg >> 2, hh = pr >> 1 & 1, w = 2 * (pr >> 2 & 1) + (pr & 1);
       const uint32_t sw = dt | ((dg >> 1 & 1) << 2);
-      f16x2 s01, s23;
-      if constexpr (V8) {
-        s01 = f16x2{(f16)ldexpf((float)ls[0], 7 - vmine), (f16)ldexpf((float)ls[1], 7 - vmine)};
-        s23 = f16x2{(f16)ldexpf((float)ls[2], 7 - vmine), (f16)ldexpf((float)ls[3], 7 - vmine)};
-      }
+      const uint2 x0 = ((const uint2 *)from.x[2 * pr])[dg], x1 = ((const uint2 *)from.x[2 * pr + 1])[dg];
+      const f16 s0 = ((const f16 *)&from.s[2 * pr])[dt], s1 = ((const f16 *)&from.s[2 * pr + 1])[dt];
+      const f16x2 sv = {(f16)ldexpf((float)s0, 7 - vmine), (f16)ldexpf((float)s1, 7 - vmine)};
 #pragma unroll
       for (uint32_t e = 0; e < 8; e++) {
         const uint32_t at = (hh * 32 + 8 * (dg & 3) + e) ^ sw;
-        if constexpr (V8) {
-          const uint32_t sel = 0x0c040c00u + (e & 3) * 0x00010001u;
-          const f16x2 v01 = widen(word(ld[1], e >> 2), word(ld[0], e >> 2), sel);
-          const f16x2 v23 = widen(word(ld[3], e >> 2), word(ld[2], e >> 2), sel);
-          const f16x2 h01 = v01 * s01, h23 = v23 * s23;
-          ((uint2 *)&s.v[0][ks][dt][at])[half] = make_uint2(as_u32(h01), as_u32(h23));
-          ((uint2 *)&s.v[V8 ? 1 : 0][ks][dt][at])[half] =
-              make_uint2(as_u32(__builtin_elementwise_fma(v01, s01, -h01)), as_u32(__builtin_elementwise_fma(v23, s23, -h23)));
-        } else {
-          const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
-          ((uint2 *)&s.v[0][ks][dt][at])[half] =
-              make_uint2(__builtin_amdgcn_perm(word(ld[1], e >> 1), word(ld[0], e >> 1), sel),
-                         __builtin_amdgcn_perm(word(ld[3], e >> 1), word(ld[2], e >> 1), sel));
-        }
+        const f16x2 v = widen(e < 4 ? x1.x : x1.y, e < 4 ? x0.x : x0.y, 0x0c040c00u + (e & 3) * 0x00010001u);
+        const f16x2 hi = v * sv;
+        ((uint32_t *)&st.vh[step & 1][0][pr >> 3][dt][at])[w] = as_u32(hi);
+        ((uint32_t *)&st.vh[step & 1][1][pr >> 3][dt][at])[w] = as_u32(__builtin_elementwise_fma(v, sv, -hi));
       }
     }
   };
 
-  f32x16 o[4];
+  // keys of a staged step: dims 16 k + [0, 16)
+  const uint32_t kbase = col * 16 + (h ^ (col & 15));
+  auto key = [&](uint32_t step, uint32_t k) {
+    if constexpr (K8)
+      return __builtin_bit_cast(f16x8, (&st.kh[step & 1][0][0])[kbase ^ (2 * k)]);
+    else
+      return __builtin_bit_cast(f16x8, (&st.k[step % DEPTH].x[0][0])[kbase ^ (2 * k)]);
+  };
+  auto zero = [](f32x16 &x) {
 #pragma unroll
-  for (int d = 0; d < 4; d++)
-#pragma unroll
-    for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
-  float m = -INFINITY, l = 0.0f;
-  look(begin);
-  load(begin);
-  look(min(begin + STEP, end - 1));
-  put(stage[0]);
-  uint32_t buf = 0;
-  for (uint32_t at = begin; at < end; at += STEP, buf ^= 1) {
-    __syncthreads();  // this step is staged, and the other stage read
-    const bool more = at + STEP < end;
-    if (more) {
-      load(at + STEP);
-      look(min(at + 2 * STEP, end - 1));
-    }
-    const WideStage<K8, V8> &s = stage[buf];
+    for (int r = 0; r < 16; r++) x[r] = 0.0f;
+  };
+  // scores of a staged step; 8-bit keys: blocks of 32 dims times their scales
+  auto scores = [&](uint32_t step) {
     f32x16 sc;
-#pragma unroll
-    for (int r = 0; r < 16; r++) sc[r] = 0.0f;
-    auto key = [&](uint32_t k) { return __builtin_bit_cast(f16x8, s.k[k][lane ^ (k | (h << 3))]); };
+    zero(sc);
     if constexpr (K8) {
 #pragma unroll
       for (uint32_t b = 0; b < 4; b++) {
         f32x16 x;
-#pragma unroll
-        for (int r = 0; r < 16; r++) x[r] = 0.0f;
+        zero(x);
 #pragma unroll
         for (uint32_t k = 2 * b; k < 2 * b + 2; k++) {
-          const f16x8 w = key(k);
+          const f16x8 w = key(step, k);
           x = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, ql[k], x, 0, 0, 0);
           x = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, qh[k], x, 0, 0, 0);
         }
 #pragma unroll
         for (uint32_t j = 0; j < 4; j++) {
-          const float4 f = *(const float4 *)&s.ks[b][8 * j + 4 * h];
+          const float4 f = *(const float4 *)&st.ks[step & 1][b][8 * j + 4 * h];
           sc[4 * j] = __builtin_fmaf(f.x, x[4 * j], sc[4 * j]);
           sc[4 * j + 1] = __builtin_fmaf(f.y, x[4 * j + 1], sc[4 * j + 1]);
           sc[4 * j + 2] = __builtin_fmaf(f.z, x[4 * j + 2], sc[4 * j + 2]);
@@ -614,10 +627,69 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
     } else {
 #pragma unroll
       for (uint32_t k = 0; k < 8; k++) {
-        const f16x8 w = key(k);
+        const f16x8 w = key(step, k);
         sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, ql[k], sc, 0, 0, 0);
         sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, qh[k], sc, 0, 0, 0);
       }
+    }
+    return sc;
+  };
+  // values of a staged step: k-step k, dims 32 d + [0, 32)
+  typedef __fp16 half4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) half4 LdsHalf4;
+  const uint32_t lr = lane >> 2 & 3;
+  const uint32_t vbase = (4 * h + lr) * 256 + 32 * (lane >> 4 & 1) + 8 * (lane & 3);
+  auto value = [&](uint32_t step, int part_, uint32_t k, uint32_t d) {
+    if constexpr (V8) {
+      return __builtin_bit_cast(f16x8, st.vh[step & 1][part_][k][d][lane ^ (d | ((lane >> 4 & 1) << 2))]);
+    } else {
+      const uint32_t at = lds_addr(&st.v[step % DEPTH].x[16 * k][0]) + vbase + ((d ^ lr) << 6);
+      const half4 x = __builtin_amdgcn_ds_read_tr16_b64_v4f16((LdsHalf4 *)(uintptr_t)at);
+      const half4 y = __builtin_amdgcn_ds_read_tr16_b64_v4f16((LdsHalf4 *)(uintptr_t)(at + 8 * 256));
+      const f16x4 u = __builtin_bit_cast(f16x4, x), v = __builtin_bit_cast(f16x4, y);
+      return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  };
+
+  f32x16 o[4];
+#pragma unroll
+  for (int d = 0; d < 4; d++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
+  float m = -INFINITY, l = 0.0f;
+  // Step s's values are loaded with step s + VK's keys: keys (scores come a step ahead) and 8-bit
+  // rows (converted a step ahead) are free for the next load a step before f16 values.
+  constexpr uint32_t VK = !V8, LEAD = DEPTH - 1 + V8;  // ... at the top of step s - LEAD
+  for (uint32_t s = 0; s < DEPTH; s++) {
+    load_keys(s, look(s));
+    if (s < LEAD) load_values(s, look(s));
+  }
+  dl_wait_vm<0>();
+  __syncthreads();
+  convert_keys(0);
+  convert_values(0);
+  __syncthreads();
+  f32x16 sc;
+  if constexpr (AHEAD) {
+    sc = scores(0);
+    __syncthreads();  // before the loop's first loads write its keys
+  }
+  const uint32_t n_steps = (end - begin + STEP - 1) / STEP;
+  Rows vat = look(LEAD), kat = look(LEAD + VK);
+  for (uint32_t step = 0; step < n_steps; step++) {
+    // here: this step's scores (AHEAD), and what is multiplied below lies in LDS, converted; what the
+    // loads write is read
+    load_values(step + LEAD, vat);
+    load_keys(step + LEAD + VK, kat);
+    vat = look(step + 1 + LEAD);
+    kat = look(step + 1 + LEAD + VK);
+    const uint32_t at = begin + step * STEP;
+    f16x8 kf[3];
+    if constexpr (AHEAD) {
+      kf[0] = key(step + 1, 0);
+      kf[1] = key(step + 1, 1);
+    } else {
+      sc = scores(step);
     }
     if (at + STEP > end) {  // the run's last positions
 #pragma unroll
@@ -637,31 +709,60 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
       for (int d = 0; d < 4; d++) o[d] *= down;
     }
     const float c = 7.0f - (m > -INFINITY ? m : 0.0f);
-    f16x8 ph[2], pl[2];
+    f16x8 ph[2], pl[2];  // e 2^7: cut to f16, and what that left
+    auto weigh = [&](uint32_t n) {  // scores 2 n and 2 n + 1
+      const uint32_t k = n >> 2, e = 2 * (n & 3);
+      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * n], inv, c));
+      const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * n + 1], inv, c));
+      l += x;
+      l += y;
+      const f16x2 hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x, y));
+      const f16x2 lo = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)hi.x, -1.0f, x),
+                                                                            __builtin_fmaf((float)hi.y, -1.0f, y)));
+      ph[k][e] = hi.x, ph[k][e + 1] = hi.y;
+      pl[k][e] = lo.x, pl[k][e + 1] = lo.y;
+    };
+    f16x8 vf[V8 ? 2 : 1][3];
+    auto read_values = [&](uint32_t n) {  // of product n: k-step n / 4, dims 32 (n % 4) + [0, 32)
+      vf[0][n % 3] = value(step, 0, n >> 2, n & 3);
+      if constexpr (V8) vf[V8 ? 1 : 0][n % 3] = value(step, 1, n >> 2, n & 3);
+    };
+    f32x16 next;
+    if constexpr (AHEAD) {
+      zero(next);
 #pragma unroll
-    for (int k = 0; k < 2; k++)
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k + e], inv, c));
-        l += x;
-        ph[k][e] = (f16)x;
-        pl[k][e] = (f16)(x - (float)ph[k][e]);
+      for (uint32_t k = 0; k < 8; k++) {
+        if (k < 6)
+          kf[(k + 2) % 3] = key(step + 1, k + 2);
+        else
+          read_values(k - 6);
+        next = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k % 3], ql[k], next, 0, 0, 0);
+        weigh(k);
+        next = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k % 3], qh[k], next, 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
       }
+    } else {
 #pragma unroll
-    for (uint32_t k = 0; k < 2; k++)
+      for (uint32_t k = 0; k < 8; k++) weigh(k);
+      read_values(0);
+      read_values(1);
+    }
 #pragma unroll
-      for (uint32_t d = 0; d < 4; d++) {
-        const uint32_t from = lane ^ (d | ((lane >> 4 & 1) << 2));
-        const f16x8 vh = __builtin_bit_cast(f16x8, s.v[0][k][d][from]);
-        if constexpr (V8) {
-          const f16x8 vl = __builtin_bit_cast(f16x8, s.v[V8 ? 1 : 0][k][d][from]);
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[k], o[d], 0, 0, 0);
-        }
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[k], o[d], 0, 0, 0);
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[k], o[d], 0, 0, 0);
-      }
-    if (more) put(stage[buf ^ 1]);
+    for (uint32_t n = 0; n < 8; n++) {
+      const uint32_t k = n >> 2, d = n & 3;
+      if (n < 6) read_values(n + 2);
+      if constexpr (V8) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[V8 ? 1 : 0][n % 3], ph[k], o[d], 0, 0, 0);
+      o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[0][n % 3], pl[k], o[d], 0, 0, 0);
+      o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[0][n % 3], ph[k], o[d], 0, 0, 0);
+      if (n == 1) convert_values(step + 1);
+      if (n == 3) convert_keys(step + 1);
+      if constexpr (AHEAD) __builtin_amdgcn_sched_barrier(0);
+    }
+    dl_wait_vm<4 * (DEPTH - 2)>();
+    __syncthreads();
+    if constexpr (AHEAD) sc = next;
   }
+  dl_wait_vm<0>();  // nothing is left to write this workgroup's LDS
   l += __shfl_xor(l, 32, 64);
   if (!live) return;
   float *out = a + p.part_off + ((row * p.n_kv * rep + kvh * rep + head) * (p.n_shared + p.n_own) + part) * PART;

@@ -120,6 +120,13 @@ SK_DEV void dl_load16(const u32x4 &res, uint32_t lds, uint32_t voff, uint32_t so
                : "s"(lds), "v"(voff), "s"(res), "s"(soff)
                : "memory", "m0");
 }
+// the same, 4 B per lane
+SK_DEV void dl_load4(const u32x4 &res, uint32_t lds, uint32_t voff, uint32_t soff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
+               :
+               : "s"(lds), "v"(voff), "s"(res), "s"(soff)
+               : "memory", "m0");
+}
 #pragma clang diagnostic pop
 SK_DEV uint32_t lds_addr(const void *p) { return (uint32_t)(uintptr_t)(dl_lds *)p; }
 
