@@ -48,6 +48,7 @@ struct LogitsPush {
       mask_stride;
 };
 
+SK_DEV float max3(float a, float b, float c) { return __builtin_fmaxf(__builtin_fmaxf(a, b), c); }
 SK_DEV float wave_max(float v) {
 #pragma unroll
   for (int d = 32; d >= 1; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, 64));
@@ -523,16 +524,16 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
 #pragma unroll
     for (uint32_t j = 0; j < 2; j++) {
       const uint32_t n = 4 * j + (lane >> 4), piece = (lane & 15) ^ (is_v ? (n & 3) << 2 : (n_at + n) & 15);
-      dl_load16(res, lds_addr(&to.x[n_at + 4 * j][0]), (min(n, at.room) * kv_dim + 8 * piece) * 2,
+      dl_load16(res, lds_addr(&to.x[n_at + 4 * j][0]), (__umul24(min(n, at.room), kv_dim) + 8 * piece) * 2,
                 (at.first * kv_dim + kvh * HD) * 2);
     }
   };
   auto load_q8 = [&](RawRows<1> &to, const u32x4 &res, const u32x4 &sres, const Rows &at) {
-    dl_load16(res, lds_addr(&to.x[n_at][0]), min(lane >> 3, at.room) * kv_dim + 16 * (lane & 7),
+    dl_load16(res, lds_addr(&to.x[n_at][0]), __umul24(min(lane >> 3, at.room), kv_dim) + 16 * (lane & 7),
               at.first * kv_dim + kvh * HD);
     const uint32_t base = __builtin_amdgcn_readfirstlane(at.first * (kv_dim / 16) + kvh * 8);
     if (lane < 16)
-      dl_load4(sres, lds_addr(&to.s[n_at]), min(lane >> 1, at.room) * (kv_dim / 16) + 4 * (lane & 1), base);
+      dl_load4(sres, lds_addr(&to.s[n_at]), __umul24(min(lane >> 1, at.room), kv_dim / 16) + 4 * (lane & 1), base);
   };
   auto load_keys = [&](uint32_t step, const Rows &at) {
     if constexpr (K8)
@@ -676,7 +677,8 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
   }
   const uint32_t n_steps = (end - begin + STEP - 1) / STEP;
   Rows vat = look(LEAD), kat = look(LEAD + VK);
-  for (uint32_t step = 0; step < n_steps; step++) {
+  // `sc`: this step's scores; into `next` the next step's
+  auto do_step = [&](uint32_t step, f32x16 &sc, f32x16 &next) {
     // here: this step's scores (AHEAD), and what is multiplied below lies in LDS, converted; what the
     // loads write is read
     load_values(step + LEAD, vat);
@@ -696,9 +698,10 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
       for (uint32_t r = 0; r < 16; r++)
         if (at + 8 * (r >> 2) + 4 * h + (r & 3) >= end) sc[r] = -INFINITY;
     }
-    float mt = sc[0];
+    float mt = max3(sc[0], sc[1], sc[2]);
 #pragma unroll
-    for (int r = 1; r < 16; r++) mt = fmaxf(mt, sc[r]);
+    for (int r = 3; r < 15; r += 2) mt = max3(mt, sc[r], sc[r + 1]);
+    mt = fmaxf(mt, sc[15]);
     mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * inv;
     if (__any(mt > m + 8.0f)) {
       const float mn = mt > m + 8.0f ? mt : m;
@@ -727,7 +730,6 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
       vf[0][n % 3] = value(step, 0, n >> 2, n & 3);
       if constexpr (V8) vf[V8 ? 1 : 0][n % 3] = value(step, 1, n >> 2, n & 3);
     };
-    f32x16 next;
     if constexpr (AHEAD) {
       zero(next);
 #pragma unroll
@@ -760,7 +762,20 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
     }
     dl_wait_vm<4 * (DEPTH - 2)>();
     __syncthreads();
-    if constexpr (AHEAD) sc = next;
+  };
+  f32x16 other;
+  if constexpr (V8) {  // two steps a round would need more registers than two waves a SIMD have
+    for (uint32_t step = 0; step < n_steps; step++) {
+      do_step(step, sc, other);
+      if constexpr (AHEAD) sc = other;
+    }
+  } else {
+    uint32_t step = 0;
+    for (; step + 2 <= n_steps; step += 2) {
+      do_step(step, sc, other);
+      do_step(step + 1, other, sc);
+    }
+    if (step < n_steps) do_step(step, sc, other);
   }
   dl_wait_vm<0>();  // nothing is left to write this workgroup's LDS
   l += __shfl_xor(l, 32, 64);

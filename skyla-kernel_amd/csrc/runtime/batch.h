@@ -25,7 +25,8 @@ inline Op op_of(const char *name) {
 constexpr uint32_t kHead = 128, kPart = kHead + 2;
 constexpr uint32_t kMaxSlots = 1024;      // partials of a row and head
 constexpr uint32_t kMaxGrid = 65535;      // rows of a dispatch
-constexpr uint32_t kMergeParts = 16;      // partials above which eight waves merge a head
+constexpr uint32_t kMergeParts = 16;      // partials above which eight waves merge a head,
+constexpr uint32_t kMergeHeads = 1024;    // where there are fewer rows of heads than this
 constexpr uint32_t kLogitsWide = 512;     // workgroups of 4096 tokens from which a logits launch takes 16384 each
 constexpr uint32_t kNarrow = 32;          // query rows of a key head up to which the shared run takes waves of 16
 constexpr uint32_t kMaxWork = 1u << 24;   // waves of an attention launch
@@ -205,7 +206,7 @@ inline Shape shape(Op op, const uint32_t *spec, const uint32_t *w, uint32_t rows
     s.groups[1] = 1;
     s.extra = {rows, wide};
   } else if (op == kMerge) {
-    s.form = w[4] + w[5] > kMergeParts;
+    s.form = w[4] + w[5] > kMergeParts && rows * w[3] < kMergeHeads;
     s.groups[0] = s.form ? w[3] : (w[3] + 3) / 4;
     s.threads = s.form ? 512 : 256;
   } else {
