@@ -20,13 +20,15 @@
 // Words that name no page or sequence reach no memory outside the pool: a row of such a sequence
 // counts as one of len 0, a length past the table's ends there, keys and values of such a page
 // are not stored, and a read of it goes to the pool's last page.
+#include <type_traits>
+
 #include "matmul_common.h"
 
 namespace {
 
 constexpr uint32_t HD = 128;         // head width
 constexpr uint32_t PART = HD + 2;    // one partial: m, l, acc[128]
-constexpr uint32_t TILE = 64;        // positions a wave takes at a time
+constexpr uint32_t TILE = 64;        // the parts of a run are whole multiples of it
 constexpr float F16_MAX = 65504.0f;
 
 struct AppendPush {
@@ -164,231 +166,278 @@ SK_DEV void append_body(const float *w, float *a, const uint32_t *ctl, f16 *kv, 
   }
 }
 
-// The state of 16 query rows (row c = lane % 16) over the positions seen so far: m the largest
-// score (in powers of two), l the sum of e = 2^(score - m), o[d] the sums of e v for the dims
-// 8 (4 g + r) + d (g = lane / 16), times 2^15 and, with 8-bit values, 2^(7 - ve).
-struct Rows16 {
-  f16x8 qh[4], ql[4];  // the query row's dims 8 g + 32 k + [0, 8) times 2^sh, in two f16 parts
-  int sh;
-  float m, l;
-  f32x4 o[8];
-  int ve;  // 8-bit values: the exponent of the largest scale so far of the dims this lane holds (block g)
+// What both forms of the attention share.  A query row is held as two f16 parts of q scale log2(e)
+// 2^sh (22 bits of its largest value; a product with an f16 key is exact), scores are in powers of
+// two.  The largest score is followed loosely: the sums are scaled down only where a score passes
+// the reference m by 2^LOOSE.  e = 2^(score - m) is held times 2^(15 - LOOSE), so that it stays in
+// f16's range, as two f16 parts (21 bits from 2^-14 of it on).
+constexpr float LOOSE = 8.0f;
+constexpr int E_SHIFT = 7;
+SK_DEV int query_shift(float big) { return big > 0.0f && big < INFINITY ? 11 - __builtin_amdgcn_frexp_expf(big) : 0; }
+// scores a and b as weights: x + y into l, the parts at elements e and e + 1
+SK_DEV void weigh(float a, float b, float inv, float c, float &l, f16x8 &ph, f16x8 &pl, int e) {
+  const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(a, inv, c));
+  const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(b, inv, c));
+  l += x;
+  l += y;
+  const f16x2 hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x, y));
+  const f16x2 lo = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)hi.x, -1.0f, x),
+                                                                        __builtin_fmaf((float)hi.y, -1.0f, y)));
+  ph[e] = hi.x, ph[e + 1] = hi.y;
+  pl[e] = lo.x, pl[e + 1] = lo.y;
+}
+// two bytes picked by sel as an f16 pair: 1024 + (byte ^ 0x80), minus 1152
+SK_DEV f16x2 widen(uint32_t x1, uint32_t x0, uint32_t sel) {
+  const f16x2 off = {(f16)1152.0f, (f16)1152.0f};
+  return as_f16x2((__builtin_amdgcn_perm(x1, x0, sel) ^ 0x00800080u) | 0x64006400u) - off;
+}
+SK_DEV f16x8 widen8(uint2 x) {
+  return __builtin_bit_cast(f16x8, make_uint4(as_u32(widen(x.x, x.x, 0x0c010c00u)), as_u32(widen(x.x, x.x, 0x0c030c02u)),
+                                              as_u32(widen(x.y, x.y, 0x0c010c00u)), as_u32(widen(x.y, x.y, 0x0c030c02u))));
+}
+// The page table through the scalar cache: nothing writes it while the kernel runs, and a vector
+// load's wait would be one for the cache rows in flight, too.
+typedef const __attribute__((address_space(4))) uint32_t ConstWord;
+struct Pages {
+  ConstWord *table;
+  uint32_t n_pages, log2;
+  __device__ __forceinline__ uint32_t slot(uint32_t pos) const {
+    const uint32_t page = min(table[pos >> log2], n_pages - 1);
+    return (page << log2) + (pos & ((1u << log2) - 1));
+  }
 };
-
-// The query row at `q` (this lane's row), scaled to scores in powers of two.
-SK_DEV void load_query(Rows16 &s, const float *q, float scale, uint32_t g) {
-  float v[4][8], big = 0.0f;
-#pragma unroll
-  for (int k = 0; k < 4; k++) {
-    const float4 u0 = *(const float4 *)(q + 8 * g + 32 * k), u1 = *(const float4 *)(q + 8 * g + 32 * k + 4);
-    const float u[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      v[k][e] = u[e] * (scale * 1.44269504088896340736f);
-      big = fmaxf(big, fabsf(v[k][e]));
-    }
-  }
-  big = fmaxf(big, __shfl_xor(big, 16, 64));
-  big = fmaxf(big, __shfl_xor(big, 32, 64));
-  s.sh = big > 0.0f && big < INFINITY ? 11 - __builtin_amdgcn_frexp_expf(big) : 0;
-#pragma unroll
-  for (int k = 0; k < 4; k++)
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const float x = ldexpf(v[k][e], s.sh);
-      s.qh[k][e] = (f16)x;
-      s.ql[k][e] = (f16)(x - (float)s.qh[k][e]);
-    }
-  s.m = -INFINITY;
-  s.l = 0.0f;
-  s.ve = -200;
-#pragma unroll
-  for (int d = 0; d < 8; d++) s.o[d] = {0.0f, 0.0f, 0.0f, 0.0f};
+SK_DEV Pages pages_of(const uint32_t *ctl, const PagedPush &p, uint32_t seq) {
+  return {(ConstWord *)(uintptr_t)(ctl + p.table_off + seq * p.table_stride), p.n_pages, p.page_log2};
 }
 
-// One tile of positions into the state: group t of 16 starts at pool slot slot[t], positions
-// [lo, hi) of the tile are live.  Loads of the others go to live positions of the tile, and their
-// scores are -inf, so what lies there reaches nothing.
+// A run of positions through one wave, for 16 query rows (this lane's, row c = lane % 16, at q), and
+// their partial into out if `live`.  A step takes HALF = 32 positions, two groups of 16; the next
+// step's rows are in flight while one is computed.  Nothing passes through LDS:
+//   S^T = K Q^T   v_mfma_f32_16x16x32_f16, A = key rows as loaded (row: position 16 t + c, dims 8 g +
+//                 32 k, g = lane / 16), B = query rows; a lane then has row c's scores at 16 t + 4 g + r
+//   O^T = V^T P^T B = those weights: element e of group g is position 16 (e / 4) + 4 g + e % 4; A =
+//                 value rows of these positions, lane c holding dims 8 c + [0, 8): tile d takes dim
+//                 8 c + d as row c, so the transposition is 8 x 8 inside a lane
+// Loads of positions outside [lo, hi) go to ones inside, and their scores are -inf, so what lies
+// there reaches nothing.  8-bit values are two f16 parts of q s 2^(4 - ve), ve the exponent of the
+// largest scale of the 32 dims, followed as loosely.
+constexpr uint32_t HALF = 32;
 template <int K8, int V8>
-SK_DEV void tile_step(Rows16 &s, const f16 *kv, const int8_t *kv8, const PagedPush &p, uint32_t kvh,
-                      const uint32_t (&slot)[4], uint32_t lo, uint32_t hi) {
-  const uint32_t lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, kv_dim = p.n_kv * HD;
-  // the pool row of position i of group t, moved to a live one
-  auto at = [&](uint32_t t, uint32_t i) {
-    const uint32_t pos = min(max(16 * t + i, lo), hi - 1), tt = pos >> 4;
-    const uint32_t first = tt == 0 ? slot[0] : tt == 1 ? slot[1] : tt == 2 ? slot[2] : slot[3];
-    return first + (pos & 15);
-  };
-  uint4 kr[4][4];
-#pragma unroll
-  for (uint32_t t = 0; t < 4; t++) {
-    const uint32_t src = p.kc_off + at(t, c) * kv_dim + kvh * HD + 8 * g;
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-      if constexpr (K8) {
-        const uint2 r = *(const uint2 *)(kv8 + src + 32 * k);
-        kr[t][k] = make_uint4(r.x, r.y, 0u, 0u);
-      } else {
-        kr[t][k] = *(const uint4 *)(kv + src + 32 * k);
-      }
-    }
-  }
-  f16x4 ks[4][4];
-  if constexpr (K8)
-#pragma unroll
-    for (uint32_t t = 0; t < 4; t++)
-#pragma unroll
-      for (uint32_t r = 0; r < 4; r++)
-        ks[t][r] = *(const f16x4 *)(kv + p.ks_off + at(t, 4 * g + r) * (kv_dim / 32) + kvh * 4);
-  uint4 vr[2][8];
-  f16 vs[2][8];
-#pragma unroll
-  for (uint32_t u = 0; u < 2; u++)
-#pragma unroll
-    for (uint32_t e = 0; e < 8; e++) {
-      const uint32_t row = at(2 * u + (e >> 2), 4 * g + (e & 3)), src = p.vc_off + row * kv_dim + kvh * HD + 8 * c;
-      if constexpr (V8) {
-        const uint2 r = *(const uint2 *)(kv8 + src);
-        vr[u][e] = make_uint4(r.x, r.y, 0u, 0u);
-        vs[u][e] = kv[p.vs_off + row * (kv_dim / 32) + kvh * 4 + (c >> 2)];
-      } else {
-        vr[u][e] = *(const uint4 *)(kv + src);
-      }
-    }
-  // two bytes picked by sel as an f16 pair: 1024 + (byte ^ 0x80), minus 1152
-  auto widen = [](uint32_t x1, uint32_t x0, uint32_t sel) {
-    const f16x2 off = {(f16)1152.0f, (f16)1152.0f};
-    return as_u32(as_f16x2((__builtin_amdgcn_perm(x1, x0, sel) ^ 0x00800080u) | 0x64006400u) - off);
-  };
-  // scores: lane holds row c's at positions 16 t + 4 g + r
-  float sc[4][4], m = s.m;
-#pragma unroll
-  for (uint32_t t = 0; t < 4; t++) {
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-      if constexpr (K8) {
-        const uint32_t x = kr[t][k].x, y = kr[t][k].y;
-        const f16x8 b = __builtin_bit_cast(f16x8, make_uint4(widen(x, x, 0x0c010c00u), widen(x, x, 0x0c030c02u),
-                                                             widen(y, y, 0x0c010c00u), widen(y, y, 0x0c030c02u)));
-        f32x4 part = {0.0f, 0.0f, 0.0f, 0.0f};
-        part = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, s.ql[k], part, 0, 0, 0);
-        part = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, s.qh[k], part, 0, 0, 0);
-#pragma unroll
-        for (int r = 0; r < 4; r++) acc[r] = __builtin_fmaf((float)ks[t][r][k], part[r], acc[r]);
-      } else {
-        const f16x8 b = __builtin_bit_cast(f16x8, kr[t][k]);
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, s.ql[k], acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, s.qh[k], acc, 0, 0, 0);
-      }
-    }
-#pragma unroll
-    for (uint32_t r = 0; r < 4; r++) {
-      const uint32_t pos = 16 * t + 4 * g + r;
-      sc[t][r] = pos >= lo && pos < hi ? ldexpf(acc[r], -s.sh) : -INFINITY;
-      m = fmaxf(m, sc[t][r]);
-    }
-  }
-  m = fmaxf(m, __shfl_xor(m, 16, 64));
-  m = fmaxf(m, __shfl_xor(m, 32, 64));
-  const float mu = m > -INFINITY ? m : 0.0f;  // scores of -inf alone: every e is 0
-  float down = __builtin_amdgcn_exp2f(s.m - mu);  // 0 for the first tile
-  s.m = m;
-  float l = 0.0f;
-  f16x8 ph[2], pl[2];  // e 2^15 in two parts: 22 bits from e = 2^-18 on, 2^-40 of the largest below
-#pragma unroll
-  for (uint32_t t = 0; t < 4; t++)
-#pragma unroll
-    for (uint32_t r = 0; r < 4; r++) {
-      const float e = __builtin_amdgcn_exp2f(sc[t][r] - mu), x = e * 32768.0f;
-      l += e;
-      const uint32_t i = 4 * (t & 1) + r;
-      ph[t >> 1][i] = (f16)x;
-      pl[t >> 1][i] = (f16)(x - (float)ph[t >> 1][i]);
-    }
-  l += __shfl_xor(l, 16, 64);
-  l += __shfl_xor(l, 32, 64);
-  s.l = __builtin_fmaf(s.l, down, l);
-  if constexpr (V8) {  // the scales of a block, largest first: to [64, 128), and the sums with them
-    float top = 0.0f;
-#pragma unroll
-    for (int u = 0; u < 2; u++)
-#pragma unroll
-      for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf((float)vs[u][e]));
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const int mine = __shfl(s.ve, (int)(16 * (c >> 2)), 64);  // this lane's values' block is c / 4
-    const int ve = top > 0.0f ? max(mine, __builtin_amdgcn_frexp_expf(top)) : mine;
-#pragma unroll
-    for (int u = 0; u < 2; u++)
-#pragma unroll
-      for (int e = 0; e < 8; e++) vs[u][e] = (f16)ldexpf((float)vs[u][e], 7 - ve);
-    const int next = __shfl(ve, (int)(4 * g), 64);
-    down = ldexpf(down, s.ve - next);
-    s.ve = next;
-  }
-#pragma unroll
-  for (int d = 0; d < 8; d++) s.o[d] *= down;
-  auto word = [](const uint4 &u, int i) { return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w; };
-#pragma unroll
-  for (int d = 0; d < 8; d++) {
-#pragma unroll
-    for (int u = 0; u < 2; u++) {
-      f16x8 vh, vl;
-      if constexpr (V8) {
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const uint32_t sel = 0x0c040c00u + (d & 3) * 0x00010001u;
-          const f16x2 v = as_f16x2(widen(word(vr[u][e + 1], d >> 2), word(vr[u][e], d >> 2), sel));
-          const f16x2 sv = {vs[u][e], vs[u][e + 1]};
-          const f16x2 hi = v * sv, rest = __builtin_elementwise_fma(v, sv, -hi);
-          vh[e] = hi.x, vh[e + 1] = hi.y;
-          vl[e] = rest.x, vl[e + 1] = rest.y;
-        }
-        s.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[u], s.o[d], 0, 0, 0);
-      } else {
-        const uint32_t sel = d & 1 ? 0x07060302u : 0x05040100u;
-        uint32_t x[4];
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-          x[e] = __builtin_amdgcn_perm(word(vr[u][2 * e + 1], d >> 1), word(vr[u][2 * e], d >> 1), sel);
-        vh = __builtin_bit_cast(f16x8, make_uint4(x[0], x[1], x[2], x[3]));
-      }
-      s.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl[u], s.o[d], 0, 0, 0);
-      s.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[u], s.o[d], 0, 0, 0);
-    }
-  }
-}
-
-// A run of positions through one wave for 16 query rows, and their partial.  `live`: the lane's
-// row is written.
+struct HalfRows {
+  typename std::conditional<K8, uint2, uint4>::type k[2][4];
+  f16x4 ks[K8 ? 2 : 1][4];
+  typename std::conditional<V8, uint2, uint4>::type v[8];
+  f16 vs[V8 ? 8 : 1];
+};
 template <int K8, int V8>
 SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t *kv8, const PagedPush &p, uint32_t kvh,
-                     const float *q, float *out, bool live, uint32_t seq, uint32_t lo, uint32_t hi, const Split &sp,
-                     uint32_t first, uint32_t last) {
-  const uint32_t g = (threadIdx.x & 63) >> 4;
-  Rows16 s;
-  load_query(s, q, p.scale, g);
-  const uint32_t *table = ctl + p.table_off + seq * p.table_stride;
-  for (uint32_t tile = first; tile < last; tile++) {
-    const uint32_t begin = sp.base + tile * TILE;
-    uint32_t slot[4];
+                     const float *q, float *out, bool live, uint32_t seq, uint32_t lo, uint32_t hi, uint32_t begin,
+                     uint32_t end) {
+  const uint32_t lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, kv_dim = p.n_kv * HD;
+  // wave-uniform, and known to be
+  lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
+  begin = __builtin_amdgcn_readfirstlane(begin), end = __builtin_amdgcn_readfirstlane(end);
+  kvh = __builtin_amdgcn_readfirstlane(kvh);
+  const Pages pages = pages_of(ctl, p, __builtin_amdgcn_readfirstlane(seq));
+  struct Groups {
+    uint32_t pos[2], slot[2];  // a step's groups of 16, moved to ones with live positions
+  };
+  auto look = [&](uint32_t at) {
+    Groups x;
 #pragma unroll
-    for (uint32_t t = 0; t < 4; t++) {
-      const uint32_t pos = min(begin + 16 * t, (hi - 1) & ~15u);
-      const uint32_t page = min(table[pos >> p.page_log2], p.n_pages - 1);
-      slot[t] = (page << p.page_log2) + (pos & ((1u << p.page_log2) - 1));
+    for (int t = 0; t < 2; t++) {
+      x.pos[t] = min(max(at + 16 * t, lo & ~15u), (hi - 1) & ~15u);
+      x.slot[t] = pages.slot(x.pos[t]);
     }
-    tile_step<K8, V8>(s, kv, kv8, p, kvh, slot, max(lo, begin) - begin, min(hi - begin, TILE));
+    return x;
+  };
+  auto load = [&](HalfRows<K8, V8> &r, const Groups &x) {
+    auto row = [&](uint32_t t, uint32_t i) { return x.slot[t] + min(max(x.pos[t] + i, lo), hi - 1) - x.pos[t]; };
+#pragma unroll
+    for (uint32_t t = 0; t < 2; t++) {
+      const uint32_t src = p.kc_off + row(t, c) * kv_dim + kvh * HD + 8 * g;
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        if constexpr (K8)
+          r.k[t][k] = *(const uint2 *)(kv8 + src + 32 * k);
+        else
+          r.k[t][k] = *(const uint4 *)(kv + src + 32 * k);
+      }
+      if constexpr (K8)
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++)
+          r.ks[t][i] = *(const f16x4 *)(kv + p.ks_off + row(t, 4 * g + i) * (kv_dim / 32) + kvh * 4);
+    }
+#pragma unroll
+    for (uint32_t e = 0; e < 8; e++) {
+      const uint32_t n = row(e >> 2, 4 * g + (e & 3)), src = p.vc_off + n * kv_dim + kvh * HD + 8 * c;
+      if constexpr (V8) {
+        r.v[e] = *(const uint2 *)(kv8 + src);
+        r.vs[e] = kv[p.vs_off + n * (kv_dim / 32) + kvh * 4 + (c >> 2)];
+      } else {
+        r.v[e] = *(const uint4 *)(kv + src);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);  // in flight before what is computed next
+  };
+
+  Groups now = look(begin), soon = look(begin + HALF);
+  HalfRows<K8, V8> ra, rb;
+  load(ra, now);
+  f16x8 qh[4], ql[4];
+  float inv;
+  {
+    float u[4][8], big = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const float4 x = *(const float4 *)(q + 8 * g + 32 * k), y = *(const float4 *)(q + 8 * g + 32 * k + 4);
+      const float w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        u[k][e] = w[e] * (p.scale * 1.44269504088896340736f);
+        big = fmaxf(big, fabsf(u[k][e]));
+      }
+    }
+    big = fmaxf(big, __shfl_xor(big, 16, 64));
+    big = fmaxf(big, __shfl_xor(big, 32, 64));
+    const int sh = query_shift(big);
+    inv = ldexpf(1.0f, -sh);
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float x = ldexpf(u[k][e], sh);
+        qh[k][e] = (f16)x;
+        ql[k][e] = (f16)(x - (float)qh[k][e]);
+      }
   }
+  float m = -INFINITY, l = 0.0f;
+  int ve = -200, vo = -200;  // of the dims that this lane's values and sums hold (blocks c / 4 and g)
+  f32x4 o[8];
+#pragma unroll
+  for (int d = 0; d < 8; d++) o[d] = {0.0f, 0.0f, 0.0f, 0.0f};
+  auto word = [](const auto &u, int i) {
+    if constexpr (sizeof(u) == 8)
+      return i == 0 ? u.x : u.y;
+    else
+      return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w;
+  };
+  auto compute = [&](const HalfRows<K8, V8> &r, uint32_t at) {
+    float sc[2][4];
+#pragma unroll
+    for (uint32_t t = 0; t < 2; t++) {
+      f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        if constexpr (K8) {
+          const f16x8 b = widen8(r.k[t][k]);
+          f32x4 part = {0.0f, 0.0f, 0.0f, 0.0f};
+          part = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, ql[k], part, 0, 0, 0);
+          part = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, qh[k], part, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < 4; i++) acc[i] = __builtin_fmaf((float)r.ks[t][i][k], part[i], acc[i]);
+        } else {
+          const f16x8 b = __builtin_bit_cast(f16x8, r.k[t][k]);
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, ql[k], acc, 0, 0, 0);
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, qh[k], acc, 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < 4; i++) sc[t][i] = acc[i];
+    }
+    if (at < lo || at + HALF > hi) {
+#pragma unroll
+      for (uint32_t t = 0; t < 2; t++)
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+          const uint32_t pos = at + 16 * t + 4 * g + i;
+          if (pos < lo || pos >= hi) sc[t][i] = -INFINITY;
+        }
+    }
+    float mt = max3(sc[0][0], sc[0][1], sc[0][2]);
+    mt = max3(mt, sc[0][3], sc[1][0]);
+    mt = max3(mt, sc[1][1], sc[1][2]);
+    mt = fmaxf(mt, sc[1][3]);
+    mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
+    mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * inv;
+    int top = -200;  // the scales' largest exponent
+    if constexpr (V8) {
+      float f = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; e++) f = fmaxf(f, fabsf((float)r.vs[e]));
+      f = fmaxf(f, __shfl_xor(f, 16, 64));
+      f = fmaxf(f, __shfl_xor(f, 32, 64));
+      top = f > 0.0f && f < INFINITY ? __builtin_amdgcn_frexp_expf(f) : -200;
+    }
+    if (__any(mt > m + LOOSE || top > ve + 5)) {
+      const float mn = mt > m + LOOSE ? mt : m;
+      float down = mn > -INFINITY ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
+      m = mn;
+      l *= down;
+      if constexpr (V8) {
+        if (top > ve + 5) ve = top;
+        const int vn = __shfl(ve, (int)(4 * g), 64);
+        down = ldexpf(down, vo - vn);
+        vo = vn;
+      }
+#pragma unroll
+      for (int d = 0; d < 8; d++) o[d] *= down;
+    }
+    const float cm = (float)E_SHIFT - (m > -INFINITY ? m : 0.0f);
+    f16x8 ph, pl;
+#pragma unroll
+    for (int n = 0; n < 4; n++) weigh(sc[n >> 1][2 * (n & 1)], sc[n >> 1][2 * (n & 1) + 1], inv, cm, l, ph, pl, 2 * n);
+    f16x2 sv[V8 ? 4 : 1];
+    if constexpr (V8)
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        sv[e] = f16x2{(f16)ldexpf((float)r.vs[2 * e], 4 - ve), (f16)ldexpf((float)r.vs[2 * e + 1], 4 - ve)};
+#pragma unroll
+    for (int d = 0; d < 8; d++) {
+      uint32_t x[4], y[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        if constexpr (V8) {
+          const f16x2 v = widen(word(r.v[2 * e + 1], d >> 2), word(r.v[2 * e], d >> 2), 0x0c040c00u + (d & 3) * 0x00010001u);
+          const f16x2 hi_ = v * sv[e];
+          x[e] = as_u32(hi_);
+          y[e] = as_u32(__builtin_elementwise_fma(v, sv[e], -hi_));
+        } else {
+          x[e] = __builtin_amdgcn_perm(word(r.v[2 * e + 1], d >> 1), word(r.v[2 * e], d >> 1), d & 1 ? 0x07060302u : 0x05040100u);
+        }
+      }
+      const f16x8 vh = __builtin_bit_cast(f16x8, make_uint4(x[0], x[1], x[2], x[3]));
+      if constexpr (V8)
+        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, make_uint4(y[0], y[1], y[2], y[3])), ph,
+                                                      o[d], 0, 0, 0);
+      o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl, o[d], 0, 0, 0);
+      o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph, o[d], 0, 0, 0);
+    }
+  };
+  for (uint32_t at = begin;; at += 2 * HALF) {
+    if (at + HALF < end) {
+      load(rb, soon);
+      soon = look(at + 2 * HALF);
+    }
+    compute(ra, at);
+    if (at + HALF >= end) break;
+    if (at + 2 * HALF < end) {
+      load(ra, soon);
+      soon = look(at + 3 * HALF);
+    }
+    compute(rb, at + HALF);
+    if (at + 2 * HALF >= end) break;
+  }
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
   if (!live) return;
-  const int back = V8 ? s.ve - 22 : -15;
+  const int back = V8 ? vo - 4 - E_SHIFT : -E_SHIFT;
 #pragma unroll
   for (int r = 0; r < 4; r++)
 #pragma unroll
     for (int d = 0; d < 8; d += 2)
-      *(float2 *)(out + 2 + 8 * (4 * g + r) + d) = make_float2(ldexpf(s.o[d][r], back), ldexpf(s.o[d + 1][r], back));
-  if (g == 0) *(float2 *)out = make_float2(s.m, s.l);
+      *(float2 *)(out + 2 + 8 * (4 * g + r) + d) = make_float2(ldexpf(o[d][r], back), ldexpf(o[d + 1][r], back));
+  if (g == 0) *(float2 *)out = make_float2(m, ldexpf(l, -E_SHIFT));
 }
 
 // The shared run for WIDE = 128 query rows a workgroup, 32 a wave: what 16 rows a wave read from
@@ -408,9 +457,7 @@ SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
 // With f16 keys a step multiplies the next step's scores while it makes this one's e, so that the
 // matrix pipe and the vector ALU work side by side in one wave; reads from LDS run two products
 // ahead.  (8-bit keys' block sums leave no registers for a second step's scores.)
-// The largest score is followed loosely: sums are scaled down only where a score passes the
-// reference by 2^8 (e is held times 2^7, so that it stays in f16's range), which after the first
-// steps is rare.  8-bit values are held as two f16 parts of q s 2^(7 - ve), ve the exponent of the
+// 8-bit values are held as two f16 parts of q s 2^(7 - ve), ve the exponent of the
 // part's largest scale of the 32 dims, found first.
 constexpr uint32_t WIDE = 128, STEP = 32;
 template <int Q8>
@@ -441,79 +488,17 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
   const uint32_t i = tile * WIDE + wave * 32 + col;
   uint32_t row = i / rep;
   const uint32_t head = i % rep;
-  const bool live =
-      row < n_rows && row_range(ctl, p.rows_off, row, shared, p.n_seq, p.table_stride, p.page_log2).member;
-  if (!__syncthreads_or(live)) return;
-  row = min(row, n_rows - 1);
-  const uint32_t *table = ctl + p.table_off + ctl[4] * p.table_stride;
-  auto slot_of = [&](uint32_t pos) {
-    const uint32_t page = min(table[pos >> p.page_log2], p.n_pages - 1);
-    return (page << p.page_log2) + (pos & ((1u << p.page_log2) - 1));
-  };
+  const Pages pages = pages_of(ctl, p, __builtin_amdgcn_readfirstlane(ctl[4]));
 
-  // this wave's query rows
-  f16x8 qh[8], ql[8];
-  float inv;
-  {
-    const float *q = a + p.q_off + row * p.q_stride + (kvh * rep + head) * HD + 8 * h;
-    float u[8][8], big = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 8; k++) {
-      const float4 x = *(const float4 *)(q + 16 * k), y = *(const float4 *)(q + 16 * k + 4);
-      const float w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        u[k][e] = w[e] * (p.scale * 1.44269504088896340736f);
-        big = fmaxf(big, fabsf(u[k][e]));
-      }
-    }
-    big = fmaxf(big, __shfl_xor(big, 32, 64));
-    const int sh = big > 0.0f && big < INFINITY ? 11 - __builtin_amdgcn_frexp_expf(big) : 0;
-    inv = ldexpf(1.0f, -sh);
-#pragma unroll
-    for (int k = 0; k < 8; k++)
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const float x = ldexpf(u[k][e], sh);
-        qh[k][e] = (f16)x;
-        ql[k][e] = (f16)(x - (float)qh[k][e]);
-      }
-  }
-
-  int ve[4] = {0, 0, 0, 0};
-  if constexpr (V8) {
-    float top[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t pos = begin + t; pos < end; pos += 256) {
-      const f16x4 s = *(const f16x4 *)(kv + p.vs_off + slot_of(pos) * (kv_dim / 32) + kvh * 4);
-#pragma unroll
-      for (int b = 0; b < 4; b++) top[b] = fmaxf(top[b], fabsf((float)s[b]));
-    }
-#pragma unroll
-    for (int b = 0; b < 4; b++) {
-      top[b] = wave_max(top[b]);
-      if (lane == 0) tops[wave][b] = top[b];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int b = 0; b < 4; b++) {
-      const float m = fmaxf(fmaxf(tops[0][b], tops[1][b]), fmaxf(tops[2][b], tops[3][b]));
-      ve[b] = m > 0.0f && m < INFINITY ? __builtin_amdgcn_frexp_expf(m) : 0;
-    }
-  }
-
-  // Staging.  Positions past the end are read as the last one.  The page table is read through
-  // the scalar cache: a vector load's wait would be one for the rows in flight, too.
+  // Staging.  Positions past the end are read as the last one.
   constexpr int DEPTH = WideStage<K8, V8>::DEPTH;
-  typedef const __attribute__((address_space(4))) uint32_t ConstWord;
-  ConstWord *pages = (ConstWord *)(uintptr_t)table;
   const uint32_t n_at = 8 * wave;  // the wave's first position of a step
   struct Rows {
     uint32_t first, room;  // that position's pool row, and how many live positions follow it
   };
   auto look = [&](uint32_t step) {
     const uint32_t pos = min(begin + step * STEP + n_at, end - 1);
-    const uint32_t page = min(pages[pos >> p.page_log2], p.n_pages - 1);
-    return Rows{(page << p.page_log2) + (pos & ((1u << p.page_log2) - 1)), end - 1 - pos};
+    return Rows{pages.slot(pos), end - 1 - pos};
   };
   const uint64_t pool = (uint64_t)(p.n_pages << p.page_log2) * kv_dim;
   const u32x4 kres = K8 ? dl_res(kv8 + p.kc_off, pool) : dl_res(kv + p.kc_off, 2 * pool);
@@ -548,12 +533,74 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
       load_f16(st.v[step % DEPTH], vres, at, true);
   };
 
+  // The first steps' rows are on their way before anything else is waited for.
+  // Step s's values are loaded with step s + VK's keys: keys (scores come a step ahead) and 8-bit
+  // rows (converted a step ahead) are free for the next load a step before f16 values.
+  constexpr uint32_t VK = !V8, LEAD = DEPTH - 1 + V8;  // ... at the top of step s - LEAD
+  for (uint32_t s = 0; s < DEPTH; s++) {
+    load_keys(s, look(s));
+    if (s < LEAD) load_values(s, look(s));
+  }
+
+  const bool live =
+      row < n_rows && row_range(ctl, p.rows_off, row, shared, p.n_seq, p.table_stride, p.page_log2).member;
+  row = min(row, n_rows - 1);
+  // this wave's query rows
+  f16x8 qh[8], ql[8];
+  float inv;
+  {
+    const float *q = a + p.q_off + row * p.q_stride + (kvh * rep + head) * HD + 8 * h;
+    float u[8][8], big = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const float4 x = *(const float4 *)(q + 16 * k), y = *(const float4 *)(q + 16 * k + 4);
+      const float w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        u[k][e] = w[e] * (p.scale * 1.44269504088896340736f);
+        big = fmaxf(big, fabsf(u[k][e]));
+      }
+    }
+    big = fmaxf(big, __shfl_xor(big, 32, 64));
+    if (!__syncthreads_or(live)) {
+      dl_wait_vm<0>();
+      return;
+    }
+    const int sh = query_shift(big);
+    inv = ldexpf(1.0f, -sh);
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float x = ldexpf(u[k][e], sh);
+        qh[k][e] = (f16)x;
+        ql[k][e] = (f16)(x - (float)qh[k][e]);
+      }
+  }
+
+  int ve[4] = {0, 0, 0, 0};
+  if constexpr (V8) {
+    float top[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t pos = begin + t; pos < end; pos += 256) {
+      const f16x4 s = *(const f16x4 *)(kv + p.vs_off + pages.slot(pos) * (kv_dim / 32) + kvh * 4);
+#pragma unroll
+      for (int b = 0; b < 4; b++) top[b] = fmaxf(top[b], fabsf((float)s[b]));
+    }
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+      top[b] = wave_max(top[b]);
+      if (lane == 0) tops[wave][b] = top[b];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+      const float m = fmaxf(fmaxf(tops[0][b], tops[1][b]), fmaxf(tops[2][b], tops[3][b]));
+      ve[b] = m > 0.0f && m < INFINITY ? __builtin_amdgcn_frexp_expf(m) : 0;
+    }
+  }
+
   // 8-bit rows to f16: dims 8 dg + [0, 8) of positions 2 pr and 2 pr + 1
   const uint32_t dg = t & 15, pr = t >> 4;
-  auto widen = [](uint32_t x1, uint32_t x0, uint32_t sel) {
-    const f16x2 off = {(f16)1152.0f, (f16)1152.0f};
-    return as_f16x2((__builtin_amdgcn_perm(x1, x0, sel) ^ 0x00800080u) | 0x64006400u) - off;
-  };
   int vmine = ve[0];
   if constexpr (V8) vmine = dg >> 2 == 0 ? ve[0] : dg >> 2 == 1 ? ve[1] : dg >> 2 == 2 ? ve[2] : ve[3];
   constexpr bool AHEAD = !K8;
@@ -563,9 +610,7 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
       for (uint32_t j = 0; j < 2; j++) {
         const uint32_t pos = 2 * pr + j;
         const uint2 x = ((const uint2 *)st.k[step % DEPTH].x[pos])[dg];
-        st.kh[step & 1][pos][dg ^ (pos & 15)] =
-            make_uint4(as_u32(widen(x.x, x.x, 0x0c010c00u)), as_u32(widen(x.x, x.x, 0x0c030c02u)),
-                       as_u32(widen(x.y, x.y, 0x0c010c00u)), as_u32(widen(x.y, x.y, 0x0c030c02u)));
+        st.kh[step & 1][pos][dg ^ (pos & 15)] = __builtin_bit_cast(uint4, widen8(x));
       }
       if (t < 4 * STEP) st.ks[step & 1][t & 3][t >> 2] = (float)((const f16 *)st.k[step % DEPTH].s)[t];
     }
@@ -658,13 +703,6 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
 #pragma unroll
     for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
   float m = -INFINITY, l = 0.0f;
-  // Step s's values are loaded with step s + VK's keys: keys (scores come a step ahead) and 8-bit
-  // rows (converted a step ahead) are free for the next load a step before f16 values.
-  constexpr uint32_t VK = !V8, LEAD = DEPTH - 1 + V8;  // ... at the top of step s - LEAD
-  for (uint32_t s = 0; s < DEPTH; s++) {
-    load_keys(s, look(s));
-    if (s < LEAD) load_values(s, look(s));
-  }
   dl_wait_vm<0>();
   __syncthreads();
   convert_keys(0);
@@ -703,28 +741,17 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
     for (int r = 3; r < 15; r += 2) mt = max3(mt, sc[r], sc[r + 1]);
     mt = fmaxf(mt, sc[15]);
     mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * inv;
-    if (__any(mt > m + 8.0f)) {
-      const float mn = mt > m + 8.0f ? mt : m;
+    if (__any(mt > m + LOOSE)) {  // rare after the first steps
+      const float mn = mt > m + LOOSE ? mt : m;
       const float down = mn > -INFINITY ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
       m = mn;
       l *= down;
 #pragma unroll
       for (int d = 0; d < 4; d++) o[d] *= down;
     }
-    const float c = 7.0f - (m > -INFINITY ? m : 0.0f);
-    f16x8 ph[2], pl[2];  // e 2^7: cut to f16, and what that left
-    auto weigh = [&](uint32_t n) {  // scores 2 n and 2 n + 1
-      const uint32_t k = n >> 2, e = 2 * (n & 3);
-      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * n], inv, c));
-      const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * n + 1], inv, c));
-      l += x;
-      l += y;
-      const f16x2 hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x, y));
-      const f16x2 lo = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)hi.x, -1.0f, x),
-                                                                            __builtin_fmaf((float)hi.y, -1.0f, y)));
-      ph[k][e] = hi.x, ph[k][e + 1] = hi.y;
-      pl[k][e] = lo.x, pl[k][e + 1] = lo.y;
-    };
+    const float c = (float)E_SHIFT - (m > -INFINITY ? m : 0.0f);
+    f16x8 ph[2], pl[2];
+    auto weigh2 = [&](uint32_t n) { weigh(sc[2 * n], sc[2 * n + 1], inv, c, l, ph[n >> 2], pl[n >> 2], 2 * (n & 3)); };
     f16x8 vf[V8 ? 2 : 1][3];
     auto read_values = [&](uint32_t n) {  // of product n: k-step n / 4, dims 32 (n % 4) + [0, 32)
       vf[0][n % 3] = value(step, 0, n >> 2, n & 3);
@@ -739,15 +766,15 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
         else
           read_values(k - 6);
         next = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k % 3], ql[k], next, 0, 0, 0);
-        weigh(k);
+        weigh2(k);
         next = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k % 3], qh[k], next, 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
       }
     } else {
-#pragma unroll
-      for (uint32_t k = 0; k < 8; k++) weigh(k);
       read_values(0);
       read_values(1);
+#pragma unroll
+      for (uint32_t k = 0; k < 4; k++) weigh2(k);
     }
 #pragma unroll
     for (uint32_t n = 0; n < 8; n++) {
@@ -756,9 +783,11 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
       if constexpr (V8) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[V8 ? 1 : 0][n % 3], ph[k], o[d], 0, 0, 0);
       o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[0][n % 3], pl[k], o[d], 0, 0, 0);
       o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[0][n % 3], ph[k], o[d], 0, 0, 0);
-      if (n == 1) convert_values(step + 1);
-      if (n == 3) convert_keys(step + 1);
-      if constexpr (AHEAD) __builtin_amdgcn_sched_barrier(0);
+      if constexpr (!AHEAD)
+        if (n < 4) weigh2(n + 4);
+      if (n == (AHEAD ? 1 : 4)) convert_values(step + 1);
+      if (n == 5) convert_keys(step + 1);
+      __builtin_amdgcn_sched_barrier(0);
     }
     dl_wait_vm<4 * (DEPTH - 2)>();
     __syncthreads();
@@ -785,12 +814,12 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
   for (int d = 0; d < 4; d++)
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      const float f = ldexpf(1.0f, V8 ? ve[d] - 14 : -7);
+      const float f = ldexpf(1.0f, V8 ? ve[d] - 7 - E_SHIFT : -E_SHIFT);
       float *to = out + 2 + 32 * d + 8 * j + 4 * h;
       *(float2 *)to = make_float2(o[d][4 * j] * f, o[d][4 * j + 1] * f);
       *(float2 *)(to + 2) = make_float2(o[d][4 * j + 2] * f, o[d][4 * j + 3] * f);
     }
-  if (h == 0) *(float2 *)out = make_float2(m, l * 0.0078125f);
+  if (h == 0) *(float2 *)out = make_float2(m, ldexpf(l, -E_SHIFT));
 }
 
 // Workgroups of four waves: first those of the shared run (`wide`: wide_run, the row tiles of a
@@ -826,7 +855,7 @@ SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_
       if (!__any(live) || first >= last) return;
       wave_run<K8, V8>(a, ctl, kv, kv8, p, kvh, a + p.q_off + row * p.q_stride + (kvh * N_REP + head) * HD,
                        a + p.part_off + ((row * p.n_kv * N_REP + kvh * N_REP + head) * slots + part) * PART, live, ctl[4],
-                       0, shared, sp, first, last);
+                       0, shared, first * TILE, min(last * TILE, shared));
       return;
     }
     w -= n;
@@ -839,7 +868,7 @@ SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_
   if (first >= last) return;
   wave_run<K8, V8>(a, ctl, kv, kv8, p, kvh, a + p.q_off + row * p.q_stride + (kvh * N_REP + head) * HD,
                    a + p.part_off + ((row * p.n_kv * N_REP + kvh * N_REP + head) * slots + p.n_shared + part) * PART,
-                   c < N_REP, r.seq, r.start, r.len, sp, first, last);
+                   c < N_REP, r.seq, r.start, r.len, sp.base + first * TILE, min(sp.base + last * TILE, r.len));
 }
 
 }  // namespace

@@ -83,8 +83,9 @@ def splits(rows: int, n_kv: int, rep: int, shared: int, own: int) -> tuple[int, 
     q = rows * rep
     if shared == 0:
         n_shared = 0
-    elif q > NARROW:  # workgroups of 128 query rows: two a compute unit
-        n_shared = parts(shared, n_kv * -(-q // 128), 512, 128)
+    elif q > NARROW:  # workgroups of 128 query rows: one a compute unit, two where a part stays long
+        groups = n_kv * -(-q // 128)
+        n_shared = parts(shared, groups, 512 if shared * groups >= 1024 * 512 else 256, -(-shared // 128))
     else:             # waves of 16
         n_shared = parts(shared, n_kv * -(-q // 16), 2048, 128)
     return n_shared, parts(own, n_kv * rows, 2048, 64)
