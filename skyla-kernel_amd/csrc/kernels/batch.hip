@@ -210,8 +210,8 @@ SK_DEV Pages pages_of(const uint32_t *ctl, const PagedPush &p, uint32_t seq) {
   return {(ConstWord *)(uintptr_t)(ctl + p.table_off + seq * p.table_stride), p.n_pages, p.page_log2};
 }
 
-// A run of positions through one wave, for 16 query rows (this lane's, row c = lane % 16, at q), and
-// their partial into out if `live`.  A step takes HALF = 32 positions, two groups of 16; the next
+// A run of positions [begin, end) through one wave, for 16 query rows (this lane's, row c = lane %
+// 16, at q); row c's partial goes to out[c].  Of the positions those in [lo, hi) count.  A step takes HALF = 32 positions, two groups of 16; the next
 // step's rows are in flight while one is computed.  Nothing passes through LDS:
 //   S^T = K Q^T   v_mfma_f32_16x16x32_f16, A = key rows as loaded (row: position 16 t + c, dims 8 g +
 //                 32 k, g = lane / 16), B = query rows; a lane then has row c's scores at 16 t + 4 g + r
@@ -231,7 +231,7 @@ struct HalfRows {
 };
 template <int K8, int V8>
 SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t *kv8, const PagedPush &p, uint32_t kvh,
-                     const float *q, float *out, bool live, uint32_t seq, uint32_t lo, uint32_t hi, uint32_t begin,
+                     const float *q, float (*out)[PART], uint32_t seq, uint32_t lo, uint32_t hi, uint32_t begin,
                      uint32_t end) {
   const uint32_t lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, kv_dim = p.n_kv * HD;
   // wave-uniform, and known to be
@@ -430,14 +430,13 @@ SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
   }
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
-  if (!live) return;
   const int back = V8 ? vo - 4 - E_SHIFT : -E_SHIFT;
 #pragma unroll
   for (int r = 0; r < 4; r++)
 #pragma unroll
     for (int d = 0; d < 8; d += 2)
-      *(float2 *)(out + 2 + 8 * (4 * g + r) + d) = make_float2(ldexpf(o[d][r], back), ldexpf(o[d + 1][r], back));
-  if (g == 0) *(float2 *)out = make_float2(m, ldexpf(l, -E_SHIFT));
+      *(float2 *)&out[c][2 + 8 * (4 * g + r) + d] = make_float2(ldexpf(o[d][r], back), ldexpf(o[d + 1][r], back));
+  if (g == 0) *(float2 *)out[c] = make_float2(m, ldexpf(l, -E_SHIFT));
 }
 
 // The shared run for WIDE = 128 query rows a workgroup, 32 a wave: what 16 rows a wave read from
@@ -473,12 +472,13 @@ struct WideStage {  // at most half of the 160 KB: two workgroups a compute unit
   uint4 kh[K8 ? 2 : 1][K8 ? STEP : 1][16];        // converted keys,
   float ks[K8 ? 2 : 1][4][K8 ? STEP : 4];         // their scales: [step][dims / 32][position]
   uint4 vh[V8 ? 2 : 1][V8 ? 2 : 1][2][4][V8 ? 64 : 1];  // and values: [step][part][k-step][dims / 32]
+  float tops[4][4];
 };
 template <int K8, int V8>
 SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t *kv8, const PagedPush &p, uint32_t rep,
-                     uint32_t kvh, uint32_t tile, uint32_t part, uint32_t shared, uint32_t n_rows) {
-  __shared__ __attribute__((aligned(1024))) WideStage<K8, V8> st;
-  __shared__ float tops[V8 ? 4 : 1][4];
+                     uint32_t kvh, uint32_t tile, uint32_t part, uint32_t shared, uint32_t n_rows,
+                     WideStage<K8, V8> &st) {
+  auto &tops = st.tops;
   const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, col = lane & 31,
                  h = lane >> 5;
   const uint32_t kv_dim = p.n_kv * HD;
@@ -822,53 +822,101 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
   if (h == 0) *(float2 *)out = make_float2(m, ldexpf(l, -E_SHIFT));
 }
 
-// Workgroups of four waves: first those of the shared run (`wide`: wide_run, the row tiles of a
-// key head's part 8 workgroups apart, so on one XCD and its L2; otherwise a wave for 16 rows of a
-// part), then a wave for each (row, part of its own run, key head).
+// Workgroups of four waves: first those of the shared run, `wide` (wide_run; the row tiles of a key
+// head's part lie 8 workgroups apart, so on one XCD and its L2) or for 16 query rows each; then one
+// for each (row, part of its own run, key head).  The latter two cut their part into the waves'
+// runs and join these in LDS.  Where a row has one part in all (slots == 1) the joined run is the
+// result.
+template <int K8, int V8>
+union PagedShared {
+  WideStage<K8, V8> wide;
+  float run[4][16][PART];
+};
 template <int N_REP, int K8, int V8>
 SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_t *kv8, const PagedPush &p,
                        uint32_t n_grid, uint32_t wide) {
-  const uint32_t lane = threadIdx.x & 63, c = lane & 15;
+  __shared__ __attribute__((aligned(1024))) PagedShared<K8, V8> st;
+  const uint32_t t = threadIdx.x, wave = t >> 6, c = t & 15;
   const uint32_t n_rows = min(ctl[2], n_grid), slots = p.n_shared + p.n_own, groups = p.n_kv * p.n_shared;
   const uint32_t shared = shared_positions(ctl, p.n_shared, p.n_seq, p.table_stride, p.page_log2);
-  uint32_t w = blockIdx.x;
+  uint32_t w = blockIdx.x, kvh, part, seq, lo, hi;
   if (n_rows == 0) return;
-  if (wide) {
-    const uint32_t tiles = (n_grid * N_REP + WIDE - 1) / WIDE, n = (groups + 7) / 8 * 8 * tiles;
-    if (w < n) {
+  const uint32_t tiles = wide ? (n_grid * N_REP + WIDE - 1) / WIDE : (n_grid * N_REP + 15) / 16;
+  const uint32_t n_first = wide ? (groups + 7) / 8 * 8 * tiles : groups * tiles;
+  const bool own = w >= n_first;
+  uint32_t i0;  // query rows i0 + [0, n_live) of the key head: row i / N_REP, head i % N_REP
+  Split sp;
+  if (!own) {
+    if (shared == 0) return;
+    if (wide) {
       const uint32_t g = w / (8 * tiles) * 8 + w % 8;
-      if (g < groups && shared) wide_run<K8, V8>(a, ctl, kv, kv8, p, N_REP, g % p.n_kv, w / 8 % tiles, g / p.n_kv, shared, n_rows);
+      if (g < groups)
+        wide_run<K8, V8>(a, ctl, kv, kv8, p, N_REP, g % p.n_kv, w / 8 % tiles, g / p.n_kv, shared, n_rows, st.wide);
       return;
     }
-    w -= n;
+    kvh = w % p.n_kv, part = w / p.n_kv % p.n_shared, i0 = w / groups * 16;
+    lo = 0, hi = shared, seq = ctl[4];
+    sp = split_of(lo, hi, p.n_shared);
+  } else {
+    w -= n_first;
+    kvh = w % p.n_kv, part = w / p.n_kv % p.n_own;
+    const uint32_t row = w / (p.n_kv * p.n_own);
+    if (row >= n_rows) return;
+    const Range r = row_range(ctl, p.rows_off, row, shared, p.n_seq, p.table_stride, p.page_log2);
+    i0 = row * N_REP, lo = r.start, hi = r.len, seq = r.seq;
+    sp = split_of(lo, hi, p.n_own);
   }
-  w = 4 * w + (threadIdx.x >> 6);
-  if (!wide) {
-    const uint32_t tiles = (n_grid * N_REP + 15) / 16, n = groups * tiles;
-    if (w < n) {
-      const uint32_t kvh = w % p.n_kv, part = w / p.n_kv % p.n_shared, i = w / groups * 16 + c;
-      const uint32_t row = min(i / N_REP, n_rows - 1), head = i % N_REP;
-      const bool live = i / N_REP < n_rows &&
-                        row_range(ctl, p.rows_off, row, shared, p.n_seq, p.table_stride, p.page_log2).member;
-      const Split sp = split_of(0, shared, p.n_shared);
-      const uint32_t first = part * sp.per, last = min(first + sp.per, sp.tiles);
-      if (!__any(live) || first >= last) return;
-      wave_run<K8, V8>(a, ctl, kv, kv8, p, kvh, a + p.q_off + row * p.q_stride + (kvh * N_REP + head) * HD,
-                       a + p.part_off + ((row * p.n_kv * N_REP + kvh * N_REP + head) * slots + part) * PART, live, ctl[4],
-                       0, shared, first * TILE, min(last * TILE, shared));
-      return;
+  const uint32_t n_live = own ? N_REP : 16;
+  const uint32_t begin = sp.base + part * sp.per * TILE, end = min(begin + sp.per * TILE, hi);
+  auto result = [&](uint32_t i, uint32_t j) -> float * {  // query row i's dims 2 j and 2 j + 1
+    return a + p.o_off + i / N_REP * p.o_stride + (kvh * N_REP + i % N_REP) * HD + 2 * j;
+  };
+  if (part * sp.per >= sp.tiles) {
+    if (slots == 1 && hi == 0)  // a row without positions
+      for (uint32_t j = t; j < N_REP * 64; j += 256) *(float2 *)result(i0 + j / 64, j % 64) = make_float2(0.0f, 0.0f);
+    return;
+  }
+  // whether query row i takes part in this run
+  auto live = [&](uint32_t i) {
+    return own || (i / N_REP < n_rows &&
+                   row_range(ctl, p.rows_off, i / N_REP, shared, p.n_seq, p.table_stride, p.page_log2).member);
+  };
+  if (!own && !__syncthreads_or(live(i0 + c))) return;
+  const uint32_t steps = (end - begin + HALF - 1) / HALF, per = (steps + 3) / 4 * HALF;
+  if (begin + wave * per < end) {
+    const uint32_t i = i0 + c % n_live, row = min(i / N_REP, n_rows - 1);
+    wave_run<K8, V8>(a, ctl, kv, kv8, p, kvh, a + p.q_off + row * p.q_stride + (kvh * N_REP + i % N_REP) * HD,
+                     st.run[wave], seq, lo, hi, begin + wave * per, min(begin + (wave + 1) * per, end));
+  }
+  const uint32_t used = (steps * HALF + per - 1) / per;  // waves with a run
+  __syncthreads();
+  for (uint32_t j = t; j < n_live * 64; j += 256) {
+    const uint32_t r = j / 64, d = j % 64, i = i0 + r;
+    if (!live(i)) continue;
+    float m = st.run[0][r][0];
+#pragma unroll
+    for (uint32_t n = 1; n < 4; n++)
+      if (n < used) m = fmaxf(m, st.run[n][r][0]);
+    const float mu = m > -INFINITY ? m : 0.0f;
+    float l = 0.0f, x = 0.0f, y = 0.0f;
+#pragma unroll
+    for (uint32_t n = 0; n < 4; n++)
+      if (n < used) {
+        const float f = __builtin_amdgcn_exp2f(st.run[n][r][0] - mu);
+        const float2 v = *(const float2 *)&st.run[n][r][2 + 2 * d];
+        l = __builtin_fmaf(f, st.run[n][r][1], l);
+        x = __builtin_fmaf(f, v.x, x);
+        y = __builtin_fmaf(f, v.y, y);
+      }
+    if (slots == 1) {
+      *(float2 *)result(i, d) = make_float2(x / l, y / l);
+    } else {
+      float *out = a + p.part_off +
+                   ((i / N_REP * p.n_kv * N_REP + kvh * N_REP + i % N_REP) * slots + (own ? p.n_shared : 0) + part) * PART;
+      *(float2 *)(out + 2 + 2 * d) = make_float2(x, y);
+      if (d == 0) *(float2 *)out = make_float2(m, l);
     }
-    w -= n;
   }
-  const uint32_t kvh = w % p.n_kv, part = w / p.n_kv % p.n_own, row = w / (p.n_kv * p.n_own), head = c % N_REP;
-  if (row >= n_rows) return;
-  const Range r = row_range(ctl, p.rows_off, row, shared, p.n_seq, p.table_stride, p.page_log2);
-  const Split sp = split_of(r.start, r.len, p.n_own);
-  const uint32_t first = part * sp.per, last = min(first + sp.per, sp.tiles);
-  if (first >= last) return;
-  wave_run<K8, V8>(a, ctl, kv, kv8, p, kvh, a + p.q_off + row * p.q_stride + (kvh * N_REP + head) * HD,
-                   a + p.part_off + ((row * p.n_kv * N_REP + kvh * N_REP + head) * slots + p.n_shared + part) * PART,
-                   c < N_REP, r.seq, r.start, r.len, sp.base + first * TILE, min(sp.base + last * TILE, r.len));
 }
 
 }  // namespace

@@ -28,8 +28,8 @@ constexpr uint32_t kMaxGrid = 65535;      // rows of a dispatch
 constexpr uint32_t kMergeParts = 16;      // partials above which eight waves merge a head,
 constexpr uint32_t kMergeHeads = 1024;    // where there are fewer rows of heads than this
 constexpr uint32_t kLogitsWide = 512;     // workgroups of 4096 tokens from which a logits launch takes 16384 each
-constexpr uint32_t kNarrow = 32;          // query rows of a key head up to which the shared run takes waves of 16
-constexpr uint32_t kMaxWork = 1u << 24;   // waves of an attention launch
+constexpr uint32_t kNarrow = 32;          // query rows of a key head up to which the shared run takes 16 a workgroup
+constexpr uint32_t kMaxWork = 1u << 23;   // workgroups of an attention launch
 
 // [off, off + stride (rows - 1) + width) in elements
 struct Region {
@@ -144,6 +144,7 @@ inline std::string refusal(Op op, const uint32_t *spec, const uint32_t *w, const
     c.holds(part, a, 2);
     check_pool(c, spec[1], spec[2], w + 5, slots, kv_dim, bytes[2], bytes[3]);
     for (const Region *r : {&q, &o, &words, &table}) c.apart(part, *r);
+    if (!(o.off == q.off && (o.stride == q.stride || rows == 1))) c.apart(o, q);
     c.apart(o, words);
     c.apart(o, table);
     if (n_kv * ((rows * spec[0] + 15) / 16 * w[11] + rows * w[12]) > kMaxWork)
@@ -152,6 +153,7 @@ inline std::string refusal(Op op, const uint32_t *spec, const uint32_t *w, const
     const uint64_t a = bytes[0] / 4, n_head = w[3], parts = (uint64_t)w[4] + w[5];
     c.need(n_head >= 1 && n_head <= 8192, "1 to 8192 heads");
     c.need(w[5] >= 1 && parts <= kMaxSlots, "a row's own positions take 1 part or more, all of them at most 1024");
+    c.need(parts > 1, "one part in all is the attention's result already");
     c.need(w[9] >= 4 && w[9] <= 12, "pages hold 16 to 4096 positions");
     if (!c.error.empty()) return c.error;
     const Region part{"the partials", w[0], 0, rows * n_head * parts * kPart, 1},
@@ -200,9 +202,9 @@ inline Shape shape(Op op, const uint32_t *spec, const uint32_t *w, uint32_t rows
     const uint32_t q = rows * spec[0], groups = w[9] * w[11], own = rows * w[9] * w[12];
     const bool wide = w[11] && q > kNarrow;
     if (wide)
-      s.groups[0] = (groups + 7) / 8 * 8 * ((q + 127) / 128) + (own + 3) / 4;
+      s.groups[0] = (groups + 7) / 8 * 8 * ((q + 127) / 128) + own;
     else
-      s.groups[0] = (groups * ((q + 15) / 16) + own + 3) / 4;
+      s.groups[0] = groups * ((q + 15) / 16) + own;
     s.groups[1] = 1;
     s.extra = {rows, wide};
   } else if (op == kMerge) {

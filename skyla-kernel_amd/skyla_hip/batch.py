@@ -24,7 +24,7 @@ import numpy as np
 from . import engine as E
 from .abi import Buffer, Context, Recorder
 
-NARROW = 32             # query rows of a key head up to which the shared run takes waves of 16 (runtime/batch.h)
+NARROW = 32             # query rows of a key head up to which the shared run takes 16 a workgroup (runtime/batch.h)
 MAX_PARTS = 1024        # partials of a row and head (runtime/batch.h)
 PAGE_SIZES = tuple(16 << i for i in range(9))  # 16 to 4096 positions
 CTL_ROWS, CTL_SHARED, CTL_LEADER = 2, 3, 4     # control words: live rows, shared positions, their sequence
@@ -77,18 +77,16 @@ def splits(rows: int, n_kv: int, rep: int, shared: int, own: int) -> tuple[int, 
     """Parts that a batch's attention cuts the shared run and each row's own run into, for
     `shared` shared positions and at most `own` of a row's own: enough workgroups to fill the
     GPU, each with some tiles of 64 positions."""
-    def parts(positions: int, groups: int, want: int, most: int) -> int:
-        tiles = -(-positions // 64)
-        return max(1, min(tiles, -(-want // groups), most))
-    q = rows * rep
+    q, tiles = rows * rep, -(-shared // 64)
     if shared == 0:
         n_shared = 0
     elif q > NARROW:  # workgroups of 128 query rows: one a compute unit, two where a part stays long
         groups = n_kv * -(-q // 128)
-        n_shared = parts(shared, groups, 512 if shared * groups >= 1024 * 512 else 256, -(-shared // 128))
-    else:             # waves of 16
-        n_shared = parts(shared, n_kv * -(-q // 16), 2048, 128)
-    return n_shared, parts(own, n_kv * rows, 2048, 64)
+        n_shared = min(-(-(512 if shared * groups >= 1024 * 512 else 256) // groups), -(-tiles // 2))
+    else:             # 16 query rows and four waves each
+        n_shared = min(-(-512 // (n_kv * -(-q // 16))), -(-tiles // 4))
+    tiles = -(-own // 64)
+    return min(n_shared, 128), max(1, min(-(-512 // (n_kv * rows)), -(-tiles // 4), 128))
 
 
 def part_size(rows: int, n_head: int, parts: tuple[int, int]) -> int:
@@ -143,6 +141,8 @@ class BatchKernels:
         push = [q[0], q[1], out[0], out[1], at.part, kv.keys(0), kv.values(0), kv.key_scales(0), kv.value_scales(0),
                 c.n_head_kv, E.f32_bits(scale), *parts, at.rows, at.table, *self._pages()]
         r.dispatch_set(self._attend, layer, [1, rows, 1], push)
+        if sum(parts) == 1:  # nothing to merge: the rows are the result
+            return
         r.barrier()
         push = [at.part, out[0], out[1], c.n_head, *parts, at.rows, self.paged.seq_pages, self.paged.n_seq,
                 self.paged.page_log2]

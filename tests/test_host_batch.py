@@ -94,7 +94,7 @@ def test_attention_words(host):
     for bad in (dict(q=A // 4), dict(q=65), dict(qs=510), dict(o=4097), dict(part=8193), dict(part=A // 4 - 100), dict(part=4096),
                 dict(part=512), dict(part=19000), dict(n_own=0), dict(n_own=1025), dict(n_shared=1024), dict(n_shared=2**32 - 1),
                 dict(n_kv=0), dict(n_kv=3), dict(n_kv=2**31), dict(kc=8), dict(ks=2, n_pages=9), dict(vs=2), dict(table=2**32 - 1),
-                dict(n_seq=0), dict(ts=2**31), dict(log2=2), dict(o=20000), dict(o=19900)):
+                dict(n_seq=0), dict(ts=2**31), dict(log2=2), dict(o=68), dict(os=516, o=64), dict(o=20000), dict(o=19900)):
         assert ok(**bad), bad
     assert ok(rows=65535)  # the partials end past the arena
     # 8-bit keys: the key rows and their scales in bytes and halves
@@ -109,7 +109,7 @@ def test_merge_words(host):
     ok = lambda rows=4, **k: _refuse(host, "attention_paged_merge", [128], list((base | k).values()), rows, [A, A])  # noqa: E731
     assert ok() == ""
     for bad in (dict(part=A // 4 - 6000), dict(part=1 << 31), dict(o=8190), dict(os=256), dict(n_head=0), dict(n_own=0),
-                dict(n_shared=1024), dict(rows=2**31), dict(log2=0), dict(o=19998)):
+                dict(n_shared=1024), dict(n_shared=0, n_own=1), dict(rows=2**31), dict(log2=0), dict(o=19998)):
         assert ok(**bad), bad
 
 
