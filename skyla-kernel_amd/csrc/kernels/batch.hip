@@ -96,73 +96,106 @@ SK_DEV Split split_of(uint32_t lo, uint32_t hi, uint32_t n) {
 }
 SK_DEV uint32_t live_parts(const Split &s) { return (s.tiles + s.per - 1) / s.per; }
 
-// Elements t and t + 64 of one head's cache row, held as attention.hip holds them but for one
-// thing: an f16 past the type's largest value is stored as that value, so that the cache has no
-// infinity (its products with the f16 parts of a query or a weight would be NaN).
+// Elements 4 t + [0, 4) and 64 + 4 t + [0, 4) (t = lane % 16) of one head's cache row, held as
+// attention.hip holds them but for one thing: an f16 past the type's largest value is stored as
+// that value, so that the cache has no infinity (its products with the f16 parts of a query or a
+// weight would be NaN).
 template <int Q8>
 SK_DEV void store_row(f16 *kv, int8_t *kv8, uint32_t cache, uint32_t scales, uint32_t kv_dim, uint32_t slot,
-                      uint32_t head, uint32_t t, float y0, float y1) {
+                      uint32_t head, uint32_t t, const float4 (&y)[2]) {
   auto fit = [](float v) { return v > F16_MAX ? F16_MAX : v < -F16_MAX ? -F16_MAX : v; };  // keeps NaN
-  const uint32_t dst = cache + slot * kv_dim + head * HD;
-  if constexpr (!Q8) {
-    kv[dst + t] = (f16)fit(y0);
-    kv[dst + t + 64] = (f16)fit(y1);
-  } else {
-    float m0 = fabsf(y0), m1 = fabsf(y1);  // blocks: the lower and upper 32 lanes
+  const uint32_t dst = cache + slot * kv_dim + head * HD + 4 * t;
 #pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) {
-      m0 = fmaxf(m0, __shfl_xor(m0, d, 64));
-      m1 = fmaxf(m1, __shfl_xor(m1, d, 64));
-    }
-    const float s0 = m0 / 127.0f, s1 = m1 / 127.0f;
-    kv8[dst + t] = (int8_t)(s0 > 0.0f ? __builtin_rintf(y0 / s0) : 0.0f);
-    kv8[dst + t + 64] = (int8_t)(s1 > 0.0f ? __builtin_rintf(y1 / s1) : 0.0f);
-    if ((t & 31) == 0) {
-      const uint32_t sd = scales + slot * (kv_dim / 32) + head * 4 + t / 32;
-      kv[sd] = (f16)fit(s0);
-      kv[sd + 2] = (f16)fit(s1);
+  for (uint32_t n = 0; n < 2; n++) {
+    const float v[4] = {y[n].x, y[n].y, y[n].z, y[n].w};
+    if constexpr (!Q8) {
+      *(f16x4 *)(kv + dst + 64 * n) = f16x4{(f16)fit(v[0]), (f16)fit(v[1]), (f16)fit(v[2]), (f16)fit(v[3])};
+    } else {  // a block: eight lanes' values
+      float m = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+      m = fmaxf(m, dpp_f<0xb1>(m));
+      m = fmaxf(m, dpp_f<0x4e>(m));
+      m = fmaxf(m, dpp_f<0x141>(m));
+      const float s = m / 127.0f;
+      uint32_t w = 0;
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        w |= ((uint32_t)(int)(s > 0.0f ? __builtin_rintf(v[e] / s) : 0.0f) & 255u) << (8 * e);
+      *(uint32_t *)(kv8 + dst + 64 * n) = w;
+      if ((t & 7) == 0) kv[scales + slot * (kv_dim / 32) + head * 4 + 2 * n + t / 8] = (f16)fit(s);
     }
   }
 }
 
-// One wave per (head, row): lane t holds the pair (t, t + 64) that the rotation turns.  The
-// angle (len - 1) f_t is formed in 64 bits as revolutions and reduced there: an f32 product is off
-// by 2^-24 of an angle of 1e5, 3e-3 of a radian.
-template <int K8, int V8>
+// A wave holds four heads of a row, 16 lanes each: lane t = lane % 16 has the pairs (d, d + 64), d
+// in 4 t + [0, 4), that the rotation turns.  A workgroup's four waves take 16 PASSES heads of one
+// row, every load in flight before the first product.  The angle (len - 1) f_d is formed in 64
+// bits as revolutions and reduced there: an f32 product is off by 2^-24 of an angle of 1e5, 3e-3
+// of a radian.  Each wave turns its row's 64 angles once, one a lane, for all its heads.
+// 16 bytes a lane and load: with 4 (a wave a head) 2048 rows of 48 heads ran 79 us from HBM.
+template <int K8, int V8, int PASSES>
 SK_DEV void append_body(const float *w, float *a, const uint32_t *ctl, f16 *kv, int8_t *kv8, const AppendPush &p) {
 #pragma clang fp contract(off)
-  const uint32_t row = blockIdx.y, t = threadIdx.x & 63, h = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= ctl[2] || h >= p.n_head + 2 * p.n_kv) return;
+  __shared__ float2 turn[4][64];
+  const uint32_t row = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, t = lane & 15;
+  if (row >= ctl[2]) return;
   const Range r = row_range(ctl, p.rows_off, row, 0, p.n_seq, p.table_stride, p.page_log2);
   if (r.len == 0) return;
-  const uint32_t pos = r.len - 1;
+  const uint32_t pos = r.len - 1, n_heads = p.n_head + 2 * p.n_kv;
+  const uint32_t h0 = (blockIdx.x * PASSES * 4 + wave) * 4 + (lane >> 4);
+  float4 x[PASSES][2];
+#pragma unroll
+  for (uint32_t n = 0; n < PASSES; n++) {
+    const uint32_t h = h0 + 16 * n;
+    if (h < n_heads) {
+      const uint32_t at = h < p.n_head            ? p.q_off + row * p.q_stride + h * HD
+                          : h < p.n_head + p.n_kv ? p.k_off + row * p.kv_stride + (h - p.n_head) * HD
+                                                  : p.v_off + row * p.kv_stride + (h - p.n_head - p.n_kv) * HD;
+      x[n][0] = *(const float4 *)(a + at + 4 * t);
+      x[n][1] = *(const float4 *)(a + at + 64 + 4 * t);
+    }
+  }
   const uint32_t page = ctl[p.table_off + r.seq * p.table_stride + (pos >> p.page_log2)];
   const uint32_t slot = (page << p.page_log2) + (pos & ((1u << p.page_log2) - 1));
   const uint32_t kv_dim = p.n_kv * HD;
-  if (h >= p.n_head + p.n_kv) {  // a value head: kept as it is
-    const uint32_t vh = h - p.n_head - p.n_kv, src = p.v_off + row * p.kv_stride + vh * HD;
-    if (page < p.n_pages) store_row<V8>(kv, kv8, p.vc_off, p.vs_off, kv_dim, slot, vh, t, a[src + t], a[src + t + 64]);
-    return;
+  {
+    const double turns = (double)pos * (double)w[p.rope_off + lane] * 0.15915494309189533577;  // 1 / (2 pi)
+    float s, c;
+    sincospif((float)(2.0 * (turns - __builtin_rint(turns))), &s, &c);
+    turn[wave][lane] = make_float2(c * p.mscale, s * p.mscale);
   }
-  const bool is_q = h < p.n_head;
-  const uint32_t head = is_q ? h : h - p.n_head;
-  const float *x = a + (is_q ? p.q_off + row * p.q_stride : p.k_off + row * p.kv_stride) + head * HD;
-  const float *nw = w + (is_q ? p.qn_off : p.kn_off);
-  const float x0 = x[t], x1 = x[t + 64];
-  const float rms = 1.0f / sqrtf(group_sum<64>(x0 * x0 + x1 * x1) / (float)HD + p.eps);
-  const float n0 = x0 * rms * nw[t], n1 = x1 * rms * nw[t + 64];
-  const double turns = (double)pos * (double)w[p.rope_off + t] * 0.15915494309189533577;  // 1 / (2 pi)
-  float s, c;
-  sincospif((float)(2.0 * (turns - __builtin_rint(turns))), &s, &c);
-  c *= p.mscale;
-  s *= p.mscale;
-  const float y0 = n0 * c - n1 * s, y1 = n0 * s + n1 * c;
-  if (is_q) {
-    float *o = a + p.o_off + row * p.o_stride + head * HD;
-    o[t] = y0;
-    o[t + 64] = y1;
-  } else if (page < p.n_pages) {
-    store_row<K8>(kv, kv8, p.kc_off, p.ks_off, kv_dim, slot, head, t, y0, y1);
+  __syncthreads();
+  const float4 cs0 = *(const float4 *)&turn[wave][4 * t], cs1 = *(const float4 *)&turn[wave][4 * t + 2];
+  const float c[4] = {cs0.x, cs0.z, cs1.x, cs1.z}, s[4] = {cs0.y, cs0.w, cs1.y, cs1.w};
+#pragma unroll
+  for (uint32_t n = 0; n < PASSES; n++) {
+    const uint32_t h = h0 + 16 * n;
+    if (h >= n_heads) break;
+    if (h >= p.n_head + p.n_kv) {  // a value head: kept as it is
+      if (page < p.n_pages) store_row<V8>(kv, kv8, p.vc_off, p.vs_off, kv_dim, slot, h - p.n_head - p.n_kv, t, x[n]);
+      continue;
+    }
+    const bool is_q = h < p.n_head;
+    const float *nw = w + (is_q ? p.qn_off : p.kn_off) + 4 * t;
+    const float u[8] = {x[n][0].x, x[n][0].y, x[n][0].z, x[n][0].w, x[n][1].x, x[n][1].y, x[n][1].z, x[n][1].w};
+    float ss = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) ss += u[e] * u[e];
+    const float rms = 1.0f / sqrtf(lane_sum<16>(ss) / (float)HD + p.eps);
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const float n0 = u[e] * rms * nw[e], n1 = u[e + 4] * rms * nw[e + 64];
+      y[e] = n0 * c[e] - n1 * s[e];
+      y[e + 4] = n0 * s[e] + n1 * c[e];
+    }
+    const float4 out[2] = {make_float4(y[0], y[1], y[2], y[3]), make_float4(y[4], y[5], y[6], y[7])};
+    if (is_q) {
+      float *o = a + p.o_off + row * p.o_stride + h * HD + 4 * t;
+      *(float4 *)o = out[0];
+      *(float4 *)(o + 64) = out[1];
+    } else if (page < p.n_pages) {
+      store_row<K8>(kv, kv8, p.kc_off, p.ks_off, kv_dim, slot, h - p.n_head, t, out);
+    }
   }
 }
 
@@ -924,7 +957,11 @@ SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_
 #define APPEND(K8, V8)                                                                                 \
   extern "C" __global__ __launch_bounds__(256) void kv_append__##K8##_##V8##_128(                      \
       const float *w, float *a, const uint32_t *ctl, f16 *kv, int8_t *kv8, AppendPush p) {              \
-    append_body<K8, V8>(w, a, ctl, kv, kv8, p);                                                         \
+    append_body<K8, V8, 1>(w, a, ctl, kv, kv8, p);                                                      \
+  }                                                                                                    \
+  extern "C" __global__ __launch_bounds__(256) void kv_append_4__##K8##_##V8##_128(                    \
+      const float *w, float *a, const uint32_t *ctl, f16 *kv, int8_t *kv8, AppendPush p) {              \
+    append_body<K8, V8, 4>(w, a, ctl, kv, kv8, p);                                                      \
   }
 APPEND(0, 0)
 APPEND(0, 1)

@@ -25,6 +25,7 @@ inline Op op_of(const char *name) {
 constexpr uint32_t kHead = 128, kPart = kHead + 2;
 constexpr uint32_t kMaxSlots = 1024;      // partials of a row and head
 constexpr uint32_t kMaxGrid = 65535;      // rows of a dispatch
+constexpr uint32_t kAppendMany = 2048;    // workgroups of 16 heads from which kv_append takes 64 each
 constexpr uint32_t kMergeParts = 16;      // partials above which eight waves merge a head,
 constexpr uint32_t kMergeHeads = 1024;    // where there are fewer rows of heads than this
 constexpr uint32_t kLogitsWide = 512;     // workgroups of 4096 tokens from which a logits launch takes 16384 each
@@ -116,7 +117,7 @@ inline std::string refusal(Op op, const uint32_t *spec, const uint32_t *w, const
     c.need(w[20] >= 1 && w[21] >= 1, "the page table is empty");
     if (!c.error.empty()) return c.error;
     const uint64_t slots = (uint64_t)w[22] << w[23];
-    for (const Region *r : {&q, &k, &v, &o}) c.holds(*r, a, 1);
+    for (const Region *r : {&q, &k, &v, &o}) c.holds(*r, a, 4);
     for (uint32_t i : {4u, 5u}) c.holds({"a norm's weights", w[i], 0, kHead, 1}, bytes[0] / 4, 1);
     c.holds({"the rotation's frequencies", w[6], 0, kHead / 2, 1}, bytes[0] / 4, 1);
     check_pool(c, spec[0], spec[1], w + 14, slots, kv_dim, bytes[3], bytes[4]);
@@ -191,13 +192,16 @@ struct Shape {
 inline std::string other_form(Op op, const std::string &symbol) {
   if (op == kLogits) return "logits_adjust_1024";
   if (op == kMerge) return "attention_paged_merge_8__128";
+  if (op == kAppend) return "kv_append_4" + symbol.substr(std::strlen("kv_append"));
   return symbol;
 }
 inline Shape shape(Op op, const uint32_t *spec, const uint32_t *w, uint32_t rows) {
   Shape s;
   s.groups[1] = rows;
   if (op == kAppend) {
-    s.groups[0] = (w[9] + 2 * w[10] + 3) / 4;  // one wave a head
+    const uint32_t heads = (w[9] + 2 * w[10] + 15) / 16;  // 16 heads a pass
+    s.form = (uint64_t)rows * heads >= kAppendMany;
+    s.groups[0] = s.form ? (heads + 3) / 4 : heads;
   } else if (op == kAttend) {
     const uint32_t q = rows * spec[0], groups = w[9] * w[11], own = rows * w[9] * w[12];
     const bool wide = w[11] && q > kNarrow;
