@@ -3,7 +3,7 @@
 //
 // Contract (bindings, push words; every grid is [1, rows, 1], and the runtime chooses the launch):
 //   kv_append              [W, A, C, KV, KV8]   24 words  spec [K_Q8, V_Q8, head_dim]
-//   attention_paged        [A, C, KV, KV8, KVS] 19 words  spec [N_REP, K_Q8, V_Q8, head_dim]
+//   attention_paged        [A, C, KV, KV8, KVS] 20 words  spec [N_REP, K_Q8, V_Q8, head_dim]
 //   attention_paged_merge  [A, C]               10 words  spec [head_dim]
 //   logits_adjust          [A, C]               12 words
 // Bindings as in attention.hip.  Heads are 128 wide.
@@ -40,7 +40,7 @@ struct AppendPush {
 struct PagedPush {
   uint32_t q_off, q_stride, o_off, o_stride, part_off, kc_off, vc_off, ks_off, vs_off, n_kv;
   float scale;
-  uint32_t n_shared, n_own, rows_off, table_off, table_stride, n_seq, n_pages, page_log2;
+  uint32_t n_shared, n_own, rows_off, table_off, table_stride, n_seq, n_pages, page_log2, wide;
 };
 struct PagedMergePush {
   uint32_t part_off, o_off, o_stride, n_head, n_shared, n_own, rows_off, table_stride, n_seq, page_log2;
@@ -867,7 +867,8 @@ union PagedShared {
 };
 template <int N_REP, int K8, int V8>
 SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_t *kv8, const PagedPush &p,
-                       uint32_t n_grid, uint32_t wide) {
+                       uint32_t n_grid) {
+  const bool wide = p.wide && p.n_shared;
   __shared__ __attribute__((aligned(1024))) PagedShared<K8, V8> st;
   const uint32_t t = threadIdx.x, wave = t >> 6, c = t & 15;
   const uint32_t n_rows = min(ctl[2], n_grid), slots = p.n_shared + p.n_own, groups = p.n_kv * p.n_shared;
@@ -971,9 +972,9 @@ APPEND(1, 1)
   extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))                  \
   void attention_paged__##R##_##K8##_##V8##_128(float *a, const uint32_t *ctl, const f16 *kv,           \
                                                 const int8_t *kv8, const f16 *kvs, PagedPush p,         \
-                                                uint32_t n_grid, uint32_t wide) {                       \
+                                                uint32_t n_grid) {                                      \
     (void)kvs;                                                                                         \
-    paged_body<R, K8, V8>(a, ctl, kv, kv8, p, n_grid, wide);                                           \
+    paged_body<R, K8, V8>(a, ctl, kv, kv8, p, n_grid);                                                 \
   }
 #define PAGED_REP(K8, V8) PAGED(1, K8, V8) PAGED(2, K8, V8) PAGED(4, K8, V8) PAGED(8, K8, V8)
 PAGED_REP(0, 0)
@@ -1105,12 +1106,21 @@ SK_DEV void logits_body(float *a, const uint32_t *ctl, const LogitsPush &p) {
       }
     };
     const uint32_t whole = n_hist & ~3u;
-    for (uint32_t i = 4 * t; i < whole; i += 4 * T) {
-      const uint4 h = *(const uint4 *)(hist + i);
-      use(i, h.x);
-      use(i + 1, h.y);
-      use(i + 2, h.z);
-      use(i + 3, h.w);
+    constexpr uint32_t U = 4;  // loads in flight
+    for (uint32_t i0 = 4 * t; i0 < whole; i0 += 4 * T * U) {
+      uint4 h[U];
+#pragma unroll
+      for (uint32_t k = 0; k < U; k++) h[k] = *(const uint4 *)(hist + min(i0 + 4 * T * k, whole - 4));
+#pragma unroll
+      for (uint32_t k = 0; k < U; k++) {
+        const uint32_t i = i0 + 4 * T * k;
+        if (i < whole) {
+          use(i, h[k].x);
+          use(i + 1, h[k].y);
+          use(i + 2, h[k].z);
+          use(i + 3, h[k].w);
+        }
+      }
     }
     if (whole + t < n_hist) use(whole + t, hist[whole + t]);
     __syncthreads();

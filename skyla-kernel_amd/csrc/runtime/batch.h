@@ -29,7 +29,6 @@ constexpr uint32_t kAppendMany = 2048;    // workgroups of 16 heads from which k
 constexpr uint32_t kMergeParts = 16;      // partials above which eight waves merge a head,
 constexpr uint32_t kMergeHeads = 1024;    // where there are fewer rows of heads than this
 constexpr uint32_t kLogitsWide = 512;     // workgroups of 4096 tokens from which a logits launch takes 16384 each
-constexpr uint32_t kNarrow = 32;          // query rows of a key head up to which the shared run takes 16 a workgroup
 constexpr uint32_t kMaxWork = 1u << 23;   // workgroups of an attention launch
 
 // [off, off + stride (rows - 1) + width) in elements
@@ -130,6 +129,7 @@ inline std::string refusal(Op op, const uint32_t *spec, const uint32_t *w, const
   } else if (op == kAttend) {
     const uint64_t a = bytes[0] / 4, n_kv = w[9], kv_dim = n_kv * kHead, n_head = n_kv * spec[0];
     const uint64_t parts = (uint64_t)w[11] + w[12];
+    c.need(w[19] <= 1, "the shared run takes 16 query rows a workgroup (0) or 128 (1)");
     c.need(n_kv >= 1 && n_kv <= 1024, "1 to 1024 key heads");
     c.need(w[12] >= 1 && parts <= kMaxSlots, "a row's own positions take 1 part or more, all of them at most 1024");
     if (!c.error.empty()) return c.error;
@@ -204,13 +204,12 @@ inline Shape shape(Op op, const uint32_t *spec, const uint32_t *w, uint32_t rows
     s.groups[0] = s.form ? (heads + 3) / 4 : heads;
   } else if (op == kAttend) {
     const uint32_t q = rows * spec[0], groups = w[9] * w[11], own = rows * w[9] * w[12];
-    const bool wide = w[11] && q > kNarrow;
-    if (wide)
+    if (w[19] && w[11])
       s.groups[0] = (groups + 7) / 8 * 8 * ((q + 127) / 128) + own;
     else
       s.groups[0] = groups * ((q + 15) / 16) + own;
     s.groups[1] = 1;
-    s.extra = {rows, wide};
+    s.extra = {rows};
   } else if (op == kMerge) {
     s.form = w[4] + w[5] > kMergeParts && rows * w[3] < kMergeHeads;
     s.groups[0] = s.form ? w[3] : (w[3] + 3) / 4;

@@ -196,7 +196,7 @@ const KernelInfo kKernels[] = {
     {"embed", 4, 8, 1, 1, -1, false, false},  // token rows from the HBM token_embd (util.hip)
     // a served batch (kernels/batch.hip): grids of [1, rows, 1]
     {"kv_append", 5, 24, 3, 3, -1, false, false},
-    {"attention_paged", 5, 19, 4, 4, -1, false, false},
+    {"attention_paged", 5, 20, 4, 4, -1, false, false},
     {"attention_paged_merge", 2, 10, 1, 1, -1, false, false},
     {"logits_adjust", 2, 12, 0, 0, -1, false, false},
 };

@@ -17,14 +17,13 @@ kernels/batch.hip.
 from __future__ import annotations
 
 import dataclasses
-from typing import Sequence
+from typing import NamedTuple, Sequence
 
 import numpy as np
 
 from . import engine as E
 from .abi import Buffer, Context, Recorder
 
-NARROW = 32             # query rows of a key head up to which the shared run takes 16 a workgroup (runtime/batch.h)
 MAX_PARTS = 1024        # partials of a row and head (runtime/batch.h)
 PAGE_SIZES = tuple(16 << i for i in range(9))  # 16 to 4096 positions
 CTL_ROWS, CTL_SHARED, CTL_LEADER = 2, 3, 4     # control words: live rows, shared positions, their sequence
@@ -73,25 +72,39 @@ class LogitsRegions:
     mask_stride: int = 0
 
 
-def splits(rows: int, n_kv: int, rep: int, shared: int, own: int) -> tuple[int, int]:
-    """Parts that a batch's attention cuts the shared run and each row's own run into, for
-    `shared` shared positions and at most `own` of a row's own: enough workgroups to fill the
-    GPU, each with some tiles of 64 positions."""
-    q, tiles = rows * rep, -(-shared // 64)
+class Parts(NamedTuple):
+    """The pieces that a batch's attention cuts the shared run (0: none is shared, whatever the rows
+    say) and each row's own run into, and whether the shared run takes 128 query rows a workgroup
+    (else 16)."""
+    shared: int
+    own: int
+    wide: bool = False
+
+
+def splits(rows: int, n_kv: int, rep: int, shared: int, own: int) -> Parts:
+    """Parts for `shared` shared positions and at most `own` of a row's own: enough workgroups to
+    fill the GPU's 256 compute units, each with some tiles of 64 positions.
+
+    128 query rows a workgroup stage keys and values once for all of them and pay for it at the
+    start: us of the shared run, 16 rows / 128 rows a workgroup (8 key heads, f16 keys, 8-bit values),
+    64 query rows a key head over 500 positions 12.0 / 15.2, 8192 25.4 / 25.3, 32768 62 / 63; 128 over 500
+    12.2 / 16.4, 2000 19.2 / 18.3, 8192 37 / 29; 256 over 500 14.9 / 17.1, 2000 28 / 21."""
+    q, tiles, own_tiles = rows * rep, -(-shared // 64), -(-own // 64)
+    n_own = max(1, min(-(-1024 // (n_kv * rows)), -(-own_tiles // 4), 128))
     if shared == 0:
-        n_shared = 0
-    elif q > NARROW:  # workgroups of 128 query rows: one a compute unit, two where a part stays long
+        return Parts(0, n_own)
+    if q > 64 and q * shared > 160 * 1024:
+        # one workgroup a compute unit, two where a part stays long: 512 query rows of 8 key heads over
+        # 32768 positions 157 / 144 us with the merge, of 4 over 8192 56 / 71, of 8 over 4000 51 / 58
         groups = n_kv * -(-q // 128)
-        n_shared = min(-(-(512 if shared * groups >= 1024 * 512 else 256) // groups), -(-tiles // 2))
-    else:             # 16 query rows and four waves each
-        n_shared = min(-(-512 // (n_kv * -(-q // 16))), -(-tiles // 4))
-    tiles = -(-own // 64)
-    return min(n_shared, 128), max(1, min(-(-512 // (n_kv * rows)), -(-tiles // 4), 128))
+        n = -(-(512 if shared * groups >= 1024 * 512 else 256) // groups)
+        return Parts(min(n, -(-tiles // 2), 128), n_own, True)
+    return Parts(min(-(-512 // (n_kv * -(-q // 16))), -(-tiles // 4), 128), n_own)
 
 
-def part_size(rows: int, n_head: int, parts: tuple[int, int]) -> int:
+def part_size(rows: int, n_head: int, parts) -> int:
     """Words of the partials' region."""
-    return rows * n_head * sum(parts) * 130
+    return rows * n_head * (parts[0] + parts[1]) * 130
 
 
 class BatchKernels:
@@ -114,7 +127,7 @@ class BatchKernels:
             return p
 
         self._append = build("kv_append", [tables, a, a], 24, [k8, v8, 128])
-        self._attend = build("attention_paged", [a, a], 19, [c.n_head // c.n_head_kv, k8, v8, 128])
+        self._attend = build("attention_paged", [a, a], 20, [c.n_head // c.n_head_kv, k8, v8, 128])
         self._merge = ctx.create_pipeline("attention_paged_merge", 2, 40, [128])
         self._merge.bind_buffers([a, a])
 
@@ -132,20 +145,19 @@ class BatchKernels:
                 at.rows, at.table, *self._pages()]
         r.dispatch_set(self._append, layer, [1, rows, 1], push)
 
-    def attend(self, r: Recorder, layer: int, at: BatchRegions, q, out, rows: int, parts: tuple[int, int]) -> None:
-        """Attention of rows of rotated q ((offset, stride)) over layer's pool into out.  `parts`:
-        how many pieces the shared positions (0: none are shared, whatever the rows say) and a
-        row's own are cut into (splits); at.part holds part_size words."""
-        c, kv = self.c, self.paged.layout
+    def attend(self, r: Recorder, layer: int, at: BatchRegions, q, out, rows: int, parts) -> None:
+        """Attention of rows of rotated q ((offset, stride)) over layer's pool into out, in `parts`
+        (splits); at.part holds part_size words."""
+        c, kv, parts = self.c, self.paged.layout, Parts(*parts)
         scale = np.float32(1.0) / np.sqrt(np.float32(c.head_dim))
         push = [q[0], q[1], out[0], out[1], at.part, kv.keys(0), kv.values(0), kv.key_scales(0), kv.value_scales(0),
-                c.n_head_kv, E.f32_bits(scale), *parts, at.rows, at.table, *self._pages()]
+                c.n_head_kv, E.f32_bits(scale), parts.shared, parts.own, at.rows, at.table, *self._pages(), parts.wide]
         r.dispatch_set(self._attend, layer, [1, rows, 1], push)
-        if sum(parts) == 1:  # nothing to merge: the rows are the result
+        if parts.shared + parts.own == 1:  # nothing to merge: the rows are the result
             return
         r.barrier()
-        push = [at.part, out[0], out[1], c.n_head, *parts, at.rows, self.paged.seq_pages, self.paged.n_seq,
-                self.paged.page_log2]
+        push = [at.part, out[0], out[1], c.n_head, parts.shared, parts.own, at.rows, self.paged.seq_pages,
+                self.paged.n_seq, self.paged.page_log2]
         r.dispatch(self._merge, [1, rows, 1], push)
 
     def free(self) -> None:
@@ -196,7 +208,7 @@ class _Sequence:
 class _BatchGraph(E.Graph):
     """A layer's dispatches with the batch's cache in place of the contiguous one."""
 
-    def __init__(self, r: Recorder, eng: "BatchEngine", batched: bool, rows: int, parts: tuple[int, int]):
+    def __init__(self, r: Recorder, eng: "BatchEngine", batched: bool, rows: int, parts: Parts):
         super().__init__(r, eng.kernels, eng.arena, eng.c, batched)
         self.eng, self.rows, self.parts = eng, rows, parts
 
@@ -410,7 +422,7 @@ class BatchEngine:
             out.append(min(2 * out[-1], most))
         return out
 
-    def _parts(self, rows: int, shared: int, own: int) -> tuple[int, int]:
+    def _parts(self, rows: int, shared: int, own: int) -> Parts:
         return splits(rows, self.c.n_head_kv, self.rep, shared, own)
 
     def _recording(self, rows: int, shared: int, own: int, head: bool):
@@ -424,7 +436,7 @@ class BatchEngine:
             self.recordings[key] = self.ctx.record(False, lambda r: self._record(r, rows, parts, head))
         return self.recordings[key]
 
-    def _record(self, r: Recorder, rows: int, parts: tuple[int, int], head: bool) -> None:
+    def _record(self, r: Recorder, rows: int, parts: Parts, head: bool) -> None:
         a, w, c, batched = self.arena, self.weights, self.c, rows > 1
         g = _BatchGraph(r, self, batched, rows, parts)
         g.embed(w.embd)

@@ -22,7 +22,7 @@ class Batch:
     """A pool and an arena for `rows` rows, with what the tests write and read in numpy."""
 
     def __init__(self, ctx, precision, n_kv, rep, page, lens, seqs=None, shares=None, shared=0, leader=0, n_seq=None,
-                 n_pages=None, parts=None, grid=None, seed=0):
+                 n_pages=None, parts=None, grid=None, seed=0, wide=None):
         g = self.g = np.random.default_rng(seed)
         self.ctx, self.lens, self.rows = ctx, np.asarray(lens), len(lens)
         self.n_kv, self.rep, self.n_head, self.dim = n_kv, rep, n_kv * rep, n_kv * 128
@@ -49,7 +49,9 @@ class Batch:
         c = self.c = E.Config(n_embd=256, n_head=self.n_head, n_head_kv=n_kv, eps=EPS, rope_theta=THETA)
         self.grid = grid or self.rows
         own = int((self.lens - np.where((self.shares > 0) & (self.lens >= shared), shared, 0)).max(initial=1))
-        self.parts = parts or B.splits(self.grid, n_kv, rep, shared, max(1, own))
+        self.parts = B.Parts(*(parts or B.splits(self.grid, n_kv, rep, shared, max(1, own))))
+        if wide is not None:
+            self.parts = self.parts._replace(wide=wide)
         size = 64
 
         def room(n):
@@ -190,9 +192,10 @@ def test_attention_of_rows_of_their_own(ctx, precision, heads, lens, page):
 
 
 @pytest.mark.parametrize("precision", list(P))
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("heads", [(2, 1), (2, 2), (1, 4), (2, 8)])
 @pytest.mark.parametrize("shared,page,n", [(1, 16, 2), (37, 16, 5), (64, 64, 17), (1000, 64, 9), (129, 32, 33)])
-def test_attention_with_shared_positions(ctx, precision, heads, shared, page, n):
+def test_attention_with_shared_positions(ctx, precision, wide, heads, shared, page, n):
     """Rows behind a shared run: one idle, one that shares nothing though it is longer, one shorter
     than the run, one that is the run and no more."""
     g = np.random.default_rng(shared + n)
@@ -202,7 +205,8 @@ def test_attention_with_shared_positions(ctx, precision, heads, shared, page, n)
         lens[0], lens[3], lens[4] = 0, max(1, shared // 2), shared
         shares[2] = 0
     leader = 1 if n > 4 else 0
-    b = Batch(ctx, P[precision], *heads, page, lens, shares=shares, shared=shared, leader=leader, seed=shared)
+    b = Batch(ctx, P[precision], *heads, page, lens, shares=shares, shared=shared, leader=leader, seed=shared,
+              wide=wide)
     try:
         b.fill()
         b.copy_shared()
@@ -213,11 +217,13 @@ def test_attention_with_shared_positions(ctx, precision, heads, shared, page, n)
 
 
 @pytest.mark.parametrize("precision", list(P))
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("shared,n", [(0, 19), (100, 40), (640, 128)])
-def test_attention_of_a_prompt_chunk(ctx, precision, shared, n):
+def test_attention_of_a_prompt_chunk(ctx, precision, wide, shared, n):
     """Rows of one sequence at consecutive positions: the run before them shared, each row its own end."""
     lens = shared + 1 + np.arange(n)
-    b = Batch(ctx, P[precision], 2, 4, 64, lens, seqs=np.zeros(n, int), shares=np.full(n, shared), shared=shared)
+    b = Batch(ctx, P[precision], 2, 4, 64, lens, seqs=np.zeros(n, int), shares=np.full(n, shared), shared=shared,
+              wide=wide)
     try:
         b.fill()
         b.rows_of(b.q, b.sq, b.n_head * 128)[:] = b.g.standard_normal((b.rows, b.n_head * 128))
@@ -227,7 +233,7 @@ def test_attention_of_a_prompt_chunk(ctx, precision, shared, n):
 
 
 @pytest.mark.parametrize("precision", list(P))
-@pytest.mark.parametrize("parts", [(1, 1), (3, 2), (64, 40), (0, 5)])
+@pytest.mark.parametrize("parts", [(1, 1), (3, 2), (64, 40), (0, 5), (1, 1, True), (3, 2, True), (21, 1, True), (0, 1)])
 def test_attention_parts(ctx, precision, parts):
     """Any number of parts gives the same attention, and none for the shared run leaves it to the rows."""
     lens = [2900, 1290, 1287, 1300]
@@ -245,11 +251,12 @@ def test_attention_parts(ctx, precision, parts):
 
 @pytest.mark.parametrize("precision", list(P))
 @pytest.mark.parametrize("bad", [np.nan, np.inf])
-def test_attention_keeps_out_what_lies_outside_a_row(ctx, precision, bad):
+@pytest.mark.parametrize("wide", [False, True])
+def test_attention_keeps_out_what_lies_outside_a_row(ctx, precision, bad, wide):
     """Everything but the rows' live positions is NaN or infinite: unused slots, the rest of a last
     page, the slots of a sequence's own page under the shared run."""
     lens, shared = [70, 45, 41, 100], 40
-    b = Batch(ctx, P[precision], 2, 2, 32, lens, shares=[40] * 4, shared=shared, leader=2)
+    b = Batch(ctx, P[precision], 2, 2, 32, lens, shares=[40] * 4, shared=shared, leader=2, wide=wide)
     try:
         b.fill()
         live = set(b.slots(2, shared).tolist())

@@ -63,7 +63,7 @@ def _append(**over):
 
 def _attend(**over):
     w = dict(q=64, qs=512, o=4096, os=512, part=8192, kc=0, vc=SLOTS * KV_DIM * 2, ks=0, vs=SLOTS * KV_DIM * 3 // 2,
-             n_kv=2, scale=0, n_shared=1, n_own=2, rows=20000, table=20100, ts=4, n_seq=3, n_pages=8, log2=5)
+             n_kv=2, scale=0, n_shared=1, n_own=2, rows=20000, table=20100, ts=4, n_seq=3, n_pages=8, log2=5, wide=0)
     assert not set(over) - set(w)
     return list((w | over).values())
 
@@ -94,7 +94,7 @@ def test_attention_words(host):
     for bad in (dict(q=A // 4), dict(q=65), dict(qs=510), dict(o=4097), dict(part=8193), dict(part=A // 4 - 100), dict(part=4096),
                 dict(part=512), dict(part=19000), dict(n_own=0), dict(n_own=1025), dict(n_shared=1024), dict(n_shared=2**32 - 1),
                 dict(n_kv=0), dict(n_kv=3), dict(n_kv=2**31), dict(kc=8), dict(ks=2, n_pages=9), dict(vs=2), dict(table=2**32 - 1),
-                dict(n_seq=0), dict(ts=2**31), dict(log2=2), dict(o=68), dict(os=516, o=64), dict(o=20000), dict(o=19900)):
+                dict(n_seq=0), dict(ts=2**31), dict(log2=2), dict(wide=2), dict(o=68), dict(os=516, o=64), dict(o=20000), dict(o=19900)):
         assert ok(**bad), bad
     assert ok(rows=65535)  # the partials end past the arena
     # 8-bit keys: the key rows and their scales in bytes and halves
@@ -144,7 +144,8 @@ def test_pages_and_parts():
         for shared in (0, 1, 64, 100000):
             for own in (1, 65, 20000):
                 for n_kv, rep in ((1, 1), (8, 4), (4, 8)):
-                    s, o = B.splits(rows, n_kv, rep, shared, own)
+                    s, o, wide = B.splits(rows, n_kv, rep, shared, own)
+                    assert not wide or shared
                     assert (s == 0) == (shared == 0) and o >= 1 and s + o <= B.MAX_PARTS
                     assert s <= max(1, -(-shared // 64)) and o <= max(1, -(-own // 64))
     assert B.part_size(3, 8, (2, 5)) == 3 * 8 * 7 * 130
