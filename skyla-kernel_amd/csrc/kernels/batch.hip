@@ -91,7 +91,7 @@ SK_DEV Split split_of(uint32_t lo, uint32_t hi, uint32_t n) {
   Split s;
   s.base = lo & ~15u;
   s.tiles = hi > lo ? (hi - s.base + TILE - 1) / TILE : 0;
-  s.per = s.tiles ? (s.tiles + n - 1) / n : 1;
+  s.per = max((s.tiles + n - 1) / n, 1u);
   return s;
 }
 SK_DEV uint32_t live_parts(const Split &s) { return (s.tiles + s.per - 1) / s.per; }
@@ -1139,7 +1139,7 @@ SK_DEV void logits_body(float *a, const uint32_t *ctl, const LogitsPush &p) {
       if (!((bits[k] >> j) & 1)) w[j] = -INFINITY;
     }
     if (i + 4 <= n) {
-      *(float4 *)(y + i) = make_float4(w[0], w[1], w[2], w[3]);
+      __builtin_nontemporal_store(f32x4{w[0], w[1], w[2], w[3]}, (f32x4 *)(y + i));
     } else if (i < n) {
       y[i] = w[0];
       if (i + 1 < n) y[i + 1] = w[1];

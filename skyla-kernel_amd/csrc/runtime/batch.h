@@ -28,7 +28,8 @@ constexpr uint32_t kMaxGrid = 65535;      // rows of a dispatch
 constexpr uint32_t kAppendMany = 2048;    // workgroups of 16 heads from which kv_append takes 64 each
 constexpr uint32_t kMergeParts = 16;      // partials above which eight waves merge a head,
 constexpr uint32_t kMergeHeads = 1024;    // where there are fewer rows of heads than this
-constexpr uint32_t kLogitsWide = 512;     // workgroups of 4096 tokens from which a logits launch takes 16384 each
+constexpr uint32_t kLogitsWide = 512;     // workgroups of 4096 tokens from which a logits launch takes 16384 each,
+constexpr uint32_t kLogitsHistory = 8192; // where each of them reads a history as long as this
 constexpr uint32_t kMaxWork = 1u << 23;   // workgroups of an attention launch
 
 // [off, off + stride (rows - 1) + width) in elements
@@ -138,6 +139,7 @@ inline std::string refusal(Op op, const uint32_t *spec, const uint32_t *w, const
     const Region words{"the rows' words", w[13], 4, 4, rows}, table{"the page table", w[14], 0, (uint64_t)w[16] * w[15], 1};
     check_pages(c, words, table, bytes[1] / 4, w[18], w[17]);
     c.need(w[15] >= 1 && w[16] >= 1, "the page table is empty");
+    c.need(w[15] <= w[17], "a sequence has more pages than the pool");  // bounds every length, and so every loop
     if (!c.error.empty()) return c.error;
     const uint64_t slots = (uint64_t)w[17] << w[18];
     c.holds(q, a, 4);
@@ -215,7 +217,7 @@ inline Shape shape(Op op, const uint32_t *spec, const uint32_t *w, uint32_t rows
     s.groups[0] = s.form ? w[3] : (w[3] + 3) / 4;
     s.threads = s.form ? 512 : 256;
   } else {
-    s.form = (uint64_t)rows * ((w[4] + 4095) / 4096) >= kLogitsWide;
+    s.form = (uint64_t)rows * ((w[4] + 4095) / 4096) >= kLogitsWide && w[7] >= kLogitsHistory;
     s.threads = s.form ? 1024 : 256;
     s.groups[0] = (w[4] + 16 * s.threads - 1) / (16 * s.threads);
   }

@@ -90,7 +90,9 @@ def splits(rows: int, n_kv: int, rep: int, shared: int, own: int) -> Parts:
     64 query rows a key head over 500 positions 12.0 / 15.2, 8192 25.4 / 25.3, 32768 62 / 63; 128 over 500
     12.2 / 16.4, 2000 19.2 / 18.3, 8192 37 / 29; 256 over 500 14.9 / 17.1, 2000 28 / 21."""
     q, tiles, own_tiles = rows * rep, -(-shared // 64), -(-own // 64)
-    n_own = max(1, min(-(-1024 // (n_kv * rows)), -(-own_tiles // 4), 128))
+    # (a workgroup without a run costs as much as a short one: 128 rows of 8 key heads in 1 / 2 / 4 parts
+    # 27 / 31 / 47 us; one row of 16384 positions in 16 / 32 / 64 20.2 / 15.3 / 16.1)
+    n_own = max(1, min(-(-512 // (n_kv * rows)), -(-own_tiles // 4), 128))
     if shared == 0:
         return Parts(0, n_own)
     if q > 64 and q * shared > 160 * 1024:
@@ -243,7 +245,8 @@ class BatchEngine:
         if max_ctx < 1:
             raise ValueError(f"max_ctx {max_ctx}")
         self.ctx, self.c, self.max_ctx, self.max_seq = ctx, c, max_ctx, max_seq
-        self.paged = Paged(precision, page, n_pages, max_seq, -(-max_ctx // page), c.n_head_kv * c.head_dim)
+        self.paged = Paged(precision, page, n_pages, max_seq, min(-(-max_ctx // page), n_pages),
+                           c.n_head_kv * c.head_dim)
         if self.paged.bytes() > ctx.max_buffer():
             raise ValueError(f"a layer's pool of {n_pages} pages needs {self.paged.bytes() >> 20} MiB, above the "
                              "allocation cap")

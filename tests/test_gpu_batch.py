@@ -4,6 +4,7 @@ end inside a page and a tile, and rows that do not share them."""
 import numpy as np
 import pytest
 
+from helpers import tactics
 from skyla_hip import batch as B
 from skyla_hip import engine as E
 from skyla_hip.abi import SkylaHipError
@@ -500,3 +501,127 @@ def test_refused_words(ctx):
             assert e.value.code == -1 and "attention_paged" in e.value.message
     finally:
         b.free()
+
+
+# ---- together, as a decode step runs them ------------------------------------------------------
+@pytest.mark.parametrize("precision", list(P))
+def test_a_recorded_step_replayed(ctx, precision):
+    """Append and attend of four layers (here the same pool) as one HIP graph, replayed as the
+    sequences grow, pages are handed out and rows fall idle, against direct launches: the same
+    bits; and against 64 bits."""
+    b = Batch(ctx, P[precision], 2, 4, 16, [40, 33, 90, 70, 1], shares=[32] * 5, shared=32, parts=(2, 3, True), n_pages=60)
+    try:
+        g, f, u = b.g, b.arena.as_f32(), b.arena.as_u32()
+        b.fill()
+        b.copy_shared()
+        qn, kn, rope = b.norms
+        for n in (qn, kn):
+            f[n: n + 128] = g.uniform(0.5, 1.5, 128)
+        f[rope: rope + 64] = THETA ** (-2.0 * np.arange(64) / 128)
+        b.arena.upload()
+        b.pool.upload()
+
+        def body(r):
+            for _ in range(4):
+                b.kernels.append(r, 0, b.at, (b.q, b.sq), (b.k, b.skv), b.v, (b.q, b.sq), qn, kn, rope, b.grid)
+                r.barrier()
+                b.kernels.attend(r, 0, b.at, (b.q, b.sq), (b.out, b.sq), b.grid, b.parts)
+                r.barrier()
+        with tactics(nograph="0"):
+            graph = ctx.record(False, body)
+        with tactics(nograph="1"):
+            direct = ctx.record(False, body)
+        assert graph.launches() == 12
+        for step in range(5):
+            lens = b.lens + step
+            lens[step % 4] = 0 if step else lens[0]
+            u[b.at.rows + 1: b.at.rows + 4 * b.rows: 4] = lens
+            x = [g.standard_normal((b.rows, w)).astype(np.float32) for w in (b.n_head * 128, b.dim, b.dim)]
+            outs = []
+            for rec in (direct, graph):
+                for (off, stride), rows in zip(((b.q, b.sq), (b.k, b.skv), (b.v, b.skv)), x):
+                    b.rows_of(off, stride, rows.shape[1])[:] = rows
+                b.arena.upload()
+                ctx.replay(rec)
+                b.arena.download()
+                outs.append((b.rows_of(b.out, b.sq, b.n_head * 128).copy(), b.rows_of(b.q, b.sq, b.n_head * 128).copy()))
+            assert np.array_equal(*[o[0] for o in outs]) and np.array_equal(*[o[1] for o in outs])
+            b.pool.download()
+            keep, b.lens = b.lens, lens
+            want = b.want().reshape(b.rows, -1)
+            b.lens = keep
+            for r in range(b.rows):
+                assert np.linalg.norm(outs[0][0][r] - want[r]) <= BAR * np.linalg.norm(want[r]), (step, r)
+        graph.free()
+        direct.free()
+    finally:
+        b.free()
+
+
+@pytest.mark.parametrize("precision", list(P))
+@pytest.mark.parametrize("wide", [False, True])
+def test_pages_at_the_end_of_a_large_pool(ctx, precision, wide):
+    """A pool of nearly 4 GiB, the sequences in its last pages: the bits of the same rows in a small
+    pool (offsets past 2^31 entries and bytes)."""
+    n_kv, page = 8, 4096
+    bits = P[precision]
+    per = sum((n_kv * 128 + n_kv * 8) if q8 else 2 * n_kv * 128 for q8 in (bits.keys_q8, bits.values_q8))
+    far = (4 << 30) // (per * page)
+    lens, shares = [130, 4200, 200], [100] * 3
+    small = Batch(ctx, bits, n_kv, 2, page, lens, shares=shares, shared=100, parts=(1, 1, wide), n_pages=6, seed=4)
+    big = Batch(ctx, bits, n_kv, 2, page, lens, shares=shares, shared=100, parts=(1, 1, wide), n_pages=far, seed=4)
+    try:
+        assert small.table.max() < 6
+        small.fill()
+        small.copy_shared()
+        q = small.g.standard_normal((3, small.n_head * 128)).astype(np.float32)
+        k, v = (small.g.standard_normal((3, small.dim)).astype(np.float32) for _ in range(2))
+        small.pool.upload()
+        # page i of the small pool lies in page far - 6 + i of the large one
+        for off, sc, q8 in (("keys", "key_scales", bits.keys_q8), ("values", "value_scales", bits.values_q8)):
+            for name, size, width in ((off, 1 if q8 else 2, small.dim), (sc, 2, small.dim // 32)) if q8 else ((off, 2, small.dim),):
+                a, z = (getattr(x.paged.layout, name)(0) * size for x in (small, big))
+                n = page * width * size
+                big.pool.copy_from(z + (far - 6) * n, small.pool, a, 6 * n)
+        outs = []
+        for b, first in ((small, 0), (big, far - 6)):
+            f, u = b.arena.as_f32(), b.arena.as_u32()
+            u[b.at.table: b.at.table + b.table.size] = small.table.ravel() + first
+            qn, kn, rope = b.norms
+            f[qn: qn + 128] = f[kn: kn + 128] = 1.25
+            f[rope: rope + 64] = 0.01
+            b.rows_of(b.q, b.sq, q.shape[1])[:] = q
+            b.rows_of(b.k, b.skv, b.dim)[:] = k
+            b.rows_of(b.v, b.skv, b.dim)[:] = v
+            b.arena.upload()
+
+            def body(r, b=b):
+                b.kernels.append(r, 0, b.at, (b.q, b.sq), (b.k, b.skv), b.v, (b.q, b.sq), qn, kn, rope, 3)
+                r.barrier()
+                b.kernels.attend(r, 0, b.at, (b.q, b.sq), (b.out, b.sq), 3, b.parts)
+            rec = ctx.record(False, body)
+            ctx.replay(rec)
+            rec.free()
+            b.arena.download()
+            outs.append(b.rows_of(b.out, b.sq, b.n_head * 128).copy())
+        assert np.isfinite(outs[0]).all() and np.array_equal(*outs)
+    finally:
+        small.free()
+        big.free()
+
+
+def test_attention_in_place(ctx):
+    """The output over the queries, with one part (written by the attention) and with several."""
+    for parts in ((0, 1), (1, 1, True), (1, 2)):
+        b = Batch(ctx, P["f16k_q8v"], 2, 4, 32, [60, 45, 0, 130], shares=[40] * 4, shared=40, parts=parts)
+        try:
+            b.fill()
+            b.copy_shared()
+            b.rows_of(b.q, b.sq, b.n_head * 128)[:] = b.g.standard_normal((b.rows, b.n_head * 128))
+            want = b.want()
+            b.run(lambda r: b.kernels.attend(r, 0, b.at, (b.q, b.sq), (b.q, b.sq), b.grid, b.parts))
+            got = b.rows_of(b.q, b.sq, b.n_head * 128).astype(np.float64).reshape(want.shape)
+            for r in range(b.rows):
+                assert np.linalg.norm(got[r] - want[r]) <= BAR * np.linalg.norm(want[r]), (parts, r)
+        finally:
+            b.free()

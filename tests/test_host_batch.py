@@ -94,7 +94,7 @@ def test_attention_words(host):
     for bad in (dict(q=A // 4), dict(q=65), dict(qs=510), dict(o=4097), dict(part=8193), dict(part=A // 4 - 100), dict(part=4096),
                 dict(part=512), dict(part=19000), dict(n_own=0), dict(n_own=1025), dict(n_shared=1024), dict(n_shared=2**32 - 1),
                 dict(n_kv=0), dict(n_kv=3), dict(n_kv=2**31), dict(kc=8), dict(ks=2, n_pages=9), dict(vs=2), dict(table=2**32 - 1),
-                dict(n_seq=0), dict(ts=2**31), dict(log2=2), dict(wide=2), dict(o=68), dict(os=516, o=64), dict(o=20000), dict(o=19900)):
+                dict(n_seq=0), dict(ts=9), dict(ts=2**31), dict(log2=2), dict(wide=2), dict(o=68), dict(os=516, o=64), dict(o=20000), dict(o=19900)):
         assert ok(**bad), bad
     assert ok(rows=65535)  # the partials end past the arena
     # 8-bit keys: the key rows and their scales in bytes and halves
