@@ -87,7 +87,10 @@ int skyla_hip_buffer_copy(skyla_hip_buffer *dst, uint64_t dst_off, const skyla_h
 
 /* Context::create_pipeline_sets(shader, n_buffers, push_size, spec, n_sets).
  * `name` is the reference shader name (matvec_q4k, matvec_q6k, matvec_q8_0, matmul,
- * moe_logits, moe_route, moe_sort, moe_combine, silu_mul, to_half, bandwidth).  The
+ * moe_logits, moe_route, moe_sort, moe_combine, silu_mul, to_half, bandwidth), or one of a
+ * served batch's, which the reference lacks: kv_append, attention_paged,
+ * attention_paged_merge, logits_adjust.  Their push words and grid are checked against the
+ * bound buffers when they are dispatched (SKYLA_HIP_E_ARG).  The
  * kernel is the gfx950 instantiation for `spec`; an unknown (name, spec) fails with
  * SKYLA_HIP_E_NO_KERNEL, as a shader that does not compile fails pipeline creation.
  * n_buffers and push_size must match the kernel's bindings and push struct.
@@ -134,7 +137,8 @@ uint32_t skyla_hip_recording_len(const skyla_hip_recording *rec);
  * (at most 4; environment SKYLA_HIP_FUSE=0 turns this off).  Profilers see launches. */
 uint32_t skyla_hip_recording_launches(const skyla_hip_recording *rec);
 
-/* Context::replay: run the recording (as one HIP graph) and wait for it. */
+/* Context::replay: run the recording (as one HIP graph, or, one of at most six launches, as
+ * those launches) and wait for it. */
 int skyla_hip_replay(skyla_hip_context *ctx, const skyla_hip_recording *rec);
 /* Replay and report the device time between its first and last work, in ns, measured
  * with HIP events on the context stream. */

@@ -20,6 +20,8 @@
 // Words that name no page or sequence reach no memory outside the pool: a row of such a sequence
 // counts as one of len 0, a length past the table's ends there, keys and values of such a page
 // are not stored, and a read of it goes to the pool's last page.
+// Keys and values are finite (kv_append stores no others but NaN): a row that attends to a NaN or an
+// infinity is not finite where that reaches, and what a row does not attend to reaches nothing.
 #include <type_traits>
 
 #include "matmul_common.h"
@@ -131,7 +133,10 @@ SK_DEV void store_row(f16 *kv, int8_t *kv8, uint32_t cache, uint32_t scales, uin
 // row, every load in flight before the first product.  The angle (len - 1) f_d is formed in 64
 // bits as revolutions and reduced there: an f32 product is off by 2^-24 of an angle of 1e5, 3e-3
 // of a radian.  Each wave turns its row's 64 angles once, one a lane, for all its heads.
-// 16 bytes a lane and load: with 4 (a wave a head) 2048 rows of 48 heads ran 79 us from HBM.
+// Measured (MI355X): 2048 rows of 48 heads, f16 keys and 8-bit values, 34 us from HBM (90 MB, 2.6
+// TB/s; 18 us from the caches), 79 with a wave a head and 4 bytes a lane and load: bound by the bytes
+// in flight.  PASSES = 4 from 2048 workgroups of one pass on (1000 rows 10.6 us against 13.1), below
+// it more workgroups are better (1 row 2.5 us: the launch and two dependent round trips).
 template <int K8, int V8, int PASSES>
 SK_DEV void append_body(const float *w, float *a, const uint32_t *ctl, f16 *kv, int8_t *kv8, const AppendPush &p) {
 #pragma clang fp contract(off)
@@ -202,8 +207,10 @@ SK_DEV void append_body(const float *w, float *a, const uint32_t *ctl, f16 *kv, 
 // What both forms of the attention share.  A query row is held as two f16 parts of q scale log2(e)
 // 2^sh (22 bits of its largest value; a product with an f16 key is exact), scores are in powers of
 // two.  The largest score is followed loosely: the sums are scaled down only where a score passes
-// the reference m by 2^LOOSE.  e = 2^(score - m) is held times 2^(15 - LOOSE), so that it stays in
-// f16's range, as two f16 parts (21 bits from 2^-14 of it on).
+// the reference m by LOOSE.  e = 2^(score - m) is held times 2^E_SHIFT = 2^(15 - LOOSE), so that it
+// stays in f16's range, as two f16 parts cut off (21 bits of it, 2^-31 of the row's largest e at
+// least); products are f16 by f16 with f32 sums, each value by both parts.  One part of either
+// would halve the products and cost 2^-12 of a result, 50 times what f32 loses.
 constexpr float LOOSE = 8.0f;
 constexpr int E_SHIFT = 7;
 SK_DEV int query_shift(float big) { return big > 0.0f && big < INFINITY ? 11 - __builtin_amdgcn_frexp_expf(big) : 0; }
@@ -244,8 +251,9 @@ SK_DEV Pages pages_of(const uint32_t *ctl, const PagedPush &p, uint32_t seq) {
 }
 
 // A run of positions [begin, end) through one wave, for 16 query rows (this lane's, row c = lane %
-// 16, at q); row c's partial goes to out[c].  Of the positions those in [lo, hi) count.  A step takes HALF = 32 positions, two groups of 16; the next
-// step's rows are in flight while one is computed.  Nothing passes through LDS:
+// 16, at q); row c's partial goes to out[c].  Of the positions those in [lo, hi) count.  A step
+// takes HALF = 32 positions, two groups of 16; the next step's rows are in flight while one is
+// computed.  No row of the cache passes through LDS:
 //   S^T = K Q^T   v_mfma_f32_16x16x32_f16, A = key rows as loaded (row: position 16 t + c, dims 8 g +
 //                 32 k, g = lane / 16), B = query rows; a lane then has row c's scores at 16 t + 4 g + r
 //   O^T = V^T P^T B = those weights: element e of group g is position 16 (e / 4) + 4 g + e % 4; A =
@@ -254,6 +262,11 @@ SK_DEV Pages pages_of(const uint32_t *ctl, const PagedPush &p, uint32_t seq) {
 // Loads of positions outside [lo, hi) go to ones inside, and their scores are -inf, so what lies
 // there reaches nothing.  8-bit values are two f16 parts of q s 2^(4 - ve), ve the exponent of the
 // largest scale of the 32 dims, followed as loosely.
+// Measured (MI355X, with the waves' join): one row of 16384 positions of 8 key heads, f16 keys and
+// 8-bit values, 15.5 us (50 MB, 3.2 TB/s); 128 rows of up to 512 own positions in f16 28 us (135 MB,
+// 4.8 TB/s, what a copy reaches); 8 rows of up to 100 positions 5.9 us.  Bound by HBM where rows are
+// many, by a workgroup's dependent round trips (control words, row words, page numbers, rows) where
+// runs are short.  Without the step in flight the first ran 24 us.
 constexpr uint32_t HALF = 32;
 template <int K8, int V8>
 struct HalfRows {
@@ -489,8 +502,14 @@ SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
 // With f16 keys a step multiplies the next step's scores while it makes this one's e, so that the
 // matrix pipe and the vector ALU work side by side in one wave; reads from LDS run two products
 // ahead.  (8-bit keys' block sums leave no registers for a second step's scores.)
-// 8-bit values are held as two f16 parts of q s 2^(7 - ve), ve the exponent of the
-// part's largest scale of the 32 dims, found first.
+// 8-bit values are held as two f16 parts of q s 2^(7 - ve), ve the exponent of the part's largest
+// scale of the 32 dims, found first.
+// Measured (MI355X): 128 rows of 32 heads over 32768 positions of 8 key heads, f16: 134 us, 137 GFLOP
+// of f16 products, 1.02 PFLOP/s, where an 8192-cube f16 library product reaches 1.31 (16 rows a wave
+// 460, keys and values through registers into LDS 147); 8-bit values 183 (five products for four);
+// 8-bit keys too 209.  Bound by the matrix pipe (busy 52% of the cycles, at the 1.87 GHz that such
+// work is clocked down to) with the vector ALU's issue beside it; under 1000 positions a part, by
+// what a workgroup does once: 15 us of round trips, the query rows' parts and the partials' writes.
 constexpr uint32_t WIDE = 128, STEP = 32;
 template <int Q8>
 struct RawRows {
@@ -983,7 +1002,9 @@ PAGED_REP(1, 1)
 
 // o = sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s over a row's live partials, W waves of a
 // (head, row), lane t dims 2 t and 2 t + 1, wave w the partials w + W i, the waves' sums added in
-// order.
+// order.  Eight partials of a wave are in flight together.  Measured (MI355X): 128 rows of 32 heads
+// and 17 partials 10 us (36 MB, 3.5 TB/s), one row's 32 heads of 64 partials 4.1 us with eight waves a
+// head (79 us with one and a load at a time): bound by the launch and three round trips.
 template <uint32_t W>
 SK_DEV void paged_merge(float *a, const uint32_t *ctl, const PagedMergePush &p, uint32_t h, uint32_t row, uint32_t wave,
                         uint32_t lane) {
@@ -1057,6 +1078,11 @@ extern "C" __global__ __launch_bounds__(512) void attention_paged_merge_8__128(f
 // A workgroup of T threads takes 16 T tokens of a row: it loads its logits, counts the history's
 // tokens among them in LDS meanwhile (integer counts, so any order gives the same), and writes the
 // row's part once.  Its biases come last, each by the thread whose entry is the last of its id.
+// Measured (MI355X), a vocabulary of 151936, half of the rows masked: 128 rows of histories to 32768
+// 44 us (169 MB, 3.8 TB/s; 49 with T = 256, whose 38 workgroups a row each read the history, and 215
+// with a load of it at a time and two counts a token), of 100 27 us (5.8 TB/s), 48 rows of 4096 12.5 us,
+// 1 row 5.2 us.  Bound by HBM, with long histories by their counting; non-temporal stores save 1 to
+// 2 us of a launch of many rows.
 template <uint32_t T>
 SK_DEV void logits_body(float *a, const uint32_t *ctl, const LogitsPush &p) {
 #pragma clang fp contract(off)
