@@ -135,8 +135,9 @@ SK_DEV void store_row(f16 *kv, int8_t *kv8, uint32_t cache, uint32_t scales, uin
 // of a radian.  Each wave turns its row's 64 angles once, one a lane, for all its heads.
 // Measured (MI355X): 2048 rows of 48 heads, f16 keys and 8-bit values, 34 us from HBM (90 MB, 2.6
 // TB/s; 18 us from the caches), 79 with a wave a head and 4 bytes a lane and load: bound by the bytes
-// in flight.  PASSES = 4 from 2048 workgroups of one pass on (1000 rows 10.6 us against 13.1), below
-// it more workgroups are better (1 row 2.5 us: the launch and two dependent round trips).
+// in flight.  PASSES = 4 where 16 heads a workgroup would make 4096 of them or more (2048 rows 33.5 us
+// against 36), below it more workgroups are better (1000 rows 24 against 26.5).  1 row 2.5 us: the
+// launch and two dependent round trips.
 template <int K8, int V8, int PASSES>
 SK_DEV void append_body(const float *w, float *a, const uint32_t *ctl, f16 *kv, int8_t *kv8, const AppendPush &p) {
 #pragma clang fp contract(off)
@@ -505,11 +506,12 @@ SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
 // 8-bit values are held as two f16 parts of q s 2^(7 - ve), ve the exponent of the part's largest
 // scale of the 32 dims, found first.
 // Measured (MI355X): 128 rows of 32 heads over 32768 positions of 8 key heads, f16: 134 us, 137 GFLOP
-// of f16 products, 1.02 PFLOP/s, where an 8192-cube f16 library product reaches 1.31 (16 rows a wave
-// 460, keys and values through registers into LDS 147); 8-bit values 183 (five products for four);
-// 8-bit keys too 209.  Bound by the matrix pipe (busy 52% of the cycles, at the 1.87 GHz that such
-// work is clocked down to) with the vector ALU's issue beside it; under 1000 positions a part, by
-// what a workgroup does once: 15 us of round trips, the query rows' parts and the partials' writes.
+// of f16 products, 1.02 PFLOP/s, where an 8192-cube f16 library product reaches 1.31 (keys and
+// values through registers into LDS 147); 8-bit values 183 (five products for four); 8-bit keys too
+// 209.  With up to 512 own positions a row beside the run 152 to 164, 492 with 16 rows a wave.  Bound
+// by the matrix pipe (busy 52% of the cycles, at the 1.87 GHz that such work is clocked down to) with
+// the vector ALU's issue beside it; under 1000 positions a part, by what a workgroup does once: 15 us
+// of round trips, the query rows' parts and the partials' writes.
 constexpr uint32_t WIDE = 128, STEP = 32;
 template <int Q8>
 struct RawRows {
@@ -1004,7 +1006,8 @@ PAGED_REP(1, 1)
 // (head, row), lane t dims 2 t and 2 t + 1, wave w the partials w + W i, the waves' sums added in
 // order.  Eight partials of a wave are in flight together.  Measured (MI355X): 128 rows of 32 heads
 // and 17 partials 10 us (36 MB, 3.5 TB/s), one row's 32 heads of 64 partials 4.1 us with eight waves a
-// head (79 us with one and a load at a time): bound by the launch and three round trips.
+// head; one row of 256 partials took 79 us with one wave and a load at a time.  Bound by the launch
+// and three round trips.
 template <uint32_t W>
 SK_DEV void paged_merge(float *a, const uint32_t *ctl, const PagedMergePush &p, uint32_t h, uint32_t row, uint32_t wave,
                         uint32_t lane) {
@@ -1079,10 +1082,10 @@ extern "C" __global__ __launch_bounds__(512) void attention_paged_merge_8__128(f
 // tokens among them in LDS meanwhile (integer counts, so any order gives the same), and writes the
 // row's part once.  Its biases come last, each by the thread whose entry is the last of its id.
 // Measured (MI355X), a vocabulary of 151936, half of the rows masked: 128 rows of histories to 32768
-// 44 us (169 MB, 3.8 TB/s; 49 with T = 256, whose 38 workgroups a row each read the history, and 215
-// with a load of it at a time and two counts a token), of 100 27 us (5.8 TB/s), 48 rows of 4096 12.5 us,
-// 1 row 5.2 us.  Bound by HBM, with long histories by their counting; non-temporal stores save 1 to
-// 2 us of a launch of many rows.
+// 45 us (169 MB, 3.8 TB/s; 50 with T = 256, whose 38 workgroups a row each read the history, and 215
+// with a load of it at a time and two counts a token), of 100 27 us (5.8 TB/s), 48 rows of 4096 12.6 us,
+// 1 row of 1000 5.7 us.  Bound by HBM, with long histories by their counting; non-temporal stores
+// save 1 to 2 us of a launch of many rows.
 template <uint32_t T>
 SK_DEV void logits_body(float *a, const uint32_t *ctl, const LogitsPush &p) {
 #pragma clang fp contract(off)

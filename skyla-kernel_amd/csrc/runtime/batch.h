@@ -25,11 +25,18 @@ inline Op op_of(const char *name) {
 constexpr uint32_t kHead = 128, kPart = kHead + 2;
 constexpr uint32_t kMaxSlots = 1024;      // partials of a row and head
 constexpr uint32_t kMaxGrid = 65535;      // rows of a dispatch
-constexpr uint32_t kAppendMany = 2048;    // workgroups of 16 heads from which kv_append takes 64 each
-constexpr uint32_t kMergeParts = 16;      // partials above which eight waves merge a head,
-constexpr uint32_t kMergeHeads = 1024;    // where there are fewer rows of heads than this
-constexpr uint32_t kLogitsWide = 512;     // workgroups of 4096 tokens from which a logits launch takes 16384 each,
-constexpr uint32_t kLogitsHistory = 8192; // where each of them reads a history as long as this
+// Workgroups of 16 heads from which kv_append takes 64 heads each (48 heads a row, f16 keys and 8-bit
+// values, us, 16 / 64: 2048 rows 36 / 33.5, 1000 rows 24 / 26.5, 300 rows 15.4 / 16, 64 rows 10.4 / 10.4).
+constexpr uint32_t kAppendMany = 4096;
+// Partials above which eight waves merge a head, where rows times heads make two such workgroups a
+// compute unit at most (32 heads, us, one wave / eight: 1 row of 12 parts 3.9 / 4.0, of 32 5.3 / 4.0, of 64
+// 6.8 / 4.1; 16 rows of 17 4.8 / 5.0, of 32 5.4 / 5.0, of 64 7.1 / 5.0; 24 rows of 32 5.6 / 6.8; 128 of 17
+// 11.8 / 25.1).
+constexpr uint32_t kMergeParts = 16, kMergeHeads = 512;
+// Room for a history from which a logits workgroup takes 16384 tokens for 4096, so that a quarter of
+// them read it (us, 4096 / 16384: 128 rows of 32768 50 / 45, of 8192 33.7 / 33.3, of 1000 28 / 29; 12
+// rows of 30000 12.2 / 9.9, of 4096 7.4 / 8.0; 1 row of 30000 9.7 / 8.6, of 1000 5.7 / 6.4).
+constexpr uint32_t kLogitsHistory = 8192;
 constexpr uint32_t kMaxWork = 1u << 23;   // workgroups of an attention launch
 
 // [off, off + stride (rows - 1) + width) in elements
@@ -213,11 +220,11 @@ inline Shape shape(Op op, const uint32_t *spec, const uint32_t *w, uint32_t rows
     s.groups[1] = 1;
     s.extra = {rows};
   } else if (op == kMerge) {
-    s.form = w[4] + w[5] > kMergeParts && rows * w[3] < kMergeHeads;
+    s.form = w[4] + w[5] > kMergeParts && rows * w[3] <= kMergeHeads;
     s.groups[0] = s.form ? w[3] : (w[3] + 3) / 4;
     s.threads = s.form ? 512 : 256;
   } else {
-    s.form = (uint64_t)rows * ((w[4] + 4095) / 4096) >= kLogitsWide && w[7] >= kLogitsHistory;
+    s.form = w[7] >= kLogitsHistory;
     s.threads = s.form ? 1024 : 256;
     s.groups[0] = (w[4] + 16 * s.threads - 1) / (16 * s.threads);
   }
