@@ -625,3 +625,86 @@ def test_attention_in_place(ctx):
                 assert np.linalg.norm(got[r] - want[r]) <= BAR * np.linalg.norm(want[r]), (parts, r)
         finally:
             b.free()
+
+
+@pytest.mark.parametrize("precision", list(P))
+@pytest.mark.parametrize("heads,grid", [((2, 1), 4100), ((16, 4), 690)])
+def test_append_of_many_rows(ctx, precision, heads, grid):
+    """A launch of many rows, most of them idle, against one of the live rows alone: the same bits in
+    the output and in the pool, nothing written for the rest."""
+    b = Batch(ctx, P[precision], *heads, 16, [5, 0, 17, 100, 64], seed=3, grid=grid, parts=(0, 1))
+    try:
+        f = b.arena.as_f32()
+        for off, stride, width in ((b.q, b.sq, b.n_head * 128), (b.k, b.skv, b.dim), (b.v, b.skv, b.dim)):
+            b.rows_of(off, stride, width, grid)[:] = b.g.standard_normal((grid, width))
+        qn, kn, rope = b.norms
+        f[qn: qn + 128] = f[kn: kn + 128] = b.g.uniform(0.5, 1.5, 128)
+        f[rope: rope + 64] = THETA ** (-2.0 * np.arange(64) / 128)
+        b.fill()
+        pool, out = b.pool.host().copy(), b.rows_of(b.out, b.sq, b.sq, grid).copy()
+        got = []
+        for rows in (b.rows, grid):
+            b.pool.host()[:] = pool
+            b.rows_of(b.out, b.sq, b.sq, grid)[:] = out
+            b.run(lambda r: b.kernels.append(r, 0, b.at, (b.q, b.sq), (b.k, b.skv), b.v, (b.out, b.sq), qn, kn, rope, rows))
+            got.append((b.rows_of(b.out, b.sq, b.sq, grid).copy(), b.pool.host().copy()))
+        (o, p), (o_many, p_many) = got
+        assert np.array_equal(o, o_many) and np.array_equal(p, p_many)
+        assert not np.array_equal(o[0], out[0]) and (o[b.rows:] == 7.5).all() and not np.array_equal(p, pool)
+    finally:
+        b.free()
+
+
+@pytest.mark.parametrize("v", [1, 16384, 16385, 40001])
+def test_logits_adjust_of_long_histories(ctx, v):
+    """Histories of none, one and thousands of tokens, the same ones thousands of times."""
+    g = np.random.default_rng(v)
+    rows, grid, h, nb = 6, 7, 9004, 3
+    sx, sm = _pad(v), -(-v // 32)
+    size, off = 64, {}
+    for name, n in (("ctrl", 8 * grid), ("x", sx * grid), ("hist", h * grid), ("bias", 2 * nb * grid), ("mask", sm * grid)):
+        off[name], size = size, size + _pad(n)
+    a = ctx.alloc_host(size * 4)
+    k = B.LogitsKernels(ctx, a)
+    try:
+        f, u = a.as_f32(), a.as_u32()
+        f[:] = 7.5
+        u[:64] = 0
+        u[2] = rows
+        x = (g.standard_normal((rows, v)) * 4).astype(np.float32)
+        hist = np.minimum(g.integers(0, v + 5, (rows, h)), g.integers(0, v + 5, (rows, h))).astype(np.uint32)
+        hist[3] = v - 1
+        n, prompt = np.array([0, 1, h, h, 8999, 4097]), np.array([0, 0, 1000, 0, 9004, 4096])
+        par = np.array([[1.25, .01, .5]] * rows, np.float32)
+        bits = g.random((rows, v)) < 0.5
+        bias = [[(v - 1, np.float32(2.5)), (v, np.float32(1))]] * rows
+        for r in range(rows):
+            f[off["x"] + r * sx: off["x"] + r * sx + v] = x[r]
+            u[off["hist"] + r * h: off["hist"] + (r + 1) * h] = hist[r]
+            for i, (t, w) in enumerate(bias[r]):
+                u[off["bias"] + 2 * nb * r + 2 * i] = t
+                f[off["bias"] + 2 * nb * r + 2 * i + 1] = w
+            packed = np.packbits(np.concatenate([bits[r], np.zeros(-v % 32, bool)]), bitorder="little").view("<u4")
+            u[off["mask"] + r * sm: off["mask"] + r * sm + len(packed)] = packed
+            c = off["ctrl"] + 8 * r
+            u[c: c + 4] = n[r], prompt[r], len(bias[r]), r & 1
+            f[c + 4: c + 7] = par[r]
+        a.upload()
+        at = B.LogitsRegions(off["ctrl"], off["hist"], h, off["bias"], 2 * nb, off["mask"], sm)
+        rec = ctx.record(False, lambda r: k.adjust(r, at, (off["x"], sx), (off["x"], sx), v, grid))
+        ctx.replay(rec)
+        rec.free()
+        a.download()
+        out = a.as_f32()[off["x"]: off["x"] + sx * grid].reshape(grid, sx)
+        for r in range(rows):
+            want, got = _adjust64(x[r], hist[r], n[r], prompt[r], bias[r], bits[r] if r & 1 else None, *par[r]), out[r, :v]
+            fin = np.isfinite(want)
+            assert np.array_equal(np.isneginf(got), np.isneginf(want)), r
+            # one rounding for each of the four steps (a product, f made and its sum with g, two sums)
+            # of numbers up to the largest on the way: 30 and 9004 times 0.01 here
+            assert np.abs(got[fin] - want[fin]).max(initial=0) <= 5 * 2.0 ** -24 * 130, r
+            assert (out[r, v:] == 7.5).all()
+        assert (out[rows:] == 7.5).all()
+    finally:
+        k.free()
+        a.free()
