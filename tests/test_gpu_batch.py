@@ -708,3 +708,62 @@ def test_logits_adjust_of_long_histories(ctx, v):
     finally:
         k.free()
         a.free()
+
+
+class _Direct:
+    """A recorder's calls as single dispatches, or as timed ones of the same words."""
+
+    def __init__(self, ctx, reps):
+        self.ctx, self.reps = ctx, reps
+
+    def dispatch(self, p, groups, push):
+        if self.reps:
+            ns = self.ctx.time_dispatch(p, groups, push, self.reps)
+            assert len(ns) == self.reps and min(ns) > 0
+        else:
+            self.ctx.dispatch_noalloc(p, groups, push)
+
+    def dispatch_set(self, p, i, groups, push):
+        assert i == 0
+        self.dispatch(p, groups, push)
+
+    def barrier(self):
+        pass
+
+
+@pytest.mark.parametrize("precision", list(P))
+@pytest.mark.parametrize("reps", [0, 3])
+@pytest.mark.parametrize("parts", [(1, 2, True), (2, 1), (3, 30)])
+def test_single_dispatches(ctx, precision, reps, parts):
+    """dispatch_noalloc and time_dispatch of the operators: the bits of a recording, the same refusals."""
+    b = Batch(ctx, P[precision], 2, 4, 16, [140, 33, 0, 70, 45], shares=[32] * 5, shared=32, parts=parts, grid=7)
+    try:
+        f = b.arena.as_f32()
+        for off, stride, width in ((b.q, b.sq, b.n_head * 128), (b.k, b.skv, b.dim), (b.v, b.skv, b.dim)):
+            b.rows_of(off, stride, width)[:] = b.g.standard_normal((b.rows, width))
+        qn, kn, rope = b.norms
+        f[qn: qn + 128] = f[kn: kn + 128] = 1
+        f[rope: rope + 64] = THETA ** (-2.0 * np.arange(64) / 128)
+        b.fill()
+        b.copy_shared()
+
+        def step(r):  # the queries stay raw, so that it can run any number of times
+            b.kernels.append(r, 0, b.at, (b.q, b.sq), (b.k, b.skv), b.v, (b.out, b.sq), qn, kn, rope, b.grid)
+            r.barrier()
+            b.kernels.attend(r, 0, b.at, (b.q, b.sq), (b.out, b.sq), b.grid, parts)
+        start, pool = f.copy(), b.pool.host().copy()
+        b.run(step)
+        want, stored = b.rows_of(b.out, b.sq, b.sq, b.grid).copy(), b.pool.host().copy()
+        f[:], b.pool.host()[:] = start, pool
+        b.arena.upload()
+        b.pool.upload()
+        step(_Direct(ctx, reps))
+        b.arena.download()
+        b.pool.download()
+        assert np.array_equal(b.rows_of(b.out, b.sq, b.sq, b.grid), want) and np.array_equal(b.pool.host(), stored)
+        assert not np.array_equal(stored, pool) and np.isfinite(want[: b.rows, : b.n_head * 128]).all()
+        with pytest.raises(SkylaHipError) as e:
+            b.kernels.attend(_Direct(ctx, reps), 0, b.at, (b.arena.size // 4, 1024), (b.out, b.sq), b.grid, parts)
+        assert e.value.code == -1
+    finally:
+        b.free()
