@@ -32,6 +32,7 @@ constexpr uint32_t HD = 128;         // head width
 constexpr uint32_t PART = HD + 2;    // one partial: m, l, acc[128]
 constexpr uint32_t TILE = 64;        // the parts of a run are whole multiples of it
 constexpr float F16_MAX = 65504.0f;
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 struct AppendPush {
   uint32_t q_off, k_off, v_off, o_off, qn_off, kn_off, rope_off;
@@ -227,6 +228,17 @@ SK_DEV void weigh(float a, float b, float inv, float c, float &l, f16x8 &ph, f16
   ph[e] = hi.x, ph[e + 1] = hi.y;
   pl[e] = lo.x, pl[e + 1] = lo.y;
 }
+// A block's scale s 2^up as the f16 that 8-bit values are multiplied by: 0 outside [2^-14, 2^TOP), where
+// it would lose bits or has been taken; infinities and NaN stay.  Scales below this window are
+// taken by a further run over the positions with up WINDOW more.
+template <int TOP>
+constexpr int WINDOW = TOP + 14;
+template <int TOP>
+SK_DEV f16 scale_in(f16 s, int up) {
+  const f16 x = __builtin_ldexpf16(s, up), y = __builtin_fabsf16(x);
+  const bool out = y < (f16)0x1p-14f || (y >= (f16)(float)(1 << TOP) && __builtin_fabsf16(s) < (f16)INFINITY);
+  return out ? (f16)0.0f : x;
+}
 // two bytes picked by sel as an f16 pair: 1024 + (byte ^ 0x80), minus 1152
 SK_DEV f16x2 widen(uint32_t x1, uint32_t x0, uint32_t sel) {
   const f16x2 off = {(f16)1152.0f, (f16)1152.0f};
@@ -261,8 +273,10 @@ SK_DEV Pages pages_of(const uint32_t *ctl, const PagedPush &p, uint32_t seq) {
 //                 value rows of these positions, lane c holding dims 8 c + [0, 8): tile d takes dim
 //                 8 c + d as row c, so the transposition is 8 x 8 inside a lane
 // Loads of positions outside [lo, hi) go to ones inside, and their scores are -inf, so what lies
-// there reaches nothing.  8-bit values are two f16 parts of q s 2^(4 - ve), ve the exponent of the
-// largest scale of the 32 dims, followed as loosely.
+// there reaches nothing.  8-bit values are two f16 parts, exact, of q s 2^(4 - ve), ve the exponent of
+// the largest scale of the 32 dims, followed as loosely.  Scales 2^18 below it, whose positions may be
+// those that a row attends to, would lose bits: a run that meets one is run again with the m and ve that
+// it found, once for each window of scales.
 // Measured (MI355X, with the waves' join): one row of 16384 positions of 8 key heads, f16 keys and
 // 8-bit values, 15.5 us (50 MB, 3.2 TB/s); 128 rows of up to 512 own positions in f16 28 us (135 MB,
 // 4.8 TB/s, what a copy reaches); 8 rows of up to 100 positions 5.9 us.  Bound by HBM where rows are
@@ -328,9 +342,17 @@ SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
     __builtin_amdgcn_sched_barrier(0);  // in flight before what is computed next
   };
 
-  Groups now = look(begin), soon = look(begin + HALF);
+  Groups soon;
   HalfRows<K8, V8> ra, rb;
-  load(ra, now);
+  auto start = [&] {  // (not from a known position: its addresses would be kept in registers for the next run)
+    const uint32_t at = begin + (V8 ? opaque_mask(0) : 0);
+    const Groups now = look(at);
+    soon = look(at + HALF);
+    load(ra, now);
+  };
+  start();
+  uint64_t more;  // lanes of a step with scales below the window
+  int run = 0, window = 0;
   f16x8 qh[4], ql[4];
   float inv;
   {
@@ -358,11 +380,9 @@ SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
         ql[k][e] = (f16)(x - (float)qh[k][e]);
       }
   }
-  float m = -INFINITY, l = 0.0f;
+  float m = -INFINITY, l;
   int ve = -200, vo = -200;  // of the dims that this lane's values and sums hold (blocks c / 4 and g)
   f32x4 o[8];
-#pragma unroll
-  for (int d = 0; d < 8; d++) o[d] = {0.0f, 0.0f, 0.0f, 0.0f};
   auto word = [](const auto &u, int i) {
     if constexpr (sizeof(u) == 8)
       return i == 0 ? u.x : u.y;
@@ -407,11 +427,18 @@ SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
     mt = fmaxf(mt, sc[1][3]);
     mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
     mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * inv;
-    int top = -200;  // the scales' largest exponent
+    int top = -200;      // the scales' largest exponent
+    float least = 0.0f;  // and the smallest of this lane's that is not 0
     if constexpr (V8) {
-      float f = 0.0f;
+      u16x2 big = {0, 0}, low = {0, 0};  // by their bits w: the largest w and the largest -w (0: none above 0)
 #pragma unroll
-      for (int e = 0; e < 8; e++) f = fmaxf(f, fabsf((float)r.vs[e]));
+      for (int e = 0; e < 4; e++) {
+        const u16x2 w = __builtin_bit_cast(u16x2, as_u32(f16x2{r.vs[2 * e], r.vs[2 * e + 1]}) & 0x7fff7fffu);
+        big = __builtin_elementwise_max(big, w);
+        low = __builtin_elementwise_max(low, (u16x2){0, 0} - w);
+      }
+      float f = f16_bits_to_f32(max(big.x, big.y));
+      least = f16_bits_to_f32((uint16_t)-max(low.x, low.y));
       f = fmaxf(f, __shfl_xor(f, 16, 64));
       f = fmaxf(f, __shfl_xor(f, 32, 64));
       top = f > 0.0f && f < INFINITY ? __builtin_amdgcn_frexp_expf(f) : -200;
@@ -435,10 +462,17 @@ SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
 #pragma unroll
     for (int n = 0; n < 4; n++) weigh(sc[n >> 1][2 * (n & 1)], sc[n >> 1][2 * (n & 1) + 1], inv, cm, l, ph, pl, 2 * n);
     f16x2 sv[V8 ? 4 : 1];
-    if constexpr (V8)
+    if constexpr (V8) {
+      const int up = 4 - ve + WINDOW<9> * window;
+      more |= __ballot(least > 0.0f && ldexpf(least, up) < 0x1p-14f);
+      if (run) {
 #pragma unroll
-      for (int e = 0; e < 4; e++)
-        sv[e] = f16x2{(f16)ldexpf((float)r.vs[2 * e], 4 - ve), (f16)ldexpf((float)r.vs[2 * e + 1], 4 - ve)};
+        for (int e = 0; e < 8; e++) sv[e >> 1][e & 1] = scale_in<9>(r.vs[e], up);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) sv[e >> 1][e & 1] = __builtin_ldexpf16(r.vs[e], up);
+      }
+    }
 #pragma unroll
     for (int d = 0; d < 8; d++) {
       uint32_t x[4], y[4];
@@ -461,28 +495,50 @@ SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
       o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph, o[d], 0, 0, 0);
     }
   };
-  for (uint32_t at = begin;; at += 2 * HALF) {
-    if (at + HALF < end) {
-      load(rb, soon);
-      soon = look(at + 2 * HALF);
+  for (;; run++) {
+    more = 0, l = 0.0f;
+#pragma unroll
+    for (int d = 0; d < 8; d++) o[d] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t at = begin;; at += 2 * HALF) {
+      if (at + HALF < end) {
+        load(rb, soon);
+        soon = look(at + 2 * HALF);
+      }
+      compute(ra, at);
+      if (at + HALF >= end) break;
+      if (at + 2 * HALF < end) {
+        load(ra, soon);
+        soon = look(at + 3 * HALF);
+      }
+      compute(rb, at + HALF);
+      if (at + 2 * HALF >= end) break;
     }
-    compute(ra, at);
-    if (at + HALF >= end) break;
-    if (at + 2 * HALF < end) {
-      load(ra, soon);
-      soon = look(at + 3 * HALF);
+    // the first run is the result, or its m and ve are where the second starts; a window a run from there
+    if (!V8 || run || !more) {
+      const int back = V8 ? vo - WINDOW<9> * window - 4 - E_SHIFT : -E_SHIFT;
+#pragma unroll
+      for (int d = 0; d < 8; d++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) o[d][r] = ldexpf(o[d][r], back);
+      float *to = &out[c][2 + 8 * (4 * g)];
+      if (V8 && window) {
+#pragma unroll
+        for (int d = 0; d < 8; d++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) o[d][r] += to[8 * r + d];
+      }
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int d = 0; d < 8; d += 2) *(float2 *)(to + 8 * r + d) = make_float2(o[d][r], o[d + 1][r]);
     }
-    compute(rb, at + HALF);
-    if (at + 2 * HALF >= end) break;
+    if (!V8 || !more) break;
+    window = run;
+    start();
+    __builtin_amdgcn_s_waitcnt(0);  // as behind the first run's queries: the loop waits for none of them
   }
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
-  const int back = V8 ? vo - 4 - E_SHIFT : -E_SHIFT;
-#pragma unroll
-  for (int r = 0; r < 4; r++)
-#pragma unroll
-    for (int d = 0; d < 8; d += 2)
-      *(float2 *)&out[c][2 + 8 * (4 * g + r) + d] = make_float2(ldexpf(o[d][r], back), ldexpf(o[d + 1][r], back));
   if (g == 0) *(float2 *)out[c] = make_float2(m, ldexpf(l, -E_SHIFT));
 }
 
@@ -503,8 +559,9 @@ SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
 // With f16 keys a step multiplies the next step's scores while it makes this one's e, so that the
 // matrix pipe and the vector ALU work side by side in one wave; reads from LDS run two products
 // ahead.  (8-bit keys' block sums leave no registers for a second step's scores.)
-// 8-bit values are held as two f16 parts of q s 2^(7 - ve), ve the exponent of the part's largest
-// scale of the 32 dims, found first.
+// 8-bit values are held as two f16 parts, exact, of q s 2^(7 - ve), ve the exponent of the part's
+// largest scale of the 32 dims, found first.  A part with scales 2^21 below it is run again for each
+// window of them, with the largest score that the first run found.
 // Measured (MI355X): 128 rows of 32 heads over 32768 positions of 8 key heads, f16: 134 us, 137 GFLOP
 // of f16 products, 1.02 PFLOP/s, where an 8192-cube f16 library product reaches 1.31 (keys and
 // values through registers into LDS 147); 8-bit values 183 (five products for four); 8-bit keys too
@@ -526,13 +583,12 @@ struct WideStage {  // at most half of the 160 KB: two workgroups a compute unit
   uint4 kh[K8 ? 2 : 1][K8 ? STEP : 1][16];        // converted keys,
   float ks[K8 ? 2 : 1][4][K8 ? STEP : 4];         // their scales: [step][dims / 32][position]
   uint4 vh[V8 ? 2 : 1][V8 ? 2 : 1][2][4][V8 ? 64 : 1];  // and values: [step][part][k-step][dims / 32]
-  float tops[4][4];
+  u16x2 ends[4][4];
 };
 template <int K8, int V8>
 SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t *kv8, const PagedPush &p, uint32_t rep,
                      uint32_t kvh, uint32_t tile, uint32_t part, uint32_t shared, uint32_t n_rows,
                      WideStage<K8, V8> &st) {
-  auto &tops = st.tops;
   const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, col = lane & 31,
                  h = lane >> 5;
   const uint32_t kv_dim = p.n_kv * HD;
@@ -591,10 +647,15 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
   // Step s's values are loaded with step s + VK's keys: keys (scores come a step ahead) and 8-bit
   // rows (converted a step ahead) are free for the next load a step before f16 values.
   constexpr uint32_t VK = !V8, LEAD = DEPTH - 1 + V8;  // ... at the top of step s - LEAD
-  for (uint32_t s = 0; s < DEPTH; s++) {
-    load_keys(s, look(s));
-    if (s < LEAD) load_values(s, look(s));
-  }
+  // (not from a constant: the addresses would be kept in registers from run to run)
+  auto prime = [&] {
+    const uint32_t first = V8 ? opaque_mask(0) : 0;
+    for (uint32_t s = 0; s < DEPTH; s++) {
+      load_keys(first + s, look(first + s));
+      if (s < LEAD) load_values(first + s, look(first + s));
+    }
+  };
+  prime();
 
   const bool live =
       row < n_rows && row_range(ctl, p.rows_off, row, shared, p.n_seq, p.table_stride, p.page_log2).member;
@@ -633,24 +694,36 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
   }
 
   int ve[4] = {0, 0, 0, 0};
+  int runs = 1;  // of the part: a window of scales each
   if constexpr (V8) {
-    float top[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    u16x2 ends[4] = {};  // a block's scales by their bits w: the largest w and the largest -w (0: none above 0)
     for (uint32_t pos = begin + t; pos < end; pos += 256) {
       const f16x4 s = *(const f16x4 *)(kv + p.vs_off + pages.slot(pos) * (kv_dim / 32) + kvh * 4);
 #pragma unroll
-      for (int b = 0; b < 4; b++) top[b] = fmaxf(top[b], fabsf((float)s[b]));
+      for (int b = 0; b < 4; b++) {
+        const f16 x = s[b];  // (a bit cast of an element itself takes element 0)
+        const uint16_t w = __builtin_bit_cast(uint16_t, x) & 0x7fff;
+        ends[b] = __builtin_elementwise_max(ends[b], u16x2{w, (uint16_t)-w});
+      }
     }
 #pragma unroll
     for (int b = 0; b < 4; b++) {
-      top[b] = wave_max(top[b]);
-      if (lane == 0) tops[wave][b] = top[b];
+#pragma unroll
+      for (int d = 32; d >= 1; d >>= 1)
+        ends[b] = __builtin_elementwise_max(
+            ends[b], __builtin_bit_cast(u16x2, __shfl_xor(__builtin_bit_cast(uint32_t, ends[b]), d, 64)));
+      if (lane == 0) st.ends[wave][b] = ends[b];
     }
     __syncthreads();
 #pragma unroll
     for (int b = 0; b < 4; b++) {
-      const float m = fmaxf(fmaxf(tops[0][b], tops[1][b]), fmaxf(tops[2][b], tops[3][b]));
-      ve[b] = m > 0.0f && m < INFINITY ? __builtin_amdgcn_frexp_expf(m) : 0;
+      const u16x2 e = __builtin_elementwise_max(__builtin_elementwise_max(st.ends[0][b], st.ends[1][b]),
+                                                __builtin_elementwise_max(st.ends[2][b], st.ends[3][b]));
+      const float m = f16_bits_to_f32(e.x), n = f16_bits_to_f32((uint16_t)-e.y);
+      ve[b] = __builtin_amdgcn_readfirstlane(m > 0.0f && m < INFINITY ? __builtin_amdgcn_frexp_expf(m) : 0);
+      for (int k = 1; n > 0.0f && ldexpf(n, 7 - ve[b] + WINDOW<7> * (k - 1)) < 0x1p-14f; k++) runs = max(runs, k + 1);
     }
+    runs = __builtin_amdgcn_readfirstlane(runs);
   }
 
   // 8-bit rows to f16: dims 8 dg + [0, 8) of positions 2 pr and 2 pr + 1
@@ -676,7 +749,7 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
       const uint32_t sw = dt | ((dg >> 1 & 1) << 2);
       const uint2 x0 = ((const uint2 *)from.x[2 * pr])[dg], x1 = ((const uint2 *)from.x[2 * pr + 1])[dg];
       const f16 s0 = ((const f16 *)&from.s[2 * pr])[dt], s1 = ((const f16 *)&from.s[2 * pr + 1])[dt];
-      const f16x2 sv = {(f16)ldexpf((float)s0, 7 - vmine), (f16)ldexpf((float)s1, 7 - vmine)};
+      const f16x2 sv = {scale_in<7>(s0, 7 - vmine), scale_in<7>(s1, 7 - vmine)};
 #pragma unroll
       for (uint32_t e = 0; e < 8; e++) {
         const uint32_t at = (hh * 32 + 8 * (dg & 3) + e) ^ sw;
@@ -689,7 +762,7 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
   };
 
   // keys of a staged step: dims 16 k + [0, 16)
-  const uint32_t kbase = col * 16 + (h ^ (col & 15));
+  uint32_t kbase = col * 16 + (h ^ (col & 15));
   auto key = [&](uint32_t step, uint32_t k) {
     if constexpr (K8)
       return __builtin_bit_cast(f16x8, (&st.kh[step & 1][0][0])[kbase ^ (2 * k)]);
@@ -752,23 +825,9 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
   };
 
   f32x16 o[4];
-#pragma unroll
-  for (int d = 0; d < 4; d++)
-#pragma unroll
-    for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
-  float m = -INFINITY, l = 0.0f;
-  dl_wait_vm<0>();
-  __syncthreads();
-  convert_keys(0);
-  convert_values(0);
-  __syncthreads();
-  f32x16 sc;
-  if constexpr (AHEAD) {
-    sc = scores(0);
-    __syncthreads();  // before the loop's first loads write its keys
-  }
+  float m = -INFINITY, l;
   const uint32_t n_steps = (end - begin + STEP - 1) / STEP;
-  Rows vat = look(LEAD), kat = look(LEAD + VK);
+  Rows vat, kat;
   // `sc`: this step's scores; into `next` the next step's
   auto do_step = [&](uint32_t step, f32x16 &sc, f32x16 &next) {
     // here: this step's scores (AHEAD), and what is multiplied below lies in LDS, converted; what the
@@ -846,34 +905,65 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
     dl_wait_vm<4 * (DEPTH - 2)>();
     __syncthreads();
   };
-  f32x16 other;
-  if constexpr (V8) {  // two steps a round would need more registers than two waves a SIMD have
-    for (uint32_t step = 0; step < n_steps; step++) {
-      do_step(step, sc, other);
-      if constexpr (AHEAD) sc = other;
+  for (int run = 0;; run++) {
+#pragma unroll
+    for (int d = 0; d < 4; d++) zero(o[d]);
+    l = 0.0f;
+    dl_wait_vm<0>();
+    __syncthreads();
+    const uint32_t first = V8 ? opaque_mask(0) : 0;
+    if constexpr (V8) asm volatile("" : "+v"(kbase));  // (as prime's: nothing of it is kept from run to run)
+    convert_keys(first);
+    convert_values(first);
+    __syncthreads();
+    f32x16 sc, other;
+    if constexpr (AHEAD) {
+      sc = scores(first);
+      __syncthreads();  // before the loop's first loads write its keys
     }
-  } else {
-    uint32_t step = 0;
-    for (; step + 2 <= n_steps; step += 2) {
-      do_step(step, sc, other);
-      do_step(step + 1, other, sc);
+    vat = look(LEAD), kat = look(LEAD + VK);
+    if constexpr (V8) {  // two steps a round would need more registers than two waves a SIMD have
+      for (uint32_t step = 0; step < n_steps; step++) {
+        do_step(step, sc, other);
+        if constexpr (AHEAD) sc = other;
+      }
+    } else {
+      uint32_t step = 0;
+      for (; step + 2 <= n_steps; step += 2) {
+        do_step(step, sc, other);
+        do_step(step + 1, other, sc);
+      }
+      if (step < n_steps) do_step(step, sc, other);
     }
-    if (step < n_steps) do_step(step, sc, other);
+    dl_wait_vm<0>();  // nothing is left to write this workgroup's LDS
+    uint32_t me;  // the lane again: no register held it through the loop
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=&v"(me));
+    const uint32_t mine = me >> 5, to = tile * WIDE + wave * 32 + (me & 31);
+    l += __shfl_xor(l, 32, 64);
+    if (live) {
+      float *out = a + p.part_off +
+                   ((to / rep * p.n_kv * rep + kvh * rep + to % rep) * (p.n_shared + p.n_own) + part) * PART;
+      float *dims = out + 2 + 4 * mine;
+#pragma unroll
+      for (int d = 0; d < 4; d++) o[d] *= ldexpf(1.0f, V8 ? ve[d] - WINDOW<7> * run - 7 - E_SHIFT : -E_SHIFT);
+      if (V8 && run) {
+#pragma unroll
+        for (int d = 0; d < 4; d++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) o[d][r] += dims[32 * d + 8 * (r >> 2) + (r & 3)];
+      }
+#pragma unroll
+      for (int d = 0; d < 4; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r += 2)
+          *(float2 *)(dims + 32 * d + 8 * (r >> 2) + (r & 3)) = make_float2(o[d][r], o[d][r + 1]);
+      if (mine == 0) *(float2 *)out = make_float2(m, ldexpf(l, -E_SHIFT));
+    }
+    if (!V8 || run + 1 == runs) return;
+    // (every wave is past the last step's reads)
+    prime();
+    vmine -= WINDOW<7>;
   }
-  dl_wait_vm<0>();  // nothing is left to write this workgroup's LDS
-  l += __shfl_xor(l, 32, 64);
-  if (!live) return;
-  float *out = a + p.part_off + ((row * p.n_kv * rep + kvh * rep + head) * (p.n_shared + p.n_own) + part) * PART;
-#pragma unroll
-  for (int d = 0; d < 4; d++)
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const float f = ldexpf(1.0f, V8 ? ve[d] - 7 - E_SHIFT : -E_SHIFT);
-      float *to = out + 2 + 32 * d + 8 * j + 4 * h;
-      *(float2 *)to = make_float2(o[d][4 * j] * f, o[d][4 * j + 1] * f);
-      *(float2 *)(to + 2) = make_float2(o[d][4 * j + 2] * f, o[d][4 * j + 3] * f);
-    }
-  if (h == 0) *(float2 *)out = make_float2(m, ldexpf(l, -E_SHIFT));
 }
 
 // Workgroups of four waves: first those of the shared run, `wide` (wide_run; the row tiles of a key

@@ -1,0 +1,76 @@
+"""The batch operators where their number formats end: scales of a cache far apart."""
+import numpy as np
+import pytest
+
+from test_gpu_batch import Batch, P
+
+pytestmark = pytest.mark.gpu
+
+
+def _reference(b):
+    """The rows' attention in 64 bits, and that of the values' sizes: (o, sum p |v|)."""
+    q = b.rows_of(b.q, b.sq, b.n_head * 128).astype(np.float64).reshape(b.rows, b.n_head, 128)
+    o, size = np.zeros((2, b.rows, b.n_head, 128))
+    for r in range(b.rows):
+        K, V = b.read64(b.slots(b.seqs[r], int(b.lens[r])))
+        for h in range(b.n_head):
+            s = K[:, h // b.rep] @ q[r, h] / np.sqrt(128.0)
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            o[r, h], size[r, h] = p @ V[:, h // b.rep], p @ np.abs(V[:, h // b.rep])
+    return o, size
+
+
+def _two_kinds(b, small, gap):
+    """Keys and queries along one direction: positions of `small` score `gap` nats above the others."""
+    u = np.where(b.g.random(128) < 0.5, -1.0, 1.0)
+    # q . k / sqrt(128) = +- gap / 2 for q = gap / (4 * 128) sqrt(128) u, k = +- 2 u
+    b.rows_of(b.q, b.sq, b.n_head * 128)[:] = np.tile(u * gap / (4 * np.sqrt(128.0)), (b.rows, b.n_head))
+    (k, ks), _ = b.halves()
+    sign = np.where(small, 1, -1)[:, None]
+    if ks is None:
+        k[:] = sign * np.tile(2 * u, b.n_kv)
+    else:
+        k[:] = sign * np.tile(64 * u, b.n_kv).astype(int)
+        ks[:] = 2.0 ** -5
+
+
+@pytest.mark.parametrize("precision", ["q8", "f16k_q8v"])
+@pytest.mark.parametrize("form", ["own", "narrow", "wide"])
+@pytest.mark.parametrize("order", ["first", "last", "mixed"])
+def test_scales_far_apart(ctx, precision, form, order):
+    """Values with scales from 2^-20 to 2^12 in one run, the rows attending to the small ones: what a row
+    leaves out does not cost what it takes its bits."""
+    shared = 0 if form == "own" else 400
+    lens = [400 + n for n in (1, 77, 33)]
+    b = Batch(ctx, P[precision], 2, 4, 16, lens, shares=[shared] * 3, shared=shared, wide=form == "wide",
+              parts=None if form == "own" else (2, 1))
+    try:
+        b.fill()
+        small = np.zeros(b.n_pages * b.page, bool)
+        for r in range(3):
+            at = b.slots(r, lens[r])
+            place = {"first": np.arange(lens[r]) < 130, "last": np.arange(lens[r]) >= 330,
+                     "mixed": b.g.random(lens[r]) < 0.3}[order]
+            if r and shared:
+                place[:shared] = small[b.slots(0, shared)]
+            small[at] = place
+        _two_kinds(b, small, 100.0)
+        _, (v, vs) = b.halves()
+        vs[:] = np.where(small[:, None], 2.0 ** b.g.uniform(-20, -16, vs.shape), 2.0 ** b.g.uniform(8, 12, vs.shape))
+        vs[::5, ::3] = 0    # and blocks of nothing
+        if shared:
+            b.copy_shared()
+        want, size = _reference(b)
+        assert 0 < np.linalg.norm(want) < 1e-2  # the others' weight is 1e-43
+        got = b.attend()
+        # queries and keys are exact, so a score is off by f32's sum: 2^-24 of 72 powers of two a product,
+        # common to the positions of a kind.  Weights are within 2^-23, values exact, f32 sums of n <= 477
+        # terms within sqrt(n) 2^-24 of sum p |v|: 2e-6 in all
+        for r in range(3):
+            for h in range(b.n_head):
+                for k in range(0, 128, 32):
+                    d = slice(k, k + 32)
+                    assert np.linalg.norm(got[r, h, d] - want[r, h, d]) <= 2e-6 * np.linalg.norm(size[r, h, d]), (r, h, k)
+    finally:
+        b.free()
