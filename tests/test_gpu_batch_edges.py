@@ -1,4 +1,4 @@
-"""The batch operators where their number formats end: scales of a cache far apart."""
+"""The batch operators where their number formats end: scales of a cache far apart, weights' rounding."""
 import numpy as np
 import pytest
 
@@ -72,5 +72,57 @@ def test_scales_far_apart(ctx, precision, form, order):
                 for k in range(0, 128, 32):
                     d = slice(k, k + 32)
                     assert np.linalg.norm(got[r, h, d] - want[r, h, d]) <= 2e-6 * np.linalg.norm(size[r, h, d]), (r, h, k)
+    finally:
+        b.free()
+
+
+@pytest.mark.parametrize("precision", ["f16", "f16k_q8v"])
+@pytest.mark.parametrize("form", ["own", "narrow", "wide"])
+def test_weights_far_below_the_largest(ctx, precision, form):
+    """Values 2^16 times the others' where the weights are 2^-20: a weight is held to 2^-32 of the row's
+    largest, so their share, a sixteenth of the sum, to 2^-12."""
+    shared = 0 if form == "own" else 256
+    b = Batch(ctx, P[precision], 1, 4, 16, [300, 290], shares=[shared] * 2, shared=shared, wide=form == "wide",
+              parts=None if form == "own" else (1, 1))
+    try:
+        b.fill()
+        small = b.g.random(b.n_pages * b.page) < 0.5
+        gap = 20.37 * np.log(2.0)
+        _two_kinds(b, small, gap)
+        _, (v, vs) = b.halves()
+        if vs is None:
+            v[:] = np.where(small[:, None], 0.25, 2.0 ** 14) * b.g.uniform(0.5, 1, v.shape)
+        else:
+            v[:] = b.g.integers(64, 128, v.shape)
+            vs[:] = np.where(small[:, None], 2.0 ** -9, 2.0 ** 7)
+        if shared:
+            b.copy_shared()
+        want, size = _reference(b)
+        got = b.attend()
+        # the big values' weights 2^-20.4 +- 2^-32 each (alike, so off alike): 2^-11.6 of a share of 2^16
+        # 2^-20.4 of the sum are 1.6e-5 of it; weights 2^-23, f32 sums sqrt(300) 2^-24, scores (20 powers of
+        # two) 20 2^-24 ln 2: 3e-6
+        assert (np.abs(got - want) <= 2e-5 * size).all()
+    finally:
+        b.free()
+
+
+@pytest.mark.parametrize("precision", list(P))
+@pytest.mark.parametrize("form", ["own", "narrow", "wide"])
+def test_one_position_is_its_value(ctx, precision, form):
+    """A weight's two parts hold all of it (of one position the largest), so the quotient is the value
+    to a rounding of the product and one of the quotient."""
+    shared = 0 if form == "own" else 1
+    rows = 64
+    b = Batch(ctx, P[precision], 2, 2, 16, [1] * rows, shares=[shared] * rows, shared=shared, wide=form == "wide",
+              parts=(0, 1) if form == "own" else (1, 1))
+    try:
+        b.fill()
+        b.copy_shared()
+        q = b.rows_of(b.q, b.sq, b.n_head * 128)
+        q[:] = b.g.standard_normal(q.shape) * 3
+        want, _ = _reference(b)
+        got = b.attend()
+        assert (np.abs(got - want) <= 2.0 ** -23 * np.abs(want)).all()
     finally:
         b.free()
