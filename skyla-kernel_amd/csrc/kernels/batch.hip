@@ -100,9 +100,10 @@ SK_DEV Split split_of(uint32_t lo, uint32_t hi, uint32_t n) {
 SK_DEV uint32_t live_parts(const Split &s) { return (s.tiles + s.per - 1) / s.per; }
 
 // Elements 4 t + [0, 4) and 64 + 4 t + [0, 4) (t = lane % 16) of one head's cache row, held as
-// attention.hip holds them but for one thing: an f16 past the type's largest value is stored as
-// that value, so that the cache has no infinity (its products with the f16 parts of a query or a
-// weight would be NaN).
+// attention.hip holds them but for two things: an f16 past the type's largest value is stored as
+// that value, and a block's scale too, its values as at most 127 of it, so that the cache has no
+// infinity (its products with the f16 parts of a query or a weight would be NaN); and a block that
+// holds a NaN has one for its scale.
 template <int Q8>
 SK_DEV void store_row(f16 *kv, int8_t *kv8, uint32_t cache, uint32_t scales, uint32_t kv_dim, uint32_t slot,
                       uint32_t head, uint32_t t, const float4 (&y)[2]) {
@@ -114,17 +115,20 @@ SK_DEV void store_row(f16 *kv, int8_t *kv8, uint32_t cache, uint32_t scales, uin
     if constexpr (!Q8) {
       *(f16x4 *)(kv + dst + 64 * n) = f16x4{(f16)fit(v[0]), (f16)fit(v[1]), (f16)fit(v[2]), (f16)fit(v[3])};
     } else {  // a block: eight lanes' values
-      float m = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
-      m = fmaxf(m, dpp_f<0xb1>(m));
-      m = fmaxf(m, dpp_f<0x4e>(m));
-      m = fmaxf(m, dpp_f<0x141>(m));
-      const float s = m / 127.0f;
+      auto bits = [](float x) { return __builtin_bit_cast(uint32_t, fabsf(x)); };  // in the values' order, NaN above all
+      uint32_t m = max(max(bits(v[0]), bits(v[1])), max(bits(v[2]), bits(v[3])));
+      m = max(m, bits(dpp_f<0xb1>(__builtin_bit_cast(float, m))));
+      m = max(m, bits(dpp_f<0x4e>(__builtin_bit_cast(float, m))));
+      m = max(m, bits(dpp_f<0x141>(__builtin_bit_cast(float, m))));
+      const float s = fit(__builtin_bit_cast(float, m) / 127.0f);
       uint32_t w = 0;
 #pragma unroll
-      for (int e = 0; e < 4; e++)
-        w |= ((uint32_t)(int)(s > 0.0f ? __builtin_rintf(v[e] / s) : 0.0f) & 255u) << (8 * e);
+      for (int e = 0; e < 4; e++) {
+        const float x = s > 0.0f ? __builtin_amdgcn_fmed3f(__builtin_rintf(v[e] / s), -127.0f, 127.0f) : 0.0f;
+        w |= ((uint32_t)(int)x & 255u) << (8 * e);
+      }
       *(uint32_t *)(kv8 + dst + 64 * n) = w;
-      if ((t & 7) == 0) kv[scales + slot * (kv_dim / 32) + head * 4 + 2 * n + t / 8] = (f16)fit(s);
+      if ((t & 7) == 0) kv[scales + slot * (kv_dim / 32) + head * 4 + 2 * n + t / 8] = (f16)s;
     }
   }
 }

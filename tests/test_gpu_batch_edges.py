@@ -1,4 +1,5 @@
-"""The batch operators where their number formats end: scales of a cache far apart, weights' rounding."""
+"""The batch operators where their number formats end: scales of a cache far apart, weights' rounding,
+what an 8-bit cache makes of NaN, infinities and values past its largest."""
 import numpy as np
 import pytest
 
@@ -124,5 +125,69 @@ def test_one_position_is_its_value(ctx, precision, form):
         want, _ = _reference(b)
         got = b.attend()
         assert (np.abs(got - want) <= 2.0 ** -23 * np.abs(want)).all()
+    finally:
+        b.free()
+
+
+def test_an_8_bit_cache_of_no_numbers_and_large_ones(ctx):
+    """A block of 32 that holds a NaN is NaN; an infinity or a value past 127 of the largest scale is
+    held as that, and the block's other values to half a step of it."""
+    b = Batch(ctx, P["q8"], 1, 2, 16, [3, 20], parts=(0, 1))
+    try:
+        f = b.arena.as_f32()
+        for off, stride, width in ((b.q, b.sq, b.n_head * 128), (b.k, b.skv, b.dim), (b.v, b.skv, b.dim)):
+            b.rows_of(off, stride, width)[:] = b.g.standard_normal((b.rows, width))
+        v, k = b.rows_of(b.v, b.skv, b.dim), b.rows_of(b.k, b.skv, b.dim)
+        v[0, 5] = np.nan
+        v[0, 32:36] = 1e9, 8e6, -2e5, 40000
+        v[0, 64:67] = np.inf, -np.inf, -7e6
+        v[1, 96:98] = np.nan, np.inf
+        k[1, 7] = np.nan
+        qn, kn, rope = b.norms
+        f[qn: qn + 128] = f[kn: kn + 128] = 1
+        f[rope: rope + 64] = 1
+        b.run(lambda r: b.kernels.append(r, 0, b.at, (b.q, b.sq), (b.k, b.skv), b.v, (b.out, b.sq), qn, kn, rope, 2))
+        (_, ks), (e, s) = b.halves()
+        top = 127 * 65504.0
+        for r, nan in ((0, [0]), (1, [3])):
+            slot = b.table[r, (b.lens[r] - 1) // 16] * 16 + (b.lens[r] - 1) % 16
+            for blk in range(4):
+                d = slice(32 * blk, 32 * blk + 32)
+                if blk in nan:
+                    assert np.isnan(s[slot, blk])
+                    continue
+                step = float(s[slot, blk])
+                y = np.clip(v[r, d].astype(np.float64), -top, top)
+                assert 0 < step <= 65504
+                # half a step, and the scale's own rounding of at most 127 steps
+                assert (np.abs(e[slot, d] * step - y) <= (0.5 + 127 * 2.0 ** -11 + 1e-6) * step).all(), (r, blk)
+            if r == 1:  # a NaN in a key makes its norm one: the whole head
+                assert np.isnan(ks[slot]).all()
+    finally:
+        b.free()
+
+
+@pytest.mark.parametrize("precision", list(P))
+@pytest.mark.parametrize("half", ["keys", "values"])
+def test_a_row_that_attends_to_no_number(ctx, precision, half):
+    """NaN at a position of one row's own run: what it reaches of that row is NaN, nothing else."""
+    shared = 40
+    b = Batch(ctx, P[precision], 2, 2, 16, [90, 70, 140], shares=[shared] * 3, shared=shared)
+    try:
+        b.fill()
+        b.copy_shared()
+        b.rows_of(b.q, b.sq, b.n_head * 128)[:] = b.g.standard_normal((b.rows, b.n_head * 128))
+        want = b.want()
+        e, s = b.halves()[half == "values"]
+        at = b.slots(1, 70)[55]
+        (e if s is None else s)[at, (128 + 35) // (1 if s is None else 32)] = np.nan  # dim 35 of key head 1
+        got = b.attend()
+        bad = np.zeros(want.shape, bool)
+        if half == "keys":
+            bad[1, 2:] = True
+        else:
+            bad[1, 2:, 35 if s is None else slice(32, 64)] = True
+        assert np.isnan(got[bad]).all() and np.isfinite(got[~bad]).all()
+        assert np.abs(got - want)[~bad].max() <= 4e-6 * np.abs(want).max()
     finally:
         b.free()
