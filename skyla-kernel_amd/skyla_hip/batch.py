@@ -202,9 +202,20 @@ class Controls:
 
 
 class _Sequence:
-    def __init__(self, pages=(), tokens=(), n_prompt=0, controls=None):
-        self.pages, self.tokens = list(pages), list(tokens)
-        self.n_prompt, self.controls = n_prompt, controls or Controls()
+    """A sequence's pages, the tokens of its prompts and those that it generated (a conversation's
+    follow in turns; what acts on the logits asks only which), its controls, and how many words of
+    its history, the prompts' tokens before the others, lie in the arena."""
+
+    def __init__(self, pages=(), prompt=(), made=(), controls=None):
+        self.pages, self.prompt, self.made = list(pages), list(prompt), list(made)
+        self.controls, self.placed = controls or Controls(), 0
+
+    def __len__(self):
+        return len(self.prompt) + len(self.made)
+
+    def add_prompt(self, tokens):
+        self.placed = min(self.placed, len(self.prompt))
+        self.prompt += tokens
 
 
 class _BatchGraph(E.Graph):
@@ -293,19 +304,19 @@ class BatchEngine:
 
     def length(self, seq: int) -> int:
         """Positions in a sequence's cache."""
-        return len(self._get(seq).tokens)
+        return len(self._get(seq))
 
     def fork(self, seq: int) -> int:
         """A new sequence that goes on from where `seq` is, with its controls."""
         s, page = self._get(seq), self.paged.page
-        whole, rest = divmod(len(s.tokens), page)
+        whole, rest = divmod(len(s), page)
         if len(self.sequences) == self.max_seq:
             raise ValueError(f"all {self.max_seq} sequences are open")
         own = self._take(1 if rest else 0)
         self.uses[s.pages[:whole]] += 1
         if rest:
             self._copy_page(s.pages[whole], own[0], rest)
-        n = self._add(_Sequence(s.pages[:whole] + own, s.tokens, s.n_prompt, s.controls))
+        n = self._add(_Sequence(s.pages[:whole] + own, s.prompt, s.made, s.controls))
         self._upload_table(n)
         return n
 
@@ -358,9 +369,9 @@ class BatchEngine:
         page, new = self.paged.page, {}
         for seq, n in need.items():
             s = self._get(seq)
-            if len(s.tokens) + n > self.max_ctx:
+            if len(s) + n > self.max_ctx:
                 raise ValueError(f"sequence {seq}: context full ({self.max_ctx} tokens)")
-            new[seq] = -(-(len(s.tokens) + n) // page) - len(s.pages)
+            new[seq] = -(-(len(s) + n) // page) - len(s.pages)
         if sum(new.values()) > len(self.free_pages):
             raise ValueError(f"{sum(new.values())} pages needed, {len(self.free_pages)} free")
         for seq, n in new.items():
@@ -376,12 +387,15 @@ class BatchEngine:
         if pages:
             a.buffer.upload(off * 4, len(pages) * 4)
 
-    def _upload_history(self, seq: int, first: int = 0) -> None:
-        a, tokens = self.arena, self._get(seq).tokens
-        off = self.logits_at.history + seq * self.s_hist
-        if len(tokens) > first:
-            a.u32()[off + first: off + len(tokens)] = tokens[first:]
-            a.buffer.upload((off + first) * 4, (len(tokens) - first) * 4)
+    def _upload_history(self, seq: int) -> None:
+        a, s = self.arena, self._get(seq)
+        n = s.placed - len(s.prompt)
+        new = s.made[n:] if n >= 0 else s.prompt[n:] + s.made
+        off = self.logits_at.history + seq * self.s_hist + s.placed
+        if new:
+            a.u32()[off: off + len(new)] = new
+            a.buffer.upload(off * 4, len(new) * 4)
+        s.placed = len(s)
 
     def _upload_controls(self, seq: int) -> None:
         a, k = self.arena, self._get(seq).controls
@@ -398,8 +412,6 @@ class BatchEngine:
             bits[: self.c.n_vocab] = k.allowed
             u[mask: mask + self.s_mask] = np.packbits(bits, bitorder="little").view("<u4")
             a.buffer.upload(mask * 4, self.s_mask * 4)
-        if k.counts:
-            self._upload_history(seq)
 
     def _words(self, live: int, rows: np.ndarray, tokens: Sequence[int], shared: int, leader: int) -> None:
         a = self.arena
@@ -456,20 +468,18 @@ class BatchEngine:
 
     # ---- decoding ----
     def extend(self, seq: int, tokens) -> None:
-        """Puts tokens into a sequence's cache, as its prompt: BATCH of them at a time."""
+        """Puts tokens into a sequence's cache, as its prompt or a further turn's, BATCH of them at a
+        time.  What it generated before counts as generated still."""
         s, tokens = self._get(seq), self._check(tokens)
         self._room({seq: len(tokens)})
         for i in range(0, len(tokens), E.BATCH):
-            chunk, pos = tokens[i: i + E.BATCH], len(s.tokens)
+            chunk, pos = tokens[i: i + E.BATCH], len(s)
             n = len(chunk)
             rows = np.zeros((n, 4), np.uint32)
             rows[:, 0], rows[:, 1], rows[:, 2] = seq, pos + 1 + np.arange(n), pos
             self._words(n, rows, chunk, pos, seq)
             self.ctx.replay(self._recording(n, pos, n, False))
-            s.tokens += chunk
-        s.n_prompt = len(s.tokens)
-        if s.controls.counts:
-            self._upload_history(seq, len(s.tokens) - len(tokens))
+            s.add_prompt(chunk)
 
     def shared_run(self, seqs) -> tuple[int, list[int]]:
         """The positions that sequences of a step read once for all: (how many, whose).  Of the
@@ -490,8 +500,8 @@ class BatchEngine:
 
     def step(self, tokens: dict, prompt=()) -> np.ndarray:
         """One token of each of several sequences ({sequence: token}): the logits after them, a row
-        each in the order given.  `prompt`: sequences whose token is their prompt's last (the
-        others' count as generated)."""
+        each in the order given.  `prompt`: sequences whose token is a prompt's (the others' count as
+        generated)."""
         if not tokens:
             raise ValueError("step needs a token of at least one sequence")
         values, seqs = self._check(tokens.values()), list(tokens)
@@ -503,13 +513,14 @@ class BatchEngine:
         rows, ids, own = np.zeros((live, 4), np.uint32), np.zeros(live, np.uint32), 1
         for q, t in zip(seqs, values):
             s = self._get(q)
-            s.tokens.append(t)
             if q in prompt:
-                s.n_prompt = len(s.tokens)
-            n, take = len(s.tokens), shared if q in members and len(s.tokens) >= shared else 0
+                s.add_prompt([t])
+            else:
+                s.made.append(t)
+            n, take = len(s), shared if q in members and len(s) >= shared else 0
             rows[q], ids[q], own = (q, n, take, 0), t, max(own, n - take)
             if s.controls.counts:
-                self._upload_history(q, n - 1)
+                self._upload_history(q)
         self._words(live, rows, ids, shared, members[0] if members else 0)
         self._control_words(live)
         self.ctx.replay(self._recording(live, shared, own, True))
@@ -527,7 +538,7 @@ class BatchEngine:
         for q in range(live):
             s, o = self.sequences.get(q), off + 8 * q
             k = s.controls if s else Controls()
-            u[o: o + 4] = (len(s.tokens), s.n_prompt, len(k.bias), k.allowed is not None) if s else 0
+            u[o: o + 4] = (len(s), len(s.prompt), len(k.bias), k.allowed is not None) if s else 0
             f[o + 4: o + 7] = k.repetition, k.frequency, k.presence
         a.buffer.upload(off * 4, live * 32)
 

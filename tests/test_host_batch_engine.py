@@ -1,0 +1,136 @@
+"""CPU tests of BatchEngine's host side: what lies in the device's buffers when a step is replayed,
+with a context that keeps them in memory and computes nothing."""
+import numpy as np
+import pytest
+
+from skyla_hip import batch as B
+from skyla_hip import engine as E
+
+
+class _Buffer:
+    """A buffer whose device side is an array of its own, reached by upload and download alone."""
+
+    def __init__(self, size):
+        self.size, self.mirror, self.device = size, np.zeros(size, np.uint8), np.zeros(size, np.uint8)
+
+    def host(self):
+        return self.mirror
+
+    def as_f32(self):
+        return self.mirror.view("<f4")
+
+    def as_u32(self):
+        return self.mirror.view("<u4")
+
+    def upload(self, off=0, length=None):
+        end = self.size if length is None else off + length
+        self.device[off:end] = self.mirror[off:end]
+
+    def download(self, off=0, length=None):
+        end = self.size if length is None else off + length
+        self.mirror[off:end] = self.device[off:end]
+
+    def copy_from(self, dst, src, at, length):
+        self.device[dst: dst + length] = src.device[at: at + length]
+
+    def free(self):
+        pass
+
+
+class _Context:
+    def __init__(self):
+        self.fails, self.steps = None, []
+
+    def alloc_host(self, size):
+        return _Buffer(size)
+
+    def max_buffer(self):
+        return 4 << 30
+
+    def record(self, profile, body):
+        if self.fails == "record":
+            raise MemoryError("record")
+        return object()
+
+    def replay(self, rec):
+        if self.fails == "replay":
+            raise RuntimeError("replay")
+        self.steps.append(self.eng.seen())
+
+
+class _Weights:
+    buffers, embd, layers, output, out_norm, rope = [_Buffer(64)], type("T", (), {"dtype": E.DType.Q8_0})(), [], None, 0, 0
+
+
+@pytest.fixture
+def make(monkeypatch):
+    """engine(...): a BatchEngine over such a context; its device's rows at each replay are in ctx.steps."""
+    for where, name in ((E, "load_weights"), (E, "Kernels"), (B, "BatchKernels"), (B, "LogitsKernels")):
+        monkeypatch.setattr(where, name, lambda *a, **k: _Weights())
+
+    class Engine(B.BatchEngine):
+        def seen(self):
+            """The live rows as the device has them: words, token, controls, history, biases, mask."""
+            u = self.arena.buffer.device.view("<u4").copy()
+            f, at, rows = u.view("<f4"), self.logits_at, []
+            for r in range(u[2]):
+                k = at.controls + 8 * r
+                h, b, m = (o + r * n for o, n in ((at.history, at.history_stride), (at.bias, at.bias_stride),
+                                                  (at.mask, at.mask_stride)))
+                bits = np.unpackbits(u[m: m + at.mask_stride].view(np.uint8), bitorder="little")[: self.c.n_vocab]
+                seq, n = (int(x) for x in u[self.at.rows + 4 * r:][:2])
+                table = u[self.at.table + seq * self.paged.seq_pages:][: -(-n // self.paged.page)]
+                rows.append(dict(
+                    seq=seq, len=n, share=int(u[self.at.rows + 4 * r + 2]), token=int(u[self.arena.tokens + r]),
+                    prompt=int(u[k + 1]), history=u[h: h + u[k]].tolist(), pages=table.tolist(),
+                    bias=dict(zip(u[b: b + 2 * u[k + 2]: 2].tolist(), f[b + 1: b + 1 + 2 * u[k + 2]: 2].tolist())),
+                    allowed=bits.astype(bool) if u[k + 3] else None, penalties=f[k + 4: k + 7].tolist()))
+                if r < self.max_seq:  # the device's answer: the row's token in every logit
+                    self.arena.buffer.device.view("<f4")[self.arena.extra["logits"] + r * self.s_vocab:][: self.c.n_vocab] = (
+                        rows[-1]["token"])
+            return rows
+
+    def engine(**over):
+        ctx = _Context()
+        c = E.Config(n_embd=256, n_ff=256, n_head=2, n_head_kv=1, head_dim=128, n_vocab=1000, n_layer=2)
+        eng = ctx.eng = Engine(ctx, {}, c, **(dict(max_ctx=300, n_pages=40, page=16, max_seq=6) | over))
+        return eng, ctx
+    return engine
+
+
+def _row(ctx, seq):
+    rows = [r for r in ctx.steps[-1] if r["len"] and r["seq"] == seq]
+    assert len(rows) == 1
+    return rows[0]
+
+
+def test_generated_tokens_stay_generated(make):
+    """A conversation: prompts and answers in turns.  The frequency and presence penalties count every
+    answer's tokens, none of the prompts'."""
+    eng, ctx = make()
+    a = eng.open()
+    eng.control(a, B.Controls(frequency=0.5))
+    eng.extend(a, [1, 2, 3])
+    eng.step({a: 4}, prompt=[a])
+    for t in (10, 11, 10):
+        eng.step({a: t})
+    eng.extend(a, [])
+    eng.step({a: 12})
+    r = _row(ctx, a)
+    assert (r["len"], r["prompt"], r["history"]) == (8, 4, [1, 2, 3, 4, 10, 11, 10, 12])
+    eng.extend(a, range(20, 29))
+    eng.step({a: 30}, prompt=[a])
+    eng.step({a: 13})
+    r = _row(ctx, a)
+    assert r["len"] == eng.length(a) == 19 and r["prompt"] == 14
+    assert r["history"] == [1, 2, 3, 4, *range(20, 29), 30, 10, 11, 10, 12, 13]
+    # a fork goes on from there, and penalties set later find the whole history
+    b = eng.fork(a)
+    eng.control(a, B.Controls())
+    eng.step({a: 14, b: 15})
+    eng.step({a: 16})
+    eng.control(a, B.Controls(presence=1.0))
+    eng.step({a: 17, b: 18}, prompt=[b])
+    assert _row(ctx, a)["history"] == [1, 2, 3, 4, *range(20, 29), 30, 10, 11, 10, 12, 13, 14, 16, 17]
+    assert _row(ctx, b)["history"] == [1, 2, 3, 4, *range(20, 29), 30, 18, 10, 11, 10, 12, 13, 15]
+    assert (_row(ctx, a)["prompt"], _row(ctx, b)["prompt"]) == (14, 15)
