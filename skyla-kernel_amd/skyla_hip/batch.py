@@ -325,16 +325,24 @@ class BatchEngine:
         del self.sequences[seq]
 
     def control(self, seq: int, controls: Controls) -> None:
-        """Sets what acts on a sequence's logits from its next step on."""
+        """Sets what acts on a sequence's logits from its next step on: `controls` as they are now (what
+        the caller changes in them later acts on nothing)."""
         s = self._get(seq)
-        values = [controls.repetition, controls.frequency, controls.presence, *controls.bias.values()]
-        if not controls.repetition > 0 or any(np.isnan(v) for v in values) or not np.isfinite(values[:3]).all():
-            raise ValueError("a repetition penalty above 0, finite penalties, biases that are numbers")
-        if len(controls.bias) > self.MAX_BIASES or any(not 0 <= int(t) < self.c.n_vocab for t in controls.bias):
+        with np.errstate(over="ignore", under="ignore"):  # as the kernel has them
+            penalties = np.float32([controls.repetition, controls.frequency, controls.presence])
+        if not penalties[0] > 0 or not np.isfinite(penalties).all():
+            raise ValueError("a repetition penalty above 0 and finite penalties, in 32 bits")
+        bias = {int(t): float(v) for t, v in controls.bias.items()}
+        if any(np.isnan(v) for v in bias.values()):
+            raise ValueError("biases that are numbers")
+        if len(bias) > self.MAX_BIASES or any(not 0 <= t < self.c.n_vocab for t in bias):
             raise ValueError(f"at most {self.MAX_BIASES} biases, of tokens of the vocabulary")
-        if controls.allowed is not None and np.shape(controls.allowed) != (self.c.n_vocab,):
-            raise ValueError(f"allowed: a truth value for each of {self.c.n_vocab} tokens")
-        s.controls = controls
+        allowed = controls.allowed
+        if allowed is not None:
+            if np.shape(allowed) != (self.c.n_vocab,):
+                raise ValueError(f"allowed: a truth value for each of {self.c.n_vocab} tokens")
+            allowed = np.array(allowed, bool)
+        s.controls = Controls(*(float(v) for v in penalties), bias, allowed)
         self._upload_controls(seq)
 
     # ---- pages ----
@@ -404,7 +412,8 @@ class BatchEngine:
         n = len(k.bias)
         if n:
             u[bias: bias + 2 * n: 2] = list(k.bias)
-            f[bias + 1: bias + 2 * n: 2] = list(k.bias.values())
+            with np.errstate(over="ignore", under="ignore"):
+                f[bias + 1: bias + 2 * n: 2] = list(k.bias.values())
             a.buffer.upload(bias * 4, n * 8)
         if k.allowed is not None:
             mask = self.logits_at.mask + self.s_mask * seq

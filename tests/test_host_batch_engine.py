@@ -134,3 +134,41 @@ def test_generated_tokens_stay_generated(make):
     assert _row(ctx, a)["history"] == [1, 2, 3, 4, *range(20, 29), 30, 10, 11, 10, 12, 13, 14, 16, 17]
     assert _row(ctx, b)["history"] == [1, 2, 3, 4, *range(20, 29), 30, 18, 10, 11, 10, 12, 13, 15]
     assert (_row(ctx, a)["prompt"], _row(ctx, b)["prompt"]) == (14, 15)
+
+
+def test_controls_are_taken_as_they_are(make):
+    """What the caller does to its Controls, or to what they hold, after control() acts on nothing; a
+    fork's are its own."""
+    eng, ctx = make()
+    a = eng.open()
+    allowed, bias = np.arange(1000) % 3 == 0, {5: 1.5, 7: -np.inf}
+    k = B.Controls(repetition=1.25, bias=bias, allowed=allowed)
+    eng.control(a, k)
+    b = eng.fork(a)
+    k.repetition, k.frequency, bias[9], allowed[:] = 3.0, 1.0, 2.0, False
+    del bias[5]
+    k.allowed = None
+    eng.control(b, B.Controls(presence=0.5, bias={1: 1.0}))
+    eng.step({a: 20, b: 21})
+    for want, seq in ((([1.25, 0, 0], {5: 1.5, 7: -np.inf}, np.arange(1000) % 3 == 0, [20]), a),
+                      (([1.0, 0, 0.5], {1: 1.0}, None, [21]), b)):
+        r = _row(ctx, seq)
+        assert (r["penalties"], r["bias"], r["history"]) == (want[0], want[1], want[3])
+        assert np.array_equal(r["allowed"], want[2]) if want[2] is not None else r["allowed"] is None
+    k = B.Controls()
+    eng.control(a, k)
+    k.repetition, k.bias[3] = 2.0, 1.0
+    eng.step({a: 22})
+    assert (_row(ctx, a)["penalties"], _row(ctx, a)["bias"]) == ([1, 0, 0], {})
+
+
+@pytest.mark.parametrize("bad", [dict(repetition=1e-50), dict(repetition=1e39), dict(frequency=-1e39), dict(presence=1e300),
+                                 dict(repetition=np.nan), dict(bias={-1: 0.0}), dict(allowed=True)])
+def test_controls_beyond_32_bits_are_refused(make, bad):
+    eng, ctx = make()
+    a = eng.open()
+    eng.control(a, B.Controls(repetition=1.5))
+    with pytest.raises(ValueError):
+        eng.control(a, B.Controls(**bad))
+    eng.step({a: 1})
+    assert _row(ctx, a)["penalties"] == [1.5, 0, 0]
