@@ -213,9 +213,18 @@ class _Sequence:
     def __len__(self):
         return len(self.prompt) + len(self.made)
 
-    def add_prompt(self, tokens):
-        self.placed = min(self.placed, len(self.prompt))
-        self.prompt += tokens
+    def add(self, tokens, prompt):
+        if prompt:
+            self.placed = min(self.placed, len(self.prompt))
+            self.prompt += tokens
+        else:
+            self.made += tokens
+
+    def drop(self, n, prompt):
+        """Takes the last n tokens of add back."""
+        keep = self.prompt if prompt else self.made
+        del keep[len(keep) - n:]
+        self.placed = min(self.placed, len(self.prompt) if prompt else len(self))
 
 
 class _BatchGraph(E.Graph):
@@ -359,6 +368,13 @@ class BatchEngine:
             if self.uses[p] == 0:
                 self.free_pages.append(p)
 
+    def _trim(self, seq: int) -> None:
+        """Gives back the pages past a sequence's last."""
+        s = self._get(seq)
+        keep = -(-len(s) // self.paged.page)
+        self._give(s.pages[keep:])
+        del s.pages[keep:]
+
     def _copy_page(self, src: int, dst: int, n: int) -> None:
         lay, page, dim = self.paged.layout, self.paged.page, self.c.n_head_kv * self.c.head_dim
         pr = lay.precision
@@ -481,14 +497,18 @@ class BatchEngine:
         time.  What it generated before counts as generated still."""
         s, tokens = self._get(seq), self._check(tokens)
         self._room({seq: len(tokens)})
-        for i in range(0, len(tokens), E.BATCH):
-            chunk, pos = tokens[i: i + E.BATCH], len(s)
-            n = len(chunk)
-            rows = np.zeros((n, 4), np.uint32)
-            rows[:, 0], rows[:, 1], rows[:, 2] = seq, pos + 1 + np.arange(n), pos
-            self._words(n, rows, chunk, pos, seq)
-            self.ctx.replay(self._recording(n, pos, n, False))
-            s.add_prompt(chunk)
+        try:
+            for i in range(0, len(tokens), E.BATCH):
+                chunk, pos = tokens[i: i + E.BATCH], len(s)
+                n = len(chunk)
+                rows = np.zeros((n, 4), np.uint32)
+                rows[:, 0], rows[:, 1], rows[:, 2] = seq, pos + 1 + np.arange(n), pos
+                self._words(n, rows, chunk, pos, seq)
+                self.ctx.replay(self._recording(n, pos, n, False))
+                s.add(chunk, True)
+        except BaseException:  # what was decoded stays
+            self._trim(seq)
+            raise
 
     def shared_run(self, seqs) -> tuple[int, list[int]]:
         """The positions that sequences of a step read once for all: (how many, whose).  Of the
@@ -517,22 +537,15 @@ class BatchEngine:
         if any(q not in tokens for q in prompt):
             raise ValueError("prompt: sequences of this step")
         self._room({q: 1 for q in seqs})
-        live = max(seqs) + 1
-        shared, members = self.shared_run(seqs)
-        rows, ids, own = np.zeros((live, 4), np.uint32), np.zeros(live, np.uint32), 1
         for q, t in zip(seqs, values):
-            s = self._get(q)
-            if q in prompt:
-                s.add_prompt([t])
-            else:
-                s.made.append(t)
-            n, take = len(s), shared if q in members and len(s) >= shared else 0
-            rows[q], ids[q], own = (q, n, take, 0), t, max(own, n - take)
-            if s.controls.counts:
-                self._upload_history(q)
-        self._words(live, rows, ids, shared, members[0] if members else 0)
-        self._control_words(live)
-        self.ctx.replay(self._recording(live, shared, own, True))
+            self._get(q).add([t], q in prompt)
+        try:
+            self._replay_step(seqs, values)
+        except BaseException:  # nothing was decoded: the sequences are as they were
+            for q in seqs:
+                self._get(q).drop(1, q in prompt)
+                self._trim(q)
+            raise
         a, v = self.arena, self.c.n_vocab
         out = np.empty((len(seqs), v), np.float32)
         for i, q in enumerate(seqs):
@@ -540,6 +553,21 @@ class BatchEngine:
             a.buffer.download(off * 4, v * 4)
             out[i] = a.f32()[off: off + v]
         return out
+
+    def _replay_step(self, seqs: list[int], values: list[int]) -> None:
+        """One row for each of the sequences' last tokens, through the model and its head."""
+        live = max(seqs) + 1
+        shared, members = self.shared_run(seqs)
+        rows, ids, own = np.zeros((live, 4), np.uint32), np.zeros(live, np.uint32), 1
+        for q, t in zip(seqs, values):
+            s = self._get(q)
+            n, take = len(s), shared if q in members and len(s) >= shared else 0
+            rows[q], ids[q], own = (q, n, take, 0), t, max(own, n - take)
+            if s.controls.counts:
+                self._upload_history(q)
+        self._words(live, rows, ids, shared, members[0] if members else 0)
+        self._control_words(live)
+        self.ctx.replay(self._recording(live, shared, own, True))
 
     def _control_words(self, live: int) -> None:
         a, off = self.arena, self.logits_at.controls

@@ -172,3 +172,31 @@ def test_controls_beyond_32_bits_are_refused(make, bad):
         eng.control(a, B.Controls(**bad))
     eng.step({a: 1})
     assert _row(ctx, a)["penalties"] == [1.5, 0, 0]
+
+
+@pytest.mark.parametrize("where", ["record", "replay"])
+def test_a_step_that_fails_leaves_the_sequences_as_they_were(make, where):
+    eng, ctx = make()
+    a, b = eng.open(), eng.open()
+    eng.control(a, B.Controls(frequency=1.0))
+    eng.control(b, B.Controls(repetition=1.5))
+    eng.extend(a, range(16))   # a page is full: the next token needs another
+    eng.extend(b, [1, 2])
+    eng.step({b: 3})
+    kept = eng.recordings
+    for prompt in ((), [b]):
+        free, ctx.fails, eng.recordings = len(eng.free_pages), where, {}
+        with pytest.raises((MemoryError, RuntimeError)):
+            eng.step({a: 50, b: 51}, prompt=prompt)
+        assert (eng.length(a), eng.length(b), len(eng.free_pages)) == (16, 3, free)
+    with pytest.raises((MemoryError, RuntimeError)):
+        eng.extend(a, range(100, 200))
+    assert (eng.length(a), len(eng.free_pages)) == (16, free)
+    ctx.fails, eng.recordings = None, kept
+    eng.step({a: 60, b: 61})
+    r, s = _row(ctx, a), _row(ctx, b)
+    assert (r["len"], r["prompt"], r["history"]) == (17, 16, [*range(16), 60])
+    assert (s["len"], s["prompt"], s["history"]) == (4, 2, [1, 2, 3, 61])
+    eng.close(a)
+    eng.close(b)
+    assert len(eng.free_pages) == 40 and not eng.uses.any()
