@@ -533,7 +533,7 @@ class BatchEngine:
         generated)."""
         if not tokens:
             raise ValueError("step needs a token of at least one sequence")
-        values, seqs = self._check(tokens.values()), list(tokens)
+        values, seqs, prompt = self._check(tokens.values()), list(tokens), set(prompt)
         if any(q not in tokens for q in prompt):
             raise ValueError("prompt: sequences of this step")
         self._room({q: 1 for q in seqs})

@@ -200,3 +200,16 @@ def test_a_step_that_fails_leaves_the_sequences_as_they_were(make, where):
     eng.close(a)
     eng.close(b)
     assert len(eng.free_pages) == 40 and not eng.uses.any()
+
+
+def test_prompt_may_be_any_iterable(make):
+    eng, ctx = make()
+    a = eng.open()
+    eng.control(a, B.Controls(presence=1.0))
+    eng.step({a: 1}, prompt=(q for q in [a]))
+    eng.step({a: 2}, prompt=iter([a]))
+    eng.step({a: 3})
+    assert (_row(ctx, a)["prompt"], _row(ctx, a)["history"]) == (2, [1, 2, 3])
+    with pytest.raises(ValueError):
+        eng.step({a: 4}, prompt=(q for q in [a, 5]))
+    assert eng.length(a) == 3
