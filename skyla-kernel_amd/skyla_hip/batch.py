@@ -203,12 +203,13 @@ class Controls:
 
 class _Sequence:
     """A sequence's pages, the tokens of its prompts and those that it generated (a conversation's
-    follow in turns; what acts on the logits asks only which), its controls, and how many words of
-    its history, the prompts' tokens before the others, lie in the arena."""
+    follow in turns; what acts on the logits asks only which), its controls, the row of the batch
+    that these lie in (None: they do not), and how many words of its history, the prompts' tokens
+    before the others, lie there."""
 
     def __init__(self, pages=(), prompt=(), made=(), controls=None):
         self.pages, self.prompt, self.made = list(pages), list(prompt), list(made)
-        self.controls, self.placed = controls or Controls(), 0
+        self.controls, self.row, self.placed = controls or Controls(), None, 0
 
     def __len__(self):
         return len(self.prompt) + len(self.made)
@@ -253,8 +254,10 @@ class BatchEngine:
     and returns the logits after them, with their controls applied; close() gives its pages back.
 
     A forked sequence shares the whole pages of the one it came from (the rest of the last page is
-    copied), and a step reads the pages that its sequences share once for all of them.  A
-    sequence's row in the batch is its number: sequences that a step leaves out are idle rows."""
+    copied), and a step reads the pages that its sequences share once for all of them.  A step has a
+    row for each of its sequences and no others, so that it takes what it would if they were the only
+    ones open; a sequence keeps its row from step to step while it can, since what acts on logits
+    lies by rows."""
 
     MAX_BIASES = 512
 
@@ -293,6 +296,7 @@ class BatchEngine:
         self.free_pages = list(range(n_pages - 1, -1, -1))
         self.uses = np.zeros(n_pages, np.int64)  # sequences that hold a page
         self.sequences: dict[int, _Sequence] = {}
+        self.rows: list[int | None] = [None] * max_seq  # the sequence whose controls lie in a row
 
     # ---- sequences ----
     def open(self) -> int:
@@ -303,7 +307,6 @@ class BatchEngine:
         if n is None:
             raise ValueError(f"all {self.max_seq} sequences are open")
         self.sequences[n] = s
-        self._upload_controls(n)
         return n
 
     def _get(self, seq: int) -> _Sequence:
@@ -330,7 +333,10 @@ class BatchEngine:
         return n
 
     def close(self, seq: int) -> None:
-        self._give(self._get(seq).pages)
+        s = self._get(seq)
+        self._give(s.pages)
+        if s.row is not None:
+            self.rows[s.row] = None
         del self.sequences[seq]
 
     def control(self, seq: int, controls: Controls) -> None:
@@ -352,7 +358,8 @@ class BatchEngine:
                 raise ValueError(f"allowed: a truth value for each of {self.c.n_vocab} tokens")
             allowed = np.array(allowed, bool)
         s.controls = Controls(*(float(v) for v in penalties), bias, allowed)
-        self._upload_controls(seq)
+        if s.row is not None:
+            self._upload_controls(seq)
 
     # ---- pages ----
     def _take(self, n: int) -> list[int]:
@@ -404,6 +411,21 @@ class BatchEngine:
                 self._upload_table(seq)
 
     # ---- words ----
+    def _place(self, seqs: list[int]) -> None:
+        """Gives the sequences rows 0 to len(seqs) - 1, each the one it has where that is among them."""
+        free = [r for r in range(len(seqs)) if self.rows[r] not in seqs]
+        for q in seqs:
+            s = self._get(q)
+            if s.row is not None and s.row < len(seqs):
+                continue
+            if s.row is not None:
+                self.rows[s.row] = None
+            s.row, s.placed = free.pop(0), 0
+            if self.rows[s.row] is not None:
+                self._get(self.rows[s.row]).row = None
+            self.rows[s.row] = q
+            self._upload_controls(q)
+
     def _upload_table(self, seq: int) -> None:
         a, pages = self.arena, self._get(seq).pages
         off = self.at.table + seq * self.paged.seq_pages
@@ -415,16 +437,16 @@ class BatchEngine:
         a, s = self.arena, self._get(seq)
         n = s.placed - len(s.prompt)
         new = s.made[n:] if n >= 0 else s.prompt[n:] + s.made
-        off = self.logits_at.history + seq * self.s_hist + s.placed
+        off = self.logits_at.history + s.row * self.s_hist + s.placed
         if new:
             a.u32()[off: off + len(new)] = new
             a.buffer.upload(off * 4, len(new) * 4)
         s.placed = len(s)
 
     def _upload_controls(self, seq: int) -> None:
-        a, k = self.arena, self._get(seq).controls
-        u, f = a.u32(), a.f32()
-        bias = self.logits_at.bias + 2 * self.MAX_BIASES * seq
+        a, s = self.arena, self._get(seq)
+        k, u, f = s.controls, a.u32(), a.f32()
+        bias = self.logits_at.bias + 2 * self.MAX_BIASES * s.row
         n = len(k.bias)
         if n:
             u[bias: bias + 2 * n: 2] = list(k.bias)
@@ -432,7 +454,7 @@ class BatchEngine:
                 f[bias + 1: bias + 2 * n: 2] = list(k.bias.values())
             a.buffer.upload(bias * 4, n * 8)
         if k.allowed is not None:
-            mask = self.logits_at.mask + self.s_mask * seq
+            mask = self.logits_at.mask + self.s_mask * s.row
             bits = np.zeros(32 * self.s_mask, bool)
             bits[: self.c.n_vocab] = k.allowed
             u[mask: mask + self.s_mask] = np.packbits(bits, bitorder="little").view("<u4")
@@ -549,20 +571,21 @@ class BatchEngine:
         a, v = self.arena, self.c.n_vocab
         out = np.empty((len(seqs), v), np.float32)
         for i, q in enumerate(seqs):
-            off = a.extra["logits"] + q * self.s_vocab
+            off = a.extra["logits"] + self._get(q).row * self.s_vocab
             a.buffer.download(off * 4, v * 4)
             out[i] = a.f32()[off: off + v]
         return out
 
     def _replay_step(self, seqs: list[int], values: list[int]) -> None:
         """One row for each of the sequences' last tokens, through the model and its head."""
-        live = max(seqs) + 1
+        self._place(seqs)
+        live = len(seqs)
         shared, members = self.shared_run(seqs)
         rows, ids, own = np.zeros((live, 4), np.uint32), np.zeros(live, np.uint32), 1
         for q, t in zip(seqs, values):
             s = self._get(q)
             n, take = len(s), shared if q in members and len(s) >= shared else 0
-            rows[q], ids[q], own = (q, n, take, 0), t, max(own, n - take)
+            rows[s.row], ids[s.row], own = (q, n, take, 0), t, max(own, n - take)
             if s.controls.counts:
                 self._upload_history(q)
         self._words(live, rows, ids, shared, members[0] if members else 0)
@@ -572,10 +595,10 @@ class BatchEngine:
     def _control_words(self, live: int) -> None:
         a, off = self.arena, self.logits_at.controls
         u, f = a.u32(), a.f32()
-        for q in range(live):
-            s, o = self.sequences.get(q), off + 8 * q
-            k = s.controls if s else Controls()
-            u[o: o + 4] = (len(s), len(s.prompt), len(k.bias), k.allowed is not None) if s else 0
+        for r in range(live):
+            s, o = self._get(self.rows[r]), off + 8 * r
+            k = s.controls
+            u[o: o + 4] = len(s), len(s.prompt), len(k.bias), k.allowed is not None
             f[o + 4: o + 7] = k.repetition, k.frequency, k.presence
         a.buffer.upload(off * 4, live * 32)
 

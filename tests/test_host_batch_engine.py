@@ -213,3 +213,39 @@ def test_prompt_may_be_any_iterable(make):
     with pytest.raises(ValueError):
         eng.step({a: 4}, prompt=(q for q in [a, 5]))
     assert eng.length(a) == 3
+
+
+def test_a_step_has_a_row_for_each_of_its_sequences(make):
+    """Whichever numbers the sequences have, a step's rows are theirs and no idle ones, with their own
+    controls, histories and pages."""
+    eng, ctx = make()
+    g, told = np.random.default_rng(1), {}
+    for q in range(6):
+        assert eng.open() == q
+        k = B.Controls(repetition=1 + q / 8, presence=q / 4, bias={q: 1.0 + q} if q % 2 else {},
+                       allowed=np.arange(1000) % (q + 2) == 0 if q > 2 else None)
+        eng.control(q, k)
+        eng.extend(q, [100 + q] * (10 + q))
+        told[q] = k, [100 + q] * (10 + q)
+    eng.step({4: 9})
+    assert len(ctx.steps[-1]) == 1 and _row(ctx, 4)["token"] == 9
+    told[4][1].append(9)
+    for step in range(40):
+        seqs = [int(q) for q in g.permutation(6)[: g.integers(1, 7)]]
+        if step == 20:  # a sequence goes, another comes in its place
+            eng.close(3)
+            assert eng.open() == 3
+            told[3] = B.Controls(), []
+        out = eng.step({q: 10 * step + q for q in seqs})
+        assert out[:, 0].tolist() == [10 * step + q for q in seqs]  # each its own row's answer
+        assert len(ctx.steps[-1]) == len(seqs)
+        for q in seqs:
+            k, history = told[q]
+            history.append(10 * step + q)
+            r = _row(ctx, q)
+            assert (r["len"], r["token"], r["bias"], r["penalties"]) == (
+                len(history), history[-1], k.bias, [k.repetition, k.frequency, k.presence])
+            if k.counts:
+                assert r["history"] == history
+            assert r["pages"] == eng.sequences[q].pages
+            assert np.array_equal(r["allowed"], k.allowed) if k.allowed is not None else r["allowed"] is None
