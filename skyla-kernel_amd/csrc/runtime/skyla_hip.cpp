@@ -1216,7 +1216,10 @@ Command dispatch_command(const skyla_hip_pipeline *p, const std::vector<void *> 
 int check_batch(const skyla_hip_pipeline *p, uint32_t set, const uint32_t *groups, const uint32_t *push,
                 const char *what) {
   if (!p->batch) return SKYLA_HIP_OK;
-  const std::string why = batch::refusal(p->batch, p->spec.data(), push, groups, p->set_bytes[set].data());
+  std::vector<uint64_t> at;
+  for (const void *b : p->sets[set]) at.push_back((uint64_t)(uintptr_t)b);
+  const std::string why =
+      batch::refusal(p->batch, p->spec.data(), push, groups, p->set_bytes[set].data(), at.data());
   if (why.empty()) return SKYLA_HIP_OK;
   return fail(SKYLA_HIP_E_ARG, "%s: %s: %s", what, p->symbol.c_str(), why.c_str());
 }
