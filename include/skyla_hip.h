@@ -140,8 +140,9 @@ uint32_t skyla_hip_recording_launches(const skyla_hip_recording *rec);
 /* Context::replay: run the recording (as one HIP graph, or, one of at most six launches, as
  * those launches) and wait for it. */
 int skyla_hip_replay(skyla_hip_context *ctx, const skyla_hip_recording *rec);
-/* Replay and report the device time between its first and last work, in ns, measured
- * with HIP events on the context stream. */
+/* Replay as one HIP graph (made on the first such call of a recording of at most six launches)
+ * and report the device time between its first and last work, in ns, measured with HIP events
+ * on the context stream. */
 int skyla_hip_replay_timed(skyla_hip_context *ctx, const skyla_hip_recording *rec,
                            double *ns);
 /* Context::marks (record.rs:137-148): for a profiled recording, after a replay.

@@ -64,9 +64,10 @@ int fail(int code, const char *fmt, ...) {
 constexpr uint64_t kMaxBuffer = 4ull << 30;  // keeps u32 element offsets valid
 constexpr uint32_t kMaxMarks = 2048;          // skyla-vk/src/record.rs:6
 constexpr uint64_t kMaxPinned = 1ull << 30;   // host mirrors pinned up to this size
-// Recordings of at most this many launches replay as direct launches: a graph's submission costs
-// a fixed 30 us of host time, a launch of its own 3 (us a replay of small kernels, graph / direct:
-// 1 launch 29.8 / 12.0, 2 30.2 / 15.2, 4 30.5 / 20.3, 6 32 / 25.4, 8 32.4 / 48, 12 38.9 / 64).
+// Recordings of at most this many launches replay as direct launches: a replay as a graph takes 31
+// us of host time and wait, as launches 9 and 2.2 for each up to seven, the eighth 20 more (us a
+// replay of small kernels, graph / direct: 1 launch 31.1 / 11.6, 2 31.4 / 14.4, 4 31.4 / 18.5, 6 34.3 /
+// 22.8, 7 35 / 25, 8 31.3 / 44.8, 12 36.9 / 58.6).  Six keep one away from that step.
 constexpr uint32_t kDirectLaunches = 6;
 
 // Tactics: every choice the runtime makes between kernel forms that compute the same
@@ -1151,6 +1152,8 @@ struct skyla_hip_recorder {
 struct skyla_hip_recording {
   skyla_hip_context *ctx = nullptr;
   bool profile = false;
+  bool direct = false;      // never as a graph
+  bool short_list = false;  // replayed as direct launches; its graph is made where a replay is timed
   std::vector<Command> cmds;
   std::vector<Launch> launches;
   void *workspace = nullptr;  // K-split partials and counters of the launches
@@ -1920,6 +1923,37 @@ int skyla_hip_record_mark(skyla_hip_recorder *r, const char *label) {
   return SKYLA_HIP_OK;
 }
 
+// One graph for the whole recording, captured from the launch list on the context stream (nothing
+// for one that replays as direct launches always, or that has its graph).
+static int make_graph(skyla_hip_recording *rec) {
+  if (rec->direct || rec->exec || skyla_hip_recording_len(rec) == 0) return SKYLA_HIP_OK;
+  skyla_hip_context *ctx = rec->ctx;
+  HIP_TRY(hipSetDevice(ctx->device));
+  HIP_TRY(hipStreamBeginCapture(ctx->stream, hipStreamCaptureModeThreadLocal));
+  int s = SKYLA_HIP_OK;
+  for (const Launch &l : rec->launches)
+    if (!l.mark && (s = launch(ctx->stream, l)) != SKYLA_HIP_OK) break;
+  hipGraph_t graph = nullptr;
+  hipError_t e = hipStreamEndCapture(ctx->stream, &graph);
+  if (s != SKYLA_HIP_OK) {
+    if (graph) hipGraphDestroy(graph);
+    return s;
+  }
+  if (e != hipSuccess)
+    return fail(SKYLA_HIP_E_DEVICE, "hipStreamEndCapture: %s", hipGetErrorString(e));
+  rec->graph = graph;
+  if (graph) {
+    e = hipGraphInstantiate(&rec->exec, graph, nullptr, nullptr, 0);
+    if (e != hipSuccess) {
+      hipGraphDestroy(graph);
+      rec->graph = nullptr;
+      rec->exec = nullptr;
+      return fail(SKYLA_HIP_E_DEVICE, "hipGraphInstantiate: %s", hipGetErrorString(e));
+    }
+  }
+  return SKYLA_HIP_OK;
+}
+
 int skyla_hip_record_end(skyla_hip_recorder *r, skyla_hip_recording **out) {
   if (!r) return fail(SKYLA_HIP_E_ARG, "record_end: null recorder");
   std::unique_ptr<skyla_hip_recorder> own(r);
@@ -1939,36 +1973,13 @@ int skyla_hip_record_end(skyla_hip_recorder *r, skyla_hip_recording **out) {
   rec->mark_ns.assign(rec->labels.size(), 0.0);
   HIP_TRY(hipSetDevice(rec->ctx->device));
   if (int s = bind_workspace(rec->launches, &rec->workspace)) return s;
-  // short lists, and all with the nograph tactic 1 (kernel traces of the exact launches a graph
-  // would hold, fused forms included), replay as direct launches
+  // the nograph tactic 1: every replay as direct launches (kernel traces of the exact launches a
+  // graph would hold, fused forms included); by default those of short lists
   const std::string nograph = tactic("nograph");
-  const bool direct = nograph.empty() ? skyla_hip_recording_launches(rec.get()) <= kDirectLaunches : nograph == "1";
-  if (!rec->profile && skyla_hip_recording_len(rec.get()) > 0 && !direct) {
-    // One graph for the whole recording, captured from the launch list on the stream.
-    skyla_hip_context *ctx = rec->ctx;
-    HIP_TRY(hipSetDevice(ctx->device));
-    HIP_TRY(hipStreamBeginCapture(ctx->stream, hipStreamCaptureModeThreadLocal));
-    int s = SKYLA_HIP_OK;
-    for (const Launch &l : rec->launches)
-      if (!l.mark && (s = launch(ctx->stream, l)) != SKYLA_HIP_OK) break;
-    hipGraph_t graph = nullptr;
-    hipError_t e = hipStreamEndCapture(ctx->stream, &graph);
-    if (s != SKYLA_HIP_OK) {
-      if (graph) hipGraphDestroy(graph);
-      return s;
-    }
-    if (e != hipSuccess)
-      return fail(SKYLA_HIP_E_DEVICE, "hipStreamEndCapture: %s", hipGetErrorString(e));
-    rec->graph = graph;
-    if (graph) {
-      e = hipGraphInstantiate(&rec->exec, graph, nullptr, nullptr, 0);
-      if (e != hipSuccess) {
-        hipGraphDestroy(graph);
-        rec->graph = nullptr;
-        return fail(SKYLA_HIP_E_DEVICE, "hipGraphInstantiate: %s", hipGetErrorString(e));
-      }
-    }
-  }
+  rec->direct = rec->profile || nograph == "1";
+  rec->short_list = nograph.empty() && skyla_hip_recording_launches(rec.get()) <= kDirectLaunches;
+  if (!rec->short_list)
+    if (int s = make_graph(rec.get())) return s;
   *out = rec.release();
   return SKYLA_HIP_OK;
 }
@@ -1991,10 +2002,11 @@ uint32_t skyla_hip_recording_launches(const skyla_hip_recording *rec) {
 
 namespace {
 
-// Launches a recording on the context stream.  With `events`, one event is recorded at
-// the start and one at every mark.
-static int submit(skyla_hip_context *ctx, const skyla_hip_recording *rec, std::vector<hipEvent_t> *events) {
-  if (rec->exec && !events) {
+// Launches a recording on the context stream, as its graph where `graph` and it has one.  With
+// `events`, one event is recorded at the start and one at every mark.
+static int submit(skyla_hip_context *ctx, const skyla_hip_recording *rec, bool graph,
+                  std::vector<hipEvent_t> *events) {
+  if (graph && rec->exec && !events) {
     HIP_TRY(hipGraphLaunch(rec->exec, ctx->stream));
     return SKYLA_HIP_OK;
   }
@@ -2030,7 +2042,7 @@ int skyla_hip_replay(skyla_hip_context *ctx, const skyla_hip_recording *rec) {
   if (rec->ctx != ctx) return fail(SKYLA_HIP_E_ARG, "replay: recording of another context");
   HIP_TRY(hipSetDevice(ctx->device));
   if (!rec->profile) {
-    int s = submit(ctx, rec, nullptr);
+    int s = submit(ctx, rec, !rec->short_list, nullptr);
     if (s) return s;
     HIP_TRY(hipStreamSynchronize(ctx->stream));
     return SKYLA_HIP_OK;
@@ -2038,7 +2050,7 @@ int skyla_hip_replay(skyla_hip_context *ctx, const skyla_hip_recording *rec) {
   Events e;
   int s = e.make(rec->labels.size() + 1);
   if (s) return s;
-  s = submit(ctx, rec, &e.ev);
+  s = submit(ctx, rec, false, &e.ev);
   if (s) return s;
   HIP_TRY(hipStreamSynchronize(ctx->stream));
   auto *mut = const_cast<skyla_hip_recording *>(rec);
@@ -2055,11 +2067,13 @@ int skyla_hip_replay_timed(skyla_hip_context *ctx, const skyla_hip_recording *re
   if (!ctx || !rec || !ns) return fail(SKYLA_HIP_E_ARG, "replay_timed: bad argument");
   if (rec->ctx != ctx) return fail(SKYLA_HIP_E_ARG, "replay_timed: recording of another context");
   HIP_TRY(hipSetDevice(ctx->device));
+  // as a graph, short lists too: launched one by one, the host's time between them would count
+  if (int s = make_graph(const_cast<skyla_hip_recording *>(rec))) return s;
   Events e;
   int s = e.make(2);
   if (s) return s;
   HIP_TRY(hipEventRecord(e.ev[0], ctx->stream));
-  s = submit(ctx, rec, nullptr);
+  s = submit(ctx, rec, true, nullptr);
   if (s) return s;
   HIP_TRY(hipEventRecord(e.ev[1], ctx->stream));
   HIP_TRY(hipEventSynchronize(e.ev[1]));
