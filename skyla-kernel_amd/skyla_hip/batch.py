@@ -86,16 +86,25 @@ def splits(rows: int, n_kv: int, rep: int, shared: int, own: int) -> Parts:
     fill the GPU's 256 compute units, each with some tiles of 64 positions.
 
     128 query rows a workgroup stage keys and values once for all of them and pay for it at the
-    start: us of the shared run, 16 rows / 128 rows a workgroup (8 key heads, f16 keys, 8-bit values),
-    64 query rows a key head over 500 positions 12.0 / 15.2, 8192 25.4 / 25.3, 32768 62 / 63; 128 over 500
-    12.2 / 16.4, 2000 19.2 / 18.3, 8192 37 / 29; 256 over 500 14.9 / 17.1, 2000 28 / 21."""
+    start, so they are taken where a key head has 64 query rows or more, and query rows, key heads and
+    positions make 1.5 Mi.  Attention and merge, us with 16 rows / 128 rows a workgroup, f16 and 8-bit
+    caches (f16 keys with 8-bit values between them); of 600 cases over 2, 4 and 8 key heads the line
+    is within 8% of the better form in 585:
+
+      8 key heads, 64 query rows of each, 2000 positions (1.0 Mi)  17.6 / 20.0  20.2 / 25.3
+      8, 64, 4000 (2.0 Mi)                                         24.8 / 23.0  28.3 / 28.0
+      8, 128, 1000 (1.0 Mi)                                        18.7 / 19.8  22.2 / 25.0
+      4, 256, 1000 (1.0 Mi)                                        17.4 / 19.7  20.1 / 24.8
+      2, 512, 2000 (2.0 Mi)                                        24.4 / 22.9  27.8 / 27.7
+      8, 32, 32768 (8.0 Mi, few rows)                              49.3 / 44.3  47.5 / 71.3
+      8, 512, 256 (1.0 Mi, the furthest off)                       24.1 / 20.3  28.5 / 25.0"""
     q, tiles, own_tiles = rows * rep, -(-shared // 64), -(-own // 64)
     # (a workgroup without a run costs as much as a short one: 128 rows of 8 key heads in 1 / 2 / 4 parts
     # 27 / 31 / 47 us; one row of 16384 positions in 16 / 32 / 64 20.2 / 15.3 / 16.1)
     n_own = max(1, min(-(-512 // (n_kv * rows)), -(-own_tiles // 4), 128))
     if shared == 0:
         return Parts(0, n_own)
-    if q > 64 and q * shared > 160 * 1024:
+    if q >= 64 and q * n_kv * shared >= 3 << 19:
         # one workgroup a compute unit, two where a part stays long: 512 query rows of 8 key heads over
         # 32768 positions 157 / 144 us with the merge, of 4 over 8192 56 / 71, of 8 over 4000 51 / 58
         groups = n_kv * -(-q // 128)

@@ -6,6 +6,7 @@ import subprocess
 import numpy as np
 import pytest
 
+from skyla_hip import batch as B
 from test_host_batch import RUNTIME, _append, _attend, _logits
 from test_host_batch_words import u32
 
@@ -106,3 +107,12 @@ def test_logits(shape, v):
             g, threads, form, extra = shape("logits_adjust", [0], _logits(v=v, hs=stride), rows)
             assert form == (stride >= 8192) and threads == (1024 if form else 256) and extra == []
             assert g == [-(-v // (16 * threads)), rows, 1]
+
+
+def test_the_shared_runs_form():
+    """128 query rows a workgroup on their side of the line, by key heads, query rows and positions."""
+    for n_kv, rep, rows, shared, wide in ((8, 4, 16, 2000, False), (8, 4, 16, 4000, True), (8, 4, 32, 1000, False),
+                                          (8, 4, 32, 2000, True), (4, 8, 32, 1000, False), (2, 8, 64, 2000, True),
+                                          (2, 8, 64, 1000, False), (8, 2, 16, 100000, False), (8, 1, 64, 3500, True),
+                                          (1, 1, 64, 24575, False), (1, 1, 64, 24576, True)):
+        assert B.splits(rows, n_kv, rep, shared, 1).wide == wide, (n_kv, rep, rows, shared)
