@@ -234,7 +234,9 @@ SK_DEV void weigh(float a, float b, float inv, float c, float &l, f16x8 &ph, f16
   const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(b, inv, c));
   l += x;
   l += y;
-  const f16x2 hi = pack_f16x2(x, y);
+  uint32_t both = as_u32(pack_f16x2(x, y));
+  asm("" : "+v"(both));  // known as a word alone: the compiler would round x and y again for the next line
+  const f16x2 hi = as_f16x2(both);
   const f16x2 lo = pack_f16x2(__builtin_fmaf((float)hi.x, -1.0f, x), __builtin_fmaf((float)hi.y, -1.0f, y));
   ph[e] = hi.x, ph[e + 1] = hi.y;
   pl[e] = lo.x, pl[e + 1] = lo.y;
