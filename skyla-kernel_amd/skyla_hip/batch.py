@@ -122,8 +122,7 @@ class BatchKernels:
     """kv_append and attention_paged over one pool buffer for each layer."""
 
     def __init__(self, ctx: Context, tables: Buffer, a: Buffer, pools: Sequence[Buffer], c: E.Config, paged: Paged):
-        if c.head_dim != 128 or c.n_head % c.n_head_kv or c.n_head // c.n_head_kv not in (1, 2, 4, 8):
-            raise ValueError(f"no batch attention kernels for head_dim {c.head_dim}, {c.n_head}/{c.n_head_kv} heads")
+        self.check(c)
         if paged.layout.per_layer != paged.n_pages * paged.page * c.n_head_kv * c.head_dim:
             raise ValueError("the pool's rows are not the model's")
         if any(b.size < paged.bytes() for b in pools):
@@ -141,6 +140,11 @@ class BatchKernels:
         self._attend = build("attention_paged", [a, a], 20, [c.n_head // c.n_head_kv, k8, v8, 128])
         self._merge = ctx.create_pipeline("attention_paged_merge", 2, 40, [128])
         self._merge.bind_buffers([a, a])
+
+    @staticmethod
+    def check(c: E.Config) -> None:
+        if c.head_dim != 128 or c.n_head % c.n_head_kv or c.n_head // c.n_head_kv not in (1, 2, 4, 8):
+            raise ValueError(f"no batch attention kernels for head_dim {c.head_dim}, {c.n_head}/{c.n_head_kv} heads")
 
     def _pages(self) -> list[int]:
         p = self.paged
@@ -276,6 +280,7 @@ class BatchEngine:
             raise ValueError(f"{max_seq} sequences: a batch holds 1 to {E.BATCH}")
         if max_ctx < 1:
             raise ValueError(f"max_ctx {max_ctx}")
+        BatchKernels.check(c)
         self.ctx, self.c, self.max_ctx, self.max_seq = ctx, c, max_ctx, max_seq
         self.paged = Paged(precision, page, n_pages, max_seq, min(-(-max_ctx // page), n_pages),
                            c.n_head_kv * c.head_dim)
@@ -287,13 +292,28 @@ class BatchEngine:
         self.s_hist = -(-max_ctx // 4) * 4
         part = max(part_size(r, c.n_head, self._parts(r, shared, own)) for r in self._buckets(E.BATCH)
                    for shared in [0, *self._buckets(max_ctx)] for own in self._buckets(max_ctx))
+        self.weights = self.arena = self.batch = self.logits = None
+        self.pools, self.recordings = [], {}
+        try:
+            self._allocate(model, precision, part)
+        except BaseException:  # as where the card has no room for so many pages
+            self.free()
+            raise
+        self.free_pages = list(range(n_pages - 1, -1, -1))
+        self.uses = np.zeros(n_pages, np.int64)  # sequences that hold a page
+        self.sequences: dict[int, _Sequence] = {}
+        self.rows: list[int | None] = [None] * max_seq  # the sequence whose controls lie in a row
+
+    def _allocate(self, model: dict, precision: E.KvPrecision, part: int) -> None:
+        ctx, c, max_seq = self.ctx, self.c, self.max_seq
         self.weights = E.load_weights(ctx, model, c)
         a = self.arena = E.Arena(ctx, c, extra={
             "rows": 4 * E.BATCH, "table": max_seq * self.paged.seq_pages, "part": part,
             "logits": self.s_vocab * max_seq, "controls": 8 * max_seq, "history": self.s_hist * max_seq,
             "bias": 2 * self.MAX_BIASES * max_seq, "mask": self.s_mask * max_seq})
         x = a.extra
-        self.pools = [ctx.alloc_host(self.paged.bytes()) for _ in range(c.n_layer)]
+        for _ in range(c.n_layer):
+            self.pools.append(ctx.alloc_host(self.paged.bytes()))
         self.at = BatchRegions(rows=x["rows"], table=x["table"], part=x["part"])
         self.logits_at = LogitsRegions(x["controls"], x["history"], self.s_hist, x["bias"], 2 * self.MAX_BIASES,
                                        x["mask"], self.s_mask)
@@ -301,11 +321,6 @@ class BatchEngine:
                                  embd_dtype=self.weights.embd.dtype)
         self.batch = BatchKernels(ctx, self.weights.buffers[0], a.buffer, self.pools, c, self.paged)
         self.logits = LogitsKernels(ctx, a.buffer)
-        self.recordings = {}
-        self.free_pages = list(range(n_pages - 1, -1, -1))
-        self.uses = np.zeros(n_pages, np.int64)  # sequences that hold a page
-        self.sequences: dict[int, _Sequence] = {}
-        self.rows: list[int | None] = [None] * max_seq  # the sequence whose controls lie in a row
 
     # ---- sequences ----
     def open(self) -> int:
@@ -334,9 +349,13 @@ class BatchEngine:
         if len(self.sequences) == self.max_seq:
             raise ValueError(f"all {self.max_seq} sequences are open")
         own = self._take(1 if rest else 0)
+        try:
+            if rest:
+                self._copy_page(s.pages[whole], own[0], rest)
+        except BaseException:
+            self._give(own)
+            raise
         self.uses[s.pages[:whole]] += 1
-        if rest:
-            self._copy_page(s.pages[whole], own[0], rest)
         n = self._add(_Sequence(s.pages[:whole] + own, s.prompt, s.made, s.controls))
         self._upload_table(n)
         return n
@@ -615,7 +634,8 @@ class BatchEngine:
         for rec in self.recordings.values():
             rec.free()
         self.recordings = {}
-        self.batch.free()
-        self.logits.free()
-        for b in [*self.weights.buffers, *self.pools, self.arena.buffer]:
+        for k in (self.batch, self.logits):
+            if k:
+                k.free()
+        for b in [*(self.weights.buffers if self.weights else ()), *self.pools, *([self.arena.buffer] if self.arena else ())]:
             b.free()

@@ -11,6 +11,7 @@ class _Buffer:
     """A buffer whose device side is an array of its own, reached by upload and download alone."""
 
     def __init__(self, size):
+        self.freed = 0
         self.size, self.mirror, self.device = size, np.zeros(size, np.uint8), np.zeros(size, np.uint8)
 
     def host(self):
@@ -34,15 +35,18 @@ class _Buffer:
         self.device[dst: dst + length] = src.device[at: at + length]
 
     def free(self):
-        pass
+        self.freed += 1
 
 
 class _Context:
     def __init__(self):
-        self.fails, self.steps = None, []
+        self.fails, self.steps, self.buffers, self.room = None, [], [], 100
 
     def alloc_host(self, size):
-        return _Buffer(size)
+        if len(self.buffers) == self.room:
+            raise MemoryError("alloc_host")
+        self.buffers.append(_Buffer(size))
+        return self.buffers[-1]
 
     def max_buffer(self):
         return 4 << 30
@@ -62,11 +66,22 @@ class _Weights:
     buffers, embd, layers, output, out_norm, rope = [_Buffer(64)], type("T", (), {"dtype": E.DType.Q8_0})(), [], None, 0, 0
 
 
+class _Kernels:
+    check = staticmethod(B.BatchKernels.check)
+
+    def __init__(self, *a, **k):
+        pass
+
+    def free(self):
+        pass
+
+
 @pytest.fixture
 def make(monkeypatch):
     """engine(...): a BatchEngine over such a context; its device's rows at each replay are in ctx.steps."""
-    for where, name in ((E, "load_weights"), (E, "Kernels"), (B, "BatchKernels"), (B, "LogitsKernels")):
-        monkeypatch.setattr(where, name, lambda *a, **k: _Weights())
+    monkeypatch.setattr(E, "load_weights", lambda *a: _Weights())
+    for where, name in ((E, "Kernels"), (B, "BatchKernels"), (B, "LogitsKernels")):
+        monkeypatch.setattr(where, name, _Kernels)
 
     class Engine(B.BatchEngine):
         def seen(self):
@@ -90,8 +105,8 @@ def make(monkeypatch):
                         rows[-1]["token"])
             return rows
 
-    def engine(**over):
-        ctx = _Context()
+    def engine(ctx=None, **over):
+        ctx = ctx or _Context()
         c = E.Config(n_embd=256, n_ff=256, n_head=2, n_head_kv=1, head_dim=128, n_vocab=1000, n_layer=2)
         eng = ctx.eng = Engine(ctx, {}, c, **(dict(max_ctx=300, n_pages=40, page=16, max_seq=6) | over))
         return eng, ctx
@@ -249,3 +264,29 @@ def test_a_step_has_a_row_for_each_of_its_sequences(make):
                 assert r["history"] == history
             assert r["pages"] == eng.sequences[q].pages
             assert np.array_equal(r["allowed"], k.allowed) if k.allowed is not None else r["allowed"] is None
+
+
+@pytest.mark.parametrize("room", [0, 1, 2])
+def test_an_engine_that_finds_no_room_gives_back_what_it_took(make, room):
+    ctx = _Context()
+    ctx.room = room
+    with pytest.raises(MemoryError):
+        make(ctx)
+    assert len(ctx.buffers) == room and all(b.freed == 1 for b in ctx.buffers)
+    ctx.room = 100
+    eng, _ = make(ctx)
+    eng.free()
+    assert all(b.freed == 1 for b in ctx.buffers)
+
+
+def test_a_fork_that_fails_gives_its_page_back(make, monkeypatch):
+    eng, ctx = make()
+    a = eng.open()
+    eng.extend(a, range(20))
+    with monkeypatch.context() as m:
+        m.setattr(_Buffer, "copy_from", lambda *k: 1 / 0)
+        with pytest.raises(ZeroDivisionError):
+            eng.fork(a)
+    assert len(eng.free_pages) == 38 and list(eng.sequences) == [a] and eng.uses.max() == 1
+    eng.close(a)
+    assert len(eng.free_pages) == 40
