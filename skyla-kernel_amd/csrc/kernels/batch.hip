@@ -20,8 +20,9 @@
 // Words that name no page or sequence reach no memory outside the pool: a row of such a sequence
 // counts as one of len 0, a length past the table's ends there, keys and values of such a page
 // are not stored, and a read of it goes to the pool's last page.
-// Keys and values are finite (kv_append stores no others but NaN): a row that attends to a NaN or an
-// infinity is not finite where that reaches, and what a row does not attend to reaches nothing.
+// Keys and values are finite (kv_append stores no others but NaN, in 8 bits as a block's scale): a row
+// that attends to a NaN or an infinity is not finite where that reaches, and what a row does not attend
+// to reaches nothing.
 #include <type_traits>
 
 #include "matmul_common.h"
@@ -138,11 +139,14 @@ SK_DEV void store_row(f16 *kv, int8_t *kv8, uint32_t cache, uint32_t scales, uin
 // row, every load in flight before the first product.  The angle (len - 1) f_d is formed in 64
 // bits as revolutions and reduced there: an f32 product is off by 2^-24 of an angle of 1e5, 3e-3
 // of a radian.  Each wave turns its row's 64 angles once, one a lane, for all its heads.
-// Measured (MI355X): 2048 rows of 48 heads, f16 keys and 8-bit values, 34 us from HBM (90 MB, 2.6
-// TB/s; 18 us from the caches), 79 with a wave a head and 4 bytes a lane and load: bound by the bytes
-// in flight.  PASSES = 4 where 16 heads a workgroup would make 4096 of them or more (2048 rows 33.5 us
-// against 36), below it more workgroups are better (1000 rows 24 against 26.5).  1 row 2.5 us: the
-// launch and two dependent round trips.
+// Measured (MI355X): 2048 rows of 48 heads, f16 keys and 8-bit values, 23 us where the caches hold other
+// data (90 MB, 3.9 TB/s; f16 25, 8 bits 23), 32 to 38 where a launch before left them written, 18 from
+// the caches (f16 15, 8 bits 19); 79 for 34 with a wave a head and 4 bytes a lane and load.  A pass loads
+// its norm weights behind the stores of the pass before and so waits for these; the row's words are two
+// dependent loads before all others; and 65 registers with 8-bit values leave seven workgroups a
+// compute unit for eight.  PASSES = 4 where 16 heads a workgroup would make 4096 of them or more (2048
+// rows 33.5 us against 36), below it more workgroups are better (1000 rows 24 against 26.5).  1 row 2.5
+// us: the launch and the dependent round trips.
 template <int K8, int V8, int PASSES>
 SK_DEV void append_body(const float *w, float *a, const uint32_t *ctl, f16 *kv, int8_t *kv8, const AppendPush &p) {
 #pragma clang fp contract(off)
@@ -290,11 +294,12 @@ SK_DEV Pages pages_of(const uint32_t *ctl, const PagedPush &p, uint32_t seq) {
 // the largest scale of the 32 dims, followed as loosely.  Scales 2^18 below it, whose positions may be
 // those that a row attends to, would lose bits: a run that meets one is run again with the m and ve that
 // it found, once for each window of scales.
-// Measured (MI355X, with the waves' join): one row of 16384 positions of 8 key heads, f16 keys and
-// 8-bit values, 15.5 us (50 MB, 3.2 TB/s); 128 rows of up to 512 own positions in f16 28 us (135 MB,
-// 4.8 TB/s, what a copy reaches); 8 rows of up to 100 positions 5.9 us.  Bound by HBM where rows are
-// many, by a workgroup's dependent round trips (control words, row words, page numbers, rows) where
-// runs are short.  Without the step in flight the first ran 24 us.
+// Measured (MI355X, with the waves' join; from the 256 MB cache / where it holds other data): one row of
+// 16384 positions of 8 key heads, f16 keys and 8-bit values, 15.9 / 25 us (50 MB), f16 14.9 / 24, 8 bits
+// 17 / 27; 128 rows of up to 512 own positions in f16 27 / 55 us (135 MB), f16 keys and 8-bit values 31 /
+// 57, 8 bits 37 / 58; 8 rows of up to 100 positions 5.9 us.  Bound by memory's latency: a workgroup's
+// dependent round trips (arguments, control words, row words, page numbers one after another, rows) and
+// one step in flight behind the one that is waited for.  Without that step the first ran 24 us for 15.5.
 constexpr uint32_t HALF = 32;
 template <int K8, int V8>
 struct HalfRows {
@@ -575,13 +580,15 @@ SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
 // 8-bit values are held as two f16 parts, exact, of q s 2^(7 - ve), ve the exponent of the part's
 // largest scale of the 32 dims, found first.  A part with scales 2^21 below it is run again for each
 // window of them, with the largest score that the first run found.
-// Measured (MI355X): 128 rows of 32 heads over 32768 positions of 8 key heads, f16: 134 us, 137 GFLOP
-// of f16 products, 1.02 PFLOP/s, where an 8192-cube f16 library product reaches 1.31 (keys and
-// values through registers into LDS 147); 8-bit values 183 (five products for four); 8-bit keys too
-// 209.  With up to 512 own positions a row beside the run 152 to 164, 492 with 16 rows a wave.  Bound
-// by the matrix pipe (busy 52% of the cycles, at the 1.87 GHz that such work is clocked down to) with
-// the vector ALU's issue beside it; under 1000 positions a part, by what a workgroup does once: 15 us
-// of round trips, the query rows' parts and the partials' writes.
+// Measured (MI355X): 128 rows of 32 heads over 32768 positions of 8 key heads, f16: 138 us, 137 GFLOP
+// of f16 products, 1.0 PFLOP/s, where an 8192-cube f16 library product reaches 1.31 (keys and
+// values through registers into LDS 147 for 134); 8-bit values 189 (five products for four); 8-bit keys
+// too 208.  With up to 512 own positions a row beside the run 151 to 160, 492 with 16 rows a wave.  The
+// matrix pipe is busy 52% of the cycles (at the 1.87 GHz that such work is clocked down to) and a wave
+// waits 26% of its own (each step's barrier, loads): the products share each wave's issue with the
+// vector instructions that make the weights, and neither alone binds it.  Under 1000 positions a part,
+// bound by what a workgroup does once: 15 us of round trips, the pass over the scales, the query rows'
+// parts and the partials' writes.
 constexpr uint32_t WIDE = 128, STEP = 32;
 template <int Q8>
 struct RawRows {
@@ -1181,14 +1188,16 @@ extern "C" __global__ __launch_bounds__(512) void attention_paged_merge_8__128(f
 //   not allowed      -inf
 // Ids past the vocabulary count for nothing.  Lengths are cut to the strides.
 //
-// A workgroup of T threads takes 16 T tokens of a row: it loads its logits, counts the history's
-// tokens among them in LDS meanwhile (integer counts, so any order gives the same), and writes the
+// A workgroup of T threads takes 16 T tokens of a row: it loads its logits and mask words, counts the
+// history's tokens among them in LDS (integer counts, so any order gives the same), and writes the
 // row's part once.  Its biases come last, each by the thread whose entry is the last of its id.
-// Measured (MI355X), a vocabulary of 151936, half of the rows masked: 128 rows of histories to 32768
-// 45 us (169 MB, 3.8 TB/s; 50 with T = 256, whose 38 workgroups a row each read the history, and 215
-// with a load of it at a time and two counts a token), of 100 27 us (5.8 TB/s), 48 rows of 4096 12.6 us,
-// 1 row of 1000 5.7 us.  Bound by HBM, with long histories by their counting; non-temporal stores
-// save 1 to 2 us of a launch of many rows.
+// Measured (MI355X), a vocabulary of 151936, half of the rows masked, from the 256 MB cache, where an
+// output head leaves logits / where it holds other data: 128 rows of histories to 32768 44 / 75 us (169
+// MB; 50 with T = 256, whose 38 workgroups a row each read the history, and 215 with a load of it at a
+// time and two counts a token), of 100 27 / 46, 48 rows of 4096 14.5 / 28, 1 row of 1000 5.2 / 9.5.  Long
+// histories are bound by their counting; short ones by round trips: the branches for a row's end put
+// a wait behind the first of a thread's four logits loads and, in masked rows, behind each mask word.
+// Non-temporal stores save 1 to 2 us of a launch of many rows.
 template <uint32_t T>
 SK_DEV void logits_body(float *a, const uint32_t *ctl, const LogitsPush &p) {
 #pragma clang fp contract(off)
