@@ -386,8 +386,8 @@ class BatchEngine:
                 raise ValueError(f"allowed: a truth value for each of {self.c.n_vocab} tokens")
             allowed = np.array(allowed, bool)
         s.controls = Controls(*(float(v) for v in penalties), bias, allowed)
-        if s.row is not None:
-            self._upload_controls(seq)
+        if s.row is not None:  # uploaded again where the next step places it
+            self.rows[s.row], s.row = None, None
 
     # ---- pages ----
     def _take(self, n: int) -> list[int]:
@@ -434,9 +434,13 @@ class BatchEngine:
         if sum(new.values()) > len(self.free_pages):
             raise ValueError(f"{sum(new.values())} pages needed, {len(self.free_pages)} free")
         for seq, n in new.items():
-            if n:
+            if n > 0:
                 self._get(seq).pages += self._take(n)
-                self._upload_table(seq)
+                try:
+                    self._upload_table(seq)
+                except BaseException:
+                    self._trim(seq)
+                    raise
 
     # ---- words ----
     def _place(self, seqs: list[int]) -> None:
@@ -452,7 +456,11 @@ class BatchEngine:
             if self.rows[s.row] is not None:
                 self._get(self.rows[s.row]).row = None
             self.rows[s.row] = q
-            self._upload_controls(q)
+            try:
+                self._upload_controls(q)
+            except BaseException:
+                self.rows[s.row], s.row = None, None
+                raise
 
     def _upload_table(self, seq: int) -> None:
         a, pages = self.arena, self._get(seq).pages

@@ -290,3 +290,32 @@ def test_a_fork_that_fails_gives_its_page_back(make, monkeypatch):
     assert len(eng.free_pages) == 38 and list(eng.sequences) == [a] and eng.uses.max() == 1
     eng.close(a)
     assert len(eng.free_pages) == 40
+
+
+@pytest.mark.parametrize("n", range(9))
+@pytest.mark.parametrize("what", ["step", "control"])
+def test_uploads_that_fail_are_made_again(make, monkeypatch, n, what):
+    """The n-th upload of a step fails (a table's, controls', a history's, the words'): the next step
+    brings what did not reach the device."""
+    eng, ctx = make()
+    a, b = eng.open(), eng.open()
+    allowed = np.arange(1000) % 2 == 0
+    eng.extend(a, range(16))  # a page: the next token needs another
+    if what == "control":
+        eng.step({a: 30, b: 31})
+        eng.extend(a, range(15))
+    eng.control(a, B.Controls(bias={3: 1.0}, presence=1.0, allowed=allowed))
+    up, calls, failed = _Buffer.upload, iter(range(100)), False
+    with monkeypatch.context() as m:
+        m.setattr(_Buffer, "upload", lambda s, *k: 1 / (next(calls) != n) and up(s, *k))
+        try:
+            eng.step({a: 40})
+        except ZeroDivisionError:
+            failed = True
+    assert failed == (n < 8)
+    eng.step({b: 51, a: 50})
+    r = _row(ctx, a)
+    assert r["pages"] == eng.sequences[a].pages and len(r["pages"]) == -(-r["len"] // 16)
+    assert r["bias"] == {3: 1.0} and np.array_equal(r["allowed"], allowed)
+    assert r["len"] == len(r["history"]) == eng.length(a) and r["history"][-1] == 50
+    assert _row(ctx, b)["bias"] == {} and _row(ctx, b)["pages"] == eng.sequences[b].pages
