@@ -217,12 +217,12 @@ class Controls:
 class _Sequence:
     """A sequence's pages, the tokens of its prompts and those that it generated (a conversation's
     follow in turns; what acts on the logits asks only which), its controls, the row of the batch
-    that these lie in (None: they do not), and how many words of its history, the prompts' tokens
-    before the others, lie there."""
+    that these lie in (None: they do not), how many words of its history, the prompts' tokens before
+    the others, lie there, and whether its controls do not yet."""
 
     def __init__(self, pages=(), prompt=(), made=(), controls=None):
         self.pages, self.prompt, self.made = list(pages), list(prompt), list(made)
-        self.controls, self.row, self.placed = controls or Controls(), None, 0
+        self.controls, self.row, self.placed, self.stale = controls or Controls(), None, 0, True
 
     def __len__(self):
         return len(self.prompt) + len(self.made)
@@ -386,8 +386,7 @@ class BatchEngine:
                 raise ValueError(f"allowed: a truth value for each of {self.c.n_vocab} tokens")
             allowed = np.array(allowed, bool)
         s.controls = Controls(*(float(v) for v in penalties), bias, allowed)
-        if s.row is not None:  # uploaded again where the next step places it
-            self.rows[s.row], s.row = None, None
+        s.stale = True
 
     # ---- pages ----
     def _take(self, n: int) -> list[int]:
@@ -448,19 +447,16 @@ class BatchEngine:
         free = [r for r in range(len(seqs)) if self.rows[r] not in seqs]
         for q in seqs:
             s = self._get(q)
-            if s.row is not None and s.row < len(seqs):
-                continue
-            if s.row is not None:
-                self.rows[s.row] = None
-            s.row, s.placed = free.pop(0), 0
-            if self.rows[s.row] is not None:
-                self._get(self.rows[s.row]).row = None
-            self.rows[s.row] = q
-            try:
+            if s.row is None or s.row >= len(seqs):
+                if s.row is not None:
+                    self.rows[s.row] = None
+                s.row, s.placed, s.stale = free.pop(0), 0, True
+                if self.rows[s.row] is not None:
+                    self._get(self.rows[s.row]).row = None
+                self.rows[s.row] = q
+            if s.stale:
                 self._upload_controls(q)
-            except BaseException:
-                self.rows[s.row], s.row = None, None
-                raise
+                s.stale = False
 
     def _upload_table(self, seq: int) -> None:
         a, pages = self.arena, self._get(seq).pages

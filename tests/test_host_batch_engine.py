@@ -319,3 +319,17 @@ def test_uploads_that_fail_are_made_again(make, monkeypatch, n, what):
     assert r["bias"] == {3: 1.0} and np.array_equal(r["allowed"], allowed)
     assert r["len"] == len(r["history"]) == eng.length(a) and r["history"][-1] == 50
     assert _row(ctx, b)["bias"] == {} and _row(ctx, b)["pages"] == eng.sequences[b].pages
+
+
+def test_controls_of_every_step_leave_the_history_where_it_is(make):
+    """A grammar's mask at each token: the mask and the token go to the device, not the history again."""
+    eng, ctx = make()
+    a = eng.open()
+    eng.extend(a, range(200))
+    for t in range(5):
+        eng.control(a, B.Controls(repetition=1.5, allowed=np.arange(1000) % 7 == t))
+        placed = eng.sequences[a].placed
+        eng.step({a: 300 + t})
+        r = _row(ctx, a)
+        assert r["history"] == [*range(200), *range(300, 301 + t)] and np.flatnonzero(r["allowed"])[0] == t
+        assert placed == (200 + t if t else 0)
