@@ -1,4 +1,4 @@
-// Host side of the batch operators (kernels/batch.hip): the checks of their push words against
+// Host side of the batch operators (kernels/batch.hip, sample.hip): the checks of their push words against
 // the buffers they are bound to, and the launch a dispatch of theirs becomes.  Plain C++, no HIP.
 #pragma once
 
@@ -12,13 +12,15 @@
 
 namespace batch {
 
-enum Op { kNone, kAppend, kAttend, kMerge, kLogits };
+enum Op { kNone, kAppend, kAttend, kMerge, kLogits, kSample, kDraw };
 
 inline Op op_of(const char *name) {
   if (std::strcmp(name, "kv_append") == 0) return kAppend;
   if (std::strcmp(name, "attention_paged") == 0) return kAttend;
   if (std::strcmp(name, "attention_paged_merge") == 0) return kMerge;
   if (std::strcmp(name, "logits_adjust") == 0) return kLogits;
+  if (std::strcmp(name, "logits_sample") == 0) return kSample;
+  if (std::strcmp(name, "logits_sample_draw") == 0) return kDraw;
   return kNone;
 }
 
@@ -37,6 +39,8 @@ constexpr uint32_t kMergeParts = 16, kMergeHeads = 512;
 // them read it (us, 4096 / 16384: 128 rows of 32768 50 / 45, of 8192 33.7 / 33.3, of 1000 28 / 29; 12
 // rows of 30000 12.2 / 9.9, of 4096 7.4 / 8.0; 1 row of 30000 9.7 / 8.6, of 1000 5.7 / 6.4).
 constexpr uint32_t kLogitsHistory = 8192;
+// Tokens of a logits_sample workgroup, words of its part, and the most tokens of a vocabulary (sample.hip).
+constexpr uint32_t kSampleChunk = 8192, kSamplePart = 1544, kSampleVocab = 1u << 20;
 constexpr uint32_t kMaxWork = 1u << 23;   // workgroups of an attention launch
 
 // A buffer bound to a dispatch: where it lies and how large it is.
@@ -214,6 +218,22 @@ inline std::string refusal(Op op, const uint32_t *spec, const uint32_t *w, const
     if (w[11] && w[11] < (v + 31) / 32) c.fail("a mask of %u words for %llu tokens", w[11], (unsigned long long)v);
     if (!y.same(x)) c.apart(y, x);
     c.writes({y}, {ctrl, hist, bias, mask, ctl});
+  } else if (op == kSample || op == kDraw) {
+    const uint64_t v = w[2], parts = rows * ((v + kSampleChunk - 1) / kSampleChunk);
+    c.need(v >= 1 && v <= kSampleVocab, "a vocabulary of 1 to 1048576 tokens");
+    if (!c.error.empty()) return c.error;
+    const Region x{"the logits", A, 4, w[0], w[1], v, rows}, ctrl{"the rows' words", C, 4, w[3], 8, 8, rows},
+        part{"the partials", A, 4, w[4], 0, parts * kSamplePart, 1};
+    c.holds(x, 4);
+    c.holds(ctrl, 4);
+    c.holds(part, 4);
+    if (op == kSample) {
+      c.writes({part}, {x, ctrl, ctl});
+    } else {
+      const Region out{"the tokens", A, 4, w[5], 4, 4, rows};
+      c.holds(out, 4);
+      c.writes({out}, {x, ctrl, part, ctl});
+    }
   }
   return c.error;
 }
@@ -249,6 +269,11 @@ inline Shape shape(Op op, const uint32_t *spec, const uint32_t *w, uint32_t rows
     s.form = w[4] + w[5] > kMergeParts && rows * w[3] <= kMergeHeads;
     s.groups[0] = s.form ? w[3] : (w[3] + 3) / 4;
     s.threads = s.form ? 512 : 256;
+  } else if (op == kSample) {
+    s.threads = 512;
+    s.groups[0] = (w[2] + kSampleChunk - 1) / kSampleChunk;
+  } else if (op == kDraw) {
+    s.threads = 1024;
   } else {
     s.form = w[7] >= kLogitsHistory;
     s.threads = s.form ? 1024 : 256;

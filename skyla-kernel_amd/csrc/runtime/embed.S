@@ -17,4 +17,5 @@ EMBED(skyla_co_moe, "moe.hsaco")
 EMBED(skyla_co_util, "util.hsaco")
 EMBED(skyla_co_attention, "attention.hsaco")
 EMBED(skyla_co_batch, "batch.hsaco")
+EMBED(skyla_co_sample, "sample.hsaco")
     .section .note.GNU-stack,"",@progbits

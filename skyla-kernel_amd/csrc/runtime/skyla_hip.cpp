@@ -39,6 +39,7 @@ extern "C" const unsigned char skyla_co_moe[], skyla_co_moe_end[];
 extern "C" const unsigned char skyla_co_util[], skyla_co_util_end[];
 extern "C" const unsigned char skyla_co_attention[], skyla_co_attention_end[];
 extern "C" const unsigned char skyla_co_batch[], skyla_co_batch_end[];
+extern "C" const unsigned char skyla_co_sample[], skyla_co_sample_end[];
 
 namespace {
 
@@ -200,6 +201,8 @@ const KernelInfo kKernels[] = {
     {"attention_paged", 5, 20, 4, 4, -1, false, false},
     {"attention_paged_merge", 2, 10, 1, 1, -1, false, false},
     {"logits_adjust", 2, 12, 0, 0, -1, false, false},
+    {"logits_sample", 2, 5, 0, 0, -1, false, false, 512},  // (kernels/sample.hip)
+    {"logits_sample_draw", 2, 6, 0, 0, -1, false, false, 1024},
 };
 
 const KernelInfo *find_kernel(const char *name) {
@@ -1500,7 +1503,7 @@ int skyla_hip_context_new(int device, skyla_hip_context **out) {
   ctx->warp = (uint32_t)prop.warpSize;
   HIP_TRY(hipStreamCreateWithFlags(&ctx->stream, hipStreamNonBlocking));
   const unsigned char *images[] = {skyla_co_matvec, skyla_co_matmul, skyla_co_matmul_ring, skyla_co_moe,
-                                   skyla_co_util, skyla_co_attention, skyla_co_batch};
+                                   skyla_co_util, skyla_co_attention, skyla_co_batch, skyla_co_sample};
   for (const unsigned char *img : images) {
     hipModule_t m = nullptr;
     hipError_t le = hipModuleLoadData(&m, img);

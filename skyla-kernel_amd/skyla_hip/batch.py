@@ -7,7 +7,8 @@ what a server of many needs beside it, over the same weights, arena rows and C-A
   BatchKernels    kv_append (QK-norm, rotation, keys and values into their pages) and
                   attention_paged (attention of rows over their pages, a leading run of positions
                   that many rows share read once for all of them)
-  LogitsKernels   logits_adjust (penalties for repeated tokens, biases, grammar masks)
+  LogitsKernels   logits_adjust (penalties for repeated tokens, biases, grammar masks) and
+                  logits_sample (a token of each row by temperature, top-k, min-p and top-p)
   BatchEngine     sequences of one model: open, fork, prefill, step, close
 
 The operators read the batch's rows from four words each, {sequence, length, share, 0}: the
@@ -72,6 +73,16 @@ class LogitsRegions:
     mask_stride: int = 0
 
 
+@dataclasses.dataclass
+class SampleRegions:
+    """Arena offsets of what a row's token is drawn by (eight words a row: temperature, top_p, min_p,
+    top_k, a random number of 32 bits), of what is drawn (four words a row: token, tokens kept, log
+    probability) and of sample_size words between the two."""
+    controls: int
+    out: int
+    part: int
+
+
 class Parts(NamedTuple):
     """The pieces that a batch's attention cuts the shared run (0: none is shared, whatever the rows
     say) and each row's own run into, and whether the shared run takes 128 query rows a workgroup
@@ -116,6 +127,14 @@ def splits(rows: int, n_kv: int, rep: int, shared: int, own: int) -> Parts:
 def part_size(rows: int, n_head: int, parts) -> int:
     """Words of the partials' region."""
     return rows * n_head * (parts[0] + parts[1]) * 130
+
+
+SAMPLE_CHUNK, SAMPLE_PART, SAMPLE_VOCAB = 8192, 1544, 1 << 20  # (runtime/batch.h)
+
+
+def sample_size(rows: int, n_vocab: int) -> int:
+    """Words of logits_sample's partials."""
+    return rows * -(-n_vocab // SAMPLE_CHUNK) * SAMPLE_PART
 
 
 class BatchKernels:
@@ -181,11 +200,14 @@ class BatchKernels:
 
 
 class LogitsKernels:
-    """logits_adjust over an arena's rows of logits."""
+    """logits_adjust and logits_sample over an arena's rows of logits."""
 
     def __init__(self, ctx: Context, a: Buffer):
-        self._adjust = ctx.create_pipeline("logits_adjust", 2, 48, [])
-        self._adjust.bind_buffers([a, a])
+        build = lambda name, words: ctx.create_pipeline(name, 2, 4 * words, [])  # noqa: E731
+        self._adjust, self._sample, self._draw = (build("logits_adjust", 12), build("logits_sample", 5),
+                                                  build("logits_sample_draw", 6))
+        for p in (self._adjust, self._sample, self._draw):
+            p.bind_buffers([a, a])
 
     def adjust(self, r: Recorder, at: LogitsRegions, x, y, n_vocab: int, rows: int) -> None:
         """Rows of logits x ((offset, stride)) into y, which may be x."""
@@ -193,8 +215,16 @@ class LogitsKernels:
                 at.mask, at.mask_stride]
         r.dispatch(self._adjust, [1, rows, 1], push)
 
+    def sample(self, r: Recorder, at: SampleRegions, x, n_vocab: int, rows: int) -> None:
+        """A token of each row of logits x ((offset, stride)) into at.out; at.part holds sample_size words."""
+        push = [x[0], x[1], n_vocab, at.controls, at.part]
+        r.dispatch(self._sample, [1, rows, 1], push)
+        r.barrier()
+        r.dispatch(self._draw, [1, rows, 1], push + [at.out])
+
     def free(self) -> None:
-        self._adjust.free()
+        for p in (self._adjust, self._sample, self._draw):
+            p.free()
 
 
 # ---- sequences of one model ----------------------------------------------------------------
