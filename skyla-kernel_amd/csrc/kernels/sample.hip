@@ -31,10 +31,11 @@ struct DrawPush {
 
 constexpr uint32_t THREADS = 512, EACH = 16, CHUNK = THREADS * EACH;  // tokens of a workgroup of logits_sample
 constexpr uint32_t BINS = 512;  // from a chunk's (a row's) largest value down; the last holds all below it, too
-constexpr uint32_t LIST = 256;  // a chunk's largest values that are listed, of whole bins
-// a chunk's part: {floor(t) of its largest value (f64), that value, bins listed, values listed, 0, 0, 0}, bins, list
-constexpr uint32_t HEAD = 8, PART = HEAD + 2 * BINS + 2 * LIST;
-constexpr int COUNT_AT = 50;  // a bin's word: its count from this bit on, its weights' sum times 2^36 below
+// a chunk's part: {floor(t) of its largest value (f64), that value, how many there are, 0, 0, 0, 0}, its bins, and
+// its tokens in the bins' order (16 bits each, from the chunk's first)
+constexpr uint32_t HEAD = 8, PART = HEAD + 2 * BINS + CHUNK / 2;
+// a bin's word: its weights' sum times 2^36, and from this bit on how many tokens end with it
+constexpr int COUNT_AT = 50;
 constexpr uint64_t SUM = (1ull << COUNT_AT) - 1;
 
 // What both kernels take a logit for, to the same bits.
@@ -83,13 +84,15 @@ SK_DEV T wave_scan(T v, uint32_t lane) {  // inclusive
 
 }  // namespace
 
-// A workgroup's CHUNK tokens of a row: their bins below its own largest value, and the values of the first bins.
+// A workgroup's CHUNK tokens of a row: their bins below its own largest value, and the tokens in the bins' order.
 extern "C" __global__ __launch_bounds__(THREADS) void logits_sample(float *a, const uint32_t *ctl, SamplePush p) {
 #pragma clang fp contract(off)
   constexpr uint32_t WAVES = THREADS / 64;
   __shared__ unsigned long long bin[BINS];
+  __shared__ uint32_t start[BINS];
+  __shared__ __attribute__((aligned(16))) uint16_t ids[CHUNK];
   __shared__ float big[WAVES];
-  __shared__ uint32_t counts[WAVES], n_list;
+  __shared__ uint32_t counts[WAVES];
   const uint32_t row = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = t >> 6;
   if (row >= ctl[2]) return;
   const uint32_t base = blockIdx.x * CHUNK, n = min(CHUNK, p.n_vocab - base);
@@ -118,56 +121,56 @@ extern "C" __global__ __launch_bounds__(THREADS) void logits_sample(float *a, co
   for (int d = 32; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
   if (lane == 0) big[wave] = top;
   bin[t] = 0;
-  if (t == 0) n_list = 0;
   __syncthreads();
 #pragma unroll
   for (uint32_t w = 0; w < WAVES; w++) top = fmaxf(top, big[w]);
   const double first = __builtin_floor(scaled(top, c));
-  if (!has_weight(top)) {  // nothing here: no bins, and none are read
+  if (!has_weight(top)) {  // nothing here, and nothing more is read
     if (t == 0) {
       *(double *)part = -INFINITY;
-      ((uint32_t *)part)[3] = BINS;
-      ((uint32_t *)part)[4] = 0;
+      part[2] = top;
+      ((uint32_t *)part)[3] = 0;
     }
     return;
   }
-  uint32_t at[EACH];
+  uint32_t at[EACH];  // a token's bin, and its place among those of the bin
 #pragma unroll
   for (uint32_t k = 0; k < EACH / 4; k++)
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       uint32_t &b = at[4 * k + e];
-      b = BINS;
+      b = ~0u;
       if (!has_weight(v[k][e])) continue;
       const double s = scaled(v[k][e], c), d = first - __builtin_floor(s);
       b = d < BINS ? (uint32_t)(int)d : BINS - 1;
-      const uint64_t word = fixed_weight(s, d);
-      atomicAdd(&bin[b], (unsigned long long)(word + (1ull << COUNT_AT)));
+      const uint64_t before = atomicAdd(&bin[b], (unsigned long long)(fixed_weight(s, d) + (1ull << COUNT_AT)));
+      b |= (uint32_t)(before >> COUNT_AT) << 16;
     }
   __syncthreads();
   const uint64_t mine = bin[t];
-  ((uint64_t *)(part + HEAD))[t] = mine;
-  // the bins whose values, with those above them, are LIST at most (the last bin has values of any size)
-  uint32_t sum = wave_scan((uint32_t)(mine >> COUNT_AT), lane);
-  if (lane == 63) counts[wave] = sum;
+  const uint32_t count = (uint32_t)(mine >> COUNT_AT);
+  uint32_t end = wave_scan(count, lane);
+  if (lane == 63) counts[wave] = end;
   __syncthreads();
+  uint32_t all = 0;
 #pragma unroll
-  for (uint32_t w = 0; w < WAVES; w++)
-    if (w < wave) sum += counts[w];
-  const uint32_t listed = __syncthreads_count(sum <= LIST && t < BINS - 1);
-  uint2 *list = (uint2 *)(part + HEAD + 2 * BINS);
+  for (uint32_t w = 0; w < WAVES; w++) {
+    if (w < wave) end += counts[w];
+    all += counts[w];
+  }
+  start[t] = end - count;
+  ((uint64_t *)(part + HEAD))[t] = (mine & SUM) | (uint64_t)end << COUNT_AT;
+  __syncthreads();
 #pragma unroll
   for (uint32_t i = 0; i < EACH; i++)
-    if (at[i] < listed) {
-      const float y = v[i / 4][i % 4];
-      list[atomicAdd(&n_list, 1u)] = make_uint2(__builtin_bit_cast(uint32_t, y), base + 4 * (t + THREADS * (i / 4)) + i % 4);
-    }
+    if (at[i] != ~0u) ids[start[at[i] & 0xffff] + (at[i] >> 16)] = 4 * (t + THREADS * (i / 4)) + i % 4;
   __syncthreads();
+  uint4 *list = (uint4 *)(part + HEAD + 2 * BINS);
+  for (uint32_t i = t; 8 * i < all; i += THREADS) list[i] = ((const uint4 *)ids)[i];
   if (t == 0) {
     *(double *)part = first;
     part[2] = top;
-    ((uint32_t *)part)[3] = listed;
-    ((uint32_t *)part)[4] = n_list;
+    ((uint32_t *)part)[3] = all;
   }
 }
 
@@ -181,26 +184,27 @@ constexpr uint32_t DIGITS = 2048;  // buckets of the search that takes any numbe
 
 struct DrawShared {
   union {
-    uint64_t got[MOST];   // places as they came,
-    uint64_t upto[MOST];  // and, of those in order, the sum behind each
-    double largest[CHUNKS];
+    uint64_t place[2][MOST];  // as they came, then by buckets; then in order
     struct {
       unsigned long long sum[DIGITS];
       uint32_t count[DIGITS];
     } digit;
+    struct {
+      uint64_t sum[DRAW];
+      uint32_t n[DRAW];
+      double largest[CHUNKS];
+    } half;
   };
-  uint64_t in_order[MOST];
-  double c[BINS + 1];    // C before a bin, in weights of the row's upper edge
-  uint32_t n[BINS + 1];  // tokens before it
-  uint32_t span[BINS];   // a bin's place among those looked at (~0: none)
-  uint32_t bucket[DRAW + 1];
-  double first[CHUNKS];  // the chunks' parts: floor(t) of their largest values, bins and values listed
-  uint32_t listed[CHUNKS], values[CHUNKS];
+  double c[BINS + 1];     // C before a bin, in weights of the row's upper edge
+  uint32_t n[BINS + 1];   // tokens before it
+  double edge[BINS];      // its upper edge's weight
+  uint32_t bucket[DRAW];
+  double first[CHUNKS];   // the chunks' floor(t) of their largest values
   double sums[DRAW_WAVES];
   uint64_t words[DRAW_WAVES];
   uint32_t counts[DRAW_WAVES];
   unsigned long long below;
-  uint32_t fill, found[4];
+  uint32_t fill, found[2];
 };
 
 // A row as its kernel sees it.
@@ -214,15 +218,15 @@ SK_DEV uint32_t bin_of(const Row &r, double t) {
   return d < BINS - 1 ? (uint32_t)(int)d : BINS - 1;
 }
 SK_DEV uint64_t fixed_weight(const Row &r, double t) { return fixed_weight(t, r.edge - __builtin_floor(t)); }
-// the weight of a bin's upper edge, and a sum of its weights
-SK_DEV double edge_weight(uint32_t b) { return exp2(-0.125 * (double)b); }
+// a sum of a bin's weights
 SK_DEV double sum_of(uint64_t fixed, double edge) { return (double)fixed * 0x1p-36 * edge; }
 
-// Every value of the row that may lie in a bin above t = least, its place and t: f(place, t).
+// Every value of the row that may lie in [least, most) by its t, among them all that do: f(place, t).
 template <typename F>
-SK_DEV void each_value(const Row &r, double least, F f) {
-  // the f32 below least / c, with room for both roundings
-  const float low = (float)(least / r.c), from = low - fabsf(low) * 1e-6f;
+SK_DEV void each_value(const Row &r, double least, double most, F f) {
+  // in f32, with room for both roundings (without a scale everything is taken)
+  const float low = (float)(least / r.c), high = (float)(most / r.c);
+  const float from = low - fabsf(low) * 1e-6f, to = high + fabsf(high) * 1e-6f;
   constexpr uint32_t U = 4;
   for (uint32_t i0 = 4 * threadIdx.x; i0 < r.n_vocab; i0 += 4 * DRAW * U) {
     f32x4 v[U];
@@ -242,8 +246,16 @@ SK_DEV void each_value(const Row &r, double least, F f) {
     for (uint32_t k = 0; k < U; k++)
 #pragma unroll
       for (int e = 0; e < 4; e++)
-        if (has_weight(v[k][e]) && !(v[k][e] < from)) f(place(v[k][e], i0 + 4 * DRAW * k + e), scaled(v[k][e], r.c));
+        if (has_weight(v[k][e]) && !(v[k][e] < from) && !(v[k][e] > to))
+          f(place(v[k][e], i0 + 4 * DRAW * k + e), scaled(v[k][e], r.c));
   }
+}
+// those of bin b
+template <typename F>
+SK_DEV void each_value_of(const Row &r, uint32_t b, F f) {
+  each_value(r, b < BINS - 1 ? r.edge - (double)b : -INFINITY, b ? r.edge - (double)b + 1.0 : INFINITY, [&](uint64_t place, double t) {
+    if (bin_of(r, t) == b) f(place, t);
+  });
 }
 
 // The first bin b whose end satisfies ok(end), BINS if none does; ok is false, then true.  The same in every wave.
@@ -293,7 +305,7 @@ __device__ __attribute__((noinline)) Found search(DrawShared &s, const Row r, Wa
                                 : first_bin(s.c, [&](double c) { return c > goal; });
   const uint32_t last = first_bin(s.n, [&](uint32_t n) { return n >= s.n[BINS]; });
   b = min(b, last);
-  const double edge = edge_weight(b);
+  const double edge = s.edge[b];
   Found f{0, s.n[b], s.c[b]};
   constexpr int at[5] = {53, 42, 32, 10, 0}, bits[5] = {11, 11, 10, 22, 10};
   // (ids are below 2^20: 10 bits from bit 10 on, all 22 of them compared as a prefix)
@@ -302,8 +314,8 @@ __device__ __attribute__((noinline)) Found search(DrawShared &s, const Row r, Wa
     for (uint32_t i = t; i < DIGITS; i += DRAW) s.digit.sum[i] = 0, s.digit.count[i] = 0;
     __syncthreads();
     const int above = at[k] + bits[k];
-    each_value(r, b < BINS - 1 ? r.edge - (double)b : -INFINITY, [&](uint64_t place, double v) {
-      if (bin_of(r, v) != b || (above < 64 && place >> above != f.place >> above)) return;
+    each_value_of(r, b, [&](uint64_t place, double v) {
+      if (above < 64 && place >> above != f.place >> above) return;
       const uint32_t d = (uint32_t)(place >> at[k]) & (DIGITS - 1);
       atomicAdd(&s.digit.sum[d], (unsigned long long)fixed_weight(r, v));
       atomicAdd(&s.digit.count[d], 1u);
@@ -339,18 +351,33 @@ __device__ __attribute__((noinline)) Found search(DrawShared &s, const Row r, Wa
   return f;
 }
 
-// Tokens of t >= least, all of them and their sum, least in bin b.
+// The tokens with t >= least, all of them and their sum, least in bin b.
 __device__ __attribute__((noinline)) Found search_above(DrawShared &s, const Row r, double least, uint32_t b) {
-  unsigned long long sum = 0;
+  uint64_t sum = 0;
   uint32_t n = 0;
-  each_value(r, least, [&](uint64_t, double v) {
-    if (v >= least && bin_of(r, v) == b) sum += fixed_weight(r, v), n++;
+  each_value_of(r, b, [&](uint64_t, double v) {
+    if (v >= least) sum += fixed_weight(r, v), n++;
   });
   uint64_t all;
   uint32_t count;
-  block_scan((uint64_t)sum, s.words, all);
+  block_scan(sum, s.words, all);
   block_scan(n, s.counts, count);
-  return {0, s.n[b] + count, s.c[b] + sum_of(all, edge_weight(b))};
+  return {0, s.n[b] + count, s.c[b] + sum_of(all, s.edge[b])};
+}
+
+// The first of [0, n) that satisfies ok, n if none does; ok is false, then true.  The same in every wave.
+template <typename F>
+SK_DEV uint32_t first_of(uint32_t n, F ok) {
+  uint32_t lo = 0, hi = n;  // none before lo does, hi does
+  while (lo < hi) {
+    const uint32_t step = (hi - lo + 63) / 64, i = lo + (threadIdx.x & 63) * step + step - 1;
+    const uint64_t m = __ballot(i >= hi || ok(i));
+    if (!m) return hi;
+    const uint32_t k = (uint32_t)__builtin_ctzll(m);
+    hi = min(hi, lo + k * step + step - 1);
+    lo += k * step;
+  }
+  return hi;
 }
 
 }  // namespace
@@ -367,85 +394,80 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
   const float *parts = a + p.part_off + (size_t)row * n_chunks * PART;
   uint32_t *out = (uint32_t *)a + p.out_off + 4 * row;
   Row r{a + p.x_off + (size_t)row * p.x_stride, p.n_vocab, scale_of(T), -INFINITY};
-  float top = -INFINITY;
   if (t < CHUNKS) {
     const float *part = parts + (size_t)min(t, n_chunks - 1) * PART;
-    const double first = *(const double *)part;
-    s.first[t] = first;
-    if (first > -INFINITY) s.largest[t] = part[2];
-    else s.largest[t] = -INFINITY;
-    s.listed[t] = ((const uint32_t *)part)[3];
-    s.values[t] = ((const uint32_t *)part)[4];
+    s.first[t] = *(const double *)part;
+    s.half.largest[t] = part[2];
   }
+  if (t < BINS) s.edge[t] = exp2(-0.125 * (double)t);
+  s.bucket[t] = 0;
+  if (t == 0) s.below = 0, s.fill = 0;
   __syncthreads();
+  float top;
   {
     const uint32_t lane = t & 63;
-    double big = fmax(s.largest[lane], s.largest[lane + 64]);
+    double big = fmax(s.half.largest[lane], s.half.largest[lane + 64]);
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1) big = fmax(big, __shfl_xor(big, d, 64));
     top = (float)big;
-    r.edge = __builtin_floor(scaled(top, r.c));
   }
   if (!has_weight(top)) {
     if (t == 0) *(uint4 *)out = make_uint4(~0u, 0, 0xff800000u, 0);
     return;
   }
+  const double t_top = scaled(top, r.c);
+  r.edge = __builtin_floor(t_top);
 
   // the row's bins: thread t has bin t % BINS of every other chunk
   {
     const uint32_t b = t % BINS;
-    uint32_t n = 0;
+    uint32_t n = 0;  // tokens that end with it
     uint64_t sum = 0;
-    if (t == 0) s.below = 0, s.fill = 0;
-    __syncthreads();
     constexpr uint32_t U = 10, STEP = DRAW / BINS;  // chunks whose loads are in flight
     for (uint32_t i0 = t / BINS; i0 < n_chunks; i0 += U * STEP) {
       uint64_t w[U];
+      bool last[U];
 #pragma unroll
       for (uint32_t j = 0; j < U; j++) {
         const uint32_t i = min(i0 + j * STEP, n_chunks - 1);
         const double d = r.edge - s.first[i];  // the chunk's bins lie so many below the row's
         const uint32_t down = d < BINS ? (uint32_t)(int)d : BINS;
-        w[j] = ((const uint64_t *)(parts + (size_t)i * PART + HEAD))[b >= down ? b - down : 0];
-        if (i0 + j * STEP >= n_chunks || b < down || b == BINS - 1) w[j] = 0;
+        const bool any = i0 + j * STEP < n_chunks && s.first[i] > -INFINITY;
+        last[j] = any && b == BINS - 1;
+        // (of the row's last bin: how many the chunk has)
+        w[j] = any && (b >= down || last[j]) ? ((const uint64_t *)(parts + (size_t)i * PART + HEAD))[last[j] ? b : b - down] : 0;
       }
 #pragma unroll
       for (uint32_t j = 0; j < U; j++) {
         n += (uint32_t)(w[j] >> COUNT_AT);
-        sum += w[j] & SUM;
+        sum += last[j] ? 0 : w[j] & SUM;
       }
     }
     // a chunk's bins from the row's last on go there, in weights of that one's edge
     for (uint32_t i = t / BINS; i < n_chunks; i += STEP) {
       const double d = r.edge - s.first[i];
       if (!(d < INFINITY) || (double)b + d < (double)(BINS - 1)) continue;
-      const uint64_t w = ((const uint64_t *)(parts + (size_t)i * PART + HEAD))[b];
-      if (!w) continue;
-      atomicAdd(&s.below, (unsigned long long)whole((double)(w & SUM) * exp2(((double)(BINS - 1) - (double)b - d) * 0.125)));
-      atomicAdd(&s.fill, (uint32_t)(w >> COUNT_AT));
+      const uint64_t w = ((const uint64_t *)(parts + (size_t)i * PART + HEAD))[b] & SUM;
+      if (w) atomicAdd(&s.below, (unsigned long long)whole((double)w * exp2(((double)(BINS - 1) - (double)b - d) * 0.125)));
     }
-    s.got[t] = sum;
-    s.bucket[t] = n;
+    __syncthreads();  // (the chunks' largest values are read)
+    s.half.sum[t] = sum;
+    s.half.n[t] = n;
     __syncthreads();
+    double c = 0.0, c_all;
     if (t < BINS) {
-      n += s.bucket[t + BINS];
-      sum += s.got[t + BINS];
-      if (b == BINS - 1) n = s.fill, sum = s.below;
-    } else {
-      n = 0, sum = 0;
+      s.n[t + 1] = n + s.half.n[t + BINS];
+      sum += s.half.sum[t + BINS];
+      c = sum_of(b == BINS - 1 ? s.below : sum, s.edge[b]);
     }
-    uint32_t n_all;
-    double c_all;
-    const uint32_t n_end = block_scan(n, s.counts, n_all);
-    const double c_end = block_scan(sum_of(sum, edge_weight(b)), s.sums, c_all);
-    if (t < BINS) s.n[t + 1] = n_end, s.c[t + 1] = c_end;
-    if (t == 0) s.n[0] = 0, s.c[0] = 0.0, s.fill = 0;
+    c = block_scan(c, s.sums, c_all);
+    if (t < BINS) s.c[t + 1] = c;
+    if (t == 0) s.n[0] = 0, s.c[0] = 0.0;
     __syncthreads();
   }
 
   // The bins with the borders.  What is known of C(n1) and C(n2) before these are looked at lies between lo and hi.
   const uint32_t total = s.n[BINS];
-  const double t_top = scaled(top, r.c);
   const uint32_t k = !(T > 0.0f) || min_p > 1.0f ? 1 : words[3] && words[3] < total ? words[3] : total;
   const double least = min_p > 0.0f ? t_top + 8.0 * log2(fmin((double)min_p, 1.0)) : -INFINITY;
   const uint32_t bm = min_p > 0.0f ? bin_of(r, least) : BINS;
@@ -456,182 +478,133 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
   if (b1 < BINS) {
     lo = s.c[b1], hi = s.c[b1 + 1];
     if (b1 == bk) {
-      const double more = (double)(k - s.n[bk]) * edge_weight(bk);
+      const double more = (double)(k - s.n[bk]) * s.edge[bk];
       hi = fmin(hi, lo + more);
-      if (bm != bk && bk < BINS - 1) lo += more * edge_weight(1);
+      if (bm != bk && bk < BINS - 1) lo += more * s.edge[1];
     }
-    if (b1 == 0) lo = fmax(lo, edge_weight(1));  // the largest stays
+    if (b1 == 0) lo = fmax(lo, s.edge[1]);  // the largest stays
   }
-  uint32_t p_lo = BINS, p_hi = 0;
+  const uint32_t b_last = min(b1, first_bin(s.n, [&](uint32_t n) { return n >= total; }));  // where n1 lies, or past it
   const bool by_p = top_p < 1.0f;
   const double share = fmax((double)top_p, 0.0);
-  const uint32_t b_last = min(b1, first_bin(s.n, [&](uint32_t n) { return n >= total; }));  // where n1 lies
+  uint32_t p_lo = b_last, p_hi = b_last;  // where n2 lies
   if (by_p) {
     lo *= share * LESS, hi *= share * MORE;
     p_lo = min(first_bin(s.c, [&](double c) { return c >= lo; }), b_last);
     p_hi = min(first_bin(s.c, [&](double c) { return c >= hi; }), b_last);
-    hi = fmin(s.c[p_hi + 1], hi + edge_weight(p_lo));
-    lo = fmax(lo, s.n[p_lo] ? 0.0 : edge_weight(1) * LESS);
+    hi = fmin(s.c[p_hi + 1], hi + s.edge[p_lo]);
+    lo = fmax(lo, s.edge[1] * LESS);
   }
   const double u = ((double)words[4] + 0.5) * 0x1p-32;
-  const uint32_t d_lo = min(first_bin(s.c, [&](double c) { return c > lo * u * LESS; }), by_p ? p_hi : b_last);
-  const uint32_t d_hi = min(first_bin(s.c, [&](double c) { return c > hi * u * MORE; }), by_p ? p_hi : b_last);
-  auto looked_at = [&](uint32_t b) { return b == b1 || (b >= p_lo && b <= p_hi) || (b >= d_lo && b <= d_hi); };
-
-  // their places, and how many
-  uint32_t n_spans, n_values, deepest;
-  {
-    const bool yes = t < BINS && looked_at(t) && s.n[t + 1] > s.n[t];
-    const uint32_t at = block_scan((uint32_t)yes, s.counts, n_spans);
-    if (t < BINS) s.span[t] = yes ? at - 1 : ~0u;
-    block_scan(yes ? s.n[t + 1] - s.n[t] : 0u, s.counts, n_values);
-    deepest = b1 < BINS ? b1 : by_p ? p_hi : d_hi;
+  const uint32_t d_lo = min(first_bin(s.c, [&](double c) { return c > lo * u * LESS; }), p_hi);
+  const uint32_t d_hi = min(first_bin(s.c, [&](double c) { return c > hi * u * MORE; }), p_hi);
+  // up to three runs of bins [f, e], each below the one before (one that is not there: f = ~0)
+  uint32_t f0 = d_lo, e0 = d_hi, f1 = ~0u, e1 = 0, f2 = ~0u, e2 = 0;
+  if (by_p) {
+    if (p_lo <= e0 + 1)
+      e0 = max(e0, p_hi);
+    else
+      f1 = p_lo, e1 = p_hi;
   }
-  Found n1, n2, chosen;
-  if (n_spans <= SPANS && n_values <= MOST && deepest < BINS - 1) {
-    // ---- few: their values into LDS, from the chunks' lists where these go down far enough, in buckets by t
-    const double down = t < n_chunks ? (double)deepest - (r.edge - s.first[t]) : -1.0;  // such a chunk's bin
-    const bool listed = !__syncthreads_or(t < n_chunks && down >= (double)s.listed[t]);
-    const uint32_t per = DRAW / max(n_spans, 1u);
-    auto bucket_of = [&](uint32_t b, double v) {
-      const double f = 1.0 - (v - __builtin_floor(v));
-      return s.span[b] * per + min((uint32_t)(int)(f * (double)per), per - 1);
+  if (b1 < BINS) {
+    if (b1 <= e0 + 1)
+      e0 = max(e0, b1);
+    else if (f1 != ~0u && b1 <= e1 + 1)
+      e1 = max(e1, b1);
+    else
+      f2 = e2 = b1;
+  }
+  // the bins and tokens before each run
+  uint32_t n_spans = e0 - f0 + 1, n = s.n[e0 + 1] - s.n[f0], deepest = e0, span1 = n_spans, at1 = n, span2 = 0, at2 = 0;
+  if (f1 != ~0u) n_spans += e1 - f1 + 1, n += s.n[e1 + 1] - s.n[f1], deepest = e1;
+  span2 = n_spans, at2 = n;
+  if (f2 != ~0u) n_spans++, n += s.n[e2 + 1] - s.n[f2], deepest = e2;
+  Found n2, chosen;
+  if (n_spans <= SPANS && n <= MOST && deepest < BINS - 1) {
+    // ---- few: from the chunks' lists into LDS, in buckets by t
+    const uint32_t per = DRAW / n_spans;
+    auto bucket_of = [&](double v) {
+      const double g = __builtin_floor(v), f = 1.0 - (v - g);
+      const uint32_t b = (uint32_t)(int)(r.edge - g), i = b >= f2 ? span2 + b - f2 : b >= f1 ? span1 + b - f1 : b - f0;
+      return i * per + min((uint32_t)(int)(f * (double)per), per - 1);
     };
-    s.bucket[t] = 0;
-    if (t == 0) s.bucket[DRAW] = 0;
-    __syncthreads();
-    auto take = [&](uint64_t place, double v) {
-      const uint32_t b = bin_of(r, v);
-      if (s.span[b] == ~0u) return;
-      const uint32_t at = atomicAdd(&s.fill, 1u);
-      if (at < MOST) s.got[at] = place;  // (always: so many were counted)
-      atomicAdd(&s.bucket[bucket_of(b, v)], 1u);
-    };
-    if (listed) {
-      constexpr uint32_t U = 5, STEP = DRAW / LIST;
-      for (uint32_t i0 = t / LIST; i0 < n_chunks; i0 += U * STEP) {
-        uint2 v[U];
-        bool is[U];
-#pragma unroll
-        for (uint32_t j = 0; j < U; j++) {
-          const uint32_t i = min(i0 + j * STEP, n_chunks - 1);
-          is[j] = i0 + j * STEP < n_chunks && t % LIST < s.values[i];
-          v[j] = is[j] ? ((const uint2 *)(parts + (size_t)i * PART + HEAD + 2 * BINS))[t % LIST] : make_uint2(0, 0);
-        }
-#pragma unroll
-        for (uint32_t j = 0; j < U; j++)
-          if (is[j]) {
-            const float x = __builtin_bit_cast(float, v[j].x);
-            take(place(x, v[j].y), scaled(x, r.c));
-          }
+    constexpr uint32_t LANES = 16;  // of a chunk's run
+    for (uint32_t j = t / LANES; j < n_chunks * 3; j += DRAW / LANES) {
+      const uint32_t i = j / 3, which = j % 3, f = which == 0 ? f0 : which == 1 ? f1 : f2, e = which == 0 ? e0 : which == 1 ? e1 : e2;
+      const float *part = parts + (size_t)i * PART;
+      const double d = r.edge - s.first[i];
+      if (f == ~0u || !(d <= (double)e)) continue;
+      const uint32_t down = (uint32_t)(int)d;
+      const uint64_t *bins = (const uint64_t *)(part + HEAD);
+      const uint32_t i0 = f > down ? (uint32_t)(bins[f - down - 1] >> COUNT_AT) : 0,
+                     i1 = (uint32_t)(bins[e - down] >> COUNT_AT);
+      for (uint32_t o = i0 + t % LANES; o < i1; o += LANES) {
+        const uint32_t id = i * CHUNK + ((const uint16_t *)(part + HEAD + 2 * BINS))[o];
+        const float x = r.x[id];
+        const uint32_t to = atomicAdd(&s.fill, 1u);
+        if (to < MOST) s.place[0][to] = place(x, id);  // (always: so many were counted)
+        atomicAdd(&s.bucket[bucket_of(scaled(x, r.c))], 1u);
       }
-    } else {
-      each_value(r, r.edge - (double)deepest, take);
     }
     __syncthreads();
-    const uint32_t n = min(s.fill, MOST);
     uint32_t all;
     const uint32_t mine = s.bucket[t], end = block_scan(mine, s.counts, all);
     s.bucket[t] = end - mine;  // where the bucket starts
     __syncthreads();
     for (uint32_t i = t; i < n; i += DRAW) {
-      const uint64_t v = s.got[i];
-      const double at = scaled(value_at(v), r.c);
-      s.in_order[atomicAdd(&s.bucket[bucket_of(bin_of(r, at), at)], 1u)] = v;
+      const uint64_t v = s.place[0][i];
+      s.place[1][atomicAdd(&s.bucket[bucket_of(scaled(value_at(v), r.c))], 1u)] = v;
     }
     __syncthreads();  // a bucket's word is now its end, the one before it its start
-    uint64_t v[MOST / DRAW];
-    uint32_t rank[MOST / DRAW];
-#pragma unroll
-    for (uint32_t j = 0; j < MOST / DRAW; j++) {
-      const uint32_t i = t + DRAW * j;
-      if (i >= n) continue;
-      v[j] = s.in_order[i];
-      const double at = scaled(value_at(v[j]), r.c);
-      const uint32_t b = bucket_of(bin_of(r, at), at), from = b ? s.bucket[b - 1] : 0, to = s.bucket[b];
-      rank[j] = from;
-      for (uint32_t o = from; o < to; o++) rank[j] += s.in_order[o] < v[j];
+    for (uint32_t i = t; i < n; i += DRAW) {
+      const uint64_t v = s.place[1][i];
+      const uint32_t b = bucket_of(scaled(value_at(v), r.c)), o0 = b ? s.bucket[b - 1] : 0, o1 = s.bucket[b];
+      uint32_t rank = o0;
+      for (uint32_t o = o0; o < o1; o++) rank += s.place[1][o] < v;
+      s.place[0][rank] = v;
     }
     __syncthreads();
-#pragma unroll
-    for (uint32_t j = 0; j < MOST / DRAW; j++)
-      if (t + DRAW * j < n) s.in_order[rank[j]] = v[j];
-    __syncthreads();
-    // the sum behind each: of thread t the values [8 t, 8 t + 8)
-    constexpr uint32_t OF = MOST / DRAW;
-    uint64_t w[OF], sum = 0, sum_all;
-    uint32_t bin[OF];
-#pragma unroll
-    for (uint32_t j = 0; j < OF; j++) {
-      const uint32_t i = OF * t + j;
-      bin[j] = 0, w[j] = 0;
-      if (i < n) {
-        const double at = scaled(value_at(s.in_order[i]), r.c);
-        bin[j] = bin_of(r, at);
-        w[j] = fixed_weight(r, at);
-      }
-      sum += w[j];
-    }
-    uint64_t before = block_scan(sum, s.words, sum_all) - sum;
-#pragma unroll
-    for (uint32_t j = 0; j < OF; j++) {
-      before += w[j];
-      if (OF * t + j < n) s.upto[OF * t + j] = before;
+    // the sum behind each, in place of those in buckets
+    uint64_t carry = 0, *raw = s.place[1];
+    for (uint32_t i0 = 0; i0 < n; i0 += DRAW) {
+      const uint32_t i = i0 + t;
+      const uint64_t w = i < n ? fixed_weight(r, scaled(value_at(s.place[0][i]), r.c)) : 0;
+      uint64_t sum_all;
+      const uint64_t sum = block_scan(w, s.words, sum_all) + carry;
+      if (i < n) raw[i] = sum;
+      carry += sum_all;
     }
     __syncthreads();
-    // of a looked-at bin the first place in the order; its sums start at the bin's C
-    if (t < BINS && s.span[t] != ~0u) s.bucket[s.span[t]] = t;
-    __syncthreads();
-    if (t < 64) {
-      const uint32_t b = t < n_spans ? s.bucket[t] : 0, c = t < n_spans ? s.n[b + 1] - s.n[b] : 0;
-      const uint32_t start = wave_scan(c, t) - c;
-      if (t < n_spans) s.span[b] = start;
-    }
-    __syncthreads();
-    auto upto = [&](uint32_t i, uint32_t b) {
-      const uint32_t start = s.span[b];
-      return s.c[b] + sum_of(s.upto[i] - (start ? s.upto[start - 1] : 0), edge_weight(b));
+    if (t >= 64) return;
+    // (the first wave alone)
+    auto start_of = [&](uint32_t b) {  // in the order here
+      return b >= f2 ? at2 + s.n[b] - s.n[f2] : b >= f1 ? at1 + s.n[b] - s.n[f1] : s.n[b] - s.n[f0];
     };
-    auto rank_of = [&](uint32_t i, uint32_t b) { return s.n[b] + i - s.span[b] + 1; };
     auto found_at = [&](uint32_t i) {
-      const uint64_t at = s.in_order[i];
-      const uint32_t b = bin_of(r, scaled(value_at(at), r.c));
-      return Found{at, rank_of(i, b), upto(i, b)};
+      const double v = scaled(value_at(s.place[0][i]), r.c);
+      const uint32_t b = bin_of(r, v), i0 = start_of(b);
+      return Found{s.place[0][i], s.n[b] + i - i0 + 1, s.c[b] + sum_of(raw[i] - (i0 ? raw[i0 - 1] : 0), s.edge[b])};
     };
-    // n1: the last place of bin b1 that stays
-    n1 = {0, total, s.c[BINS]};
+    // n1: of bin b1 those that stay
+    Found n1{0, total, s.c[BINS]};
     if (b1 < BINS) {
-      if (t == 0) s.found[0] = 0;
-      __syncthreads();
-#pragma unroll
-      for (uint32_t j = 0; j < OF; j++) {
-        const uint32_t i = OF * t + j;
-        if (i < n && bin[j] == b1 && rank_of(i, b1) <= k && scaled(value_at(s.in_order[i]), r.c) >= least)
-          atomicMax(&s.found[0], i + 1);
-      }
-      __syncthreads();
-      n1 = s.found[0] ? found_at(s.found[0] - 1) : Found{0, s.n[b1], s.c[b1]};
+      const uint32_t i0 = start_of(b1);
+      uint32_t some = s.n[b1 + 1] - s.n[b1];
+      if (b1 == bk) some = k - s.n[b1];
+      if (b1 == bm) some = first_of(some, [&](uint32_t i) { return scaled(value_at(s.place[0][i0 + i]), r.c) < least; });
+      n1 = some ? found_at(i0 + some - 1) : Found{0, s.n[b1], s.c[b1]};
     }
-    // the first place in bins [from, to] that meets `want`, the last of them if none does
-    auto first = [&](Want want, double goal, uint32_t most, uint32_t from, uint32_t to) {
-      __syncthreads();
-      if (t == 0) s.found[1] = ~0u, s.found[2] = 0;
-      __syncthreads();
-#pragma unroll
-      for (uint32_t j = 0; j < OF; j++) {
-        const uint32_t i = OF * t + j;
-        if (i >= n || bin[j] < from || bin[j] > to || rank_of(i, bin[j]) > most) continue;
-        if (meets(want, goal, 0, upto(i, bin[j]))) atomicMin(&s.found[1], i);
-        atomicMax(&s.found[2], i);
-      }
-      __syncthreads();
-      return found_at(s.found[1] != ~0u ? s.found[1] : s.found[2]);
+    // the first token of bins [f, e], not past the n-th, that meets `want`; the last of these if none does
+    auto first = [&](Want want, double goal, uint32_t most, uint32_t f, uint32_t e) {
+      const uint32_t i0 = start_of(f), end = max(min(s.n[e + 1], most), s.n[f]) - s.n[f];
+      const uint32_t i = first_of(end, [&](uint32_t i) { return meets(want, goal, 0, found_at(i0 + i).sum); });
+      return found_at(min(i0 + (i < end ? i : max(end, 1u) - 1), n - 1));
     };
     n2 = by_p ? first(kReach, share * n1.sum, n1.n, p_lo, p_hi) : n1;
     chosen = first(kPass, u * n2.sum, n2.n, d_lo, d_hi);
   } else {
     // ---- many
-    n1 = {0, total, s.c[BINS]};
+    Found n1{0, total, s.c[BINS]};
     if (b1 < BINS && b1 == bm) n1 = search_above(s, r, least, bm);
     if (b1 < BINS && b1 == bk) {
       const Found by_k = search(s, r, kCount, (double)k);

@@ -40,7 +40,7 @@ constexpr uint32_t kMergeParts = 16, kMergeHeads = 512;
 // rows of 30000 12.2 / 9.9, of 4096 7.4 / 8.0; 1 row of 30000 9.7 / 8.6, of 1000 5.7 / 6.4).
 constexpr uint32_t kLogitsHistory = 8192;
 // Tokens of a logits_sample workgroup, words of its part, and the most tokens of a vocabulary (sample.hip).
-constexpr uint32_t kSampleChunk = 8192, kSamplePart = 1544, kSampleVocab = 1u << 20;
+constexpr uint32_t kSampleChunk = 8192, kSamplePart = 5128, kSampleVocab = 1u << 20;
 constexpr uint32_t kMaxWork = 1u << 23;   // workgroups of an attention launch
 
 // A buffer bound to a dispatch: where it lies and how large it is.

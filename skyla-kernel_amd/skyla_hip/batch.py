@@ -129,7 +129,7 @@ def part_size(rows: int, n_head: int, parts) -> int:
     return rows * n_head * (parts[0] + parts[1]) * 130
 
 
-SAMPLE_CHUNK, SAMPLE_PART, SAMPLE_VOCAB = 8192, 1544, 1 << 20  # (runtime/batch.h)
+SAMPLE_CHUNK, SAMPLE_PART, SAMPLE_VOCAB = 8192, 5128, 1 << 20  # (runtime/batch.h)
 
 
 def sample_size(rows: int, n_vocab: int) -> int:
