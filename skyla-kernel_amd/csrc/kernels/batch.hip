@@ -3,8 +3,11 @@
 //
 // Contract (bindings, push words; every grid is [1, rows, 1], and the runtime chooses the launch):
 //   kv_append              [W, A, C, KV, KV8]   24 words  spec [K_Q8, V_Q8, head_dim]
+//   kv_append_axes         [W, A, C, KV, KV8]   26 words  spec [K_Q8, V_Q8, head_dim]
 //   attention_paged        [A, C, KV, KV8, KVS] 20 words  spec [N_REP, K_Q8, V_Q8, head_dim]
 //   attention_paged_merge  [A, C]               10 words  spec [head_dim]
+//   attention_paged_shaped       [A, C, KV, KV8, KVS] 25 words  spec [N_REP, K_Q8, V_Q8, head_dim]
+//   attention_paged_shaped_merge [A, C]         13 words  spec [head_dim]
 //   logits_adjust          [A, C]               12 words
 // Bindings as in attention.hip.  Heads are 128 wide.
 //
@@ -41,6 +44,10 @@ struct AppendPush {
   uint32_t n_head, n_kv, q_stride, kv_stride, o_stride, kc_off, vc_off, ks_off, vs_off, rows_off, table_off,
       table_stride, n_seq, n_pages, page_log2;
 };
+struct AppendAxesPush {
+  AppendPush append;
+  uint32_t axes_off, n_axes;
+};
 struct PagedPush {
   uint32_t q_off, q_stride, o_off, o_stride, part_off, kc_off, vc_off, ks_off, vs_off, n_kv;
   float scale;
@@ -49,6 +56,15 @@ struct PagedPush {
 struct PagedMergePush {
   uint32_t part_off, o_off, o_stride, n_head, n_shared, n_own, rows_off, table_stride, n_seq, page_log2;
 };
+struct ShapedPush : PagedPush {
+  uint32_t spans_off, slopes_off, window, n_lead;
+  float cap;
+};
+struct ShapedMergePush : PagedMergePush {
+  uint32_t spans_off, window, n_lead;
+};
+template <typename P>
+constexpr bool SHAPED = std::is_base_of<ShapedPush, P>::value || std::is_base_of<ShapedMergePush, P>::value;
 struct LogitsPush {
   uint32_t x_off, y_off, x_stride, y_stride, n_vocab, ctrl_off, hist_off, hist_stride, bias_off, bias_stride, mask_off,
       mask_stride;
@@ -84,6 +100,56 @@ SK_DEV Range row_range(const uint32_t *ctl, uint32_t rows_off, uint32_t row, uin
   r.member = shared != 0 && w.z != 0 && r.len >= shared;
   r.start = r.member ? shared : 0;
   return r;
+}
+
+// attention_paged_shaped: row r's token, at position i = len - 1, attends to the positions j of [lo, hi): from
+// `from`, and with a window from len - window on, up to len, or to `until` where that is more ({from, until} at
+// spans_off + 2 r; their positions are in the cache when the kernel runs).  A row of len 0, or whose mask leaves
+// nothing, gives zeros.  With s = scale q k a score is cap tanh(s / cap) (cap 0: s), less slope_h |i - j| (the
+// heads' slopes at slopes_off; ~0: none).
+// The shared run is [S, P), S the tile's end at or above ctl[5] (the shared kernels' mask is the run itself: no row
+// attends to a part of it): a row takes it with share != 0 and len >= P if it attends to all of it, lo <= S.  Its
+// own pages serve [lo, S), its lead, in n_lead parts (without lead parts lo must be S), and those from P on.
+struct ShapedRange : Range {  // tail: [start, len), len the end hi
+  uint32_t lo, at;            // lead: [lo, S) of a member; the position i
+};
+template <typename P>
+SK_DEV uint32_t shared_first(const uint32_t *ctl, const P &p, uint32_t shared) {
+  const uint32_t first = min(ctl[5], shared);
+  return (first + TILE - 1) / TILE * TILE;
+}
+template <typename P>
+SK_DEV uint32_t shared_end(const uint32_t *ctl, const P &p) {  // 0: none
+  const uint32_t shared = shared_positions(ctl, p.n_shared, p.n_seq, p.table_stride, p.page_log2);
+  if constexpr (SHAPED<P>) return shared_first(ctl, p, shared) < shared ? shared : 0;
+  return shared;
+}
+template <typename P>
+SK_DEV ShapedRange shaped_range(const uint32_t *ctl, const P &p, uint32_t row, uint32_t shared) {
+  ShapedRange r;
+  (Range &)r = row_range(ctl, p.rows_off, row, shared, p.n_seq, p.table_stride, p.page_log2);
+  const uint2 span = *(const uint2 *)(ctl + p.spans_off + 2 * row);
+  const uint64_t cap = (uint64_t)p.table_stride << p.page_log2;
+  const uint32_t len = r.len;
+  r.at = len - 1;
+  r.lo = p.window && len > p.window ? max(span.x, len - p.window) : span.x;
+  if (len && span.y > len) r.len = span.y < cap ? span.y : (uint32_t)cap;
+  if (r.lo >= r.len) {
+    r.lo = r.start = r.len = 0, r.member = false;
+    return r;
+  }
+  const uint32_t first = shared_first(ctl, p, shared);
+  r.member = r.member && (p.n_lead ? r.lo <= first : r.lo == first);
+  r.start = r.member ? shared : r.lo;
+  return r;
+}
+// a row's range, whichever kernel's
+template <typename P>
+SK_DEV auto range_of(const uint32_t *ctl, const P &p, uint32_t row, uint32_t shared) {
+  if constexpr (SHAPED<P>)
+    return shaped_range(ctl, p, row, shared);
+  else
+    return row_range(ctl, p.rows_off, row, shared, p.n_seq, p.table_stride, p.page_log2);
 }
 
 // A run of positions [lo, hi) in tiles of TILE from a multiple of 16 at or below lo, cut into at
@@ -147,8 +213,14 @@ SK_DEV void store_row(f16 *kv, int8_t *kv8, uint32_t cache, uint32_t scales, uin
 // compute unit for eight.  PASSES = 4 where 16 heads a workgroup would make 4096 of them or more (2048
 // rows 33.5 us against 36), below it more workgroups are better (1000 rows 24 against 26.5).  1 row 2.5
 // us: the launch and the dependent round trips.
-template <int K8, int V8, int PASSES>
-SK_DEV void append_body(const float *w, float *a, const uint32_t *ctl, f16 *kv, int8_t *kv8, const AppendPush &p) {
+//
+// kv_append_axes turns by positions of several axes (time, height, width of images and video): row r has four words
+// at axes_off + 4 r, and pair d's angle is the sum over the axes a < n_axes <= 4 of word a times the frequency
+// at rope_off + 64 a + d, formed in 64 bits.  A pair that one axis turns has its frequency at that axis and 0 at
+// the others, so any layout of sections is the table's.
+template <int K8, int V8, int PASSES, int AXES>
+SK_DEV void append_body(const float *w, float *a, const uint32_t *ctl, f16 *kv, int8_t *kv8, const AppendPush &p,
+                        uint32_t axes_off = 0, uint32_t n_axes = 0) {
 #pragma clang fp contract(off)
   __shared__ float2 turn[4][64];
   const uint32_t row = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, t = lane & 15;
@@ -173,7 +245,18 @@ SK_DEV void append_body(const float *w, float *a, const uint32_t *ctl, f16 *kv, 
   const uint32_t slot = (page << p.page_log2) + (pos & ((1u << p.page_log2) - 1));
   const uint32_t kv_dim = p.n_kv * HD;
   {
-    const double turns = (double)pos * (double)w[p.rope_off + lane] * 0.15915494309189533577;  // 1 / (2 pi)
+    double angle;
+    if constexpr (AXES) {
+      const uint4 at = *(const uint4 *)(ctl + axes_off + 4 * row);
+      const float *f = w + p.rope_off + lane;
+      angle = (double)at.x * (double)f[0];
+      if (n_axes > 1) angle += (double)at.y * (double)f[64];
+      if (n_axes > 2) angle += (double)at.z * (double)f[128];
+      if (n_axes > 3) angle += (double)at.w * (double)f[192];
+    } else {
+      angle = (double)pos * (double)w[p.rope_off + lane];
+    }
+    const double turns = angle * 0.15915494309189533577;  // 1 / (2 pi)
     float s, c;
     sincospif((float)(2.0 * (turns - __builtin_rint(turns))), &s, &c);
     turn[wave][lane] = make_float2(c * p.mscale, s * p.mscale);
@@ -265,6 +348,45 @@ SK_DEV f16x8 widen8(uint2 x) {
   return __builtin_bit_cast(f16x8, make_uint4(as_u32(widen(x.x, x.x, 0x0c010c00u)), as_u32(widen(x.x, x.x, 0x0c030c02u)),
                                               as_u32(widen(x.y, x.y, 0x0c010c00u)), as_u32(widen(x.y, x.y, 0x0c030c02u))));
 }
+// Scores in powers of two to what they are capped and biased to.  c tanh(s / c) = s P((s / c)^2), P the polynomial
+// of degree 4 nearest to tanh(x) / x for |x| <= 1/2 (1.3e-8 of it at most); where a wave has a larger score,
+// c (1 - e) / (1 + e), e = exp(-2 |s| / c), for those (within 4e-7).
+struct Cap {
+  float c, inv, edge, p[5];
+};
+SK_DEV float to_scalar(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+}
+SK_DEV Cap cap_of(float cap) {
+  const float c = cap * 1.44269504088896340736f, inv = 1.0f / c, k = inv * inv;
+  Cap x{c, inv, 0.5f * c, {0.99999999f, -0.33333069f * k, 0.13324779f * k * k, -0.05298608f * k * k * k, 0.01713501f * k * k * k * k}};
+  x.c = to_scalar(x.c), x.inv = to_scalar(x.inv), x.edge = to_scalar(x.edge);
+#pragma unroll
+  for (int i = 0; i < 5; i++) x.p[i] = to_scalar(x.p[i]);
+  return x;
+}
+template <int N, typename S>
+SK_DEV void cap_scores(S &s, const Cap &x) {
+  float big = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; i += 2) big = max3(big, fabsf(s[i]), fabsf(s[i + 1]));
+  const bool any = __any(!(big <= x.edge));
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    const float v = s[i], u = v * v;
+    float y = __builtin_fmaf(x.p[4], u, x.p[3]);
+    y = __builtin_fmaf(y, u, x.p[2]);
+    y = __builtin_fmaf(y, u, x.p[1]);
+    y = __builtin_fmaf(y, u, x.p[0]) * v;
+    if (any) {
+      const float e = __builtin_amdgcn_exp2f(fabsf(v) * x.inv * -2.88539008177792681472f);
+      const float far = __builtin_copysignf(x.c * (1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e), v);
+      y = fabsf(v) > x.edge ? far : y;
+    }
+    s[i] = y;
+  }
+}
+
 // The page table through the scalar cache: nothing writes it while the kernel runs, and a vector
 // load's wait would be one for the cache rows in flight, too.
 typedef const __attribute__((address_space(4))) uint32_t ConstWord;
@@ -308,10 +430,10 @@ struct HalfRows {
   typename std::conditional<V8, uint2, uint4>::type v[8];
   f16 vs[V8 ? 8 : 1];
 };
-template <int K8, int V8>
-SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t *kv8, const PagedPush &p, uint32_t kvh,
+template <int K8, int V8, typename P>
+SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t *kv8, const P &p, uint32_t kvh,
                      const float *q, float (*out)[PART], uint32_t seq, uint32_t lo, uint32_t hi, uint32_t begin,
-                     uint32_t end) {
+                     uint32_t end, float slope = 0.0f, uint32_t row_at = 0) {
   const uint32_t lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, kv_dim = p.n_kv * HD;
   // wave-uniform, and known to be
   lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
@@ -398,6 +520,11 @@ SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
         ql[k][e] = (f16)(x - (float)qh[k][e]);
       }
   }
+  [[maybe_unused]] Cap cap;
+  if constexpr (SHAPED<P>) {
+    if (p.cap > 0.0f) cap = cap_of(p.cap);
+  }
+  const float unit = SHAPED<P> ? 1.0f : inv;  // of the scores as they are weighed
   float m = -INFINITY, l;
   int ve = -200, vo = -200;  // of the dims that this lane's values and sums hold (blocks c / 4 and g)
   f32x4 o[8];
@@ -430,6 +557,16 @@ SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
 #pragma unroll
       for (uint32_t i = 0; i < 4; i++) sc[t][i] = acc[i];
     }
+    if constexpr (SHAPED<P>) {
+      float s[8];
+#pragma unroll
+      for (uint32_t i = 0; i < 8; i++) s[i] = sc[i >> 2][i & 3] * inv;
+      if (p.cap > 0.0f) cap_scores<8>(s, cap);
+      const int away = (int)(at + 4 * g - row_at);
+#pragma unroll
+      for (uint32_t i = 0; i < 8; i++)
+        sc[i >> 2][i & 3] = __builtin_fmaf(-slope, fabsf((float)(away + (int)(16 * (i >> 2) + (i & 3)))), s[i]);
+    }
     if (at < lo || at + HALF > hi) {
 #pragma unroll
       for (uint32_t t = 0; t < 2; t++)
@@ -444,7 +581,7 @@ SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
     mt = max3(mt, sc[1][1], sc[1][2]);
     mt = fmaxf(mt, sc[1][3]);
     mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
-    mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * inv;
+    mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * unit;
     int top = -200;      // the scales' largest exponent
     float least = 0.0f;  // and the smallest of this lane's that is not 0
     if constexpr (V8) {
@@ -478,7 +615,7 @@ SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
     const float cm = (float)E_SHIFT - (m > -INFINITY ? m : 0.0f);
     f16x8 ph, pl;
 #pragma unroll
-    for (int n = 0; n < 4; n++) weigh(sc[n >> 1][2 * (n & 1)], sc[n >> 1][2 * (n & 1) + 1], inv, cm, l, ph, pl, 2 * n);
+    for (int n = 0; n < 4; n++) weigh(sc[n >> 1][2 * (n & 1)], sc[n >> 1][2 * (n & 1) + 1], unit, cm, l, ph, pl, 2 * n);
     f16x2 sv[V8 ? 4 : 1];
     if constexpr (V8) {
       const int up = 4 - ve + WINDOW<9> * window;
@@ -590,6 +727,11 @@ SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
 // bound by what a workgroup does once: 15 us of round trips, the pass over the scales, the query rows'
 // parts and the partials' writes.
 constexpr uint32_t WIDE = 128, STEP = 32;
+template <typename P>
+SK_DEV uint32_t slots_of(const P &p) {  // partials of a row and head
+  if constexpr (SHAPED<P>) return p.n_shared + p.n_own + p.n_lead;
+  return p.n_shared + p.n_own;
+}
 template <int Q8>
 struct RawRows {
   uint4 x[STEP][Q8 ? 8 : 16];
@@ -605,15 +747,17 @@ struct WideStage {  // at most half of the 160 KB: two workgroups a compute unit
   uint4 vh[V8 ? 2 : 1][V8 ? 2 : 1][2][4][V8 ? 64 : 1];  // and values: [step][part][k-step][dims / 32]
   u16x2 ends[4][4];
 };
-template <int K8, int V8>
-SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t *kv8, const PagedPush &p, uint32_t rep,
+template <int K8, int V8, typename P>
+SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t *kv8, const P &p, uint32_t rep,
                      uint32_t kvh, uint32_t tile, uint32_t part, uint32_t shared, uint32_t n_rows,
                      WideStage<K8, V8> &st) {
   const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, col = lane & 31,
                  h = lane >> 5;
   const uint32_t kv_dim = p.n_kv * HD;
-  const Split sp = split_of(0, shared, p.n_shared);
-  const uint32_t begin = part * sp.per * TILE, end = min(begin + sp.per * TILE, shared);
+  uint32_t first_at = 0;
+  if constexpr (SHAPED<P>) first_at = shared_first(ctl, p, shared);
+  const Split sp = split_of(first_at, shared, p.n_shared);
+  const uint32_t begin = first_at + part * sp.per * TILE, end = min(begin + sp.per * TILE, shared);
   if (begin >= end) return;
   const uint32_t i = tile * WIDE + wave * 32 + col;
   uint32_t row = i / rep;
@@ -677,9 +821,16 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
   };
   prime();
 
-  const bool live =
-      row < n_rows && row_range(ctl, p.rows_off, row, shared, p.n_seq, p.table_stride, p.page_log2).member;
+  const bool live = row < n_rows && range_of(ctl, p, row, shared).member;
   row = min(row, n_rows - 1);
+  [[maybe_unused]] Cap cap;
+  [[maybe_unused]] float slope = 0.0f;
+  [[maybe_unused]] uint32_t row_at = 0;
+  if constexpr (SHAPED<P>) {
+    if (p.cap > 0.0f) cap = cap_of(p.cap);
+    if (p.slopes_off != ~0u) slope = __builtin_bit_cast(float, ctl[p.slopes_off + kvh * rep + head]) * 1.44269504088896340736f;
+    row_at = range_of(ctl, p, row, shared).at;
+  }
   // this wave's query rows
   f16x8 qh[8], ql[8];
   float inv;
@@ -846,6 +997,7 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
 
   f32x16 o[4];
   float m = -INFINITY, l;
+  const float unit = SHAPED<P> ? 1.0f : inv;  // of the scores as they are weighed
   const uint32_t n_steps = (end - begin + STEP - 1) / STEP;
   Rows vat, kat;
   // `sc`: this step's scores; into `next` the next step's
@@ -864,6 +1016,16 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
     } else {
       sc = scores(step);
     }
+    if constexpr (SHAPED<P>) {
+#pragma unroll
+      for (uint32_t r = 0; r < 16; r++) sc[r] *= inv;
+      if (p.cap > 0.0f) cap_scores<16>(sc, cap);
+      if (p.slopes_off != ~0u) {  // (every position is below the row's)
+        const float away = (float)(int)(at + 4 * h - row_at) * slope;
+#pragma unroll
+        for (uint32_t r = 0; r < 16; r++) sc[r] += __builtin_fmaf(slope, (float)(8 * (r >> 2) + (r & 3)), away);
+      }
+    }
     if (at + STEP > end) {  // the run's last positions
 #pragma unroll
       for (uint32_t r = 0; r < 16; r++)
@@ -873,7 +1035,7 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
 #pragma unroll
     for (int r = 3; r < 15; r += 2) mt = max3(mt, sc[r], sc[r + 1]);
     mt = fmaxf(mt, sc[15]);
-    mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * inv;
+    mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * unit;
     if (__any(mt > m + LOOSE)) {  // rare after the first steps
       const float mn = mt > m + LOOSE ? mt : m;
       const float down = mn > -INFINITY ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
@@ -884,7 +1046,7 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
     }
     const float c = (float)E_SHIFT - (m > -INFINITY ? m : 0.0f);
     f16x8 ph[2], pl[2];
-    auto weigh2 = [&](uint32_t n) { weigh(sc[2 * n], sc[2 * n + 1], inv, c, l, ph[n >> 2], pl[n >> 2], 2 * (n & 3)); };
+    auto weigh2 = [&](uint32_t n) { weigh(sc[2 * n], sc[2 * n + 1], unit, c, l, ph[n >> 2], pl[n >> 2], 2 * (n & 3)); };
     f16x8 vf[V8 ? 2 : 1][3];
     auto read_values = [&](uint32_t n) {  // of product n: k-step n / 4, dims 32 (n % 4) + [0, 32)
       vf[0][n % 3] = value(step, 0, n >> 2, n & 3);
@@ -962,7 +1124,7 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
     l += __shfl_xor(l, 32, 64);
     if (live) {
       float *out = a + p.part_off +
-                   ((to / rep * p.n_kv * rep + kvh * rep + to % rep) * (p.n_shared + p.n_own) + part) * PART;
+                   ((to / rep * p.n_kv * rep + kvh * rep + to % rep) * slots_of(p) + part) * PART;
       float *dims = out + 2 + 4 * mine;
 #pragma unroll
       for (int d = 0; d < 4; d++) o[d] *= ldexpf(1.0f, V8 ? ve[d] - WINDOW<7> * run - 7 - E_SHIFT : -E_SHIFT);
@@ -996,14 +1158,13 @@ union PagedShared {
   WideStage<K8, V8> wide;
   float run[4][16][PART];
 };
-template <int N_REP, int K8, int V8>
-SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_t *kv8, const PagedPush &p,
-                       uint32_t n_grid) {
+template <int N_REP, int K8, int V8, typename P>
+SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_t *kv8, const P &p, uint32_t n_grid) {
   const bool wide = p.wide && p.n_shared;
   __shared__ __attribute__((aligned(1024))) PagedShared<K8, V8> st;
   const uint32_t t = threadIdx.x, wave = t >> 6, c = t & 15;
-  const uint32_t n_rows = min(ctl[2], n_grid), slots = p.n_shared + p.n_own, groups = p.n_kv * p.n_shared;
-  const uint32_t shared = shared_positions(ctl, p.n_shared, p.n_seq, p.table_stride, p.page_log2);
+  const uint32_t n_rows = min(ctl[2], n_grid), slots = slots_of(p), groups = p.n_kv * p.n_shared;
+  const uint32_t shared = shared_end(ctl, p);
   uint32_t w = blockIdx.x, kvh, part, seq, lo, hi;
   if (n_rows == 0) return;
   const uint32_t tiles = wide ? (n_grid * N_REP + WIDE - 1) / WIDE : (n_grid * N_REP + 15) / 16;
@@ -1011,6 +1172,7 @@ SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_
   const bool own = w >= n_first;
   uint32_t i0;  // query rows i0 + [0, n_live) of the key head: row i / N_REP, head i % N_REP
   Split sp;
+  [[maybe_unused]] uint32_t slot = 0;  // of an own run's partial
   if (!own) {
     if (shared == 0) return;
     if (wide) {
@@ -1021,15 +1183,28 @@ SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_
     }
     kvh = w % p.n_kv, part = w / p.n_kv % p.n_shared, i0 = w / groups * 16;
     lo = 0, hi = shared, seq = ctl[4];
+    if constexpr (SHAPED<P>) lo = shared_first(ctl, p, shared);
     sp = split_of(lo, hi, p.n_shared);
   } else {
     w -= n_first;
-    kvh = w % p.n_kv, part = w / p.n_kv % p.n_own;
-    const uint32_t row = w / (p.n_kv * p.n_own);
+    const uint32_t n_own = slots - p.n_shared;
+    kvh = w % p.n_kv, part = w / p.n_kv % n_own;
+    const uint32_t row = w / (p.n_kv * n_own);
     if (row >= n_rows) return;
-    const Range r = row_range(ctl, p.rows_off, row, shared, p.n_seq, p.table_stride, p.page_log2);
+    const auto r = range_of(ctl, p, row, shared);
     i0 = row * N_REP, lo = r.start, hi = r.len, seq = r.seq;
-    sp = split_of(lo, hi, p.n_own);
+    if constexpr (SHAPED<P>) {
+      slot = p.n_shared + part;
+      if (part >= p.n_own) {  // of the lead
+        if (!r.member) return;
+        part -= p.n_own, lo = r.lo, hi = shared_first(ctl, p, shared);
+        sp = split_of(lo, hi, p.n_lead);
+      } else {
+        sp = split_of(lo, hi, p.n_own);
+      }
+    } else {
+      sp = split_of(lo, hi, p.n_own);
+    }
   }
   const uint32_t n_live = own ? N_REP : 16;
   const uint32_t begin = sp.base + part * sp.per * TILE, end = min(begin + sp.per * TILE, hi);
@@ -1043,15 +1218,20 @@ SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_
   }
   // whether query row i takes part in this run
   auto live = [&](uint32_t i) {
-    return own || (i / N_REP < n_rows &&
-                   row_range(ctl, p.rows_off, i / N_REP, shared, p.n_seq, p.table_stride, p.page_log2).member);
+    return own || (i / N_REP < n_rows && range_of(ctl, p, i / N_REP, shared).member);
   };
   if (!own && !__syncthreads_or(live(i0 + c))) return;
   const uint32_t steps = (end - begin + HALF - 1) / HALF, per = (steps + 3) / 4 * HALF;
   if (begin + wave * per < end) {
     const uint32_t i = i0 + c % n_live, row = min(i / N_REP, n_rows - 1);
+    float slope = 0.0f;
+    uint32_t row_at = 0;
+    if constexpr (SHAPED<P>) {
+      if (p.slopes_off != ~0u) slope = __builtin_bit_cast(float, ctl[p.slopes_off + kvh * N_REP + i % N_REP]) * 1.44269504088896340736f;
+      row_at = range_of(ctl, p, row, shared).at;
+    }
     wave_run<K8, V8>(a, ctl, kv, kv8, p, kvh, a + p.q_off + row * p.q_stride + (kvh * N_REP + i % N_REP) * HD,
-                     st.run[wave], seq, lo, hi, begin + wave * per, min(begin + (wave + 1) * per, end));
+                     st.run[wave], seq, lo, hi, begin + wave * per, min(begin + (wave + 1) * per, end), slope, row_at);
   }
   const uint32_t used = (steps * HALF + per - 1) / per;  // waves with a run
   __syncthreads();
@@ -1077,7 +1257,7 @@ SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_
       *(float2 *)result(i, d) = make_float2(x / l, y / l);
     } else {
       float *out = a + p.part_off +
-                   ((i / N_REP * p.n_kv * N_REP + kvh * N_REP + i % N_REP) * slots + (own ? p.n_shared : 0) + part) * PART;
+                   ((i / N_REP * p.n_kv * N_REP + kvh * N_REP + i % N_REP) * slots + (SHAPED<P> && own ? slot : (own ? p.n_shared : 0) + part)) * PART;
       *(float2 *)(out + 2 + 2 * d) = make_float2(x, y);
       if (d == 0) *(float2 *)out = make_float2(m, l);
     }
@@ -1089,11 +1269,19 @@ SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_
 #define APPEND(K8, V8)                                                                                 \
   extern "C" __global__ __launch_bounds__(256) void kv_append__##K8##_##V8##_128(                      \
       const float *w, float *a, const uint32_t *ctl, f16 *kv, int8_t *kv8, AppendPush p) {              \
-    append_body<K8, V8, 1>(w, a, ctl, kv, kv8, p);                                                      \
+    append_body<K8, V8, 1, 0>(w, a, ctl, kv, kv8, p);                                                   \
   }                                                                                                    \
   extern "C" __global__ __launch_bounds__(256) void kv_append_4__##K8##_##V8##_128(                    \
       const float *w, float *a, const uint32_t *ctl, f16 *kv, int8_t *kv8, AppendPush p) {              \
-    append_body<K8, V8, 4>(w, a, ctl, kv, kv8, p);                                                      \
+    append_body<K8, V8, 4, 0>(w, a, ctl, kv, kv8, p);                                                   \
+  }                                                                                                    \
+  extern "C" __global__ __launch_bounds__(256) void kv_append_axes__##K8##_##V8##_128(                 \
+      const float *w, float *a, const uint32_t *ctl, f16 *kv, int8_t *kv8, AppendAxesPush p) {          \
+    append_body<K8, V8, 1, 1>(w, a, ctl, kv, kv8, p.append, p.axes_off, p.n_axes);                      \
+  }                                                                                                    \
+  extern "C" __global__ __launch_bounds__(256) void kv_append_axes_4__##K8##_##V8##_128(               \
+      const float *w, float *a, const uint32_t *ctl, f16 *kv, int8_t *kv8, AppendAxesPush p) {          \
+    append_body<K8, V8, 4, 1>(w, a, ctl, kv, kv8, p.append, p.axes_off, p.n_axes);                      \
   }
 APPEND(0, 0)
 APPEND(0, 1)
@@ -1104,6 +1292,13 @@ APPEND(1, 1)
   void attention_paged__##R##_##K8##_##V8##_128(float *a, const uint32_t *ctl, const f16 *kv,           \
                                                 const int8_t *kv8, const f16 *kvs, PagedPush p,         \
                                                 uint32_t n_grid) {                                      \
+    (void)kvs;                                                                                         \
+    paged_body<R, K8, V8>(a, ctl, kv, kv8, p, n_grid);                                                 \
+  }                                                                                                    \
+  extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))                  \
+  void attention_paged_shaped__##R##_##K8##_##V8##_128(float *a, const uint32_t *ctl, const f16 *kv,    \
+                                                       const int8_t *kv8, const f16 *kvs, ShapedPush p, \
+                                                       uint32_t n_grid) {                               \
     (void)kvs;                                                                                         \
     paged_body<R, K8, V8>(a, ctl, kv, kv8, p, n_grid);                                                 \
   }
@@ -1118,16 +1313,24 @@ PAGED_REP(1, 1)
 // and 17 partials 10 us (36 MB, 3.5 TB/s), one row's 32 heads of 64 partials 4.1 us with eight waves a
 // head; one row of 256 partials took 79 us with one wave and a load at a time.  Bound by the launch
 // and three round trips.
-template <uint32_t W>
-SK_DEV void paged_merge(float *a, const uint32_t *ctl, const PagedMergePush &p, uint32_t h, uint32_t row, uint32_t wave,
+template <uint32_t W, typename P>
+SK_DEV void paged_merge(float *a, const uint32_t *ctl, const P &p, uint32_t h, uint32_t row, uint32_t wave,
                         uint32_t lane) {
-  const uint32_t shared = shared_positions(ctl, p.n_shared, p.n_seq, p.table_stride, p.page_log2);
-  const Range r = row_range(ctl, p.rows_off, row, shared, p.n_seq, p.table_stride, p.page_log2);
-  const uint32_t ns = r.member ? live_parts(split_of(0, shared, p.n_shared)) : 0;
-  const uint32_t no = live_parts(split_of(r.start, r.len, p.n_own)), n = ns + no;
-  const float *part = a + p.part_off + (row * p.n_head + h) * (p.n_shared + p.n_own) * PART;
+  const uint32_t shared = shared_end(ctl, p);
+  const auto r = range_of(ctl, p, row, shared);
+  uint32_t first = 0, nl = 0;  // where the shared run starts, and a lead's partials
+  if constexpr (SHAPED<P>) {
+    first = shared_first(ctl, p, shared);
+    if (r.member && p.n_lead) nl = live_parts(split_of(r.lo, first, p.n_lead));
+  }
+  const uint32_t ns = r.member ? live_parts(split_of(first, shared, p.n_shared)) : 0;
+  const uint32_t no = live_parts(split_of(r.start, r.len, p.n_own)), n = ns + no + nl;
+  const float *part = a + p.part_off + (row * p.n_head + h) * slots_of(p) * PART;
   // live partial i
-  auto at = [&](uint32_t i) { return part + (i < ns ? i : p.n_shared + i - ns) * PART; };
+  auto at = [&](uint32_t i) {
+    if (SHAPED<P> && i >= ns + no) return part + (p.n_shared + p.n_own + i - ns - no) * PART;
+    return part + (i < ns ? i : p.n_shared + i - ns) * PART;
+  };
   float big = -INFINITY;
   for (uint32_t i = lane; i < n; i += 64) big = fmaxf(big, at(i)[0]);
   big = wave_max(big);
@@ -1174,6 +1377,17 @@ extern "C" __global__ __launch_bounds__(256) void attention_paged_merge__128(flo
 // eight waves a head
 extern "C" __global__ __launch_bounds__(512) void attention_paged_merge_8__128(float *a, const uint32_t *ctl,
                                                                                PagedMergePush p) {
+  const uint32_t h = blockIdx.x, row = blockIdx.y;
+  if (row < ctl[2]) paged_merge<8>(a, ctl, p, h, row, threadIdx.x >> 6, threadIdx.x & 63);
+}
+// and of attention_paged_shaped's partials
+extern "C" __global__ __launch_bounds__(256) void attention_paged_shaped_merge__128(float *a, const uint32_t *ctl,
+                                                                                    ShapedMergePush p) {
+  const uint32_t h = blockIdx.x * 4 + (threadIdx.x >> 6), row = blockIdx.y;
+  if (row < ctl[2] && h < p.n_head) paged_merge<1>(a, ctl, p, h, row, 0, threadIdx.x & 63);
+}
+extern "C" __global__ __launch_bounds__(512) void attention_paged_shaped_merge_8__128(float *a, const uint32_t *ctl,
+                                                                                      ShapedMergePush p) {
   const uint32_t h = blockIdx.x, row = blockIdx.y;
   if (row < ctl[2]) paged_merge<8>(a, ctl, p, h, row, threadIdx.x >> 6, threadIdx.x & 63);
 }

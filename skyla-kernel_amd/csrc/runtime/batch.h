@@ -12,13 +12,16 @@
 
 namespace batch {
 
-enum Op { kNone, kAppend, kAttend, kMerge, kLogits, kSample, kDraw };
+enum Op { kNone, kAppend, kAttend, kMerge, kLogits, kAppendAxes, kShaped, kShapedMerge, kSample, kDraw };
 
 inline Op op_of(const char *name) {
   if (std::strcmp(name, "kv_append") == 0) return kAppend;
   if (std::strcmp(name, "attention_paged") == 0) return kAttend;
   if (std::strcmp(name, "attention_paged_merge") == 0) return kMerge;
   if (std::strcmp(name, "logits_adjust") == 0) return kLogits;
+  if (std::strcmp(name, "kv_append_axes") == 0) return kAppendAxes;
+  if (std::strcmp(name, "attention_paged_shaped") == 0) return kShaped;
+  if (std::strcmp(name, "attention_paged_shaped_merge") == 0) return kShapedMerge;
   if (std::strcmp(name, "logits_sample") == 0) return kSample;
   if (std::strcmp(name, "logits_sample_draw") == 0) return kDraw;
   return kNone;
@@ -41,6 +44,7 @@ constexpr uint32_t kMergeParts = 16, kMergeHeads = 512;
 constexpr uint32_t kLogitsHistory = 8192;
 // Tokens of a logits_sample workgroup, words of its part, and the most tokens of a vocabulary (sample.hip).
 constexpr uint32_t kSampleChunk = 8192, kSamplePart = 5128, kSampleVocab = 1u << 20;
+constexpr float kMinCap = 0x1p-10f, kMaxCap = 0x1p14f;  // of scores (batch.hip, Cap: its powers stay in f32's range)
 constexpr uint32_t kMaxWork = 1u << 23;   // workgroups of an attention launch
 
 // A buffer bound to a dispatch: where it lies and how large it is.
@@ -134,14 +138,16 @@ inline std::string refusal(Op op, const uint32_t *spec, const uint32_t *w, const
   c.need(groups[0] == 1 && groups[2] == 1, "the grid is [1, rows, 1]");
   if (rows > kMaxGrid) c.fail("%llu rows: at most %u", (unsigned long long)rows, kMaxGrid);
   if (!c.error.empty() || rows == 0 || op == kNone) return c.error;
+  const bool append = op == kAppend || op == kAppendAxes;
   auto bound = [&](int i) {
     static const uint64_t place[2][5] = {{2, 0, 0, 1, 1}, {0, 0, 1, 1, 1}};
-    return Binding{at ? at[i] : place[op != kAppend][i] << 40, bytes[i]};
+    return Binding{at ? at[i] : place[!append][i] << 40, bytes[i]};
   };
-  const Binding A = bound(op == kAppend), C = bound(op == kAppend ? 2 : 1);  // arena, control words
-  const Region ctl{"the control words", C, 4, 0, 0, 5, 1};
+  const Binding A = bound(append), C = bound(append ? 2 : 1);  // arena, control words
+  const bool shaped = op == kShaped || op == kShapedMerge;
+  const Region ctl{"the control words", C, 4, 0, 0, shaped ? 6u : 5u, 1};
   c.holds(ctl, 1);
-  if (op == kAppend) {
+  if (append) {
     const uint64_t n_head = w[9], n_kv = w[10], kv_dim = n_kv * kHead;
     c.need(n_head >= 1 && n_head <= 1024 && n_kv >= 1 && n_kv <= 1024, "1 to 1024 heads");
     if (!c.error.empty()) return c.error;
@@ -151,26 +157,38 @@ inline std::string refusal(Op op, const uint32_t *spec, const uint32_t *w, const
     const Region words{"the rows' words", C, 4, w[18], 4, 4, rows},
         table{"the page table", C, 4, w[19], 0, (uint64_t)w[21] * w[20], 1};
     const Region qn{"q's norm weights", W, 4, w[4], 0, kHead, 1}, kn{"k's norm weights", W, 4, w[5], 0, kHead, 1},
-        rope{"the rotation's frequencies", W, 4, w[6], 0, kHead / 2, 1};
+        rope{"the rotation's frequencies", W, 4, w[6], 0, op == kAppendAxes ? (uint64_t)w[25] * (kHead / 2) : kHead / 2, 1};
+    const Region axes{"the rows' positions", C, 4, op == kAppendAxes ? w[24] : 0, 4, 4, op == kAppendAxes ? rows : 0};
+    if (op == kAppendAxes) c.need(w[25] >= 1 && w[25] <= 4, "1 to 4 axes");
     check_pages(c, words, table, w[23], w[22]);
     c.need(w[20] >= 1 && w[21] >= 1, "the page table is empty");
     if (!c.error.empty()) return c.error;
     for (const Region *r : {&q, &k, &v, &o}) c.holds(*r, 4);
     for (const Region *r : {&qn, &kn, &rope}) c.holds(*r, 1);
+    c.holds(axes, 4);
     std::vector<Region> written = check_pool(c, spec[0], spec[1], w + 14, (uint64_t)w[22] << w[23], kv_dim, bound(3), bound(4));
     if (!c.error.empty()) return c.error;
     for (const Region &r : written) c.apart(r, q);
     // in place, or apart: another wave may still read what this one writes
     if (!o.same(q)) c.apart(o, q);
     written.push_back(o);
-    c.writes(written, {k, v, qn, kn, rope, words, table, ctl});
-  } else if (op == kAttend) {
+    c.writes(written, {k, v, qn, kn, rope, axes, words, table, ctl});
+  } else if (op == kAttend || op == kShaped) {
     const uint64_t n_kv = w[9], kv_dim = n_kv * kHead, n_head = n_kv * spec[0];
-    const uint64_t parts = (uint64_t)w[11] + w[12];
+    const uint64_t lead = shaped ? w[23] : 0, parts = (uint64_t)w[11] + w[12] + lead;
     c.need(w[19] <= 1, "the shared run takes 16 query rows a workgroup (0) or 128 (1)");
     c.need(n_kv >= 1 && n_kv <= 1024, "1 to 1024 key heads");
     c.need(w[12] >= 1 && parts <= kMaxSlots, "a row's own positions take 1 part or more, all of them at most 1024");
+    if (shaped) {
+      float cap;
+      std::memcpy(&cap, w + 24, 4);
+      c.need(cap == 0.0f || (cap >= kMinCap && cap <= kMaxCap), "scores are capped (0: not) at 2^-10 to 2^14");
+    }
     if (!c.error.empty()) return c.error;
+    const Region spans{"the rows' spans", C, 4, shaped ? w[20] : 0, 2, 2, shaped ? rows : 0},
+        slopes{"the heads' slopes", C, 4, shaped ? w[21] : 0, 0, n_head, shaped && w[21] != ~0u ? 1u : 0u};
+    c.holds(spans, 2);
+    c.holds(slopes, 1);
     const Region q{"q", A, 4, w[0], w[1], n_head * kHead, rows}, o{"the output", A, 4, w[2], w[3], n_head * kHead, rows};
     const Region part{"the partials", A, 4, w[4], 0, rows * n_head * parts * kPart, 1};
     const Region words{"the rows' words", C, 4, w[13], 4, 4, rows},
@@ -184,14 +202,14 @@ inline std::string refusal(Op op, const uint32_t *spec, const uint32_t *w, const
     c.holds(part, 2);
     std::vector<Region> read = check_pool(c, spec[1], spec[2], w + 5, (uint64_t)w[17] << w[18], kv_dim, bound(2), bound(3));
     if (!c.error.empty()) return c.error;
-    read.insert(read.end(), {words, table, ctl});
+    read.insert(read.end(), {words, table, spans, slopes, ctl});
     if (!o.same(q)) c.apart(o, q);
     c.apart(part, q);
     c.writes({o, part}, read);
-    if (n_kv * ((rows * spec[0] + 15) / 16 * w[11] + rows * w[12]) > kMaxWork)
+    if (n_kv * ((rows * spec[0] + 15) / 16 * w[11] + rows * (w[12] + lead)) > kMaxWork)
       c.fail("%llu rows in %llu parts: too many workgroups", (unsigned long long)rows, (unsigned long long)parts);
-  } else if (op == kMerge) {
-    const uint64_t n_head = w[3], parts = (uint64_t)w[4] + w[5];
+  } else if (op == kMerge || op == kShapedMerge) {
+    const uint64_t n_head = w[3], parts = (uint64_t)w[4] + w[5] + (shaped ? w[12] : 0);
     c.need(n_head >= 1 && n_head <= 8192, "1 to 8192 heads");
     c.need(w[5] >= 1 && parts <= kMaxSlots, "a row's own positions take 1 part or more, all of them at most 1024");
     c.need(parts > 1, "one part in all is the attention's result already");
@@ -202,7 +220,9 @@ inline std::string refusal(Op op, const uint32_t *spec, const uint32_t *w, const
     c.holds(part, 2);
     c.holds(o, 2);
     c.holds(words, 4);
-    c.writes({o}, {part, words, ctl});
+    const Region spans{"the rows' spans", C, 4, shaped ? w[10] : 0, 2, 2, shaped ? rows : 0};
+    c.holds(spans, 2);
+    c.writes({o}, {part, words, spans, ctl});
   } else if (op == kLogits) {
     const uint64_t v = w[4];
     c.need(v >= 1, "an empty vocabulary");
@@ -248,25 +268,27 @@ inline std::string other_form(Op op, const std::string &symbol) {
   if (op == kLogits) return "logits_adjust_1024";
   if (op == kMerge) return "attention_paged_merge_8__128";
   if (op == kAppend) return "kv_append_4" + symbol.substr(std::strlen("kv_append"));
+  if (op == kAppendAxes) return "kv_append_axes_4" + symbol.substr(std::strlen("kv_append_axes"));
+  if (op == kShapedMerge) return "attention_paged_shaped_merge_8__128";
   return symbol;
 }
 inline Shape shape(Op op, const uint32_t *spec, const uint32_t *w, uint32_t rows) {
   Shape s;
   s.groups[1] = rows;
-  if (op == kAppend) {
+  if (op == kAppend || op == kAppendAxes) {
     const uint32_t heads = (w[9] + 2 * w[10] + 15) / 16;  // 16 heads a pass
     s.form = (uint64_t)rows * heads >= kAppendMany;
     s.groups[0] = s.form ? (heads + 3) / 4 : heads;
-  } else if (op == kAttend) {
-    const uint32_t q = rows * spec[0], groups = w[9] * w[11], own = rows * w[9] * w[12];
+  } else if (op == kAttend || op == kShaped) {
+    const uint32_t q = rows * spec[0], groups = w[9] * w[11], own = rows * w[9] * (w[12] + (op == kShaped ? w[23] : 0));
     if (w[19] && w[11])
       s.groups[0] = (groups + 7) / 8 * 8 * ((q + 127) / 128) + own;
     else
       s.groups[0] = groups * ((q + 15) / 16) + own;
     s.groups[1] = 1;
     s.extra = {rows};
-  } else if (op == kMerge) {
-    s.form = w[4] + w[5] > kMergeParts && rows * w[3] <= kMergeHeads;
+  } else if (op == kMerge || op == kShapedMerge) {
+    s.form = w[4] + w[5] + (op == kShapedMerge ? w[12] : 0) > kMergeParts && rows * w[3] <= kMergeHeads;
     s.groups[0] = s.form ? w[3] : (w[3] + 3) / 4;
     s.threads = s.form ? 512 : 256;
   } else if (op == kSample) {

@@ -4,9 +4,11 @@ The reference's engine serves one sequence over a contiguous cache (kv.rs); this
 what a server of many needs beside it, over the same weights, arena rows and C-ABI:
 
   Paged           a pool of pages in the contiguous cache's row layout, and its page table
-  BatchKernels    kv_append (QK-norm, rotation, keys and values into their pages) and
-                  attention_paged (attention of rows over their pages, a leading run of positions
-                  that many rows share read once for all of them)
+  BatchKernels    kv_append (QK-norm, rotation, keys and values into their pages), kv_append_axes
+                  (the rotation by positions of several axes), attention_paged (attention of rows
+                  over their pages, a leading run of positions that many rows share read once for
+                  all of them) and attention_paged_shaped (scores capped by a tanh or biased by
+                  distance, windows, rows that see from a document's start or to a prefix's end)
   LogitsKernels   logits_adjust (penalties for repeated tokens, biases, grammar masks) and
                   logits_sample (a token of each row by temperature, top-k, min-p and top-p)
   BatchEngine     sequences of one model: open, fork, prefill, step, close
@@ -27,7 +29,8 @@ from .abi import Buffer, Context, Recorder
 
 MAX_PARTS = 1024        # partials of a row and head (runtime/batch.h)
 PAGE_SIZES = tuple(16 << i for i in range(9))  # 16 to 4096 positions
-CTL_ROWS, CTL_SHARED, CTL_LEADER = 2, 3, 4     # control words: live rows, shared positions, their sequence
+# control words: live rows, shared positions, their sequence, the first of them (attention_paged_shaped)
+CTL_ROWS, CTL_SHARED, CTL_LEADER, CTL_FIRST = 2, 3, 4, 5
 
 
 class Paged:
@@ -54,10 +57,24 @@ class Paged:
 
 @dataclasses.dataclass
 class BatchRegions:
-    """Arena offsets of a batch: the rows' words, the page table, the attention's partials."""
+    """Arena offsets of a batch: the rows' words, the page table, the attention's partials; of
+    kv_append_axes four positions a row, of attention_paged_shaped two words a row, the first position
+    that it attends to and the end of a prefix that it sees past its own (0: none)."""
     rows: int
     table: int
     part: int = 0
+    axes: int = 0
+    spans: int = 0
+
+
+@dataclasses.dataclass
+class Shape:
+    """What attention_paged_shaped does to scores: a cap (cap tanh(s / cap); 0: none), a window (a row
+    attends to so many positions, its own the last; 0: all) and the arena offset of the heads' slopes (a
+    score at a distance d loses slope d; None: none do)."""
+    cap: float = 0.0
+    window: int = 0
+    slopes: int | None = None
 
 
 @dataclasses.dataclass
@@ -129,6 +146,27 @@ def part_size(rows: int, n_head: int, parts) -> int:
     return rows * n_head * (parts[0] + parts[1]) * 130
 
 
+class ShapedParts(NamedTuple):
+    """Parts, and the pieces of a row's positions before the shared run (its lead; 0: none has any)."""
+    shared: int
+    own: int
+    wide: bool = False
+    lead: int = 0
+
+
+def shaped_splits(rows: int, n_kv: int, rep: int, shared: int, own: int, lead: int = 0) -> ShapedParts:
+    """Parts for a shared run of `shared` positions, at most `own` of a row's own and `lead` of those
+    before the run."""
+    parts = splits(rows, n_kv, rep, shared, own)
+    n_lead = max(1, min(-(-512 // (n_kv * rows)), -(-lead // 256), 128)) if lead and shared else 0
+    return ShapedParts(*parts, n_lead)
+
+
+def shaped_part_size(rows: int, n_head: int, parts) -> int:
+    """Words of attention_paged_shaped's partials."""
+    return rows * n_head * (parts[0] + parts[1] + parts[3]) * 130
+
+
 SAMPLE_CHUNK, SAMPLE_PART, SAMPLE_VOCAB = 8192, 5128, 1 << 20  # (runtime/batch.h)
 
 
@@ -150,15 +188,19 @@ class BatchKernels:
         k8, v8 = int(paged.precision.keys_q8), int(paged.precision.values_q8)
 
         def build(name, bufs, push, spec):
-            p = ctx.create_pipeline_sets(name, len(bufs) + 2 if name == "kv_append" else 5, 4 * push, spec, len(pools))
+            p = ctx.create_pipeline_sets(name, 5, 4 * push, spec, len(pools))
             for i, kv in enumerate(pools):
-                p.bind_set_buffers(i, bufs + [kv, kv] + ([] if name == "kv_append" else [kv]))
+                p.bind_set_buffers(i, (bufs + [kv, kv, kv])[:5])
             return p
 
         self._append = build("kv_append", [tables, a, a], 24, [k8, v8, 128])
         self._attend = build("attention_paged", [a, a], 20, [c.n_head // c.n_head_kv, k8, v8, 128])
+        self._append_axes = build("kv_append_axes", [tables, a, a], 26, [k8, v8, 128])
+        self._shaped = build("attention_paged_shaped", [a, a], 25, [c.n_head // c.n_head_kv, k8, v8, 128])
         self._merge = ctx.create_pipeline("attention_paged_merge", 2, 40, [128])
         self._merge.bind_buffers([a, a])
+        self._shaped_merge = ctx.create_pipeline("attention_paged_shaped_merge", 2, 52, [128])
+        self._shaped_merge.bind_buffers([a, a])
 
     @staticmethod
     def check(c: E.Config) -> None:
@@ -173,29 +215,56 @@ class BatchKernels:
                rope: int, rows: int, mscale: float = 1.0) -> None:
         """Rows of raw q, k, v ((offset, stride); v has k's stride): q and k normed and rotated, q
         into out, k and v into layer's pool at each row's position."""
+        r.dispatch_set(self._append, layer, [1, rows, 1], self._append_push(at, q, k, v, out, q_norm, k_norm, rope, mscale))
+
+    def append_axes(self, r: Recorder, layer: int, at: BatchRegions, q, k, v: int, out, q_norm: int, k_norm: int,
+                    rope: int, n_axes: int, rows: int, mscale: float = 1.0) -> None:
+        """append, with each row turned by its `n_axes` (1 to 4) positions at at.axes: rope holds 64
+        frequencies for each axis (those of a pair's other axes 0)."""
+        push = self._append_push(at, q, k, v, out, q_norm, k_norm, rope, mscale)
+        r.dispatch_set(self._append_axes, layer, [1, rows, 1], push + [at.axes, n_axes])
+
+    def _append_push(self, at, q, k, v, out, q_norm, k_norm, rope, mscale) -> list[int]:
         c, kv = self.c, self.paged.layout
-        push = [q[0], k[0], v, out[0], q_norm, k_norm, rope, E.f32_bits(c.eps), E.f32_bits(mscale), c.n_head,
+        return [q[0], k[0], v, out[0], q_norm, k_norm, rope, E.f32_bits(c.eps), E.f32_bits(mscale), c.n_head,
                 c.n_head_kv, q[1], k[1], out[1], kv.keys(0), kv.values(0), kv.key_scales(0), kv.value_scales(0),
                 at.rows, at.table, *self._pages()]
-        r.dispatch_set(self._append, layer, [1, rows, 1], push)
 
     def attend(self, r: Recorder, layer: int, at: BatchRegions, q, out, rows: int, parts) -> None:
         """Attention of rows of rotated q ((offset, stride)) over layer's pool into out, in `parts`
         (splits); at.part holds part_size words."""
-        c, kv, parts = self.c, self.paged.layout, Parts(*parts)
-        scale = np.float32(1.0) / np.sqrt(np.float32(c.head_dim))
-        push = [q[0], q[1], out[0], out[1], at.part, kv.keys(0), kv.values(0), kv.key_scales(0), kv.value_scales(0),
-                c.n_head_kv, E.f32_bits(scale), parts.shared, parts.own, at.rows, at.table, *self._pages(), parts.wide]
-        r.dispatch_set(self._attend, layer, [1, rows, 1], push)
+        parts = Parts(*parts)
+        r.dispatch_set(self._attend, layer, [1, rows, 1], self._attend_push(at, q, out, parts))
         if parts.shared + parts.own == 1:  # nothing to merge: the rows are the result
             return
         r.barrier()
-        push = [at.part, out[0], out[1], c.n_head, parts.shared, parts.own, at.rows, self.paged.seq_pages,
+        r.dispatch(self._merge, [1, rows, 1], self._merge_push(at, out, parts))
+
+    def attend_shaped(self, r: Recorder, layer: int, at: BatchRegions, q, out, rows: int, parts, shape: Shape) -> None:
+        """attend, each row over the positions that at.spans and the window leave it, with scores as
+        `shape` has them, in `parts` (shaped_splits); at.part holds shaped_part_size words."""
+        parts = ShapedParts(*parts)
+        push = self._attend_push(at, q, out, parts)
+        push += [at.spans, 0xFFFFFFFF if shape.slopes is None else shape.slopes, shape.window, parts.lead, E.f32_bits(shape.cap)]
+        r.dispatch_set(self._shaped, layer, [1, rows, 1], push)
+        if parts.shared + parts.own + parts.lead == 1:
+            return
+        r.barrier()
+        push = self._merge_push(at, out, parts) + [at.spans, shape.window, parts.lead]
+        r.dispatch(self._shaped_merge, [1, rows, 1], push)
+
+    def _attend_push(self, at, q, out, parts) -> list[int]:
+        c, kv = self.c, self.paged.layout
+        scale = np.float32(1.0) / np.sqrt(np.float32(c.head_dim))
+        return [q[0], q[1], out[0], out[1], at.part, kv.keys(0), kv.values(0), kv.key_scales(0), kv.value_scales(0),
+                c.n_head_kv, E.f32_bits(scale), parts.shared, parts.own, at.rows, at.table, *self._pages(), parts.wide]
+
+    def _merge_push(self, at, out, parts) -> list[int]:
+        return [at.part, out[0], out[1], self.c.n_head, parts.shared, parts.own, at.rows, self.paged.seq_pages,
                 self.paged.n_seq, self.paged.page_log2]
-        r.dispatch(self._merge, [1, rows, 1], push)
 
     def free(self) -> None:
-        for p in (self._append, self._attend, self._merge):
+        for p in (self._append, self._append_axes, self._attend, self._shaped, self._merge, self._shaped_merge):
             p.free()
 
 
