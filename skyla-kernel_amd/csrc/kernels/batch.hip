@@ -7,7 +7,7 @@
 //   attention_paged        [A, C, KV, KV8, KVS] 20 words  spec [N_REP, K_Q8, V_Q8, head_dim]
 //   attention_paged_merge  [A, C]               10 words  spec [head_dim]
 //   attention_paged_shaped       [A, C, KV, KV8, KVS] 25 words  spec [N_REP, K_Q8, V_Q8, head_dim]
-//   attention_paged_shaped_merge [A, C]         13 words  spec [head_dim]
+//   attention_paged_shaped_merge [A, C]         14 words  spec [head_dim]
 //   logits_adjust          [A, C]               12 words
 // Bindings as in attention.hip.  Heads are 128 wide.
 //
@@ -60,11 +60,14 @@ struct ShapedPush : PagedPush {
   uint32_t spans_off, slopes_off, window, n_lead;
   float cap;
 };
+struct CappedPush : ShapedPush {};  // of the kernels for a cap above 0
 struct ShapedMergePush : PagedMergePush {
-  uint32_t spans_off, window, n_lead;
+  uint32_t spans_off, window, n_lead, rep;
 };
 template <typename P>
 constexpr bool SHAPED = std::is_base_of<ShapedPush, P>::value || std::is_base_of<ShapedMergePush, P>::value;
+template <typename P>
+constexpr bool CAPPED = std::is_base_of<CappedPush, P>::value;
 struct LogitsPush {
   uint32_t x_off, y_off, x_stride, y_stride, n_vocab, ctrl_off, hist_off, hist_stride, bias_off, bias_stride, mask_off,
       mask_stride;
@@ -142,6 +145,58 @@ SK_DEV ShapedRange shaped_range(const uint32_t *ctl, const P &p, uint32_t row, u
   r.member = r.member && (p.n_lead ? r.lo <= first : r.lo == first);
   r.start = r.member ? shared : r.lo;
   return r;
+}
+// Whether the T rows from row / T * T on go together: those with a token are of one sequence and at most 256
+// positions apart, as a prompt's are.  Their own runs (tails, and leads) are then one, cut into parts as one, with each
+// row's mask.  (The words through the scalar cache: nothing writes them while the kernel runs.)
+typedef const __attribute__((address_space(4))) uint32_t ConstWord;
+template <uint32_t T>
+SK_DEV bool rows_together(const uint32_t *ctl, uint32_t rows_off, uint32_t row, uint32_t n_rows) {
+  if constexpr (T == 1) return false;
+  ConstWord *w = (ConstWord *)(uintptr_t)(ctl + rows_off);
+  uint32_t seq = ~0u, least = ~0u, most = 0;
+  bool one = true;
+#pragma unroll
+  for (uint32_t i = 0; i < T; i++) {
+    const uint32_t r = min(row / T * T + i, n_rows - 1), of = w[4 * r], len = w[4 * r + 1];
+    if (len == 0) continue;
+    one = one && (seq == ~0u || of == seq);
+    seq = of, least = min(least, len), most = max(most, len);
+  }
+  return one && most != 0 && most - least <= 256;
+}
+SK_DEV bool rows_together(const uint32_t *ctl, uint32_t rows_off, uint32_t row, uint32_t n_rows, uint32_t T) {
+  return T == 16  ? rows_together<16>(ctl, rows_off, row, n_rows)
+         : T == 8 ? rows_together<8>(ctl, rows_off, row, n_rows)
+         : T == 4 ? rows_together<4>(ctl, rows_off, row, n_rows)
+                  : rows_together<2>(ctl, rows_off, row, n_rows);
+}
+// The positions of row row's own run, its tail or its lead, and of the run that it is part of.  (Whole waves: lane l
+// looks at row l % T of the rows that may go together.)
+struct OwnRun {
+  uint32_t lo, hi, all_lo, all_hi;  // the row's, and the run's; [0, 0): nothing
+  uint32_t seq, lane_lo, lane_hi;   // row l % T's, in lane l
+};
+template <typename P>
+SK_DEV OwnRun own_run(const uint32_t *ctl, const P &p, uint32_t row, uint32_t n_rows, uint32_t T, bool together, uint32_t shared, bool lead) {
+  const uint32_t lane = threadIdx.x & 63, row0 = row / T * T, mine = row0 + (lane & (T - 1));
+  uint32_t lo = 0, hi = 0, seq = 0;
+  if (mine < n_rows) {
+    const ShapedRange r = shaped_range(ctl, p, mine, shared);
+    lo = lead ? r.lo : r.start, hi = lead ? shared_first(ctl, p, shared) : r.len, seq = r.seq;
+    if (lo >= hi || (lead && !r.member)) lo = hi = 0;
+  }
+  OwnRun x;
+  x.lane_lo = lo, x.lane_hi = hi;
+  x.lo = __shfl(lo, row - row0, 64), x.hi = __shfl(hi, row - row0, 64), x.seq = __shfl(seq, row - row0, 64);
+  uint32_t from = hi ? lo : ~0u, to = hi, of = hi ? seq : 0;
+  for (uint32_t d = T / 2; d >= 1; d >>= 1) {
+    from = min(from, (uint32_t)__shfl_xor(from, d, 64)), to = max(to, (uint32_t)__shfl_xor(to, d, 64));
+    of = max(of, (uint32_t)__shfl_xor(of, d, 64));
+  }
+  if (together) x.seq = of;
+  x.all_lo = !together ? x.lo : to ? from : 0, x.all_hi = together ? to : x.hi;
+  return x;
 }
 // a row's range, whichever kernel's
 template <typename P>
@@ -315,10 +370,10 @@ SK_DEV void append_body(const float *w, float *a, const uint32_t *ctl, f16 *kv, 
 constexpr float LOOSE = 8.0f;
 constexpr int E_SHIFT = 7;
 SK_DEV int query_shift(float big) { return big > 0.0f && big < INFINITY ? 11 - __builtin_amdgcn_frexp_expf(big) : 0; }
-// scores a and b as weights: x + y into l, the parts at elements e and e + 1
-SK_DEV void weigh(float a, float b, float inv, float c, float &l, f16x8 &ph, f16x8 &pl, int e) {
-  const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(a, inv, c));
-  const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(b, inv, c));
+// scores a and b, in units of ua and ub, as weights: x + y into l, the parts at elements e and e + 1
+SK_DEV void weigh(float a, float b, float ua, float ub, float c, float &l, f16x8 &ph, f16x8 &pl, int e) {
+  const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(a, ua, c));
+  const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(b, ub, c));
   l += x;
   l += y;
   uint32_t both = as_u32(pack_f16x2(x, y));
@@ -348,9 +403,9 @@ SK_DEV f16x8 widen8(uint2 x) {
   return __builtin_bit_cast(f16x8, make_uint4(as_u32(widen(x.x, x.x, 0x0c010c00u)), as_u32(widen(x.x, x.x, 0x0c030c02u)),
                                               as_u32(widen(x.y, x.y, 0x0c010c00u)), as_u32(widen(x.y, x.y, 0x0c030c02u))));
 }
-// Scores in powers of two to what they are capped and biased to.  c tanh(s / c) = s P((s / c)^2), P the polynomial
-// of degree 4 nearest to tanh(x) / x for |x| <= 1/2 (1.3e-8 of it at most); where a wave has a larger score,
-// c (1 - e) / (1 + e), e = exp(-2 |s| / c), for those (within 4e-7).
+// Scores in powers of two to what they are capped at: c tanh(s / c) = s P((s / c)^2), P the polynomial of degree 4
+// nearest to tanh(x) / x for |x| <= 1/2 (1.3e-8 of it at most); where a wave has a larger score, c (1 - e) / (1 + e),
+// e = exp(-2 |s| / c), for those (within 4e-7).
 struct Cap {
   float c, inv, edge, p[5];
 };
@@ -359,7 +414,7 @@ SK_DEV float to_scalar(float v) {
 }
 SK_DEV Cap cap_of(float cap) {
   const float c = cap * 1.44269504088896340736f, inv = 1.0f / c, k = inv * inv;
-  Cap x{c, inv, 0.5f * c, {0.99999999f, -0.33333069f * k, 0.13324779f * k * k, -0.05298608f * k * k * k, 0.01713501f * k * k * k * k}};
+  Cap x{c, inv, 0.5f * c, {0.9999999869f, -0.3333306939f * k, 0.1332477932f * k * k, -0.0529860752f * k * k * k, 0.0171350065f * k * k * k * k}};
   x.c = to_scalar(x.c), x.inv = to_scalar(x.inv), x.edge = to_scalar(x.edge);
 #pragma unroll
   for (int i = 0; i < 5; i++) x.p[i] = to_scalar(x.p[i]);
@@ -389,7 +444,6 @@ SK_DEV void cap_scores(S &s, const Cap &x) {
 
 // The page table through the scalar cache: nothing writes it while the kernel runs, and a vector
 // load's wait would be one for the cache rows in flight, too.
-typedef const __attribute__((address_space(4))) uint32_t ConstWord;
 struct Pages {
   ConstWord *table;
   uint32_t n_pages, log2;
@@ -433,7 +487,7 @@ struct HalfRows {
 template <int K8, int V8, typename P>
 SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t *kv8, const P &p, uint32_t kvh,
                      const float *q, float (*out)[PART], uint32_t seq, uint32_t lo, uint32_t hi, uint32_t begin,
-                     uint32_t end, float slope = 0.0f, uint32_t row_at = 0) {
+                     uint32_t end, float slope = 0.0f, uint32_t row_at = 0, uint32_t my_lo = 0, uint32_t my_hi = 0) {
   const uint32_t lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, kv_dim = p.n_kv * HD;
   // wave-uniform, and known to be
   lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
@@ -521,8 +575,13 @@ SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
       }
   }
   [[maybe_unused]] Cap cap;
+  [[maybe_unused]] uint32_t all_lo = 0, all_hi = 0;  // what every row sees
+  if constexpr (CAPPED<P>) cap = cap_of(p.cap);
   if constexpr (SHAPED<P>) {
-    if (p.cap > 0.0f) cap = cap_of(p.cap);
+    all_lo = my_lo, all_hi = my_hi;
+#pragma unroll
+    for (int d = 8; d >= 1; d >>= 1) all_lo = max(all_lo, (uint32_t)__shfl_xor(all_lo, d, 64)), all_hi = min(all_hi, (uint32_t)__shfl_xor(all_hi, d, 64));
+    all_lo = __builtin_amdgcn_readfirstlane(all_lo), all_hi = __builtin_amdgcn_readfirstlane(all_hi);
   }
   const float unit = SHAPED<P> ? 1.0f : inv;  // of the scores as they are weighed
   float m = -INFINITY, l;
@@ -534,7 +593,7 @@ SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
     else
       return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w;
   };
-  auto compute = [&](const HalfRows<K8, V8> &r, uint32_t at) {
+  auto compute = [&](HalfRows<K8, V8> &r, uint32_t at) {
     float sc[2][4];
 #pragma unroll
     for (uint32_t t = 0; t < 2; t++) {
@@ -561,20 +620,40 @@ SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
       float s[8];
 #pragma unroll
       for (uint32_t i = 0; i < 8; i++) s[i] = sc[i >> 2][i & 3] * inv;
-      if (p.cap > 0.0f) cap_scores<8>(s, cap);
+      if constexpr (CAPPED<P>) cap_scores<8>(s, cap);
       const int away = (int)(at + 4 * g - row_at);
 #pragma unroll
       for (uint32_t i = 0; i < 8; i++)
         sc[i >> 2][i & 3] = __builtin_fmaf(-slope, fabsf((float)(away + (int)(16 * (i >> 2) + (i & 3)))), s[i]);
     }
-    if (at < lo || at + HALF > hi) {
+    if (SHAPED<P> ? at < all_lo || at + HALF > all_hi : at < lo || at + HALF > hi) {
 #pragma unroll
       for (uint32_t t = 0; t < 2; t++)
 #pragma unroll
         for (uint32_t i = 0; i < 4; i++) {
           const uint32_t pos = at + 16 * t + 4 * g + i;
-          if (pos < lo || pos >= hi) sc[t][i] = -INFINITY;
+          if (SHAPED<P> ? pos < my_lo || pos >= my_hi : pos < lo || pos >= hi) sc[t][i] = -INFINITY;
         }
+      if constexpr (SHAPED<P>) {
+        // A weight of 0 would not keep a value that is not finite out of a row that does not see it: such a value is
+        // taken for 0, and of the rows that see it the weight for NaN.
+#pragma unroll
+        for (uint32_t e = 0; e < 8; e++) {
+          bool odd;
+          if constexpr (V8) {
+            odd = !(__builtin_fabsf16(r.vs[e]) < (f16)INFINITY);
+            if (odd) r.vs[e] = (f16)0.0f;
+          } else {
+            uint32_t any = 0;
+#pragma unroll
+            for (int k = 0; k < 4; k++) any |= (word(r.v[e], k) & 0x7c007c00u) + 0x04000400u;
+            odd = any & 0x80008000u;
+            if (odd) r.v[e] = make_uint4(0, 0, 0, 0);
+          }
+          const uint64_t which = __ballot(odd);
+          if (which && (which >> (16 * g) & 0xffff) && sc[e >> 2][e & 3] > -INFINITY) sc[e >> 2][e & 3] = NAN;
+        }
+      }
     }
     float mt = max3(sc[0][0], sc[0][1], sc[0][2]);
     mt = max3(mt, sc[0][3], sc[1][0]);
@@ -615,7 +694,7 @@ SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
     const float cm = (float)E_SHIFT - (m > -INFINITY ? m : 0.0f);
     f16x8 ph, pl;
 #pragma unroll
-    for (int n = 0; n < 4; n++) weigh(sc[n >> 1][2 * (n & 1)], sc[n >> 1][2 * (n & 1) + 1], unit, cm, l, ph, pl, 2 * n);
+    for (int n = 0; n < 4; n++) weigh(sc[n >> 1][2 * (n & 1)], sc[n >> 1][2 * (n & 1) + 1], unit, unit, cm, l, ph, pl, 2 * n);
     f16x2 sv[V8 ? 4 : 1];
     if constexpr (V8) {
       const int up = 4 - ve + WINDOW<9> * window;
@@ -827,7 +906,7 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
   [[maybe_unused]] float slope = 0.0f;
   [[maybe_unused]] uint32_t row_at = 0;
   if constexpr (SHAPED<P>) {
-    if (p.cap > 0.0f) cap = cap_of(p.cap);
+    if constexpr (CAPPED<P>) cap = cap_of(p.cap);
     if (p.slopes_off != ~0u) slope = __builtin_bit_cast(float, ctl[p.slopes_off + kvh * rep + head]) * 1.44269504088896340736f;
     row_at = range_of(ctl, p, row, shared).at;
   }
@@ -997,7 +1076,13 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
 
   f32x16 o[4];
   float m = -INFINITY, l;
-  const float unit = SHAPED<P> ? 1.0f : inv;  // of the scores as they are weighed
+  // What the scores are weighed in: as they are times `unit`, or, capped, times c P(x^2) of x = s / c, P the polynomial
+  // of degree 3 nearest to tanh(x) / x for |x| <= 0.35 (3.5e-8 of it at most; the largest of a step's scores is past that
+  // in few steps: those, like biased ones, are capped before)
+  float unit = inv;
+  if constexpr (SHAPED<P>) unit = p.slopes_off != ~0u ? 1.0f : inv;
+  [[maybe_unused]] float over = 0.0f;
+  if constexpr (CAPPED<P>) over = inv * cap.inv;
   const uint32_t n_steps = (end - begin + STEP - 1) / STEP;
   Rows vat, kat;
   // `sc`: this step's scores; into `next` the next step's
@@ -1016,26 +1101,62 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
     } else {
       sc = scores(step);
     }
-    if constexpr (SHAPED<P>) {
+    [[maybe_unused]] float p0 = 1.0f, p1 = 0.0f, p2 = 0.0f, p3 = 0.0f;
+    [[maybe_unused]] auto lifted = [&](float x) {
+      const float u = x * x;
+      float y = __builtin_fmaf(p3, u, p2);
+      y = __builtin_fmaf(y, u, p1);
+      return __builtin_fmaf(y, u, p0);
+    };
+    const bool tail = at + STEP > end;  // the run's last positions
+    [[maybe_unused]] auto bias = [&] {  // (every position is below the row's)
+      const float away = (float)(int)(at + 4 * h - row_at) * slope;
 #pragma unroll
-      for (uint32_t r = 0; r < 16; r++) sc[r] *= inv;
-      if (p.cap > 0.0f) cap_scores<16>(sc, cap);
-      if (p.slopes_off != ~0u) {  // (every position is below the row's)
-        const float away = (float)(int)(at + 4 * h - row_at) * slope;
+      for (uint32_t r = 0; r < 16; r++) sc[r] += __builtin_fmaf(slope, (float)(8 * (r >> 2) + (r & 3)), away);
+    };
+    if constexpr (CAPPED<P>) {
+      float big = 0.0f;
 #pragma unroll
-        for (uint32_t r = 0; r < 16; r++) sc[r] += __builtin_fmaf(slope, (float)(8 * (r >> 2) + (r & 3)), away);
+      for (uint32_t r = 0; r < 16; r++) sc[r] *= over;
+#pragma unroll
+      for (uint32_t r = 0; r < 16; r += 2) big = max3(big, fabsf(sc[r]), fabsf(sc[r + 1]));
+      if (p.slopes_off == ~0u && !tail && !__any(!(big <= 0.35f))) {
+        p0 = 0.9999999653f * cap.c, p1 = -0.3333242243f * cap.c, p2 = 0.1329579931f * cap.c, p3 = -0.0489582307f * cap.c;
+      } else {
+#pragma unroll
+        for (uint32_t r = 0; r < 16; r++) sc[r] *= cap.c;
+        cap_scores<16>(sc, cap);
+        if (p.slopes_off != ~0u) bias();
+        if (tail) {  // (not infinite: it is squared)
+#pragma unroll
+          for (uint32_t r = 0; r < 16; r++)
+            if (at + 8 * (r >> 2) + 4 * h + (r & 3) >= end) sc[r] = -0x1p50f;
+        }
       }
-    }
-    if (at + STEP > end) {  // the run's last positions
+    } else {
+      if constexpr (SHAPED<P>) {
+        if (p.slopes_off != ~0u) {
 #pragma unroll
-      for (uint32_t r = 0; r < 16; r++)
-        if (at + 8 * (r >> 2) + 4 * h + (r & 3) >= end) sc[r] = -INFINITY;
+          for (uint32_t r = 0; r < 16; r++) sc[r] *= inv;
+          bias();
+        }
+      }
+      if (tail) {
+#pragma unroll
+        for (uint32_t r = 0; r < 16; r++)
+          if (at + 8 * (r >> 2) + 4 * h + (r & 3) >= end) sc[r] = -INFINITY;
+      }
     }
     float mt = max3(sc[0], sc[1], sc[2]);
 #pragma unroll
     for (int r = 3; r < 15; r += 2) mt = max3(mt, sc[r], sc[r + 1]);
     mt = fmaxf(mt, sc[15]);
-    mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * unit;
+    mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+    if constexpr (CAPPED<P>) {
+      mt *= lifted(mt);
+    } else {
+      mt *= unit;
+    }
     if (__any(mt > m + LOOSE)) {  // rare after the first steps
       const float mn = mt > m + LOOSE ? mt : m;
       const float down = mn > -INFINITY ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
@@ -1046,7 +1167,13 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
     }
     const float c = (float)E_SHIFT - (m > -INFINITY ? m : 0.0f);
     f16x8 ph[2], pl[2];
-    auto weigh2 = [&](uint32_t n) { weigh(sc[2 * n], sc[2 * n + 1], unit, c, l, ph[n >> 2], pl[n >> 2], 2 * (n & 3)); };
+    auto weigh2 = [&](uint32_t n) {
+      const float x = sc[2 * n], y = sc[2 * n + 1];
+      if constexpr (CAPPED<P>)
+        weigh(x, y, lifted(x), lifted(y), c, l, ph[n >> 2], pl[n >> 2], 2 * (n & 3));
+      else
+        weigh(x, y, unit, unit, c, l, ph[n >> 2], pl[n >> 2], 2 * (n & 3));
+    };
     f16x8 vf[V8 ? 2 : 1][3];
     auto read_values = [&](uint32_t n) {  // of product n: k-step n / 4, dims 32 (n % 4) + [0, 32)
       vf[0][n % 3] = value(step, 0, n >> 2, n & 3);
@@ -1172,7 +1299,8 @@ SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_
   const bool own = w >= n_first;
   uint32_t i0;  // query rows i0 + [0, n_live) of the key head: row i / N_REP, head i % N_REP
   Split sp;
-  [[maybe_unused]] uint32_t slot = 0;  // of an own run's partial
+  [[maybe_unused]] uint32_t slot = 0, tile0 = 0, n_own_rows = N_REP;  // of an own run's partial; of the rows that may go together
+  [[maybe_unused]] OwnRun run;
   if (!own) {
     if (shared == 0) return;
     if (wide) {
@@ -1189,24 +1317,32 @@ SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_
     w -= n_first;
     const uint32_t n_own = slots - p.n_shared;
     kvh = w % p.n_kv, part = w / p.n_kv % n_own;
-    const uint32_t row = w / (p.n_kv * n_own);
-    if (row >= n_rows) return;
-    const auto r = range_of(ctl, p, row, shared);
-    i0 = row * N_REP, lo = r.start, hi = r.len, seq = r.seq;
+    uint32_t row = w / (p.n_kv * n_own);
     if constexpr (SHAPED<P>) {
+      // (the first rows of every T come first: the others of those that go together end at once, and would else hold
+      // places up)
+      constexpr uint32_t T = 16 / N_REP;
+      const uint32_t tiles = (n_grid + T - 1) / T;
+      row = w / (p.n_kv * n_own);
+      row = row % tiles * T + row / tiles;
+      if (row >= n_rows) return;
+      const bool together = rows_together<T>(ctl, p.rows_off, row, n_rows), lead = part >= p.n_own;
+      tile0 = row / T * T;
+      if (together && row != tile0) return;
+      run = own_run(ctl, p, row, n_rows, T, together, shared, lead);
       slot = p.n_shared + part;
-      if (part >= p.n_own) {  // of the lead
-        if (!r.member) return;
-        part -= p.n_own, lo = r.lo, hi = shared_first(ctl, p, shared);
-        sp = split_of(lo, hi, p.n_lead);
-      } else {
-        sp = split_of(lo, hi, p.n_own);
-      }
+      if (together) n_own_rows = min(T, n_rows - tile0) * N_REP;
+      if (lead) part -= p.n_own;
+      i0 = row * N_REP, lo = run.all_lo, hi = run.all_hi, seq = run.seq;
+      sp = split_of(lo, hi, lead ? p.n_lead : p.n_own);
     } else {
+      if (row >= n_rows) return;
+      const auto r = range_of(ctl, p, row, shared);
+      i0 = row * N_REP, lo = r.start, hi = r.len, seq = r.seq;
       sp = split_of(lo, hi, p.n_own);
     }
   }
-  const uint32_t n_live = own ? N_REP : 16;
+  const uint32_t n_live = own ? SHAPED<P> ? n_own_rows : N_REP : 16;
   const uint32_t begin = sp.base + part * sp.per * TILE, end = min(begin + sp.per * TILE, hi);
   auto result = [&](uint32_t i, uint32_t j) -> float * {  // query row i's dims 2 j and 2 j + 1
     return a + p.o_off + i / N_REP * p.o_stride + (kvh * N_REP + i % N_REP) * HD + 2 * j;
@@ -1216,28 +1352,46 @@ SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_
       for (uint32_t j = t; j < N_REP * 64; j += 256) *(float2 *)result(i0 + j / 64, j % 64) = make_float2(0.0f, 0.0f);
     return;
   }
+  // Each row's [lo, hi) of the run (shaped): rows that go together may see parts of it.
+  [[maybe_unused]] __shared__ uint2 sees[SHAPED<P> ? 16 : 1];
+  if constexpr (SHAPED<P>) {
+    if (t < 16) {
+      const uint32_t at = own ? (i0 + c % n_live) / N_REP - tile0 : 0, from = __shfl(run.lane_lo, at, 64), to = __shfl(run.lane_hi, at, 64);
+      sees[t] = own ? make_uint2(from, to) : make_uint2(lo, hi);
+    }
+    __syncthreads();
+  }
   // whether query row i takes part in this run
   auto live = [&](uint32_t i) {
+    if constexpr (SHAPED<P>)
+      if (own) return max(sees[i - i0].x, begin) < min(sees[i - i0].y, end);
     return own || (i / N_REP < n_rows && range_of(ctl, p, i / N_REP, shared).member);
   };
   if (!own && !__syncthreads_or(live(i0 + c))) return;
   const uint32_t steps = (end - begin + HALF - 1) / HALF, per = (steps + 3) / 4 * HALF;
   if (begin + wave * per < end) {
     const uint32_t i = i0 + c % n_live, row = min(i / N_REP, n_rows - 1);
-    float slope = 0.0f;
-    uint32_t row_at = 0;
+    [[maybe_unused]] float slope = 0.0f;
+    [[maybe_unused]] uint32_t row_at = 0;
+    [[maybe_unused]] uint2 mine = {};
     if constexpr (SHAPED<P>) {
       if (p.slopes_off != ~0u) slope = __builtin_bit_cast(float, ctl[p.slopes_off + kvh * N_REP + i % N_REP]) * 1.44269504088896340736f;
-      row_at = range_of(ctl, p, row, shared).at;
+      row_at = ctl[p.rows_off + 4 * row + 1] - 1;
+      mine = sees[c % n_live];
     }
     wave_run<K8, V8>(a, ctl, kv, kv8, p, kvh, a + p.q_off + row * p.q_stride + (kvh * N_REP + i % N_REP) * HD,
-                     st.run[wave], seq, lo, hi, begin + wave * per, min(begin + (wave + 1) * per, end), slope, row_at);
+                     st.run[wave], seq, lo, hi, begin + wave * per, min(begin + (wave + 1) * per, end), slope, row_at, mine.x,
+                     mine.y);
   }
   const uint32_t used = (steps * HALF + per - 1) / per;  // waves with a run
   __syncthreads();
   for (uint32_t j = t; j < n_live * 64; j += 256) {
     const uint32_t r = j / 64, d = j % 64, i = i0 + r;
-    if (!live(i)) continue;
+    if (!live(i)) {
+      if constexpr (SHAPED<P>)  // a row without positions among others
+        if (slots == 1 && sees[r].y == 0) *(float2 *)result(i, d) = make_float2(0.0f, 0.0f);
+      continue;
+    }
     float m = st.run[0][r][0];
 #pragma unroll
     for (uint32_t n = 1; n < 4; n++)
@@ -1301,6 +1455,13 @@ APPEND(1, 1)
                                                        uint32_t n_grid) {                               \
     (void)kvs;                                                                                         \
     paged_body<R, K8, V8>(a, ctl, kv, kv8, p, n_grid);                                                 \
+  }                                                                                                    \
+  extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))                  \
+  void attention_paged_shaped_cap__##R##_##K8##_##V8##_128(float *a, const uint32_t *ctl, const f16 *kv, \
+                                                           const int8_t *kv8, const f16 *kvs, CappedPush p, \
+                                                           uint32_t n_grid) {                           \
+    (void)kvs;                                                                                         \
+    paged_body<R, K8, V8>(a, ctl, kv, kv8, p, n_grid);                                                 \
   }
 #define PAGED_REP(K8, V8) PAGED(1, K8, V8) PAGED(2, K8, V8) PAGED(4, K8, V8) PAGED(8, K8, V8)
 PAGED_REP(0, 0)
@@ -1318,18 +1479,33 @@ SK_DEV void paged_merge(float *a, const uint32_t *ctl, const P &p, uint32_t h, u
                         uint32_t lane) {
   const uint32_t shared = shared_end(ctl, p);
   const auto r = range_of(ctl, p, row, shared);
-  uint32_t first = 0, nl = 0;  // where the shared run starts, and a lead's partials
+  uint32_t ns, no, nl = 0;  // live partials: the shared run's, the row's own, its lead's
+  uint32_t o0 = p.n_shared, l0 = 0;  // the first of the latter two
   if constexpr (SHAPED<P>) {
-    first = shared_first(ctl, p, shared);
-    if (r.member && p.n_lead) nl = live_parts(split_of(r.lo, first, p.n_lead));
+    const bool together = rows_together(ctl, p.rows_off, row, ctl[2], 16 / p.rep);
+    // the parts of [x.all_lo, x.all_hi) with some of [x.lo, x.hi)
+    auto parts_of = [&](bool lead, uint32_t n_parts, uint32_t &at) {
+      const OwnRun x = own_run(ctl, p, row, ctl[2], 16 / p.rep, together, shared, lead);
+      if (x.lo >= x.hi) return 0u;
+      const Split sp = split_of(x.all_lo, x.all_hi, n_parts);
+      const uint32_t k = (x.lo - sp.base) / (sp.per * TILE);
+      at += k;
+      return (x.hi - 1 - sp.base) / (sp.per * TILE) - k + 1;
+    };
+    ns = r.member ? live_parts(split_of(shared_first(ctl, p, shared), shared, p.n_shared)) : 0;
+    no = parts_of(false, p.n_own, o0);
+    l0 = p.n_shared + p.n_own;
+    if (p.n_lead) nl = parts_of(true, p.n_lead, l0);
+  } else {
+    ns = r.member ? live_parts(split_of(0, shared, p.n_shared)) : 0;
+    no = live_parts(split_of(r.start, r.len, p.n_own));
   }
-  const uint32_t ns = r.member ? live_parts(split_of(first, shared, p.n_shared)) : 0;
-  const uint32_t no = live_parts(split_of(r.start, r.len, p.n_own)), n = ns + no + nl;
+  const uint32_t n = ns + no + nl;
   const float *part = a + p.part_off + (row * p.n_head + h) * slots_of(p) * PART;
   // live partial i
   auto at = [&](uint32_t i) {
-    if (SHAPED<P> && i >= ns + no) return part + (p.n_shared + p.n_own + i - ns - no) * PART;
-    return part + (i < ns ? i : p.n_shared + i - ns) * PART;
+    if (SHAPED<P> && i >= ns + no) return part + (l0 + i - ns - no) * PART;
+    return part + (i < ns ? i : o0 + i - ns) * PART;
   };
   float big = -INFINITY;
   for (uint32_t i = lane; i < n; i += 64) big = fmaxf(big, at(i)[0]);

@@ -206,7 +206,7 @@ inline std::string refusal(Op op, const uint32_t *spec, const uint32_t *w, const
     if (!o.same(q)) c.apart(o, q);
     c.apart(part, q);
     c.writes({o, part}, read);
-    if (n_kv * ((rows * spec[0] + 15) / 16 * w[11] + rows * (w[12] + lead)) > kMaxWork)
+    if (n_kv * ((rows * spec[0] + 15) / 16 * w[11] + (rows + (shaped ? 15 : 0)) * (w[12] + lead)) > kMaxWork)
       c.fail("%llu rows in %llu parts: too many workgroups", (unsigned long long)rows, (unsigned long long)parts);
   } else if (op == kMerge || op == kShapedMerge) {
     const uint64_t n_head = w[3], parts = (uint64_t)w[4] + w[5] + (shaped ? w[12] : 0);
@@ -221,6 +221,7 @@ inline std::string refusal(Op op, const uint32_t *spec, const uint32_t *w, const
     c.holds(o, 2);
     c.holds(words, 4);
     const Region spans{"the rows' spans", C, 4, shaped ? w[10] : 0, 2, 2, shaped ? rows : 0};
+    if (shaped) c.need((w[13] == 1 || w[13] == 2 || w[13] == 4 || w[13] == 8) && n_head % w[13] == 0, "1, 2, 4 or 8 query heads a key head");
     c.holds(spans, 2);
     c.writes({o}, {part, words, spans, ctl});
   } else if (op == kLogits) {
@@ -269,6 +270,7 @@ inline std::string other_form(Op op, const std::string &symbol) {
   if (op == kMerge) return "attention_paged_merge_8__128";
   if (op == kAppend) return "kv_append_4" + symbol.substr(std::strlen("kv_append"));
   if (op == kAppendAxes) return "kv_append_axes_4" + symbol.substr(std::strlen("kv_append_axes"));
+  if (op == kShaped) return "attention_paged_shaped_cap" + symbol.substr(std::strlen("attention_paged_shaped"));
   if (op == kShapedMerge) return "attention_paged_shaped_merge_8__128";
   return symbol;
 }
@@ -280,12 +282,14 @@ inline Shape shape(Op op, const uint32_t *spec, const uint32_t *w, uint32_t rows
     s.form = (uint64_t)rows * heads >= kAppendMany;
     s.groups[0] = s.form ? (heads + 3) / 4 : heads;
   } else if (op == kAttend || op == kShaped) {
-    const uint32_t q = rows * spec[0], groups = w[9] * w[11], own = rows * w[9] * (w[12] + (op == kShaped ? w[23] : 0));
+    const uint32_t q = rows * spec[0], groups = w[9] * w[11], T = op == kShaped ? 16 / spec[0] : 1;  // (whole T rows)
+    const uint32_t own = (rows + T - 1) / T * T * w[9] * (w[12] + (op == kShaped ? w[23] : 0));
     if (w[19] && w[11])
       s.groups[0] = (groups + 7) / 8 * 8 * ((q + 127) / 128) + own;
     else
       s.groups[0] = groups * ((q + 15) / 16) + own;
     s.groups[1] = 1;
+    s.form = op == kShaped && w[24] << 1;  // a cap (not 0, nor -0)
     s.extra = {rows};
   } else if (op == kMerge || op == kShapedMerge) {
     s.form = w[4] + w[5] + (op == kShapedMerge ? w[12] : 0) > kMergeParts && rows * w[3] <= kMergeHeads;

@@ -203,7 +203,7 @@ const KernelInfo kKernels[] = {
     {"logits_adjust", 2, 12, 0, 0, -1, false, false},
     {"kv_append_axes", 5, 26, 3, 3, -1, false, false},
     {"attention_paged_shaped", 5, 25, 4, 4, -1, false, false},
-    {"attention_paged_shaped_merge", 2, 13, 1, 1, -1, false, false},
+    {"attention_paged_shaped_merge", 2, 14, 1, 1, -1, false, false},
     {"logits_sample", 2, 5, 0, 0, -1, false, false, 512},  // (kernels/sample.hip)
     {"logits_sample_draw", 2, 6, 0, 0, -1, false, false, 1024},
 };

@@ -199,7 +199,7 @@ class BatchKernels:
         self._shaped = build("attention_paged_shaped", [a, a], 25, [c.n_head // c.n_head_kv, k8, v8, 128])
         self._merge = ctx.create_pipeline("attention_paged_merge", 2, 40, [128])
         self._merge.bind_buffers([a, a])
-        self._shaped_merge = ctx.create_pipeline("attention_paged_shaped_merge", 2, 52, [128])
+        self._shaped_merge = ctx.create_pipeline("attention_paged_shaped_merge", 2, 56, [128])
         self._shaped_merge.bind_buffers([a, a])
 
     @staticmethod
@@ -250,7 +250,7 @@ class BatchKernels:
         if parts.shared + parts.own + parts.lead == 1:
             return
         r.barrier()
-        push = self._merge_push(at, out, parts) + [at.spans, shape.window, parts.lead]
+        push = self._merge_push(at, out, parts) + [at.spans, shape.window, parts.lead, self.c.n_head // self.c.n_head_kv]
         r.dispatch(self._shaped_merge, [1, rows, 1], push)
 
     def _attend_push(self, at, q, out, parts) -> list[int]:
