@@ -14,10 +14,10 @@
 // no place; +inf counts as the type's largest value.  A row without tokens gets {~0, 0, -inf, 0}.
 //
 // Sums decide which token it is, so they are held to more than 32 bits: a row's tokens fall into bins of
-// t = x 8 log2(e) / T, one floor(t) each, in which a weight is 2^((t - floor(t) - 1) / 8) of its bin's upper
-// edge's.  A bin's count and sum of weights are integers (36 bits after the point: a weight is off by 7e-12
-// of itself at most), the same in any order, and only the tokens of the bins in which a border lies (min_p's
-// or top_k's, top_p's, the draw's) are looked at one by one, in f64.
+// t = x 8 log2(e) / T, one rint(t) each, in which a weight is 2^((t - rint(t)) / 8) of its bin's middle's.
+// A bin's count and sum of weights are integers (36 bits after the point: a weight is off by 8e-12 of itself at
+// most), the same in any order, and only the tokens of the bins in which a border lies (min_p's or top_k's,
+// top_p's, the draw's) are looked at one by one.
 #include "common.h"
 
 namespace {
@@ -31,7 +31,7 @@ struct DrawPush {
 
 constexpr uint32_t THREADS = 512, EACH = 16, CHUNK = THREADS * EACH;  // tokens of a workgroup of logits_sample
 constexpr uint32_t BINS = 512;  // from a chunk's (a row's) largest value down; the last holds all below it, too
-// a chunk's part: {floor(t) of its largest value (f64), that value, how many there are, 0, 0, 0, 0}, its bins, and
+// a chunk's part: {rint(t) of its largest value (f64), that value, how many there are, 0, 0, 0, 0}, its bins, and
 // its tokens in the bins' order (16 bits each, from the chunk's first)
 constexpr uint32_t HEAD = 8, PART = HEAD + 2 * BINS + CHUNK / 2;
 // a bin's word: its weights' sum times 2^36, and from this bit on how many tokens end with it
@@ -42,25 +42,34 @@ constexpr uint64_t SUM = (1ull << COUNT_AT) - 1;
 SK_DEV bool has_weight(float x) { return x > -INFINITY; }  // (not NaN)
 SK_DEV double scale_of(float T) { return 11.541560327111707 / (T > 0.0f ? (double)T : 1.0); }  // 8 log2(e) / T
 SK_DEV double scaled(float x, double c) { return (double)fminf(x, 3.402823466e38f) * c; }
-// 2^36 2^((f - 1) / 8), f in [0, 1): a series in f - 1/2 of which what is left out is below 6e-14
-SK_DEV double weight(double f) {
-  constexpr double S = 0x1p36;
-  const double s = f - 0.5;
-  double y = S * 5.626858230225532679e-10;
-  y = __builtin_fma(y, s, S * 3.896563422975180069e-8);
-  y = __builtin_fma(y, s, S * 2.248621090734246650e-6);
-  y = __builtin_fma(y, s, S * 1.038103838861001429e-4);
-  y = __builtin_fma(y, s, S * 3.594401424606149610e-3);
-  y = __builtin_fma(y, s, S * 8.297000176389627734e-2);
-  return __builtin_fma(y, s, S * 9.576032806985736469e-1);
+// 2^(f / 8) for |f| <= 1/2 in units of 2^-36, as the low bits of the double behind 2^52: 1 + the polynomial of degree 5
+// nearest to the rest (4e-13 of it at most).  The constants are scalar registers: known as constants they would be moved
+// into vector ones for each use.
+struct Series {
+  double a, b, c, d, e, one;
+};
+SK_DEV Series series() {
+  Series k{4.0687475846311098e-8 * 0x1p36, 2.3483805669065314e-6 * 0x1p36, 1.0840646378828406e-4 * 0x1p36,
+           3.7535391554191859e-3 * 0x1p36, 8.6643397569895267e-2 * 0x1p36, 0x1p36 + 0x1p52};
+  asm("" : "+s"(k.a), "+s"(k.b), "+s"(k.c), "+s"(k.d), "+s"(k.e), "+s"(k.one));
+  return k;
 }
-SK_DEV uint64_t whole(double v) { return (uint64_t)__builtin_rint(v); }
-// What t adds to the sum of the bin floor(t), d bins below the first.
-SK_DEV uint64_t fixed_weight(double t, double d) {
+SK_DEV uint64_t fixed_weight(const Series &k, double f) {
+  double y = __builtin_fma(k.a, f, k.b);
+  y = __builtin_fma(y, f, k.c);
+  y = __builtin_fma(y, f, k.d);
+  y = __builtin_fma(y, f, k.e);
+  y = __builtin_fma(y, f, k.one);
+  return __builtin_bit_cast(uint64_t, y) - 0x4330000000000000ull;
+}
+// what a token adds to the last bin from d bins below the first, below that one's lower edge
+SK_DEV uint64_t far_weight(const Series &k, double f, double d) {
+  return (uint64_t)__builtin_rint((double)fixed_weight(k, f) * exp2(((double)(BINS - 1) - d) * 0.125));
+}
+SK_DEV uint64_t fixed_weight_at(const Series &k, double t, double d) {
 #pragma clang fp contract(off)
-  const double y = weight(t - __builtin_floor(t));
-  if (d < BINS) return __builtin_bit_cast(uint64_t, y + 0x1p52) - 0x4330000000000000ull;  // rounded there
-  return whole(y * exp2(((double)(BINS - 1) - d) * 0.125));  // below the last bin's lower edge
+  const double f = t - __builtin_rint(t);
+  return d < BINS ? fixed_weight(k, f) : far_weight(k, f, d);
 }
 // a place in the order: the smaller, the earlier (-0 and 0 are equal)
 SK_DEV uint64_t place(float x, uint32_t id) {
@@ -94,14 +103,12 @@ extern "C" __global__ __launch_bounds__(THREADS) void logits_sample(float *a, co
   __shared__ float big[WAVES];
   __shared__ uint32_t counts[WAVES];
   const uint32_t row = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  if (row >= ctl[2]) return;
   const uint32_t base = blockIdx.x * CHUNK, n = min(CHUNK, p.n_vocab - base);
   const float *x = a + p.x_off + (size_t)row * p.x_stride + base;
   float *part = a + p.part_off + ((size_t)row * gridDim.x + blockIdx.x) * PART;
-  const double c = scale_of(__builtin_bit_cast(float, ctl[p.ctrl_off + 8 * row]));
   f32x4 v[EACH / 4];
 #pragma unroll
-  for (uint32_t k = 0; k < EACH / 4; k++) {  // tokens 4 (t + THREADS k) + [0, 4)
+  for (uint32_t k = 0; k < EACH / 4; k++) {  // tokens 4 (t + THREADS k) + [0, 4); on their way before anything is known
     const uint32_t i = 4 * (t + THREADS * k);
     v[k] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
     if (i + 4 <= n) {
@@ -112,6 +119,8 @@ extern "C" __global__ __launch_bounds__(THREADS) void logits_sample(float *a, co
       if (i + 2 < n) v[k][2] = x[i + 2];
     }
   }
+  if (row >= ctl[2]) return;
+  const double c = scale_of(__builtin_bit_cast(float, ctl[p.ctrl_off + 8 * row]));
   float top = -INFINITY;
 #pragma unroll
   for (uint32_t k = 0; k < EACH / 4; k++)
@@ -124,7 +133,7 @@ extern "C" __global__ __launch_bounds__(THREADS) void logits_sample(float *a, co
   __syncthreads();
 #pragma unroll
   for (uint32_t w = 0; w < WAVES; w++) top = fmaxf(top, big[w]);
-  const double first = __builtin_floor(scaled(top, c));
+  const double first = __builtin_rint(scaled(top, c));
   if (!has_weight(top)) {  // nothing here, and nothing more is read
     if (t == 0) {
       *(double *)part = -INFINITY;
@@ -133,19 +142,44 @@ extern "C" __global__ __launch_bounds__(THREADS) void logits_sample(float *a, co
     }
     return;
   }
-  uint32_t at[EACH];  // a token's bin, and its place among those of the bin
+  const Series series_ = series();
+  uint32_t at[EACH];  // a token's bin, and its place among those of the bin; ~0: none yet
+  uint32_t far = 0;   // one bit each: below the last bin, as most of a row are where T is low
 #pragma unroll
-  for (uint32_t k = 0; k < EACH / 4; k++)
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      uint32_t &b = at[4 * k + e];
-      b = ~0u;
-      if (!has_weight(v[k][e])) continue;
-      const double s = scaled(v[k][e], c), d = first - __builtin_floor(s);
-      b = d < BINS ? (uint32_t)(int)d : BINS - 1;
-      const uint64_t before = atomicAdd(&bin[b], (unsigned long long)(fixed_weight(s, d) + (1ull << COUNT_AT)));
-      b |= (uint32_t)(before >> COUNT_AT) << 16;
+  for (uint32_t i = 0; i < EACH; i++) {
+    const float y = v[i / 4][i % 4];
+    const double s = scaled(y, c), g = __builtin_rint(s), d = first - g;
+    const uint64_t word = fixed_weight(series_, s - g) + (1ull << COUNT_AT);
+    const uint32_t b = (uint32_t)(int)fmin(d, 2.0 * BINS);
+    at[i] = ~0u;
+    if (has_weight(y)) {
+      if (b < BINS)
+        at[i] = b | (uint32_t)(atomicAdd(&bin[b], (unsigned long long)word) >> COUNT_AT) << 16;
+      else
+        far |= 1u << i;
     }
+  }
+  if (__any(far != 0)) {
+    uint32_t near = 0;  // those whose weights count: 2^-36 of the last bin's middle's and above
+#pragma unroll
+    for (uint32_t i = 0; i < EACH; i++) {
+      const uint64_t m = __ballot(far >> i & 1);
+      if (!m) continue;
+      uint64_t before = 0;
+      if (lane == 0) before = atomicAdd(&bin[BINS - 1], (unsigned long long)__builtin_popcountll(m) << COUNT_AT);
+      const uint32_t rank = __builtin_amdgcn_readfirstlane((uint32_t)(before >> COUNT_AT)) +
+                            __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+      if (far >> i & 1) {
+        at[i] = (BINS - 1) | rank << 16;
+        if (first - __builtin_rint(scaled(v[i / 4][i % 4], c)) < BINS + 8 * 37) near |= 1u << i;
+      }
+    }
+    for (; near; near &= near - 1) {
+      const uint32_t i = (uint32_t)__builtin_ctz(near);
+      const double s = scaled(x[4 * (t + THREADS * (i / 4)) + i % 4], c), g = __builtin_rint(s);
+      atomicAdd(&bin[BINS - 1], (unsigned long long)far_weight(series_, s - g, first - g));
+    }
+  }
   __syncthreads();
   const uint64_t mine = bin[t];
   const uint32_t count = (uint32_t)(mine >> COUNT_AT);
@@ -195,11 +229,11 @@ struct DrawShared {
       double largest[CHUNKS];
     } half;
   };
-  double c[BINS + 1];     // C before a bin, in weights of the row's upper edge
+  double c[BINS + 1];     // C before a bin, in weights of the first bin's middle
   uint32_t n[BINS + 1];   // tokens before it
-  double edge[BINS];      // its upper edge's weight
+  double edge[BINS];      // its middle's weight
   uint32_t bucket[DRAW];
-  double first[CHUNKS];   // the chunks' floor(t) of their largest values
+  double first[CHUNKS];   // the chunks' rint(t) of their largest values
   double sums[DRAW_WAVES];
   uint64_t words[DRAW_WAVES];
   uint32_t counts[DRAW_WAVES];
@@ -211,15 +245,16 @@ struct DrawShared {
 struct Row {
   const float *x;
   uint32_t n_vocab;
-  double c, edge;  // t = x c; floor(t) of the largest value
+  double c, edge;  // t = x c; rint(t) of the largest value
 };
 SK_DEV uint32_t bin_of(const Row &r, double t) {
-  const double d = r.edge - __builtin_floor(t);
+  const double d = r.edge - __builtin_rint(t);
   return d < BINS - 1 ? (uint32_t)(int)d : BINS - 1;
 }
-SK_DEV uint64_t fixed_weight(const Row &r, double t) { return fixed_weight(t, r.edge - __builtin_floor(t)); }
+SK_DEV uint64_t fixed_weight(const Series &k, const Row &r, double t) { return fixed_weight_at(k, t, r.edge - __builtin_rint(t)); }
 // a sum of a bin's weights
 SK_DEV double sum_of(uint64_t fixed, double edge) { return (double)fixed * 0x1p-36 * edge; }
+constexpr double UP = 1.0442737824274138, DOWN = 0.9576032806985737;  // 2^(1/16), 2^(-1/16): a weight of its bin's middle's
 
 // Every value of the row that may lie in [least, most) by its t, among them all that do: f(place, t).
 template <typename F>
@@ -253,7 +288,8 @@ SK_DEV void each_value(const Row &r, double least, double most, F f) {
 // those of bin b
 template <typename F>
 SK_DEV void each_value_of(const Row &r, uint32_t b, F f) {
-  each_value(r, b < BINS - 1 ? r.edge - (double)b : -INFINITY, b ? r.edge - (double)b + 1.0 : INFINITY, [&](uint64_t place, double t) {
+  each_value(r, b < BINS - 1 ? r.edge - (double)b - 0.5 : -INFINITY, b ? r.edge - (double)b + 0.5 : INFINITY,
+             [&](uint64_t place, double t) {
     if (bin_of(r, t) == b) f(place, t);
   });
 }
@@ -306,6 +342,7 @@ __device__ __attribute__((noinline)) Found search(DrawShared &s, const Row r, Wa
   const uint32_t last = first_bin(s.n, [&](uint32_t n) { return n >= s.n[BINS]; });
   b = min(b, last);
   const double edge = s.edge[b];
+  const Series series_ = series();
   Found f{0, s.n[b], s.c[b]};
   constexpr int at[5] = {53, 42, 32, 10, 0}, bits[5] = {11, 11, 10, 22, 10};
   // (ids are below 2^20: 10 bits from bit 10 on, all 22 of them compared as a prefix)
@@ -317,7 +354,7 @@ __device__ __attribute__((noinline)) Found search(DrawShared &s, const Row r, Wa
     each_value_of(r, b, [&](uint64_t place, double v) {
       if (above < 64 && place >> above != f.place >> above) return;
       const uint32_t d = (uint32_t)(place >> at[k]) & (DIGITS - 1);
-      atomicAdd(&s.digit.sum[d], (unsigned long long)fixed_weight(r, v));
+      atomicAdd(&s.digit.sum[d], (unsigned long long)fixed_weight(series_, r, v));
       atomicAdd(&s.digit.count[d], 1u);
     });
     __syncthreads();
@@ -355,8 +392,9 @@ __device__ __attribute__((noinline)) Found search(DrawShared &s, const Row r, Wa
 __device__ __attribute__((noinline)) Found search_above(DrawShared &s, const Row r, double least, uint32_t b) {
   uint64_t sum = 0;
   uint32_t n = 0;
+  const Series series_ = series();
   each_value_of(r, b, [&](uint64_t, double v) {
-    if (v >= least) sum += fixed_weight(r, v), n++;
+    if (v >= least) sum += fixed_weight(series_, r, v), n++;
   });
   uint64_t all;
   uint32_t count;
@@ -416,7 +454,7 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
     return;
   }
   const double t_top = scaled(top, r.c);
-  r.edge = __builtin_floor(t_top);
+  r.edge = __builtin_rint(t_top);
 
   // the row's bins: thread t has bin t % BINS of every other chunk
   {
@@ -425,30 +463,28 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
     uint64_t sum = 0;
     constexpr uint32_t U = 10, STEP = DRAW / BINS;  // chunks whose loads are in flight
     for (uint32_t i0 = t / BINS; i0 < n_chunks; i0 += U * STEP) {
-      uint64_t w[U];
-      bool last[U];
+      uint64_t w[U], below[U];
 #pragma unroll
       for (uint32_t j = 0; j < U; j++) {
         const uint32_t i = min(i0 + j * STEP, n_chunks - 1);
         const double d = r.edge - s.first[i];  // the chunk's bins lie so many below the row's
         const uint32_t down = d < BINS ? (uint32_t)(int)d : BINS;
         const bool any = i0 + j * STEP < n_chunks && s.first[i] > -INFINITY;
-        last[j] = any && b == BINS - 1;
-        // (of the row's last bin: how many the chunk has)
-        w[j] = any && (b >= down || last[j]) ? ((const uint64_t *)(parts + (size_t)i * PART + HEAD))[last[j] ? b : b - down] : 0;
+        const uint64_t *bins = (const uint64_t *)(parts + (size_t)i * PART + HEAD);
+        w[j] = any && b >= down && b < BINS - 1 ? bins[b - down] : 0;
+        below[j] = any && b + down >= BINS - 1 ? bins[b] : 0;  // of the chunk's bin b: it lies in the row's last
       }
 #pragma unroll
       for (uint32_t j = 0; j < U; j++) {
         n += (uint32_t)(w[j] >> COUNT_AT);
-        sum += last[j] ? 0 : w[j] & SUM;
+        sum += w[j] & SUM;
+        if (b == BINS - 1) n += (uint32_t)(below[j] >> COUNT_AT);  // (how many the chunk has)
+        if (below[j] & SUM) {  // in weights of that one's middle
+          const double d = r.edge - s.first[min(i0 + j * STEP, n_chunks - 1)];
+          const double by = exp2(((double)(BINS - 1) - (double)b - d) * 0.125);
+          atomicAdd(&s.below, (unsigned long long)__builtin_rint((double)(below[j] & SUM) * by));
+        }
       }
-    }
-    // a chunk's bins from the row's last on go there, in weights of that one's edge
-    for (uint32_t i = t / BINS; i < n_chunks; i += STEP) {
-      const double d = r.edge - s.first[i];
-      if (!(d < INFINITY) || (double)b + d < (double)(BINS - 1)) continue;
-      const uint64_t w = ((const uint64_t *)(parts + (size_t)i * PART + HEAD))[b] & SUM;
-      if (w) atomicAdd(&s.below, (unsigned long long)whole((double)w * exp2(((double)(BINS - 1) - (double)b - d) * 0.125)));
     }
     __syncthreads();  // (the chunks' largest values are read)
     s.half.sum[t] = sum;
@@ -479,10 +515,10 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
     lo = s.c[b1], hi = s.c[b1 + 1];
     if (b1 == bk) {
       const double more = (double)(k - s.n[bk]) * s.edge[bk];
-      hi = fmin(hi, lo + more);
-      if (bm != bk && bk < BINS - 1) lo += more * s.edge[1];
+      hi = fmin(hi, lo + more * UP);
+      if (bm != bk && bk < BINS - 1) lo += more * DOWN;
     }
-    if (b1 == 0) lo = fmax(lo, s.edge[1]);  // the largest stays
+    if (b1 == 0) lo = fmax(lo, DOWN * LESS);  // the largest stays
   }
   const uint32_t b_last = min(b1, first_bin(s.n, [&](uint32_t n) { return n >= total; }));  // where n1 lies, or past it
   const bool by_p = top_p < 1.0f;
@@ -492,8 +528,8 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
     lo *= share * LESS, hi *= share * MORE;
     p_lo = min(first_bin(s.c, [&](double c) { return c >= lo; }), b_last);
     p_hi = min(first_bin(s.c, [&](double c) { return c >= hi; }), b_last);
-    hi = fmin(s.c[p_hi + 1], hi + s.edge[p_lo]);
-    lo = fmax(lo, s.edge[1] * LESS);
+    hi = fmin(s.c[p_hi + 1], hi + s.edge[p_lo] * UP);
+    lo = fmax(lo, DOWN * LESS);
   }
   const double u = ((double)words[4] + 0.5) * 0x1p-32;
   const uint32_t d_lo = min(first_bin(s.c, [&](double c) { return c > lo * u * LESS; }), p_hi);
@@ -524,13 +560,13 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
     // ---- few: from the chunks' lists into LDS, in buckets by t
     const uint32_t per = DRAW / n_spans;
     auto bucket_of = [&](double v) {
-      const double g = __builtin_floor(v), f = 1.0 - (v - g);
+      const double g = __builtin_rint(v), f = 0.5 - (v - g);
       const uint32_t b = (uint32_t)(int)(r.edge - g), i = b >= f2 ? span2 + b - f2 : b >= f1 ? span1 + b - f1 : b - f0;
       return i * per + min((uint32_t)(int)(f * (double)per), per - 1);
     };
-    constexpr uint32_t LANES = 16;  // of a chunk's run
+    constexpr uint32_t LANES = 16, U = 4;  // of a chunk's run, each with so many loads in flight
     for (uint32_t j = t / LANES; j < n_chunks * 3; j += DRAW / LANES) {
-      const uint32_t i = j / 3, which = j % 3, f = which == 0 ? f0 : which == 1 ? f1 : f2, e = which == 0 ? e0 : which == 1 ? e1 : e2;
+      const uint32_t i = j % n_chunks, which = j / n_chunks, f = which == 0 ? f0 : which == 1 ? f1 : f2, e = which == 0 ? e0 : which == 1 ? e1 : e2;
       const float *part = parts + (size_t)i * PART;
       const double d = r.edge - s.first[i];
       if (f == ~0u || !(d <= (double)e)) continue;
@@ -538,12 +574,21 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
       const uint64_t *bins = (const uint64_t *)(part + HEAD);
       const uint32_t i0 = f > down ? (uint32_t)(bins[f - down - 1] >> COUNT_AT) : 0,
                      i1 = (uint32_t)(bins[e - down] >> COUNT_AT);
-      for (uint32_t o = i0 + t % LANES; o < i1; o += LANES) {
-        const uint32_t id = i * CHUNK + ((const uint16_t *)(part + HEAD + 2 * BINS))[o];
-        const float x = r.x[id];
-        const uint32_t to = atomicAdd(&s.fill, 1u);
-        if (to < MOST) s.place[0][to] = place(x, id);  // (always: so many were counted)
-        atomicAdd(&s.bucket[bucket_of(scaled(x, r.c))], 1u);
+      const uint16_t *ids = (const uint16_t *)(part + HEAD + 2 * BINS);
+      for (uint32_t o = i0 + t % LANES; o < i1; o += U * LANES) {
+        uint32_t id[U];
+        float x[U];
+#pragma unroll
+        for (uint32_t u = 0; u < U; u++) id[u] = i * CHUNK + ids[min(o + u * LANES, i1 - 1)];
+#pragma unroll
+        for (uint32_t u = 0; u < U; u++) x[u] = r.x[id[u]];
+#pragma unroll
+        for (uint32_t u = 0; u < U; u++) {
+          if (o + u * LANES >= i1) break;
+          const uint32_t to = atomicAdd(&s.fill, 1u);
+          if (to < MOST) s.place[0][to] = place(x[u], id[u]);  // (always: so many were counted)
+          atomicAdd(&s.bucket[bucket_of(scaled(x[u], r.c))], 1u);
+        }
       }
     }
     __syncthreads();
@@ -566,9 +611,10 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
     __syncthreads();
     // the sum behind each, in place of those in buckets
     uint64_t carry = 0, *raw = s.place[1];
+    const Series series_ = series();
     for (uint32_t i0 = 0; i0 < n; i0 += DRAW) {
       const uint32_t i = i0 + t;
-      const uint64_t w = i < n ? fixed_weight(r, scaled(value_at(s.place[0][i]), r.c)) : 0;
+      const uint64_t w = i < n ? fixed_weight(series_, r, scaled(value_at(s.place[0][i]), r.c)) : 0;
       uint64_t sum_all;
       const uint64_t sum = block_scan(w, s.words, sum_all) + carry;
       if (i < n) raw[i] = sum;
@@ -619,7 +665,7 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
     if (chosen.n > n2.n) chosen = search(s, r, kCount, (double)n2.n);
   }
   if (t == 0) {
-    const double y = (scaled(value_at(chosen.place), r.c) - r.edge - 1.0) * 0.125 * 0.69314718055994530942 - log(n2.sum);
+    const double y = (scaled(value_at(chosen.place), r.c) - r.edge) * 0.125 * 0.69314718055994530942 - log(n2.sum);
     *(uint4 *)out = make_uint4((uint32_t)chosen.place, n2.n, __builtin_bit_cast(uint32_t, n2.n == 1 ? 0.0f : (float)y), 0);
   }
 }
