@@ -81,14 +81,40 @@ SK_DEV float value_at(uint64_t place) {
   return __builtin_bit_cast(float, u & 0x80000000u ? u : ~u & 0x7fffffffu);
 }
 
-template <typename T>
-SK_DEV T wave_scan(T v, uint32_t lane) {  // inclusive
-#pragma unroll
-  for (uint32_t d = 1; d < 64; d <<= 1) {
-    const T u = __shfl_up(v, d, 64);
-    if (lane >= d) v += u;
+// Sums over the lanes up to each (inclusive) and the largest of all, by moves between lanes: 1, 2, 4 and 8 lanes up
+// within a row of 16, then a row's last lane into the rows above it.
+template <int CTRL, int ROWS>
+SK_DEV uint32_t moved(uint32_t v, uint32_t none) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS = 0xf, typename T>
+SK_DEV T moved_or_0(T v) {
+  if constexpr (sizeof(T) == 8) {
+    const uint2 u = __builtin_bit_cast(uint2, v);
+    return __builtin_bit_cast(T, make_uint2(moved<CTRL, ROWS>(u.x, 0), moved<CTRL, ROWS>(u.y, 0)));
+  } else {
+    return __builtin_bit_cast(T, moved<CTRL, ROWS>(__builtin_bit_cast(uint32_t, v), 0));
   }
+}
+template <typename T>
+SK_DEV T wave_scan(T v) {
+  v += moved_or_0<0x111>(v);
+  v += moved_or_0<0x112>(v);
+  v += moved_or_0<0x114>(v);
+  v += moved_or_0<0x118>(v);
+  v += moved_or_0<0x142, 0xa>(v);
+  v += moved_or_0<0x143, 0xc>(v);
   return v;
+}
+template <int CTRL, int ROWS = 0xf>
+SK_DEV float larger(float v) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  return fmaxf(v, __builtin_bit_cast(float, moved<CTRL, ROWS>(u, u)));
+}
+SK_DEV float wave_max(float v) {
+  v = larger<0x118>(larger<0x114>(larger<0x112>(larger<0x111>(v))));
+  v = larger<0x143, 0xc>(larger<0x142, 0xa>(v));
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
 }  // namespace
@@ -97,7 +123,7 @@ SK_DEV T wave_scan(T v, uint32_t lane) {  // inclusive
 extern "C" __global__ __launch_bounds__(THREADS) void logits_sample(float *a, const uint32_t *ctl, SamplePush p) {
 #pragma clang fp contract(off)
   constexpr uint32_t WAVES = THREADS / 64;
-  __shared__ unsigned long long bin[BINS];
+  __shared__ unsigned long long bin[BINS + 64];  // and a lane's own for what is in none
   __shared__ uint32_t start[BINS];
   __shared__ __attribute__((aligned(16))) uint16_t ids[CHUNK];
   __shared__ float big[WAVES];
@@ -126,10 +152,9 @@ extern "C" __global__ __launch_bounds__(THREADS) void logits_sample(float *a, co
   for (uint32_t k = 0; k < EACH / 4; k++)
 #pragma unroll
     for (int e = 0; e < 4; e++) top = fmaxf(top, v[k][e]);  // (leaves NaN aside)
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+  top = wave_max(top);
   if (lane == 0) big[wave] = top;
-  bin[t] = 0;
+  if (t < BINS) bin[t] = 0;
   __syncthreads();
 #pragma unroll
   for (uint32_t w = 0; w < WAVES; w++) top = fmaxf(top, big[w]);
@@ -143,24 +168,28 @@ extern "C" __global__ __launch_bounds__(THREADS) void logits_sample(float *a, co
     return;
   }
   const Series series_ = series();
-  uint32_t at[EACH];  // a token's bin, and its place among those of the bin; ~0: none yet
+  uint32_t at[EACH];  // a token's bin (BINS and above: none), and its place among those of the bin
   uint32_t far = 0;   // one bit each: below the last bin, as most of a row are where T is low
+  constexpr uint32_t U = 4;
 #pragma unroll
-  for (uint32_t i = 0; i < EACH; i++) {
-    const float y = v[i / 4][i % 4];
-    const double s = scaled(y, c), g = __builtin_rint(s), d = first - g;
-    const uint64_t word = fixed_weight(series_, s - g) + (1ull << COUNT_AT);
-    const uint32_t b = (uint32_t)(int)fmin(d, 2.0 * BINS);
-    at[i] = ~0u;
-    if (has_weight(y)) {
-      if (b < BINS)
-        at[i] = b | (uint32_t)(atomicAdd(&bin[b], (unsigned long long)word) >> COUNT_AT) << 16;
-      else
-        far |= 1u << i;
+  for (uint32_t i0 = 0; i0 < EACH; i0 += U) {  // (without branches, so that U are under way at once)
+    uint64_t word[U];
+    uint32_t b[U];
+#pragma unroll
+    for (uint32_t j = 0; j < U; j++) {
+      const float y = v[(i0 + j) / 4][(i0 + j) % 4];
+      const double s = scaled(y, c), g = __builtin_rint(s);
+      word[j] = fixed_weight(series_, s - g) + (1ull << COUNT_AT);
+      b[j] = (uint32_t)(int)fmin(first - g, 2.0 * BINS);
+      far |= has_weight(y) && b[j] >= BINS ? 1u << (i0 + j) : 0;
+      b[j] = has_weight(y) && b[j] < BINS ? b[j] : BINS + lane;
     }
+#pragma unroll
+    for (uint32_t j = 0; j < U; j++) word[j] = atomicAdd(&bin[b[j]], (unsigned long long)word[j]);
+#pragma unroll
+    for (uint32_t j = 0; j < U; j++) at[i0 + j] = b[j] | (uint32_t)(word[j] >> COUNT_AT) << 16;
   }
   if (__any(far != 0)) {
-    uint32_t near = 0;  // those whose weights count: 2^-36 of the last bin's middle's and above
 #pragma unroll
     for (uint32_t i = 0; i < EACH; i++) {
       const uint64_t m = __ballot(far >> i & 1);
@@ -169,21 +198,19 @@ extern "C" __global__ __launch_bounds__(THREADS) void logits_sample(float *a, co
       if (lane == 0) before = atomicAdd(&bin[BINS - 1], (unsigned long long)__builtin_popcountll(m) << COUNT_AT);
       const uint32_t rank = __builtin_amdgcn_readfirstlane((uint32_t)(before >> COUNT_AT)) +
                             __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
-      if (far >> i & 1) {
-        at[i] = (BINS - 1) | rank << 16;
-        if (first - __builtin_rint(scaled(v[i / 4][i % 4], c)) < BINS + 8 * 37) near |= 1u << i;
-      }
+      if (far >> i & 1) at[i] = (BINS - 1) | rank << 16;
     }
-    for (; near; near &= near - 1) {
-      const uint32_t i = (uint32_t)__builtin_ctz(near);
+    for (; far; far &= far - 1) {  // (read again: the registers are used)
+      const uint32_t i = (uint32_t)__builtin_ctz(far);
       const double s = scaled(x[4 * (t + THREADS * (i / 4)) + i % 4], c), g = __builtin_rint(s);
-      atomicAdd(&bin[BINS - 1], (unsigned long long)far_weight(series_, s - g, first - g));
+      // what is 2^-37 of the last bin's middle's or less adds nothing
+      if (first - g < BINS + 8 * 37) atomicAdd(&bin[BINS - 1], (unsigned long long)far_weight(series_, s - g, first - g));
     }
   }
   __syncthreads();
-  const uint64_t mine = bin[t];
+  const uint64_t mine = t < BINS ? bin[t] : 0;
   const uint32_t count = (uint32_t)(mine >> COUNT_AT);
-  uint32_t end = wave_scan(count, lane);
+  uint32_t end = wave_scan(count);
   if (lane == 63) counts[wave] = end;
   __syncthreads();
   uint32_t all = 0;
@@ -192,12 +219,14 @@ extern "C" __global__ __launch_bounds__(THREADS) void logits_sample(float *a, co
     if (w < wave) end += counts[w];
     all += counts[w];
   }
-  start[t] = end - count;
-  ((uint64_t *)(part + HEAD))[t] = (mine & SUM) | (uint64_t)end << COUNT_AT;
+  if (t < BINS) {
+    start[t] = end - count;
+    ((uint64_t *)(part + HEAD))[t] = (mine & SUM) | (uint64_t)end << COUNT_AT;
+  }
   __syncthreads();
 #pragma unroll
   for (uint32_t i = 0; i < EACH; i++)
-    if (at[i] != ~0u) ids[start[at[i] & 0xffff] + (at[i] >> 16)] = 4 * (t + THREADS * (i / 4)) + i % 4;
+    if ((at[i] & 0xffff) < BINS) ids[start[at[i] & 0xffff] + (at[i] >> 16)] = 4 * (t + THREADS * (i / 4)) + i % 4;
   __syncthreads();
   uint4 *list = (uint4 *)(part + HEAD + 2 * BINS);
   for (uint32_t i = t; 8 * i < all; i += THREADS) list[i] = ((const uint4 *)ids)[i];
@@ -226,7 +255,7 @@ struct DrawShared {
     struct {
       uint64_t sum[DRAW];
       uint32_t n[DRAW];
-      double largest[CHUNKS];
+      float largest[CHUNKS];
     } half;
   };
   double c[BINS + 1];     // C before a bin, in weights of the first bin's middle
@@ -307,7 +336,7 @@ SK_DEV uint32_t first_bin(const A *before, F ok) {
 template <typename T>
 SK_DEV T block_scan(T v, T *waves, T &total) {  // inclusive, over DRAW threads; a barrier at its start and one inside
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  v = wave_scan(v, lane);
+  v = wave_scan(v);
   __syncthreads();
   if (lane == 63) waves[wave] = v;
   __syncthreads();
@@ -441,14 +470,7 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
   s.bucket[t] = 0;
   if (t == 0) s.below = 0, s.fill = 0;
   __syncthreads();
-  float top;
-  {
-    const uint32_t lane = t & 63;
-    double big = fmax(s.half.largest[lane], s.half.largest[lane + 64]);
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) big = fmax(big, __shfl_xor(big, d, 64));
-    top = (float)big;
-  }
+  const float top = wave_max(fmaxf(s.half.largest[t & 63], s.half.largest[64 + (t & 63)]));
   if (!has_weight(top)) {
     if (t == 0) *(uint4 *)out = make_uint4(~0u, 0, 0xff800000u, 0);
     return;
@@ -587,42 +609,49 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
           if (o + u * LANES >= i1) break;
           const uint32_t to = atomicAdd(&s.fill, 1u);
           if (to < MOST) s.place[0][to] = place(x[u], id[u]);  // (always: so many were counted)
-          atomicAdd(&s.bucket[bucket_of(scaled(x[u], r.c))], 1u);
+          if (n > 64) atomicAdd(&s.bucket[bucket_of(scaled(x[u], r.c))], 1u);
         }
       }
     }
     __syncthreads();
-    uint32_t all;
-    const uint32_t mine = s.bucket[t], end = block_scan(mine, s.counts, all);
-    s.bucket[t] = end - mine;  // where the bucket starts
-    __syncthreads();
-    for (uint32_t i = t; i < n; i += DRAW) {
-      const uint64_t v = s.place[0][i];
-      s.place[1][atomicAdd(&s.bucket[bucket_of(scaled(value_at(v), r.c))], 1u)] = v;
-    }
-    __syncthreads();  // a bucket's word is now its end, the one before it its start
-    for (uint32_t i = t; i < n; i += DRAW) {
-      const uint64_t v = s.place[1][i];
-      const uint32_t b = bucket_of(scaled(value_at(v), r.c)), o0 = b ? s.bucket[b - 1] : 0, o1 = s.bucket[b];
-      uint32_t rank = o0;
-      for (uint32_t o = o0; o < o1; o++) rank += s.place[1][o] < v;
-      s.place[0][rank] = v;
-    }
-    __syncthreads();
-    // the sum behind each, in place of those in buckets
-    uint64_t carry = 0, *raw = s.place[1];
     const Series series_ = series();
-    for (uint32_t i0 = 0; i0 < n; i0 += DRAW) {
-      const uint32_t i = i0 + t;
-      const uint64_t w = i < n ? fixed_weight(series_, r, scaled(value_at(s.place[0][i]), r.c)) : 0;
-      uint64_t sum_all;
-      const uint64_t sum = block_scan(w, s.words, sum_all) + carry;
-      if (i < n) raw[i] = sum;
-      carry += sum_all;
+    uint64_t *raw = s.place[1];  // in the end, the sum behind each of those in order
+    auto weight_of = [&](uint64_t v) { return fixed_weight(series_, r, scaled(value_at(v), r.c)); };
+    if (n > 64) {
+      uint32_t all;
+      const uint32_t mine = s.bucket[t], end = block_scan(mine, s.counts, all);
+      s.bucket[t] = end - mine;  // where the bucket starts
+      __syncthreads();
+      for (uint32_t i = t; i < n; i += DRAW) {
+        const uint64_t v = s.place[0][i];
+        s.place[1][atomicAdd(&s.bucket[bucket_of(scaled(value_at(v), r.c))], 1u)] = v;
+      }
+      __syncthreads();  // a bucket's word is now its end, the one before it its start
+      for (uint32_t i = t; i < n; i += DRAW) {
+        const uint64_t v = s.place[1][i];
+        const uint32_t b = bucket_of(scaled(value_at(v), r.c)), o0 = b ? s.bucket[b - 1] : 0, o1 = s.bucket[b];
+        uint32_t rank = o0;
+        for (uint32_t o = o0; o < o1; o++) rank += s.place[1][o] < v;
+        s.place[0][rank] = v;
+      }
+      __syncthreads();
+      const uint32_t each = (n + DRAW - 1) / DRAW, i0 = t * each, i1 = min(i0 + each, n);
+      uint64_t sum = 0, sum_all;
+      for (uint32_t i = i0; i < i1; i++) raw[i] = sum += weight_of(s.place[0][i]);
+      const uint64_t before = block_scan(sum, s.words, sum_all) - sum;
+      for (uint32_t i = i0; i < i1; i++) raw[i] += before;
+      __syncthreads();
     }
-    __syncthreads();
     if (t >= 64) return;
     // (the first wave alone)
+    if (n <= 64) {
+      const uint64_t v = t < n ? s.place[0][t] : ~0ull;
+      uint32_t rank = 0;
+      for (uint32_t i = 0; i < n; i++) rank += s.place[0][i] < v;
+      if (t < n) s.place[0][rank] = v;
+      const uint64_t sum = wave_scan(t < n ? weight_of(s.place[0][t]) : 0);
+      if (t < n) raw[t] = sum;
+    }
     auto start_of = [&](uint32_t b) {  // in the order here
       return b >= f2 ? at2 + s.n[b] - s.n[f2] : b >= f1 ? at1 + s.n[b] - s.n[f1] : s.n[b] - s.n[f0];
     };
