@@ -245,19 +245,25 @@ constexpr uint32_t SPANS = 64;     // such bins
 constexpr uint32_t CHUNKS = 128;   // of a row
 constexpr uint32_t DIGITS = 2048;  // buckets of the search that takes any number of them
 
+// Where a row's borders lie: of bin b1 some tokens stay (BINS: all of all bins), as min_p has it if that is bm, as top_k
+// if bk; n2 ends in bins [p_lo, p_hi] and the draw falls into [d_lo, d_hi].
+struct Borders {
+  double least;  // min_p's t
+  uint32_t k, bm, bk, b1, p_lo, p_hi, d_lo, d_hi;
+};
 struct DrawShared {
   union {
-    uint64_t place[2][MOST];  // as they came, then by buckets; then in order
+    uint64_t place[2][MOST];  // as they came and then in order; by buckets, then the sums behind them, then C there
     struct {
       unsigned long long sum[DIGITS];
       uint32_t count[DIGITS];
     } digit;
-    struct {
-      uint64_t sum[DRAW];
-      uint32_t n[DRAW];
-      float largest[CHUNKS];
-    } half;
+    uint16_t ends[CHUNKS][BINS];  // of a chunk's tokens, those that end with a bin
   };
+  uint64_t half_sum[BINS];
+  uint32_t half_n[BINS];
+  float largest[CHUNKS];
+  uint32_t down[CHUNKS];  // how many bins below the row's a chunk's lie (BINS: that or more; ~0: it has none)
   double c[BINS + 1];     // C before a bin, in weights of the first bin's middle
   uint32_t n[BINS + 1];   // tokens before it
   double edge[BINS];      // its middle's weight
@@ -267,6 +273,8 @@ struct DrawShared {
   uint64_t words[DRAW_WAVES];
   uint32_t counts[DRAW_WAVES];
   unsigned long long below;
+  Borders at;
+  uint2 runs[3 * CHUNKS];  // of the chunks' lists, the tokens in each run of bins
   uint32_t fill, found[2];
 };
 
@@ -325,12 +333,12 @@ SK_DEV void each_value_of(const Row &r, uint32_t b, F f) {
 
 // The first bin b whose end satisfies ok(end), BINS if none does; ok is false, then true.  The same in every wave.
 template <typename A, typename F>
-SK_DEV uint32_t first_bin(const A *before, F ok) {
+SK_DEV uint32_t first_bin(const A *before, F ok) {  // (without branches: two of them go on side by side)
   const uint32_t lane = threadIdx.x & 63;
   const uint64_t m = __ballot(ok(before[8 * lane + 8]));
-  if (!m) return BINS;
-  const uint32_t b = 8 * (uint32_t)__builtin_ctzll(m);
-  return b + (uint32_t)__builtin_ctzll(__ballot(lane >= 7 || ok(before[b + lane % 8 + 1])));
+  const uint32_t b = 8 * (uint32_t)__builtin_ctzll(m | 1ull << 63);
+  const uint32_t e = b + (uint32_t)__builtin_ctzll(__ballot(lane >= 7 || ok(before[b + lane % 8 + 1])));
+  return m ? e : BINS;
 }
 
 template <typename T>
@@ -464,19 +472,24 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
   if (t < CHUNKS) {
     const float *part = parts + (size_t)min(t, n_chunks - 1) * PART;
     s.first[t] = *(const double *)part;
-    s.half.largest[t] = part[2];
+    s.largest[t] = part[2];
   }
   if (t < BINS) s.edge[t] = exp2(-0.125 * (double)t);
   s.bucket[t] = 0;
   if (t == 0) s.below = 0, s.fill = 0;
   __syncthreads();
-  const float top = wave_max(fmaxf(s.half.largest[t & 63], s.half.largest[64 + (t & 63)]));
+  const float top = wave_max(fmaxf(s.largest[t & 63], s.largest[64 + (t & 63)]));
   if (!has_weight(top)) {
     if (t == 0) *(uint4 *)out = make_uint4(~0u, 0, 0xff800000u, 0);
     return;
   }
   const double t_top = scaled(top, r.c);
   r.edge = __builtin_rint(t_top);
+  if (t < n_chunks) {
+    const double d = r.edge - s.first[t];
+    s.down[t] = d < BINS ? (uint32_t)(int)d : d < INFINITY ? BINS : ~0u;
+  }
+  __syncthreads();
 
   // the row's bins: thread t has bin t % BINS of every other chunk
   {
@@ -485,37 +498,39 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
     uint64_t sum = 0;
     constexpr uint32_t U = 10, STEP = DRAW / BINS;  // chunks whose loads are in flight
     for (uint32_t i0 = t / BINS; i0 < n_chunks; i0 += U * STEP) {
-      uint64_t w[U], below[U];
+      uint64_t w[U], low[U];
+      uint32_t downs[U];
 #pragma unroll
       for (uint32_t j = 0; j < U; j++) {
         const uint32_t i = min(i0 + j * STEP, n_chunks - 1);
-        const double d = r.edge - s.first[i];  // the chunk's bins lie so many below the row's
-        const uint32_t down = d < BINS ? (uint32_t)(int)d : BINS;
-        const bool any = i0 + j * STEP < n_chunks && s.first[i] > -INFINITY;
         const uint64_t *bins = (const uint64_t *)(parts + (size_t)i * PART + HEAD);
-        w[j] = any && b >= down && b < BINS - 1 ? bins[b - down] : 0;
-        below[j] = any && b + down >= BINS - 1 ? bins[b] : 0;  // of the chunk's bin b: it lies in the row's last
+        downs[j] = i0 + j * STEP < n_chunks ? s.down[i] : ~0u;
+        w[j] = bins[b >= downs[j] ? b - downs[j] : 0];
+        // the chunk's bin b, if it lies in the row's last
+        low[j] = downs[j] != ~0u && b + downs[j] >= BINS - 1 ? bins[b] : 0;
       }
 #pragma unroll
       for (uint32_t j = 0; j < U; j++) {
-        n += (uint32_t)(w[j] >> COUNT_AT);
-        sum += w[j] & SUM;
-        if (b == BINS - 1) n += (uint32_t)(below[j] >> COUNT_AT);  // (how many the chunk has)
-        if (below[j] & SUM) {  // in weights of that one's middle
-          const double d = r.edge - s.first[min(i0 + j * STEP, n_chunks - 1)];
-          const double by = exp2(((double)(BINS - 1) - (double)b - d) * 0.125);
-          atomicAdd(&s.below, (unsigned long long)__builtin_rint((double)(below[j] & SUM) * by));
+        const uint32_t i = i0 + j * STEP;
+        if (b < BINS - 1 && b >= downs[j]) {
+          const uint32_t end = (uint32_t)(w[j] >> COUNT_AT);
+          n += end;
+          sum += w[j] & SUM;
+          s.ends[i][b - downs[j]] = end;
+        }
+        if (b == BINS - 1) n += (uint32_t)(low[j] >> COUNT_AT);  // how many the chunk has
+        if (low[j] & SUM) {  // in weights of the last bin's middle
+          const double by = exp2(((double)(BINS - 1) - (double)b - (r.edge - s.first[i])) * 0.125);
+          atomicAdd(&s.below, (unsigned long long)__builtin_rint((double)(low[j] & SUM) * by));
         }
       }
     }
-    __syncthreads();  // (the chunks' largest values are read)
-    s.half.sum[t] = sum;
-    s.half.n[t] = n;
+    if (t >= BINS) s.half_sum[b] = sum, s.half_n[b] = n;
     __syncthreads();
     double c = 0.0, c_all;
     if (t < BINS) {
-      s.n[t + 1] = n + s.half.n[t + BINS];
-      sum += s.half.sum[t + BINS];
+      s.n[t + 1] = n + s.half_n[t];
+      sum += s.half_sum[t];
       c = sum_of(b == BINS - 1 ? s.below : sum, s.edge[b]);
     }
     c = block_scan(c, s.sums, c_all);
@@ -524,38 +539,45 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
     __syncthreads();
   }
 
-  // The bins with the borders.  What is known of C(n1) and C(n2) before these are looked at lies between lo and hi.
+  // The bins with the borders, by the first wave.  What is known of C(n1) and C(n2) before these are looked at lies
+  // between lo and hi.
   const uint32_t total = s.n[BINS];
-  const uint32_t k = !(T > 0.0f) || min_p > 1.0f ? 1 : words[3] && words[3] < total ? words[3] : total;
-  const double least = min_p > 0.0f ? t_top + 8.0 * log2(fmin((double)min_p, 1.0)) : -INFINITY;
-  const uint32_t bm = min_p > 0.0f ? bin_of(r, least) : BINS;
-  const uint32_t bk = k < total ? first_bin(s.n, [&](uint32_t n) { return n >= k; }) : BINS;
-  const uint32_t b1 = min(bm < BINS && s.n[bm] < total ? bm : BINS, bk);  // (BINS: all tokens stay)
-  constexpr double MORE = 1.0 + 1e-9, LESS = 1.0 - 1e-9;
-  double lo = s.c[BINS], hi = lo;
-  if (b1 < BINS) {
-    lo = s.c[b1], hi = s.c[b1 + 1];
-    if (b1 == bk) {
-      const double more = (double)(k - s.n[bk]) * s.edge[bk];
-      hi = fmin(hi, lo + more * UP);
-      if (bm != bk && bk < BINS - 1) lo += more * DOWN;
-    }
-    if (b1 == 0) lo = fmax(lo, DOWN * LESS);  // the largest stays
-  }
-  const uint32_t b_last = min(b1, first_bin(s.n, [&](uint32_t n) { return n >= total; }));  // where n1 lies, or past it
   const bool by_p = top_p < 1.0f;
-  const double share = fmax((double)top_p, 0.0);
-  uint32_t p_lo = b_last, p_hi = b_last;  // where n2 lies
-  if (by_p) {
-    lo *= share * LESS, hi *= share * MORE;
-    p_lo = min(first_bin(s.c, [&](double c) { return c >= lo; }), b_last);
-    p_hi = min(first_bin(s.c, [&](double c) { return c >= hi; }), b_last);
-    hi = fmin(s.c[p_hi + 1], hi + s.edge[p_lo] * UP);
-    lo = fmax(lo, DOWN * LESS);
+  const double share = fmax((double)top_p, 0.0), u = ((double)words[4] + 0.5) * 0x1p-32;
+  if (t < 64) {
+    const uint32_t k = !(T > 0.0f) || min_p > 1.0f ? 1 : words[3] && words[3] < total ? words[3] : total;
+    const double least = min_p > 0.0f ? t_top + 8.0 * log2(fmin((double)min_p, 1.0)) : -INFINITY;
+    const uint32_t bm = min_p > 0.0f ? bin_of(r, least) : BINS;
+    const uint32_t bk = k < total ? first_bin(s.n, [&](uint32_t n) { return n >= k; }) : BINS;
+    const uint32_t b1 = min(bm < BINS && s.n[bm] < total ? bm : BINS, bk);  // (BINS: all tokens stay)
+    constexpr double MORE = 1.0 + 1e-9, LESS = 1.0 - 1e-9;
+    double lo = s.c[BINS], hi = lo;
+    if (b1 < BINS) {
+      lo = s.c[b1], hi = s.c[b1 + 1];
+      if (b1 == bk) {
+        const double more = (double)(k - s.n[bk]) * s.edge[bk];
+        hi = fmin(hi, lo + more * UP);
+        if (bm != bk && bk < BINS - 1) lo += more * DOWN;
+      }
+      if (b1 == 0) lo = fmax(lo, DOWN * LESS);  // the largest stays
+    }
+    const uint32_t b_last = min(b1, first_bin(s.n, [&](uint32_t n) { return n >= total; }));  // where n1 lies, or past it
+    uint32_t p_lo = b_last, p_hi = b_last;  // where n2 lies
+    if (by_p) {
+      lo *= share * LESS, hi *= share * MORE;
+      p_lo = min(first_bin(s.c, [&](double c) { return c >= lo; }), b_last);
+      p_hi = min(first_bin(s.c, [&](double c) { return c >= hi; }), b_last);
+      hi = fmin(s.c[p_hi + 1], hi + s.edge[p_lo] * UP);
+      lo = fmax(lo, DOWN * LESS);
+    }
+    const uint32_t d_lo = min(first_bin(s.c, [&](double c) { return c > lo * u * LESS; }), p_hi);
+    const uint32_t d_hi = min(first_bin(s.c, [&](double c) { return c > hi * u * MORE; }), p_hi);
+    if (t == 0) s.at = {least, k, bm, bk, b1, p_lo, p_hi, d_lo, d_hi};
   }
-  const double u = ((double)words[4] + 0.5) * 0x1p-32;
-  const uint32_t d_lo = min(first_bin(s.c, [&](double c) { return c > lo * u * LESS; }), p_hi);
-  const uint32_t d_hi = min(first_bin(s.c, [&](double c) { return c > hi * u * MORE; }), p_hi);
+  __syncthreads();
+  const double least = s.at.least;
+  const uint32_t k = s.at.k, bm = s.at.bm, bk = s.at.bk, b1 = s.at.b1, p_lo = s.at.p_lo, p_hi = s.at.p_hi, d_lo = s.at.d_lo,
+                 d_hi = s.at.d_hi;
   // up to three runs of bins [f, e], each below the one before (one that is not there: f = ~0)
   uint32_t f0 = d_lo, e0 = d_hi, f1 = ~0u, e1 = 0, f2 = ~0u, e2 = 0;
   if (by_p) {
@@ -586,27 +608,30 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
       const uint32_t b = (uint32_t)(int)(r.edge - g), i = b >= f2 ? span2 + b - f2 : b >= f1 ? span1 + b - f1 : b - f0;
       return i * per + min((uint32_t)(int)(f * (double)per), per - 1);
     };
-    constexpr uint32_t LANES = 16, U = 4;  // of a chunk's run, each with so many loads in flight
-    for (uint32_t j = t / LANES; j < n_chunks * 3; j += DRAW / LANES) {
-      const uint32_t i = j % n_chunks, which = j / n_chunks, f = which == 0 ? f0 : which == 1 ? f1 : f2, e = which == 0 ? e0 : which == 1 ? e1 : e2;
+    // a chunk's run takes 16 lanes or more, each with U loads in flight
+    const uint32_t runs = 1 + (f1 != ~0u) + (f2 != ~0u), lanes = n_chunks * runs <= 16 ? 64 : n_chunks * runs <= 32 ? 32 : 16;
+    constexpr uint32_t U = 4;
+    if (t < n_chunks * runs) {
+      const uint32_t i = t % n_chunks, which = t / n_chunks;
+      const uint32_t f = which == 0 ? f0 : which == 1 && f1 != ~0u ? f1 : f2, e = which == 0 ? e0 : which == 1 && f1 != ~0u ? e1 : e2;
+      const uint32_t down = s.down[i];
+      s.runs[t] = down > e ? make_uint2(0, 0) : make_uint2(f > down ? s.ends[i][f - down - 1] : 0, s.ends[i][e - down]);
+    }
+    __syncthreads();
+    for (uint32_t j = t / lanes; j < n_chunks * runs; j += DRAW / lanes) {
+      const uint32_t i = j % n_chunks, i0 = s.runs[j].x, i1 = s.runs[j].y;
       const float *part = parts + (size_t)i * PART;
-      const double d = r.edge - s.first[i];
-      if (f == ~0u || !(d <= (double)e)) continue;
-      const uint32_t down = (uint32_t)(int)d;
-      const uint64_t *bins = (const uint64_t *)(part + HEAD);
-      const uint32_t i0 = f > down ? (uint32_t)(bins[f - down - 1] >> COUNT_AT) : 0,
-                     i1 = (uint32_t)(bins[e - down] >> COUNT_AT);
       const uint16_t *ids = (const uint16_t *)(part + HEAD + 2 * BINS);
-      for (uint32_t o = i0 + t % LANES; o < i1; o += U * LANES) {
+      for (uint32_t o = i0 + t % lanes; o < i1; o += U * lanes) {
         uint32_t id[U];
         float x[U];
 #pragma unroll
-        for (uint32_t u = 0; u < U; u++) id[u] = i * CHUNK + ids[min(o + u * LANES, i1 - 1)];
+        for (uint32_t u = 0; u < U; u++) id[u] = i * CHUNK + ids[min(o + u * lanes, i1 - 1)];
 #pragma unroll
         for (uint32_t u = 0; u < U; u++) x[u] = r.x[id[u]];
 #pragma unroll
         for (uint32_t u = 0; u < U; u++) {
-          if (o + u * LANES >= i1) break;
+          if (o + u * lanes >= i1) break;
           const uint32_t to = atomicAdd(&s.fill, 1u);
           if (to < MOST) s.place[0][to] = place(x[u], id[u]);  // (always: so many were counted)
           if (n > 64) atomicAdd(&s.bucket[bucket_of(scaled(x[u], r.c))], 1u);
@@ -615,8 +640,16 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
     }
     __syncthreads();
     const Series series_ = series();
-    uint64_t *raw = s.place[1];  // in the end, the sum behind each of those in order
+    uint64_t *raw = s.place[1];
+    double *upto = (double *)s.place[1];
     auto weight_of = [&](uint64_t v) { return fixed_weight(series_, r, scaled(value_at(v), r.c)); };
+    auto start_of = [&](uint32_t b) {  // bin b's first place in the order here
+      return b >= f2 ? at2 + s.n[b] - s.n[f2] : b >= f1 ? at1 + s.n[b] - s.n[f1] : s.n[b] - s.n[f0];
+    };
+    auto c_at = [&](uint32_t i) {  // from the sums
+      const uint32_t b = bin_of(r, scaled(value_at(s.place[0][i]), r.c)), i0 = start_of(b);
+      return s.c[b] + sum_of(raw[i] - (i0 ? raw[i0 - 1] : 0), s.edge[b]);
+    };
     if (n > 64) {
       uint32_t all;
       const uint32_t mine = s.bucket[t], end = block_scan(mine, s.counts, all);
@@ -641,6 +674,15 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
       const uint64_t before = block_scan(sum, s.words, sum_all) - sum;
       for (uint32_t i = i0; i < i1; i++) raw[i] += before;
       __syncthreads();
+      double c[MOST / DRAW];
+#pragma unroll
+      for (uint32_t j = 0; j < MOST / DRAW; j++)
+        if (t + j * DRAW < n) c[j] = c_at(t + j * DRAW);
+      __syncthreads();
+#pragma unroll
+      for (uint32_t j = 0; j < MOST / DRAW; j++)
+        if (t + j * DRAW < n) upto[t + j * DRAW] = c[j];
+      __syncthreads();
     }
     if (t >= 64) return;
     // (the first wave alone)
@@ -651,14 +693,13 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
       if (t < n) s.place[0][rank] = v;
       const uint64_t sum = wave_scan(t < n ? weight_of(s.place[0][t]) : 0);
       if (t < n) raw[t] = sum;
+      const double c = t < n ? c_at(t) : 0.0;
+      if (t < n) upto[t] = c;
     }
-    auto start_of = [&](uint32_t b) {  // in the order here
-      return b >= f2 ? at2 + s.n[b] - s.n[f2] : b >= f1 ? at1 + s.n[b] - s.n[f1] : s.n[b] - s.n[f0];
-    };
+    // the token at place i of the order here (within a run of bins places and ranks go together)
     auto found_at = [&](uint32_t i) {
-      const double v = scaled(value_at(s.place[0][i]), r.c);
-      const uint32_t b = bin_of(r, v), i0 = start_of(b);
-      return Found{s.place[0][i], s.n[b] + i - i0 + 1, s.c[b] + sum_of(raw[i] - (i0 ? raw[i0 - 1] : 0), s.edge[b])};
+      const uint32_t rank = i >= at2 && f2 != ~0u ? s.n[f2] + i - at2 : i >= at1 && f1 != ~0u ? s.n[f1] + i - at1 : s.n[f0] + i;
+      return Found{s.place[0][i], rank + 1, upto[i]};
     };
     // n1: of bin b1 those that stay
     Found n1{0, total, s.c[BINS]};
@@ -672,7 +713,7 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
     // the first token of bins [f, e], not past the n-th, that meets `want`; the last of these if none does
     auto first = [&](Want want, double goal, uint32_t most, uint32_t f, uint32_t e) {
       const uint32_t i0 = start_of(f), end = max(min(s.n[e + 1], most), s.n[f]) - s.n[f];
-      const uint32_t i = first_of(end, [&](uint32_t i) { return meets(want, goal, 0, found_at(i0 + i).sum); });
+      const uint32_t i = first_of(end, [&](uint32_t i) { return want == kReach ? upto[i0 + i] >= goal : upto[i0 + i] > goal; });
       return found_at(min(i0 + (i < end ? i : max(end, 1u) - 1), n - 1));
     };
     n2 = by_p ? first(kReach, share * n1.sum, n1.n, p_lo, p_hi) : n1;
