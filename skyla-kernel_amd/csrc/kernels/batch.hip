@@ -110,15 +110,17 @@ SK_DEV Range row_range(const uint32_t *ctl, uint32_t rows_off, uint32_t row, uin
 // spans_off + 2 r; their positions are in the cache when the kernel runs).  A row of len 0, or whose mask leaves
 // nothing, gives zeros.  With s = scale q k a score is cap tanh(s / cap) (cap 0: s), less slope_h |i - j| (the
 // heads' slopes at slopes_off; ~0: none).
-// The shared run is [S, P), S the tile's end at or above ctl[5] (the shared kernels' mask is the run itself: no row
-// attends to a part of it): a row takes it with share != 0 and len >= P if it attends to all of it, lo <= S.  Its
-// own pages serve [lo, S), its lead, in n_lead parts (without lead parts lo must be S), and those from P on.
+// The shared run is [S, P), S the tile's end at or above ctl[5], and with a window at or above ctl[6] - window, ctl[6]
+// the longest of the rows (0: ctl[5] alone; layers of one step may have windows of their own).  No row attends to a
+// part of it: a row takes it with share != 0 and len >= P if it attends to all of it, lo <= S.  Its own pages serve
+// [lo, S), its lead, in n_lead parts (without lead parts lo must be S), and those from P on.
 struct ShapedRange : Range {  // tail: [start, len), len the end hi
   uint32_t lo, at;            // lead: [lo, S) of a member; the position i
 };
 template <typename P>
 SK_DEV uint32_t shared_first(const uint32_t *ctl, const P &p, uint32_t shared) {
-  const uint32_t first = min(ctl[5], shared);
+  const uint32_t longest = ctl[6], window = p.window && longest > p.window ? longest - p.window : 0;
+  const uint32_t first = min(max(ctl[5], window), shared);
   return (first + TILE - 1) / TILE * TILE;
 }
 template <typename P>

@@ -145,7 +145,7 @@ inline std::string refusal(Op op, const uint32_t *spec, const uint32_t *w, const
   };
   const Binding A = bound(append), C = bound(append ? 2 : 1);  // arena, control words
   const bool shaped = op == kShaped || op == kShapedMerge;
-  const Region ctl{"the control words", C, 4, 0, 0, shaped ? 6u : 5u, 1};
+  const Region ctl{"the control words", C, 4, 0, 0, shaped ? 7u : 5u, 1};
   c.holds(ctl, 1);
   if (append) {
     const uint64_t n_head = w[9], n_kv = w[10], kv_dim = n_kv * kHead;

@@ -29,8 +29,10 @@ from .abi import Buffer, Context, Recorder
 
 MAX_PARTS = 1024        # partials of a row and head (runtime/batch.h)
 PAGE_SIZES = tuple(16 << i for i in range(9))  # 16 to 4096 positions
-# control words: live rows, shared positions, their sequence, the first of them (attention_paged_shaped)
-CTL_ROWS, CTL_SHARED, CTL_LEADER, CTL_FIRST = 2, 3, 4, 5
+# control words: live rows, shared positions, their sequence, and for attention_paged_shaped the first of them and the
+# longest row's length
+CTL_ROWS, CTL_SHARED, CTL_LEADER, CTL_FIRST, CTL_LONGEST = 2, 3, 4, 5, 6
+MIN_CAP, MAX_CAP = 2.0**-10, 2.0**14           # of scores (runtime/batch.h)
 
 
 class Paged:
@@ -313,15 +315,36 @@ class Controls:
         return self.repetition != 1.0 or self.frequency != 0.0 or self.presence != 0.0
 
 
+@dataclasses.dataclass
+class Sampling:
+    """How a sequence's tokens are drawn (logits_sample): at a temperature (0: the likeliest token), among the
+    top_k likeliest (0: any number of them), those at least min_p as likely as the likeliest, and the likeliest
+    that make up top_p of these."""
+    temperature: float = 1.0
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+
+
+class Drawn(NamedTuple):
+    """A step's tokens, a row each (-1: its controls leave none), the log probabilities that they were drawn
+    with, and among how many tokens."""
+    token: np.ndarray
+    logprob: np.ndarray
+    kept: np.ndarray
+
+
 class _Sequence:
     """A sequence's pages, the tokens of its prompts and those that it generated (a conversation's
     follow in turns; what acts on the logits asks only which), its controls, the row of the batch
     that these lie in (None: they do not), how many words of its history, the prompts' tokens before
-    the others, lie there, and whether its controls do not yet."""
+    the others, lie there, whether its controls do not yet, how its tokens are drawn, and how far the
+    rotation's positions of further text are past the cache's (behind images, mostly below 0)."""
 
-    def __init__(self, pages=(), prompt=(), made=(), controls=None):
+    def __init__(self, pages=(), prompt=(), made=(), controls=None, sampling=None, shift=0):
         self.pages, self.prompt, self.made = list(pages), list(prompt), list(made)
         self.controls, self.row, self.placed, self.stale = controls or Controls(), None, 0, True
+        self.sampling, self.shift = sampling or Sampling(), shift
 
     def __len__(self):
         return len(self.prompt) + len(self.made)
@@ -341,29 +364,40 @@ class _Sequence:
 
 
 class _BatchGraph(E.Graph):
-    """A layer's dispatches with the batch's cache in place of the contiguous one."""
+    """A layer's dispatches with the batch's cache in place of the contiguous one; `parts` by the layers'
+    windows where scores are shaped."""
 
-    def __init__(self, r: Recorder, eng: "BatchEngine", batched: bool, rows: int, parts: Parts):
+    def __init__(self, r: Recorder, eng: "BatchEngine", batched: bool, rows: int, parts):
         super().__init__(r, eng.kernels, eng.arena, eng.c, batched)
         self.eng, self.rows, self.parts = eng, rows, parts
 
     def qk_rope(self, l: int, q_norm: int, k_norm: int, rope: int) -> None:
-        a = self.a
+        a, e = self.a, self.eng
         q = (a.q, a.s_q)
-        self.eng.batch.append(self.r, l, self.eng.at, q, (a.k, a.s_kv), a.v, q, q_norm, k_norm, rope, self.rows,
-                              self.c.rope_mscale)
+        if e.n_axes:
+            e.batch.append_axes(self.r, l, e.at, q, (a.k, a.s_kv), a.v, q, q_norm, k_norm, e.weights.rope_axes, e.n_axes,
+                                self.rows, self.c.rope_mscale)
+        else:
+            e.batch.append(self.r, l, e.at, q, (a.k, a.s_kv), a.v, q, q_norm, k_norm, rope, self.rows, self.c.rope_mscale)
         self.stage("kv append")
 
     def attend(self, l: int) -> None:
-        a = self.a
-        self.eng.batch.attend(self.r, l, self.eng.at, (a.q, a.s_q), (a.attn, a.s_attn), self.rows, self.parts)
+        a, e = self.a, self.eng
+        q, out = (a.q, a.s_q), (a.attn, a.s_attn)
+        if isinstance(self.parts, Parts):
+            e.batch.attend(self.r, l, e.at, q, out, self.rows, self.parts)
+        else:
+            window = e.window(l)
+            shape = Shape(self.c.score_cap, window, e.slopes)
+            e.batch.attend_shaped(self.r, l, e.at, q, out, self.rows, dict(self.parts)[window], shape)
         self.stage("attention")
 
 
 class BatchEngine:
     """Up to BATCH sequences of one model, decoded together.  A sequence is a number from open() or
     fork(); extend() puts tokens into its cache, step() takes a token of each of several sequences
-    and returns the logits after them, with their controls applied; close() gives its pages back.
+    and returns the logits after them, with their controls applied, sample() the tokens drawn from
+    these; close() gives its pages back.
 
     A forked sequence shares the whole pages of the one it came from (the rest of the last page is
     copied), and a step reads the pages that its sequences share once for all of them.  A step has a
@@ -380,6 +414,7 @@ class BatchEngine:
         if max_ctx < 1:
             raise ValueError(f"max_ctx {max_ctx}")
         BatchKernels.check(c)
+        self._check_shape(c)
         self.ctx, self.c, self.max_ctx, self.max_seq = ctx, c, max_ctx, max_seq
         self.paged = Paged(precision, page, n_pages, max_seq, min(-(-max_ctx // page), n_pages),
                            c.n_head_kv * c.head_dim)
@@ -389,8 +424,13 @@ class BatchEngine:
         self.rep = c.n_head // c.n_head_kv
         self.s_vocab, self.s_mask = E._next64(c.n_vocab), -(-c.n_vocab // 32)
         self.s_hist = -(-max_ctx // 4) * 4
-        part = max(part_size(r, c.n_head, self._parts(r, shared, own)) for r in self._buckets(E.BATCH)
-                   for shared in [0, *self._buckets(max_ctx)] for own in self._buckets(max_ctx))
+        self.n_axes = max(c.axes) + 1 if c.axes is not None else 0
+        self.windows = sorted(set(c.windows or [0]))
+        part = max(max(part_size(r, c.n_head, self._parts(r, shared, own)),
+                       *(shaped_part_size(r, c.n_head, p) for lead in (False, True)
+                         for _, p in self._shaped_parts(r, shared, own, lead)))
+                   for r in self._buckets(E.BATCH) for shared in [0, *self._buckets(max_ctx)]
+                   for own in self._buckets(max_ctx))
         self.weights = self.arena = self.batch = self.logits = None
         self.pools, self.recordings = [], {}
         try:
@@ -409,17 +449,41 @@ class BatchEngine:
         a = self.arena = E.Arena(ctx, c, extra={
             "rows": 4 * E.BATCH, "table": max_seq * self.paged.seq_pages, "part": part,
             "logits": self.s_vocab * max_seq, "controls": 8 * max_seq, "history": self.s_hist * max_seq,
-            "bias": 2 * self.MAX_BIASES * max_seq, "mask": self.s_mask * max_seq})
+            "bias": 2 * self.MAX_BIASES * max_seq, "mask": self.s_mask * max_seq,
+            "axes": 4 * E.BATCH, "spans": 2 * E.BATCH, "slopes": c.n_head, "sampling": 8 * max_seq,
+            "drawn": 4 * max_seq, "sample": sample_size(max_seq, c.n_vocab)})
         x = a.extra
         for _ in range(c.n_layer):
             self.pools.append(ctx.alloc_host(self.paged.bytes()))
-        self.at = BatchRegions(rows=x["rows"], table=x["table"], part=x["part"])
+        self.at = BatchRegions(rows=x["rows"], table=x["table"], part=x["part"], axes=x["axes"], spans=x["spans"])
+        self.sample_at = SampleRegions(controls=x["sampling"], out=x["drawn"], part=x["sample"])
+        self.slopes = None
+        if c.slopes is not None:
+            self.slopes = x["slopes"]
+            a.f32()[self.slopes: self.slopes + c.n_head] = c.slopes
+            a.buffer.upload(self.slopes * 4, c.n_head * 4)
         self.logits_at = LogitsRegions(x["controls"], x["history"], self.s_hist, x["bias"], 2 * self.MAX_BIASES,
                                        x["mask"], self.s_mask)
         self.kernels = E.Kernels(ctx, self.weights.buffers, a.buffer, kv=self.pools[0], c=c, precision=precision,
                                  embd_dtype=self.weights.embd.dtype)
         self.batch = BatchKernels(ctx, self.weights.buffers[0], a.buffer, self.pools, c, self.paged)
         self.logits = LogitsKernels(ctx, a.buffer)
+
+    @staticmethod
+    def _check_shape(c: E.Config) -> None:
+        if c.n_vocab > SAMPLE_VOCAB:
+            raise ValueError(f"a vocabulary of {c.n_vocab} tokens: at most {SAMPLE_VOCAB}")
+        if c.axes is not None and (len(c.axes) != c.head_dim // 2 or any(a not in (0, 1, 2, 3) for a in c.axes)):
+            raise ValueError(f"axes: one of 0 to 3 for each of {c.head_dim // 2} pairs")
+        if c.score_cap != 0 and not MIN_CAP <= c.score_cap <= MAX_CAP:
+            raise ValueError(f"scores capped at {c.score_cap}: {MIN_CAP} to {MAX_CAP}, or 0")
+        if c.windows is not None and (len(c.windows) != c.n_layer or any(not 0 <= w < 2**32 for w in c.windows)):
+            raise ValueError(f"windows: a number of positions for each of {c.n_layer} layers (0: all)")
+        if c.slopes is not None and (len(c.slopes) != c.n_head or not np.isfinite(np.float32(c.slopes)).all()):
+            raise ValueError(f"slopes: a number for each of {c.n_head} heads")
+
+    def window(self, layer: int) -> int:
+        return self.c.windows[layer] if self.c.windows is not None else 0
 
     # ---- sequences ----
     def open(self) -> int:
@@ -455,7 +519,7 @@ class BatchEngine:
             self._give(own)
             raise
         self.uses[s.pages[:whole]] += 1
-        n = self._add(_Sequence(s.pages[:whole] + own, s.prompt, s.made, s.controls))
+        n = self._add(_Sequence(s.pages[:whole] + own, s.prompt, s.made, s.controls, s.sampling, s.shift))
         self._upload_table(n)
         return n
 
@@ -486,6 +550,17 @@ class BatchEngine:
             allowed = np.array(allowed, bool)
         s.controls = Controls(*(float(v) for v in penalties), bias, allowed)
         s.stale = True
+
+    def sampling(self, seq: int, sampling: Sampling) -> None:
+        """Sets how a sequence's tokens are drawn from its next sample() on: `sampling` as it is now."""
+        s = self._get(seq)
+        with np.errstate(over="ignore", under="ignore"):
+            t, p, m = (float(np.float32(v)) for v in (sampling.temperature, sampling.top_p, sampling.min_p))
+        if not 0 <= t < np.inf or not 0 < p <= 1 or not 0 <= m <= 1:
+            raise ValueError("a temperature of 0 or more, top_p in (0, 1] and min_p in [0, 1], in 32 bits")
+        if not 0 <= sampling.top_k < 2**32:
+            raise ValueError("top_k: a number of tokens (0: any)")
+        s.sampling = Sampling(t, int(sampling.top_k), p, m)
 
     # ---- pages ----
     def _take(self, n: int) -> list[int]:
@@ -591,15 +666,22 @@ class BatchEngine:
             u[mask: mask + self.s_mask] = np.packbits(bits, bitorder="little").view("<u4")
             a.buffer.upload(mask * 4, self.s_mask * 4)
 
-    def _words(self, live: int, rows: np.ndarray, tokens: Sequence[int], shared: int, leader: int) -> None:
+    def _words(self, live: int, rows: np.ndarray, tokens: Sequence[int], shared: int, leader: int, axes=None,
+               spans=None, first: int = 0) -> None:
         a = self.arena
         u, n = a.u32(), len(rows)
         u[a.tokens: a.tokens + n] = tokens
         u[self.at.rows: self.at.rows + 4 * n] = rows.ravel()
-        u[0], u[1], u[2], u[3], u[4] = int(tokens[0]), 0, live, shared, leader
+        u[0], u[1], u[2], u[3], u[4], u[5], u[6] = int(tokens[0]), 0, live, shared, leader, first, rows[:, 1].max()
         a.buffer.upload(0, 64 * 4)
         a.buffer.upload(a.tokens * 4, n * 4)
         a.buffer.upload(self.at.rows * 4, n * 16)
+        if spans is not None or self.c.shapes_scores:
+            u[self.at.spans: self.at.spans + 2 * n] = np.broadcast_to(spans or (0, 0), (n, 2)).ravel()
+            a.buffer.upload(self.at.spans * 4, n * 8)
+        if self.n_axes:
+            u[self.at.axes: self.at.axes + 4 * n] = np.broadcast_to(axes, (n, 4)).ravel()
+            a.buffer.upload(self.at.axes * 4, n * 16)
 
     def _check(self, tokens) -> list[int]:
         tokens = [int(t) for t in tokens]
@@ -618,21 +700,36 @@ class BatchEngine:
     def _parts(self, rows: int, shared: int, own: int) -> Parts:
         return splits(rows, self.c.n_head_kv, self.rep, shared, own)
 
-    def _recording(self, rows: int, shared: int, own: int, head: bool):
+    def _shaped_parts(self, rows: int, shared: int, own: int, lead: bool) -> tuple:
+        """((window, its layers' parts), ...): a window leaves that much of the shared run at most, and of a row that
+        does not take the run; rows' leads are as long as the rows' lengths differ, or end a tile."""
+        def parts(w):
+            run, alone = (min(shared, w), min(shared + own, w)) if w else (shared, own)
+            return shaped_splits(rows, self.c.n_head_kv, self.rep, run, max(alone, 1), max(own, 64) if w or lead else 0)
+        return tuple((w, parts(w)) for w in self.windows)
+
+    def _recording(self, rows: int, shared: int, own: int, head: bool, shaped: bool = False, lead: bool = False,
+                   sample: bool = False, vectors: bool = False):
         """The recording for up to `rows` rows over `shared` shared and `own` positions of their own,
-        with the output head and the logits' controls or without (extend)."""
+        with the output head and the logits' controls or without (extend); with shaped scores or spans, some of
+        which start inside a tile (lead); with tokens drawn; of rows given as vectors."""
         up = lambda n, most: next(b for b in self._buckets(most) if b >= n)  # noqa: E731
         rows = up(rows, E.BATCH)
-        parts = self._parts(rows, up(shared, self.max_ctx) if shared else 0, up(own, self.max_ctx))
-        key = rows, parts, head
+        shared, own = up(shared, self.max_ctx) if shared else 0, up(own, self.max_ctx)
+        if shaped or self.c.shapes_scores:
+            parts = self._shaped_parts(rows, shared, own, lead)
+        else:
+            parts = self._parts(rows, shared, own)
+        key = rows, parts, head, sample, vectors
         if key not in self.recordings:
-            self.recordings[key] = self.ctx.record(False, lambda r: self._record(r, rows, parts, head))
+            self.recordings[key] = self.ctx.record(False, lambda r: self._record(r, rows, parts, head, sample, vectors))
         return self.recordings[key]
 
-    def _record(self, r: Recorder, rows: int, parts: Parts, head: bool) -> None:
+    def _record(self, r: Recorder, rows: int, parts, head: bool, sample: bool = False, vectors: bool = False) -> None:
         a, w, c, batched = self.arena, self.weights, self.c, rows > 1
         g = _BatchGraph(r, self, batched, rows, parts)
-        g.embed(w.embd)
+        if not vectors:
+            g.embed(w.embd)
         for l, lw in enumerate(w.layers):
             g.layer(l, lw, w.rope)
         if head:
@@ -642,26 +739,64 @@ class BatchEngine:
             g.matvec(w.output, (a.n, a.s_embd), y, False, batched)
             g.stage("matvec output")
             self.logits.adjust(r, self.logits_at, y, y, c.n_vocab, min(rows, self.max_seq))
+            if sample:
+                r.barrier()
+                self.logits.sample(r, self.sample_at, y, c.n_vocab, min(rows, self.max_seq))
         r.host_barrier()
 
     # ---- decoding ----
-    def extend(self, seq: int, tokens) -> None:
+    def extend(self, seq: int, tokens, axes=None, vectors=None, since: int = 0, together: bool = False) -> None:
         """Puts tokens into a sequence's cache, as its prompt or a further turn's, BATCH of them at a
-        time.  What it generated before counts as generated still."""
+        time.  What it generated before counts as generated still.
+
+        axes: the tokens' positions for the rotation, a row each and a column for each of the model's axes, as an
+        image's patches or a video's have them; without, they follow one another as text, which goes on behind the
+        largest so far.  vectors: rows of n_embd numbers in place of the tokens' own (an image's; the tokens then
+        are what the history says of them).  since: the first position that the tokens attend to, as where a document
+        of its own begins.  together: the tokens, BATCH at most, attend to one another, later ones too."""
         s, tokens = self._get(seq), self._check(tokens)
-        self._room({seq: len(tokens)})
+        n_all = len(tokens)
+        if axes is not None:
+            axes = np.asarray(axes)
+            if not self.n_axes:
+                raise ValueError("axes: the model's rotation has one position")
+            if axes.shape != (n_all, self.n_axes) or (n_all and (axes.dtype.kind not in "iu" or axes.min() < 0 or
+                                                                 axes.max() >= 2**31)):
+                raise ValueError(f"axes: {n_all} rows of {self.n_axes} positions")
+            axes = np.concatenate([axes.astype(np.int64), np.zeros((n_all, 4 - self.n_axes), np.int64)], 1)
+        if vectors is not None:
+            vectors = np.asarray(vectors, np.float32)
+            if vectors.shape != (n_all, self.c.n_embd):
+                raise ValueError(f"vectors: {n_all} rows of {self.c.n_embd} numbers")
+        if not 0 <= since <= len(s):
+            raise ValueError(f"since: a position of the sequence or its end (0 to {len(s)})")
+        if together and n_all > E.BATCH:
+            raise ValueError(f"together: at most {E.BATCH} tokens see one another")
+        self._room({seq: n_all})
+        shaped = since > 0 or together
         try:
-            for i in range(0, len(tokens), E.BATCH):
+            for i in range(0, n_all, E.BATCH):
                 chunk, pos = tokens[i: i + E.BATCH], len(s)
                 n = len(chunk)
                 rows = np.zeros((n, 4), np.uint32)
                 rows[:, 0], rows[:, 1], rows[:, 2] = seq, pos + 1 + np.arange(n), pos
-                self._words(n, rows, chunk, pos, seq)
-                self.ctx.replay(self._recording(n, pos, n, False))
+                turn = axes[i: i + n] if axes is not None else (pos + s.shift + np.arange(n))[:, None]
+                if vectors is not None:
+                    self._upload_vectors(vectors[i: i + n])
+                spans = (since, pos + n if together else 0) if shaped else None
+                self._words(n, rows, chunk, pos, seq, turn, spans, since)
+                self.ctx.replay(self._recording(n, pos, n, False, shaped, since > 0, vectors=vectors is not None))
                 s.add(chunk, True)
+                if axes is not None:
+                    s.shift = max(int(turn.max()) + 1, pos + s.shift) - len(s)
         except BaseException:  # what was decoded stays
             self._trim(seq)
             raise
+
+    def _upload_vectors(self, vectors: np.ndarray) -> None:
+        a, (n, width) = self.arena, vectors.shape
+        a.f32()[a.x: a.x + n * a.s_embd].reshape(n, a.s_embd)[:, :width] = vectors
+        a.buffer.upload(a.x * 4, n * a.s_embd * 4)
 
     def shared_run(self, seqs) -> tuple[int, list[int]]:
         """The positions that sequences of a step read once for all: (how many, whose).  Of the
@@ -684,6 +819,33 @@ class BatchEngine:
         """One token of each of several sequences ({sequence: token}): the logits after them, a row
         each in the order given.  `prompt`: sequences whose token is a prompt's (the others' count as
         generated)."""
+        seqs = self._step(tokens, prompt)
+        a, v = self.arena, self.c.n_vocab
+        out = np.empty((len(seqs), v), np.float32)
+        for i, q in enumerate(seqs):
+            off = a.extra["logits"] + self._get(q).row * self.s_vocab
+            a.buffer.download(off * 4, v * 4)
+            out[i] = a.f32()[off: off + v]
+        return out
+
+    def sample(self, tokens: dict, draws: dict, prompt=()) -> Drawn:
+        """step(), but the tokens that come next, each drawn as its sequence's sampling has it from the logits after
+        its controls, by its random number draws[sequence], an integer of 32 bits: the same number draws the same
+        token, whatever else is in the batch."""
+        if set(draws) != set(tokens):
+            raise ValueError("draws: a random number for each sequence of this step")
+        draws = {q: int(d) for q, d in draws.items()}
+        if any(not 0 <= d < 2**32 for d in draws.values()):
+            raise ValueError("draws: integers of 32 bits")
+        seqs = self._step(tokens, prompt, draws)
+        a, off, live = self.arena, self.sample_at.out, len(seqs)
+        a.buffer.download(off * 4, live * 16)
+        order = [self._get(q).row for q in seqs]
+        out = a.u32()[off: off + 4 * live].reshape(live, 4)[order].copy()
+        return Drawn(out[:, 0].astype(np.int32).astype(np.int64), out[:, 2].copy().view(np.float32), out[:, 1].astype(np.int64))
+
+    def _step(self, tokens: dict, prompt, draws: dict | None = None) -> list[int]:
+        """Decodes one token of each sequence; the sequences."""
         if not tokens:
             raise ValueError("step needs a token of at least one sequence")
         values, seqs, prompt = self._check(tokens.values()), list(tokens), set(prompt)
@@ -693,35 +855,33 @@ class BatchEngine:
         for q, t in zip(seqs, values):
             self._get(q).add([t], q in prompt)
         try:
-            self._replay_step(seqs, values)
+            self._replay_step(seqs, values, draws)
         except BaseException:  # nothing was decoded: the sequences are as they were
             for q in seqs:
                 self._get(q).drop(1, q in prompt)
                 self._trim(q)
             raise
-        a, v = self.arena, self.c.n_vocab
-        out = np.empty((len(seqs), v), np.float32)
-        for i, q in enumerate(seqs):
-            off = a.extra["logits"] + self._get(q).row * self.s_vocab
-            a.buffer.download(off * 4, v * 4)
-            out[i] = a.f32()[off: off + v]
-        return out
+        return seqs
 
-    def _replay_step(self, seqs: list[int], values: list[int]) -> None:
+    def _replay_step(self, seqs: list[int], values: list[int], draws: dict | None) -> None:
         """One row for each of the sequences' last tokens, through the model and its head."""
         self._place(seqs)
         live = len(seqs)
         shared, members = self.shared_run(seqs)
         rows, ids, own = np.zeros((live, 4), np.uint32), np.zeros(live, np.uint32), 1
+        turn = np.zeros((live, 1), np.int64)
         for q, t in zip(seqs, values):
             s = self._get(q)
             n, take = len(s), shared if q in members and len(s) >= shared else 0
             rows[s.row], ids[s.row], own = (q, n, take, 0), t, max(own, n - take)
+            turn[s.row] = n - 1 + s.shift
             if s.controls.counts:
                 self._upload_history(q)
-        self._words(live, rows, ids, shared, members[0] if members else 0)
+        self._words(live, rows, ids, shared, members[0] if members else 0, turn)
         self._control_words(live)
-        self.ctx.replay(self._recording(live, shared, own, True))
+        if draws is not None:
+            self._sampling_words(live, draws)
+        self.ctx.replay(self._recording(live, shared, own, True, sample=draws is not None))
 
     def _control_words(self, live: int) -> None:
         a, off = self.arena, self.logits_at.controls
@@ -731,6 +891,15 @@ class BatchEngine:
             k = s.controls
             u[o: o + 4] = len(s), len(s.prompt), len(k.bias), k.allowed is not None
             f[o + 4: o + 7] = k.repetition, k.frequency, k.presence
+        a.buffer.upload(off * 4, live * 32)
+
+    def _sampling_words(self, live: int, draws: dict) -> None:
+        a, off = self.arena, self.sample_at.controls
+        u, f = a.u32(), a.f32()
+        for r in range(live):
+            k, o = self._get(self.rows[r]).sampling, off + 8 * r
+            f[o: o + 3] = k.temperature, k.top_p, k.min_p
+            u[o + 3: o + 8] = k.top_k, draws[self.rows[r]], 0, 0, 0
         a.buffer.upload(off * 4, live * 32)
 
     def free(self) -> None:

@@ -341,11 +341,23 @@ class Config:
     rope_theta: float = 1e6
     # YaRN (rope.rs:7-31): (factor, original context length, attn_factor), or None
     rope_scaling: tuple | None = None
+    # What BatchEngine serves beyond the reference's models: the axis (0 to 3: time, height, width, ...) whose position
+    # turns each of the head_dim / 2 pairs (None: one position turns all); scores capped at score_cap by a tanh (0: not);
+    # each layer's window of positions (0: all; None: all layers see all); each head's loss of score a position of
+    # distance (None: none)
+    axes: tuple | None = None
+    score_cap: float = 0.0
+    windows: tuple | None = None
+    slopes: tuple | None = None
 
     @property
     def rope_mscale(self) -> float:
         """rope.rs:56: the magnitude YaRN puts on every rotated pair (1 without scaling)."""
         return rope_table(self)[1]
+
+    @property
+    def shapes_scores(self) -> bool:
+        return self.score_cap != 0.0 or bool(self.windows and any(self.windows)) or self.slopes is not None
 
 
 _libm = None
@@ -398,6 +410,12 @@ def rope_table(c: Config) -> tuple[np.ndarray, float]:
         out.append(f32(f * f32(f32(freq_scale * f32(f32(1.0) - mix)) + mix)))
     mscale = f32(attn_factor * f32(f32(1.0) + f32(f32(0.1) * f32(_libm_f32("logf")(f32(f32(1.0) / freq_scale))))))
     return np.asarray(out, np.float32), float(mscale)
+
+
+def rope_axes_table(c: Config) -> np.ndarray:
+    """[axes][head_dim / 2]: each pair's frequency at the axis that turns it, 0 at the others."""
+    f, axis = rope_frequencies(c), np.asarray(c.axes)
+    return np.where(axis == np.arange(axis.max() + 1)[:, None], f, np.float32(0.0))
 
 
 def rope_frequencies(c: Config) -> np.ndarray:
@@ -880,6 +898,7 @@ class Weights:
     out_norm: int
     rope: int
     layers: list
+    rope_axes: int = 0  # rope_axes_table's, of a model with axes
 
 
 def load_weights(ctx: Context, model: dict, c: Config) -> Weights:
@@ -899,6 +918,8 @@ def load_weights(ctx: Context, model: dict, c: Config) -> Weights:
                       p.table(model[n("attn_q_norm")]), p.table(model[n("attn_k_norm")]),
                       p.table(model[n("ffn_gate_inp")]) if moe else None))
 
+    rope_axes = p.table(rope_axes_table(c)) if c.axes is not None else 0
+
     def mat(name):  # expert tensors hold n_expert matrices of n_out rows (QMatrix.n_out per expert)
         t = model[name]
         return p.matrix(t[0], t[1], t[2], t[3])
@@ -912,7 +933,7 @@ def load_weights(ctx: Context, model: dict, c: Config) -> Weights:
         at = AttnWeights(q_norm, k_norm, mat(n("attn_q")), mat(n("attn_k")), mat(n("attn_v")), mat(n("attn_output")))
         gate, up, down = (mat(n(ffn(s))) for s in ("ffn_gate", "ffn_up", "ffn_down"))
         layers.append(LayerWeights(attn_norm, ffn_norm, at, gate, up, down, router))
-    return Weights(upload_weights(ctx, p), output, embd, out_norm, rope, layers)
+    return Weights(upload_weights(ctx, p), output, embd, out_norm, rope, layers, rope_axes)
 
 
 # ---- graph.rs::record, engine.rs ---------------------------------------------------------
@@ -960,6 +981,8 @@ class Engine:
         others, the head unfused; "none" keeps graph.rs's launches.  Measured on MI355X
         (tok/s, qkv / ffn / all): config 5 (Qwen3-8B Q4_K_M) at 1k context 495 / 513 / 474,
         at 16k 382 / 394 / 371; config 1 (Qwen3-0.6B Q8_0, no pair form) 890 / 886 / 970."""
+        if c.shapes_scores:
+            raise ValueError("capped, windowed or biased scores: batch.BatchEngine serves such models")
         self.ctx, self.c = ctx, c
         self.weights = load_weights(ctx, model, c)
         self.arena = Arena(ctx, c, max_ctx, precision)
