@@ -109,7 +109,8 @@ SK_DEV Range row_range(const uint32_t *ctl, uint32_t rows_off, uint32_t row, uin
 // `from`, and with a window from len - window on, up to len, or to `until` where that is more ({from, until} at
 // spans_off + 2 r; their positions are in the cache when the kernel runs).  A row of len 0, or whose mask leaves
 // nothing, gives zeros.  With s = scale q k a score is cap tanh(s / cap) (cap 0: s), less slope_h |i - j| (the
-// heads' slopes at slopes_off; ~0: none).
+// heads' slopes at slopes_off, of 2^16 at most; ~0: none).  A row that attends to a NaN or an infinity may be not finite
+// in all of a head's dims.
 // The shared run is [S, P), S the tile's end at or above ctl[5], and with a window at or above ctl[6] - window, ctl[6]
 // the longest of the rows (0: ctl[5] alone; layers of one step may have windows of their own).  No row attends to a
 // part of it: a row takes it with share != 0 and len >= P if it attends to all of it, lo <= S.  Its own pages serve
@@ -199,6 +200,12 @@ SK_DEV OwnRun own_run(const uint32_t *ctl, const P &p, uint32_t row, uint32_t n_
   if (together) x.seq = of;
   x.all_lo = !together ? x.lo : to ? from : 0, x.all_hi = together ? to : x.hi;
   return x;
+}
+// A head's slope in powers of two, so that no bias reaches what masked scores are set to.
+template <typename P>
+SK_DEV float slope_of(const uint32_t *ctl, const P &p, uint32_t head) {
+  if (p.slopes_off == ~0u) return 0.0f;
+  return __builtin_amdgcn_fmed3f(__builtin_bit_cast(float, ctl[p.slopes_off + head]), -0x1p16f, 0x1p16f) * 1.44269504088896340736f;
 }
 // a row's range, whichever kernel's
 template <typename P>
@@ -909,7 +916,7 @@ SK_DEV void wide_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
   [[maybe_unused]] uint32_t row_at = 0;
   if constexpr (SHAPED<P>) {
     if constexpr (CAPPED<P>) cap = cap_of(p.cap);
-    if (p.slopes_off != ~0u) slope = __builtin_bit_cast(float, ctl[p.slopes_off + kvh * rep + head]) * 1.44269504088896340736f;
+    slope = slope_of(ctl, p, kvh * rep + head);
     row_at = range_of(ctl, p, row, shared).at;
   }
   // this wave's query rows
@@ -1325,7 +1332,6 @@ SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_
       // places up)
       constexpr uint32_t T = 16 / N_REP;
       const uint32_t tiles = (n_grid + T - 1) / T;
-      row = w / (p.n_kv * n_own);
       row = row % tiles * T + row / tiles;
       if (row >= n_rows) return;
       const bool together = rows_together<T>(ctl, p.rows_off, row, n_rows), lead = part >= p.n_own;
@@ -1377,8 +1383,8 @@ SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_
     [[maybe_unused]] uint32_t row_at = 0;
     [[maybe_unused]] uint2 mine = {};
     if constexpr (SHAPED<P>) {
-      if (p.slopes_off != ~0u) slope = __builtin_bit_cast(float, ctl[p.slopes_off + kvh * N_REP + i % N_REP]) * 1.44269504088896340736f;
-      row_at = ctl[p.rows_off + 4 * row + 1] - 1;
+      slope = slope_of(ctl, p, kvh * N_REP + i % N_REP);
+      row_at = range_of(ctl, p, row, shared).at;
       mine = sees[c % n_live];
     }
     wave_run<K8, V8>(a, ctl, kv, kv8, p, kvh, a + p.q_off + row * p.q_stride + (kvh * N_REP + i % N_REP) * HD,
@@ -1484,15 +1490,16 @@ SK_DEV void paged_merge(float *a, const uint32_t *ctl, const P &p, uint32_t h, u
   uint32_t ns, no, nl = 0;  // live partials: the shared run's, the row's own, its lead's
   uint32_t o0 = p.n_shared, l0 = 0;  // the first of the latter two
   if constexpr (SHAPED<P>) {
-    const bool together = rows_together(ctl, p.rows_off, row, ctl[2], 16 / p.rep);
+    const uint32_t n_rows = min(ctl[2], gridDim.y);  // the attention's
+    const bool together = rows_together(ctl, p.rows_off, row, n_rows, 16 / p.rep);
     // the parts of [x.all_lo, x.all_hi) with some of [x.lo, x.hi)
     auto parts_of = [&](bool lead, uint32_t n_parts, uint32_t &at) {
-      const OwnRun x = own_run(ctl, p, row, ctl[2], 16 / p.rep, together, shared, lead);
+      const OwnRun x = own_run(ctl, p, row, n_rows, 16 / p.rep, together, shared, lead);
       if (x.lo >= x.hi) return 0u;
       const Split sp = split_of(x.all_lo, x.all_hi, n_parts);
-      const uint32_t k = (x.lo - sp.base) / (sp.per * TILE);
+      const uint32_t k = min((x.lo - sp.base) / TILE / sp.per, n_parts - 1);
       at += k;
-      return (x.hi - 1 - sp.base) / (sp.per * TILE) - k + 1;
+      return min((x.hi - 1 - sp.base) / TILE / sp.per, n_parts - 1) - k + 1;
     };
     ns = r.member ? live_parts(split_of(shared_first(ctl, p, shared), shared, p.n_shared)) : 0;
     no = parts_of(false, p.n_own, o0);

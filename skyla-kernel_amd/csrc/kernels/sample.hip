@@ -10,6 +10,7 @@
 //   n1  the tokens whose w >= min_p (0: all), at most top_k of them (0: all), at least one
 //   n2  the first n with C(n) >= top_p C(n1) (n1 where top_p is 1 or more)
 //   the token is the first with C(n) > (draw + 1/2) 2^-32 C(n2); kept = n2, logprob = ln(w / C(n2))
+// (What a draw reads of the histograms reaches no memory outside the row, whatever they hold.)
 // T = 0 (or below 0, or no number) takes the first of the order.  Logits of -inf or NaN have no weight and
 // no place; +inf counts as the type's largest value.  A row without tokens gets {~0, 0, -inf, 0}.
 //
@@ -606,7 +607,7 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
     auto bucket_of = [&](double v) {
       const double g = __builtin_rint(v), f = 0.5 - (v - g);
       const uint32_t b = (uint32_t)(int)(r.edge - g), i = b >= f2 ? span2 + b - f2 : b >= f1 ? span1 + b - f1 : b - f0;
-      return i * per + min((uint32_t)(int)(f * (double)per), per - 1);
+      return min(i * per + min((uint32_t)(int)(f * (double)per), per - 1), DRAW - 1);
     };
     // a chunk's run takes 16 lanes or more, each with U loads in flight
     const uint32_t runs = 1 + (f1 != ~0u) + (f2 != ~0u), lanes = n_chunks * runs <= 16 ? 64 : n_chunks * runs <= 32 ? 32 : 16;
@@ -615,7 +616,7 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
       const uint32_t i = t % n_chunks, which = t / n_chunks;
       const uint32_t f = which == 0 ? f0 : which == 1 && f1 != ~0u ? f1 : f2, e = which == 0 ? e0 : which == 1 && f1 != ~0u ? e1 : e2;
       const uint32_t down = s.down[i];
-      s.runs[t] = down > e ? make_uint2(0, 0) : make_uint2(f > down ? s.ends[i][f - down - 1] : 0, s.ends[i][e - down]);
+      s.runs[t] = down > e ? make_uint2(0, 0) : make_uint2(f > down ? s.ends[i][f - down - 1] : 0, min((uint32_t)s.ends[i][e - down], CHUNK));
     }
     __syncthreads();
     for (uint32_t j = t / lanes; j < n_chunks * runs; j += DRAW / lanes) {
@@ -626,7 +627,7 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
         uint32_t id[U];
         float x[U];
 #pragma unroll
-        for (uint32_t u = 0; u < U; u++) id[u] = i * CHUNK + ids[min(o + u * lanes, i1 - 1)];
+        for (uint32_t u = 0; u < U; u++) id[u] = min(i * CHUNK + ids[min(o + u * lanes, i1 - 1)], r.n_vocab - 1);
 #pragma unroll
         for (uint32_t u = 0; u < U; u++) x[u] = r.x[id[u]];
 #pragma unroll
@@ -657,15 +658,15 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
       __syncthreads();
       for (uint32_t i = t; i < n; i += DRAW) {
         const uint64_t v = s.place[0][i];
-        s.place[1][atomicAdd(&s.bucket[bucket_of(scaled(value_at(v), r.c))], 1u)] = v;
+        s.place[1][min(atomicAdd(&s.bucket[bucket_of(scaled(value_at(v), r.c))], 1u), MOST - 1)] = v;
       }
       __syncthreads();  // a bucket's word is now its end, the one before it its start
       for (uint32_t i = t; i < n; i += DRAW) {
         const uint64_t v = s.place[1][i];
         const uint32_t b = bucket_of(scaled(value_at(v), r.c)), o0 = b ? s.bucket[b - 1] : 0, o1 = s.bucket[b];
         uint32_t rank = o0;
-        for (uint32_t o = o0; o < o1; o++) rank += s.place[1][o] < v;
-        s.place[0][rank] = v;
+        for (uint32_t o = o0; o < min(o1, n); o++) rank += s.place[1][o] < v;
+        s.place[0][min(rank, n - 1)] = v;
       }
       __syncthreads();
       const uint32_t each = (n + DRAW - 1) / DRAW, i0 = t * each, i1 = min(i0 + each, n);

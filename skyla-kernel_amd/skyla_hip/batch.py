@@ -73,7 +73,7 @@ class BatchRegions:
 class Shape:
     """What attention_paged_shaped does to scores: a cap (cap tanh(s / cap); 0: none), a window (a row
     attends to so many positions, its own the last; 0: all) and the arena offset of the heads' slopes (a
-    score at a distance d loses slope d; None: none do)."""
+    score at a distance d loses slope d, slopes of 2^16 at most; None: none do)."""
     cap: float = 0.0
     window: int = 0
     slopes: int | None = None
@@ -479,8 +479,8 @@ class BatchEngine:
             raise ValueError(f"scores capped at {c.score_cap}: {MIN_CAP} to {MAX_CAP}, or 0")
         if c.windows is not None and (len(c.windows) != c.n_layer or any(not 0 <= w < 2**32 for w in c.windows)):
             raise ValueError(f"windows: a number of positions for each of {c.n_layer} layers (0: all)")
-        if c.slopes is not None and (len(c.slopes) != c.n_head or not np.isfinite(np.float32(c.slopes)).all()):
-            raise ValueError(f"slopes: a number for each of {c.n_head} heads")
+        if c.slopes is not None and (len(c.slopes) != c.n_head or not (np.abs(c.slopes) <= 2**16).all()):
+            raise ValueError(f"slopes: a number of 2^16 at most for each of {c.n_head} heads")
 
     def window(self, layer: int) -> int:
         return self.c.windows[layer] if self.c.windows is not None else 0

@@ -318,6 +318,33 @@ def test_recorded_steps(ctx):
         b.free()
 
 
+def test_more_live_rows_than_the_grid(ctx):
+    """The control word says more rows than the recording has: those of the recording are right, the words behind
+    them (another sequence's, at their place) no part of them."""
+    lens = 200 + np.arange(6)
+    b = Shaped(ctx, P["f16"], 2, 2, 32, lens, seqs=np.zeros(6, int), shares=[100] * 6, shared=100, window=150, first=56,
+               parts=(2, 2, False, 1))
+    try:
+        b.prepare()
+        b.arena.as_u32()[2] = 5000
+        b.check()
+    finally:
+        b.free()
+
+
+@pytest.mark.parametrize("rows", [3, 16, 17])
+def test_rows_that_go_together_or_not(ctx, rows):
+    """Rows of one sequence among idle ones, rows in any order, two sequences in one tile, rows far apart."""
+    g = np.random.default_rng(rows)
+    for seqs, lens in ((np.zeros(rows, int), 300 + g.permutation(rows)),
+                       (np.zeros(rows, int), np.where(g.random(rows) < 0.4, 0, 200 + np.arange(rows))),
+                       (np.arange(rows) // 5 % 2, 100 + np.arange(rows)),
+                       (np.zeros(rows, int), 1 + 257 * (np.arange(rows) % 4) + np.arange(rows))):
+        for parts in (None, (0, 1, False, 0), (0, 7, False, 0)):
+            _check(ctx, P["f16k_q8v"], 2, 2, 16, lens, seqs=seqs, window=90, cap=20.0, parts=parts,
+                   until=np.where(np.arange(rows) % 3 == 1, lens.max(), 0))
+
+
 def test_refusals(ctx):
     b = Shaped(ctx, P["f16"], 2, 2, 16, [50, 40])
     try:
