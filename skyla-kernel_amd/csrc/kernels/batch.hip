@@ -154,51 +154,57 @@ SK_DEV ShapedRange shaped_range(const uint32_t *ctl, const P &p, uint32_t row, u
 // row's mask.  (The words through the scalar cache: nothing writes them while the kernel runs.)
 typedef const __attribute__((address_space(4))) uint32_t ConstWord;
 template <uint32_t T>
-SK_DEV bool rows_together(const uint32_t *ctl, uint32_t rows_off, uint32_t row, uint32_t n_rows) {
+SK_DEV bool rows_together(const uint32_t *ctl, uint32_t rows_off, uint32_t row, uint32_t n_rows, uint32_t n_grid) {
   if constexpr (T == 1) return false;
   ConstWord *w = (ConstWord *)(uintptr_t)(ctl + rows_off);
   uint32_t seq = ~0u, least = ~0u, most = 0;
   bool one = true;
 #pragma unroll
   for (uint32_t i = 0; i < T; i++) {
-    const uint32_t r = min(row / T * T + i, n_rows - 1), of = w[4 * r], len = w[4 * r + 1];
-    if (len == 0) continue;
-    one = one && (seq == ~0u || of == seq);
-    seq = of, least = min(least, len), most = max(most, len);
+    // (the grid's rows, so that the loads wait for no control word)
+    const uint32_t r = row / T * T + i, of = w[4 * min(r, n_grid - 1)], len = w[4 * min(r, n_grid - 1) + 1];
+    const bool live = r < n_rows && len != 0;
+    one = one && (!live || seq == ~0u || of == seq);
+    seq = live ? of : seq, least = live ? min(least, len) : least, most = live ? max(most, len) : most;
   }
   return one && most != 0 && most - least <= 256;
 }
-SK_DEV bool rows_together(const uint32_t *ctl, uint32_t rows_off, uint32_t row, uint32_t n_rows, uint32_t T) {
-  return T == 16  ? rows_together<16>(ctl, rows_off, row, n_rows)
-         : T == 8 ? rows_together<8>(ctl, rows_off, row, n_rows)
-         : T == 4 ? rows_together<4>(ctl, rows_off, row, n_rows)
-                  : rows_together<2>(ctl, rows_off, row, n_rows);
+SK_DEV bool rows_together(const uint32_t *ctl, uint32_t rows_off, uint32_t row, uint32_t n_rows, uint32_t n_grid, uint32_t T) {
+  return T == 16  ? rows_together<16>(ctl, rows_off, row, n_rows, n_grid)
+         : T == 8 ? rows_together<8>(ctl, rows_off, row, n_rows, n_grid)
+         : T == 4 ? rows_together<4>(ctl, rows_off, row, n_rows, n_grid)
+                  : rows_together<2>(ctl, rows_off, row, n_rows, n_grid);
 }
 // The positions of row row's own run, its tail or its lead, and of the run that it is part of.  (Whole waves: lane l
 // looks at row l % T of the rows that may go together.)
 struct OwnRun {
   uint32_t lo, hi, all_lo, all_hi;  // the row's, and the run's; [0, 0): nothing
-  uint32_t seq, lane_lo, lane_hi;   // row l % T's, in lane l
+  uint32_t seq, lane_lo, lane_hi, lane_at;  // row l % T's, in lane l
 };
 template <typename P>
 SK_DEV OwnRun own_run(const uint32_t *ctl, const P &p, uint32_t row, uint32_t n_rows, uint32_t T, bool together, uint32_t shared, bool lead) {
-  const uint32_t lane = threadIdx.x & 63, row0 = row / T * T, mine = row0 + (lane & (T - 1));
-  uint32_t lo = 0, hi = 0, seq = 0;
-  if (mine < n_rows) {
-    const ShapedRange r = shaped_range(ctl, p, mine, shared);
-    lo = lead ? r.lo : r.start, hi = lead ? shared_first(ctl, p, shared) : r.len, seq = r.seq;
+  uint32_t lo = 0, hi = 0, seq = 0, at = 0;
+  auto look = [&](uint32_t i) {
+    const ShapedRange r = shaped_range(ctl, p, i, shared);
+    at = r.at, lo = lead ? r.lo : r.start, hi = lead ? shared_first(ctl, p, shared) : r.len, seq = r.seq;
     if (lo >= hi || (lead && !r.member)) lo = hi = 0;
+  };
+  if (!together) {  // (the same words in every lane: scalar loads, and nothing to be passed between lanes)
+    look(row);
+    return {lo, hi, lo, hi, seq, lo, hi, at};
   }
+  const uint32_t lane = threadIdx.x & 63, row0 = row / T * T, mine = row0 + (lane & (T - 1));
+  if (mine < n_rows) look(mine);
   OwnRun x;
-  x.lane_lo = lo, x.lane_hi = hi;
-  x.lo = __shfl(lo, row - row0, 64), x.hi = __shfl(hi, row - row0, 64), x.seq = __shfl(seq, row - row0, 64);
+  x.lane_lo = lo, x.lane_hi = hi, x.lane_at = at;
+  x.lo = __shfl(lo, row - row0, 64), x.hi = __shfl(hi, row - row0, 64);
   uint32_t from = hi ? lo : ~0u, to = hi, of = hi ? seq : 0;
   for (uint32_t d = T / 2; d >= 1; d >>= 1) {
     from = min(from, (uint32_t)__shfl_xor(from, d, 64)), to = max(to, (uint32_t)__shfl_xor(to, d, 64));
     of = max(of, (uint32_t)__shfl_xor(of, d, 64));
   }
-  if (together) x.seq = of;
-  x.all_lo = !together ? x.lo : to ? from : 0, x.all_hi = together ? to : x.hi;
+  x.seq = of;
+  x.all_lo = to ? from : 0, x.all_hi = to;
   return x;
 }
 // A head's slope in powers of two, so that no bias reaches what masked scores are set to.
@@ -1302,7 +1308,8 @@ SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_
   const uint32_t n_rows = min(ctl[2], n_grid), slots = slots_of(p), groups = p.n_kv * p.n_shared;
   const uint32_t shared = shared_end(ctl, p);
   uint32_t w = blockIdx.x, kvh, part, seq, lo, hi;
-  if (n_rows == 0) return;
+  if constexpr (!SHAPED<P>)
+    if (n_rows == 0) return;
   const uint32_t tiles = wide ? (n_grid * N_REP + WIDE - 1) / WIDE : (n_grid * N_REP + 15) / 16;
   const uint32_t n_first = wide ? (groups + 7) / 8 * 8 * tiles : groups * tiles;
   const bool own = w >= n_first;
@@ -1311,7 +1318,7 @@ SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_
   [[maybe_unused]] uint32_t slot = 0, tile0 = 0, n_own_rows = N_REP;  // of an own run's partial; of the rows that may go together
   [[maybe_unused]] OwnRun run;
   if (!own) {
-    if (shared == 0) return;
+    if (shared == 0 || (SHAPED<P> && n_rows == 0)) return;
     if (wide) {
       const uint32_t g = w / (8 * tiles) * 8 + w % 8;
       if (g < groups)
@@ -1333,10 +1340,9 @@ SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_
       constexpr uint32_t T = 16 / N_REP;
       const uint32_t tiles = (n_grid + T - 1) / T;
       row = row % tiles * T + row / tiles;
-      if (row >= n_rows) return;
-      const bool together = rows_together<T>(ctl, p.rows_off, row, n_rows), lead = part >= p.n_own;
+      const bool together = rows_together<T>(ctl, p.rows_off, row, n_rows, n_grid), lead = part >= p.n_own;
       tile0 = row / T * T;
-      if (together && row != tile0) return;
+      if (row >= n_rows || (together && row != tile0)) return;
       run = own_run(ctl, p, row, n_rows, T, together, shared, lead);
       slot = p.n_shared + part;
       if (together) n_own_rows = min(T, n_rows - tile0) * N_REP;
@@ -1361,11 +1367,15 @@ SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_
     return;
   }
   // Each row's [lo, hi) of the run (shaped): rows that go together may see parts of it.
-  [[maybe_unused]] __shared__ uint2 sees[SHAPED<P> ? 16 : 1];
+  [[maybe_unused]] __shared__ uint4 sees[SHAPED<P> ? 16 : 1];  // and its position
   if constexpr (SHAPED<P>) {
     if (t < 16) {
-      const uint32_t at = own ? (i0 + c % n_live) / N_REP - tile0 : 0, from = __shfl(run.lane_lo, at, 64), to = __shfl(run.lane_hi, at, 64);
-      sees[t] = own ? make_uint2(from, to) : make_uint2(lo, hi);
+      if (own) {
+        const uint32_t at = (i0 + c % n_live) / N_REP - tile0;
+        sees[t] = make_uint4(__shfl(run.lane_lo, at, 64), __shfl(run.lane_hi, at, 64), __shfl(run.lane_at, at, 64), 0);
+      } else {
+        sees[t] = make_uint4(lo, hi, range_of(ctl, p, min((i0 + t) / N_REP, n_rows - 1), shared).at, 0);
+      }
     }
     __syncthreads();
   }
@@ -1381,11 +1391,11 @@ SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_
     const uint32_t i = i0 + c % n_live, row = min(i / N_REP, n_rows - 1);
     [[maybe_unused]] float slope = 0.0f;
     [[maybe_unused]] uint32_t row_at = 0;
-    [[maybe_unused]] uint2 mine = {};
+    [[maybe_unused]] uint4 mine = {};
     if constexpr (SHAPED<P>) {
       slope = slope_of(ctl, p, kvh * N_REP + i % N_REP);
-      row_at = range_of(ctl, p, row, shared).at;
       mine = sees[c % n_live];
+      row_at = mine.z;
     }
     wave_run<K8, V8>(a, ctl, kv, kv8, p, kvh, a + p.q_off + row * p.q_stride + (kvh * N_REP + i % N_REP) * HD,
                      st.run[wave], seq, lo, hi, begin + wave * per, min(begin + (wave + 1) * per, end), slope, row_at, mine.x,
@@ -1491,7 +1501,7 @@ SK_DEV void paged_merge(float *a, const uint32_t *ctl, const P &p, uint32_t h, u
   uint32_t o0 = p.n_shared, l0 = 0;  // the first of the latter two
   if constexpr (SHAPED<P>) {
     const uint32_t n_rows = min(ctl[2], gridDim.y);  // the attention's
-    const bool together = rows_together(ctl, p.rows_off, row, n_rows, 16 / p.rep);
+    const bool together = rows_together(ctl, p.rows_off, row, n_rows, gridDim.y, 16 / p.rep);
     // the parts of [x.all_lo, x.all_hi) with some of [x.lo, x.hi)
     auto parts_of = [&](bool lead, uint32_t n_parts, uint32_t &at) {
       const OwnRun x = own_run(ctl, p, row, n_rows, 16 / p.rep, together, shared, lead);
