@@ -244,6 +244,7 @@ constexpr uint32_t DRAW = 1024, DRAW_WAVES = DRAW / 64;
 constexpr uint32_t MOST = 8192;    // values of the bins with borders that are put in order in LDS
 constexpr uint32_t SPANS = 64;     // such bins
 constexpr uint32_t CHUNKS = 128;   // of a row
+constexpr uint32_t ID_BITS = 20;   // of a token's id
 constexpr uint32_t DIGITS = 2048;  // buckets of the search that takes any number of them
 
 // Where a row's borders lie: of bin b1 some tokens stay (BINS: all of all bins), as min_p has it if that is bm, as top_k
@@ -611,7 +612,7 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
     };
     // a chunk's run takes 16 lanes or more, each with U loads in flight
     const uint32_t runs = 1 + (f1 != ~0u) + (f2 != ~0u), lanes = n_chunks * runs <= 16 ? 64 : n_chunks * runs <= 32 ? 32 : 16;
-    constexpr uint32_t U = 4;
+    constexpr uint32_t U = 8;
     if (t < n_chunks * runs) {
       const uint32_t i = t % n_chunks, which = t / n_chunks;
       const uint32_t f = which == 0 ? f0 : which == 1 && f1 != ~0u ? f1 : f2, e = which == 0 ? e0 : which == 1 && f1 != ~0u ? e1 : e2;
@@ -634,8 +635,10 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
         for (uint32_t u = 0; u < U; u++) {
           if (o + u * lanes >= i1) break;
           const uint32_t to = atomicAdd(&s.fill, 1u);
-          if (to < MOST) s.place[0][to] = place(x[u], id[u]);  // (always: so many were counted)
-          if (n > 64) atomicAdd(&s.bucket[bucket_of(scaled(x[u], r.c))], 1u);
+          // (with the bucket above the id: it goes by the value, so that the order is the same)
+          const uint32_t b = n > 64 ? bucket_of(scaled(x[u], r.c)) : 0;
+          if (to < MOST) s.place[0][to] = place(x[u], id[u] | b << ID_BITS);  // (always: so many were counted)
+          if (n > 64) atomicAdd(&s.bucket[b], 1u);
         }
       }
     }
@@ -658,12 +661,12 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
       __syncthreads();
       for (uint32_t i = t; i < n; i += DRAW) {
         const uint64_t v = s.place[0][i];
-        s.place[1][min(atomicAdd(&s.bucket[bucket_of(scaled(value_at(v), r.c))], 1u), MOST - 1)] = v;
+        s.place[1][min(atomicAdd(&s.bucket[(uint32_t)v >> ID_BITS], 1u), MOST - 1)] = v;
       }
       __syncthreads();  // a bucket's word is now its end, the one before it its start
       for (uint32_t i = t; i < n; i += DRAW) {
         const uint64_t v = s.place[1][i];
-        const uint32_t b = bucket_of(scaled(value_at(v), r.c)), o0 = b ? s.bucket[b - 1] : 0, o1 = s.bucket[b];
+        const uint32_t b = (uint32_t)v >> ID_BITS, o0 = b ? s.bucket[b - 1] : 0, o1 = s.bucket[b];
         uint32_t rank = o0;
         for (uint32_t o = o0; o < min(o1, n); o++) rank += s.place[1][o] < v;
         s.place[0][min(rank, n - 1)] = v;
@@ -737,6 +740,6 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
   }
   if (t == 0) {
     const double y = (scaled(value_at(chosen.place), r.c) - r.edge) * 0.125 * 0.69314718055994530942 - log(n2.sum);
-    *(uint4 *)out = make_uint4((uint32_t)chosen.place, n2.n, __builtin_bit_cast(uint32_t, n2.n == 1 ? 0.0f : (float)y), 0);
+    *(uint4 *)out = make_uint4((uint32_t)chosen.place & ((1u << ID_BITS) - 1), n2.n, __builtin_bit_cast(uint32_t, n2.n == 1 ? 0.0f : (float)y), 0);
   }
 }
