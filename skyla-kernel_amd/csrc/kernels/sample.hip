@@ -241,7 +241,8 @@ extern "C" __global__ __launch_bounds__(THREADS) void logits_sample(float *a, co
 namespace {
 
 constexpr uint32_t DRAW = 1024, DRAW_WAVES = DRAW / 64;
-constexpr uint32_t MOST = 8192;    // values of the bins with borders that are put in order in LDS
+constexpr uint32_t MOST = 8192;    // values of the bins with borders that are taken into LDS
+constexpr uint32_t RANKED = 512;   // and of one bucket of these that are put in order
 constexpr uint32_t SPANS = 64;     // such bins
 constexpr uint32_t CHUNKS = 128;   // of a row
 constexpr uint32_t ID_BITS = 20;   // of a token's id
@@ -255,21 +256,24 @@ struct Borders {
 };
 struct DrawShared {
   union {
-    uint64_t place[2][MOST];  // as they came and then in order; by buckets, then the sums behind them, then C there
+    uint64_t place[2][MOST];  // as they came, then those of one bucket in order and behind them C there; by buckets
     struct {
       unsigned long long sum[DIGITS];
       uint32_t count[DIGITS];
     } digit;
     uint16_t ends[CHUNKS][BINS];  // of a chunk's tokens, those that end with a bin
   };
-  uint64_t half_sum[BINS];
+  union {
+    uint64_t half_sum[BINS];
+    uint32_t next[DRAW];  // a bucket's next free place
+  };
   uint32_t half_n[BINS];
   float largest[CHUNKS];
   uint32_t down[CHUNKS];  // how many bins below the row's a chunk's lie (BINS: that or more; ~0: it has none)
   double c[BINS + 1];     // C before a bin, in weights of the first bin's middle
   uint32_t n[BINS + 1];   // tokens before it
   double edge[BINS];      // its middle's weight
-  uint32_t bucket[DRAW];
+  unsigned long long bucket[DRAW];  // a word like a bin's
   double first[CHUNKS];   // the chunks' rint(t) of their largest values
   double sums[DRAW_WAVES];
   uint64_t words[DRAW_WAVES];
@@ -602,7 +606,8 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
   span2 = n_spans, at2 = n;
   if (f2 != ~0u) n_spans++, n += s.n[e2 + 1] - s.n[f2], deepest = e2;
   Found n2, chosen;
-  if (n_spans <= SPANS && n <= MOST && deepest < BINS - 1) {
+  bool many = n_spans > SPANS || n > MOST || deepest == BINS - 1;
+  if (!many) {
     // ---- few: from the chunks' lists into LDS, in buckets by t
     const uint32_t per = DRAW / n_spans;
     auto bucket_of = [&](double v) {
@@ -613,6 +618,7 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
     // a chunk's run takes 16 lanes or more, each with U loads in flight
     const uint32_t runs = 1 + (f1 != ~0u) + (f2 != ~0u), lanes = n_chunks * runs <= 16 ? 64 : n_chunks * runs <= 32 ? 32 : 16;
     constexpr uint32_t U = 8;
+    const Series series_ = series();
     if (t < n_chunks * runs) {
       const uint32_t i = t % n_chunks, which = t / n_chunks;
       const uint32_t f = which == 0 ? f0 : which == 1 && f1 != ~0u ? f1 : f2, e = which == 0 ? e0 : which == 1 && f1 != ~0u ? e1 : e2;
@@ -636,94 +642,124 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
           if (o + u * lanes >= i1) break;
           const uint32_t to = atomicAdd(&s.fill, 1u);
           // (with the bucket above the id: it goes by the value, so that the order is the same)
-          const uint32_t b = n > 64 ? bucket_of(scaled(x[u], r.c)) : 0;
+          const double v = scaled(x[u], r.c);
+          const uint32_t b = n > 64 ? bucket_of(v) : 0;
           if (to < MOST) s.place[0][to] = place(x[u], id[u] | b << ID_BITS);  // (always: so many were counted)
-          if (n > 64) atomicAdd(&s.bucket[b], 1u);
+          if (n > 64) atomicAdd(&s.bucket[b], (unsigned long long)fixed_weight(series_, r, v) + (1ull << COUNT_AT));
         }
       }
     }
     __syncthreads();
-    const Series series_ = series();
-    uint64_t *raw = s.place[1];
-    double *upto = (double *)s.place[1];
-    auto weight_of = [&](uint64_t v) { return fixed_weight(series_, r, scaled(value_at(v), r.c)); };
-    auto start_of = [&](uint32_t b) {  // bin b's first place in the order here
-      return b >= f2 ? at2 + s.n[b] - s.n[f2] : b >= f1 ? at1 + s.n[b] - s.n[f1] : s.n[b] - s.n[f0];
-    };
-    auto c_at = [&](uint32_t i) {  // from the sums
-      const uint32_t b = bin_of(r, scaled(value_at(s.place[0][i]), r.c)), i0 = start_of(b);
-      return s.c[b] + sum_of(raw[i] - (i0 ? raw[i0 - 1] : 0), s.edge[b]);
-    };
     if (n > 64) {
-      uint32_t all;
-      const uint32_t mine = s.bucket[t], end = block_scan(mine, s.counts, all);
-      s.bucket[t] = end - mine;  // where the bucket starts
+      uint64_t all;
+      const uint64_t mine = s.bucket[t], end = block_scan(mine, s.words, all);
+      s.bucket[t] = end;
+      s.next[t] = (uint32_t)((end - mine) >> COUNT_AT);
       __syncthreads();
       for (uint32_t i = t; i < n; i += DRAW) {
         const uint64_t v = s.place[0][i];
-        s.place[1][min(atomicAdd(&s.bucket[(uint32_t)v >> ID_BITS], 1u), MOST - 1)] = v;
-      }
-      __syncthreads();  // a bucket's word is now its end, the one before it its start
-      for (uint32_t i = t; i < n; i += DRAW) {
-        const uint64_t v = s.place[1][i];
-        const uint32_t b = (uint32_t)v >> ID_BITS, o0 = b ? s.bucket[b - 1] : 0, o1 = s.bucket[b];
-        uint32_t rank = o0;
-        for (uint32_t o = o0; o < min(o1, n); o++) rank += s.place[1][o] < v;
-        s.place[0][min(rank, n - 1)] = v;
+        s.place[1][min(atomicAdd(&s.next[(uint32_t)v >> ID_BITS], 1u), MOST - 1)] = v;
       }
       __syncthreads();
-      const uint32_t each = (n + DRAW - 1) / DRAW, i0 = t * each, i1 = min(i0 + each, n);
-      uint64_t sum = 0, sum_all;
-      for (uint32_t i = i0; i < i1; i++) raw[i] = sum += weight_of(s.place[0][i]);
-      const uint64_t before = block_scan(sum, s.words, sum_all) - sum;
-      for (uint32_t i = i0; i < i1; i++) raw[i] += before;
-      __syncthreads();
-      double c[MOST / DRAW];
-#pragma unroll
-      for (uint32_t j = 0; j < MOST / DRAW; j++)
-        if (t + j * DRAW < n) c[j] = c_at(t + j * DRAW);
-      __syncthreads();
-#pragma unroll
-      for (uint32_t j = 0; j < MOST / DRAW; j++)
-        if (t + j * DRAW < n) upto[t + j * DRAW] = c[j];
-      __syncthreads();
     }
-    if (t >= 64) return;
-    // (the first wave alone)
-    if (n <= 64) {
-      const uint64_t v = t < n ? s.place[0][t] : ~0ull;
-      uint32_t rank = 0;
-      for (uint32_t i = 0; i < n; i++) rank += s.place[0][i] < v;
-      if (t < n) s.place[0][rank] = v;
-      const uint64_t sum = wave_scan(t < n ? weight_of(s.place[0][t]) : 0);
-      if (t < n) raw[t] = sum;
-      const double c = t < n ? c_at(t) : 0.0;
-      if (t < n) upto[t] = c;
+    if (t < 64) {  // the first wave alone
+      uint32_t o0 = 0, m = n;  // of the order here, the places whose tokens lie in order
+      uint64_t *sorted = s.place[0];
+      double *upto = (double *)(s.place[0] + RANKED);
+      bool fits = true;
+      auto weight_of = [&](uint64_t v) { return fixed_weight(series_, r, scaled(value_at(v), r.c)); };
+      auto start_of = [&](uint32_t b) {  // bin b's first place in the order here
+        return b >= f2 ? at2 + s.n[b] - s.n[f2] : b >= f1 ? at1 + s.n[b] - s.n[f1] : s.n[b] - s.n[f0];
+      };
+      auto span_of = [&](uint32_t b) { return b >= f2 ? span2 + b - f2 : b >= f1 ? span1 + b - f1 : b - f0; };
+      auto count_to = [&](uint32_t q) { return (uint32_t)(s.bucket[q] >> COUNT_AT); };  // with bucket q
+      auto sum_to = [&](uint32_t q) { return s.bucket[q] & SUM; };
+      auto sum_before = [&](uint32_t q) { return q ? sum_to(q - 1) : 0; };
+      if (n <= 64) {  // all of them
+        const uint64_t v = t < n ? s.place[0][t] : ~0ull;
+        uint32_t rank = 0;
+        for (uint32_t i = 0; i < n; i++) rank += s.place[0][i] < v;
+        if (t < n) sorted[rank] = v;
+        uint64_t *raw = s.place[1];
+        const uint64_t sum = wave_scan(t < n ? weight_of(sorted[t]) : 0);
+        if (t < n) raw[t] = sum;
+        if (t < n) {
+          const uint32_t b = bin_of(r, scaled(value_at(sorted[t]), r.c)), i0 = start_of(b);
+          upto[t] = s.c[b] + sum_of(sum - (i0 ? raw[i0 - 1] : 0), s.edge[b]);
+        }
+      } else {
+        m = 0;
+      }
+      auto order = [&](uint32_t q) {  // bucket q's
+        const uint32_t i0 = q ? count_to(q - 1) : 0, size = count_to(q) - i0;
+        if (m && i0 == o0) return;
+        fits = fits && size <= RANKED;  // (if not, nothing found from here on is used)
+        o0 = i0, m = size <= RANKED ? size : 0;
+        for (uint32_t j = t; j < m; j += 64) {
+          const uint64_t v = s.place[1][o0 + j];
+          uint32_t rank = 0;
+          for (uint32_t i = 0; i < m; i++) rank += s.place[1][o0 + i] < v;
+          sorted[rank] = v;
+        }
+        const uint32_t span = q / per, b = span >= span2 ? f2 + span - span2 : span >= span1 ? f1 + span - span1 : f0 + span;
+        uint64_t before = sum_before(q) - sum_before(span * per);
+        for (uint32_t j0 = 0; j0 < m; j0 += 64) {
+          const uint32_t j = j0 + t;
+          const uint64_t sum = before + wave_scan(j < m ? weight_of(sorted[j]) : 0);
+          if (j < m) upto[j] = s.c[b] + sum_of(sum, s.edge[b]);
+          before = __shfl(sum, 63);
+        }
+      };
+      // the bucket with place i
+      auto order_at = [&](uint32_t i) {
+        if (n > 64) order(min(first_of(DRAW, [&](uint32_t q) { return count_to(q) > i; }), DRAW - 1));
+      };
+      // the token at place i of the order here (within a run of bins places and ranks go together), if it lies in order
+      auto found_at = [&](uint32_t i) {
+        const uint32_t rank = i >= at2 && f2 != ~0u ? s.n[f2] + i - at2 : i >= at1 && f1 != ~0u ? s.n[f1] + i - at1 : s.n[f0] + i;
+        const uint32_t j = min(i - o0, RANKED - 1);
+        return Found{sorted[j], rank + 1, upto[j]};
+      };
+      // n1: of bin b1 those that stay
+      Found n1{0, total, s.c[BINS]};
+      if (b1 < BINS) {
+        const uint32_t i0 = start_of(b1);
+        uint32_t some = s.n[b1 + 1] - s.n[b1];
+        if (b1 == bk) some = k - s.n[b1];
+        if (b1 == bm) {  // (what lies in the buckets before `least`'s is larger, in those behind it smaller)
+          if (n > 64) order(bucket_of(least));
+          const uint32_t at = max(o0, i0) - i0;
+          some = min(some, at + first_of(o0 + m - max(o0, i0), [&](uint32_t i) {
+            return scaled(value_at(sorted[i + max(o0, i0) - o0]), r.c) < least;
+          }));
+        }
+        if (some) order_at(i0 + some - 1);
+        n1 = some ? found_at(i0 + some - 1) : Found{0, s.n[b1], s.c[b1]};
+      }
+      // the first token of bins [f, e], not past the n-th, that meets `want`; the last of these if none does
+      auto first = [&](Want want, double goal, uint32_t most, uint32_t f, uint32_t e) {
+        const uint32_t i0 = start_of(f), i1 = min(i0 + max(min(s.n[e + 1], most), s.n[f] + 1) - s.n[f], n);
+        auto ok = [&](double c) { return want == kReach ? c >= goal : c > goal; };
+        if (n > 64) {
+          const uint32_t q0 = span_of(f) * per, n_q = (span_of(e) + 1) * per - q0;
+          const uint32_t q = q0 + first_of(n_q, [&](uint32_t i) {
+            const uint32_t span = (q0 + i) / per, b = f + span - q0 / per;
+            return ok(s.c[b] + sum_of(sum_to(q0 + i) - sum_before(span * per), s.edge[b]));
+          });
+          order_at(min(q ? count_to(q - 1) : 0, i1 - 1));
+        }
+        const uint32_t from = max(i0, o0), to = min(i1, o0 + m);
+        const uint32_t i = from + first_of(to - from, [&](uint32_t i) { return ok(upto[from + i - o0]); });
+        return found_at(min(i, to - 1));
+      };
+      n2 = by_p ? first(kReach, share * n1.sum, n1.n, p_lo, p_hi) : n1;
+      chosen = first(kPass, u * n2.sum, n2.n, d_lo, d_hi);
+      if (t == 0) s.fill = fits;
     }
-    // the token at place i of the order here (within a run of bins places and ranks go together)
-    auto found_at = [&](uint32_t i) {
-      const uint32_t rank = i >= at2 && f2 != ~0u ? s.n[f2] + i - at2 : i >= at1 && f1 != ~0u ? s.n[f1] + i - at1 : s.n[f0] + i;
-      return Found{s.place[0][i], rank + 1, upto[i]};
-    };
-    // n1: of bin b1 those that stay
-    Found n1{0, total, s.c[BINS]};
-    if (b1 < BINS) {
-      const uint32_t i0 = start_of(b1);
-      uint32_t some = s.n[b1 + 1] - s.n[b1];
-      if (b1 == bk) some = k - s.n[b1];
-      if (b1 == bm) some = first_of(some, [&](uint32_t i) { return scaled(value_at(s.place[0][i0 + i]), r.c) < least; });
-      n1 = some ? found_at(i0 + some - 1) : Found{0, s.n[b1], s.c[b1]};
-    }
-    // the first token of bins [f, e], not past the n-th, that meets `want`; the last of these if none does
-    auto first = [&](Want want, double goal, uint32_t most, uint32_t f, uint32_t e) {
-      const uint32_t i0 = start_of(f), end = max(min(s.n[e + 1], most), s.n[f]) - s.n[f];
-      const uint32_t i = first_of(end, [&](uint32_t i) { return want == kReach ? upto[i0 + i] >= goal : upto[i0 + i] > goal; });
-      return found_at(min(i0 + (i < end ? i : max(end, 1u) - 1), n - 1));
-    };
-    n2 = by_p ? first(kReach, share * n1.sum, n1.n, p_lo, p_hi) : n1;
-    chosen = first(kPass, u * n2.sum, n2.n, d_lo, d_hi);
-  } else {
-    // ---- many
+    __syncthreads();
+    many = !s.fill;
+  }
+  if (many) {
     Found n1{0, total, s.c[BINS]};
     if (b1 < BINS && b1 == bm) n1 = search_above(s, r, least, bm);
     if (b1 < BINS && b1 == bk) {

@@ -132,6 +132,16 @@ def test_equal_logits(ctx):
         _check(ctx, x, [(1.0, p, m, k, int(d)) for d in g.integers(0, 2**32, 12)])
 
 
+@pytest.mark.parametrize("v", [70, 600, 5000, 8192, 20000])
+@pytest.mark.parametrize("step", [2.0**-7, 2.0**-4, 0.5, 8.0])
+def test_logits_on_a_grid(ctx, v, step):
+    """From a few tokens of each value to thousands: those of one value are in order by their ids alone."""
+    g = np.random.default_rng(v)
+    x = (np.round(g.standard_normal((16, v)) / step) * step).astype(np.float32)
+    _check(ctx, x, [(*s[:4], int(d)) for s, d in zip(_some(g, 16), g.integers(0, 2**32, 16))])
+    _check(ctx, x, [(1.0, 0.37, 0.6, v // 3, int(d)) for d in g.integers(0, 2**32, 16)])
+
+
 @pytest.mark.parametrize("v", [5, 9000, 40000])
 def test_logits_without_a_place(ctx, v):
     """-inf and NaN are never drawn, +inf always, rows of nothing give no token; whole chunks of nothing."""
