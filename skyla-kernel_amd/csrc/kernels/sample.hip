@@ -245,6 +245,7 @@ constexpr uint32_t MOST = 8192;    // values of the bins with borders that are t
 constexpr uint32_t RANKED = 512;   // and of one bucket of these that are put in order
 constexpr uint32_t SPANS = 64;     // such bins
 constexpr uint32_t CHUNKS = 128;   // of a row
+constexpr uint32_t RUNS = 512;     // 3 * CHUNKS and more, a power of two
 constexpr uint32_t ID_BITS = 20;   // of a token's id
 constexpr uint32_t DIGITS = 2048;  // buckets of the search that takes any number of them
 
@@ -280,10 +281,14 @@ struct DrawShared {
   uint32_t counts[DRAW_WAVES];
   unsigned long long below;
   Borders at;
-  uint2 runs[3 * CHUNKS];  // of the chunks' lists, the tokens in each run of bins
-  uint32_t fill, found[2];
+  uint2 runs[RUNS];       // of the chunks' lists the tokens in each run of bins: where from, less its own place; its end here
+  uint32_t fits, found[2];
 };
 
+template <uint32_t U>
+struct Count {
+  static constexpr uint32_t value = U;
+};
 // A row as its kernel sees it.
 struct Row {
   const float *x;
@@ -482,7 +487,7 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
   }
   if (t < BINS) s.edge[t] = exp2(-0.125 * (double)t);
   s.bucket[t] = 0;
-  if (t == 0) s.below = 0, s.fill = 0;
+  if (t == 0) s.below = 0;
   __syncthreads();
   const float top = wave_max(fmaxf(s.largest[t & 63], s.largest[64 + (t & 63)]));
   if (!has_weight(top)) {
@@ -610,45 +615,61 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
   if (!many) {
     // ---- few: from the chunks' lists into LDS, in buckets by t
     const uint32_t per = DRAW / n_spans;
+    const float per_inverse = 1.0f / (float)per;
     auto bucket_of = [&](double v) {
       const double g = __builtin_rint(v), f = 0.5 - (v - g);
       const uint32_t b = (uint32_t)(int)(r.edge - g), i = b >= f2 ? span2 + b - f2 : b >= f1 ? span1 + b - f1 : b - f0;
       return min(i * per + min((uint32_t)(int)(f * (double)per), per - 1), DRAW - 1);
     };
-    // a chunk's run takes 16 lanes or more, each with U loads in flight
-    const uint32_t runs = 1 + (f1 != ~0u) + (f2 != ~0u), lanes = n_chunks * runs <= 16 ? 64 : n_chunks * runs <= 32 ? 32 : 16;
-    constexpr uint32_t U = 8;
+    const uint32_t runs = 1 + (f1 != ~0u) + (f2 != ~0u);
     const Series series_ = series();
-    if (t < n_chunks * runs) {
+    {
+      uint2 run = make_uint2(0, 0);
       const uint32_t i = t % n_chunks, which = t / n_chunks;
-      const uint32_t f = which == 0 ? f0 : which == 1 && f1 != ~0u ? f1 : f2, e = which == 0 ? e0 : which == 1 && f1 != ~0u ? e1 : e2;
-      const uint32_t down = s.down[i];
-      s.runs[t] = down > e ? make_uint2(0, 0) : make_uint2(f > down ? s.ends[i][f - down - 1] : 0, min((uint32_t)s.ends[i][e - down], CHUNK));
+      if (which < runs) {
+        const uint32_t f = which == 0 ? f0 : which == 1 && f1 != ~0u ? f1 : f2;
+        const uint32_t e = which == 0 ? e0 : which == 1 && f1 != ~0u ? e1 : e2, down = s.down[i];
+        if (down <= e) run = make_uint2(f > down ? s.ends[i][f - down - 1] : 0, min((uint32_t)s.ends[i][e - down], CHUNK));
+      }
+      uint32_t all;
+      const uint32_t end = block_scan(run.y - run.x, s.counts, all);
+      if (t < RUNS) s.runs[t] = make_uint2(run.y - end, which < runs ? end : ~0u);
     }
     __syncthreads();
-    for (uint32_t j = t / lanes; j < n_chunks * runs; j += DRAW / lanes) {
-      const uint32_t i = j % n_chunks, i0 = s.runs[j].x, i1 = s.runs[j].y;
-      const float *part = parts + (size_t)i * PART;
-      const uint16_t *ids = (const uint16_t *)(part + HEAD + 2 * BINS);
-      for (uint32_t o = i0 + t % lanes; o < i1; o += U * lanes) {
-        uint32_t id[U];
-        float x[U];
+    uint32_t half = 1;
+    while (2 * half < n_chunks * runs) half *= 2;
+    // thread t has the values t + DRAW u, all of them on their way at once
+    auto gather = [&](auto u_) {
+      constexpr uint32_t U = decltype(u_)::value;
+      uint32_t id[U], j[U];
+      float x[U];
 #pragma unroll
-        for (uint32_t u = 0; u < U; u++) id[u] = min(i * CHUNK + ids[min(o + u * lanes, i1 - 1)], r.n_vocab - 1);
+      for (uint32_t u = 0; u < U; u++) j[u] = 0;
+      for (uint32_t h = half; h; h /= 2)  // the first run that ends behind it
 #pragma unroll
-        for (uint32_t u = 0; u < U; u++) x[u] = r.x[id[u]];
+        for (uint32_t u = 0; u < U; u++) j[u] += s.runs[j[u] + h - 1].y <= min(t + DRAW * u, n - 1) ? h : 0;
 #pragma unroll
-        for (uint32_t u = 0; u < U; u++) {
-          if (o + u * lanes >= i1) break;
-          const uint32_t to = atomicAdd(&s.fill, 1u);
-          // (with the bucket above the id: it goes by the value, so that the order is the same)
-          const double v = scaled(x[u], r.c);
-          const uint32_t b = n > 64 ? bucket_of(v) : 0;
-          if (to < MOST) s.place[0][to] = place(x[u], id[u] | b << ID_BITS);  // (always: so many were counted)
-          if (n > 64) atomicAdd(&s.bucket[b], (unsigned long long)fixed_weight(series_, r, v) + (1ull << COUNT_AT));
-        }
+      for (uint32_t u = 0; u < U; u++) {
+        const uint32_t i = j[u] % n_chunks;
+        const uint16_t *ids = (const uint16_t *)(parts + (size_t)i * PART + HEAD + 2 * BINS);
+        id[u] = min(i * CHUNK + ids[min(s.runs[j[u]].x + min(t + DRAW * u, n - 1), CHUNK - 1)], r.n_vocab - 1);
       }
-    }
+#pragma unroll
+      for (uint32_t u = 0; u < U; u++) x[u] = r.x[id[u]];
+#pragma unroll
+      for (uint32_t u = 0; u < U; u++) {
+        if (t + DRAW * u >= n) break;
+        // (with the bucket above the id: it goes by the value, so that the order is the same)
+        const double v = scaled(x[u], r.c);
+        const uint32_t b = n > 64 ? bucket_of(v) : 0;
+        s.place[0][t + DRAW * u] = place(x[u], id[u] | b << ID_BITS);
+        if (n > 64) atomicAdd(&s.bucket[b], (unsigned long long)fixed_weight(series_, r, v) + (1ull << COUNT_AT));
+      }
+    };
+    if (n <= DRAW)
+      gather(Count<1>());
+    else
+      gather(Count<MOST / DRAW>());
     __syncthreads();
     if (n > 64) {
       uint64_t all;
@@ -698,6 +719,7 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
         for (uint32_t j = t; j < m; j += 64) {
           const uint64_t v = s.place[1][o0 + j];
           uint32_t rank = 0;
+#pragma unroll 4
           for (uint32_t i = 0; i < m; i++) rank += s.place[1][o0 + i] < v;
           sorted[rank] = v;
         }
@@ -743,10 +765,14 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
         if (n > 64) {
           const uint32_t q0 = span_of(f) * per, n_q = (span_of(e) + 1) * per - q0;
           const uint32_t q = q0 + first_of(n_q, [&](uint32_t i) {
-            const uint32_t span = (q0 + i) / per, b = f + span - q0 / per;
-            return ok(s.c[b] + sum_of(sum_to(q0 + i) - sum_before(span * per), s.edge[b]));
+            const uint32_t k = (uint32_t)(((float)i + 0.5f) * per_inverse);  // i / per
+            return ok(s.c[f + k] + sum_of(sum_to(q0 + i) - sum_before(q0 + k * per), s.edge[f + k]));
           });
-          order_at(min(q ? count_to(q - 1) : 0, i1 - 1));
+          const uint32_t i = q ? count_to(q - 1) : 0;
+          if (q < q0 + n_q && i < i1 && i < count_to(q))
+            order(q);
+          else
+            order_at(min(i, i1 - 1));
         }
         const uint32_t from = max(i0, o0), to = min(i1, o0 + m);
         const uint32_t i = from + first_of(to - from, [&](uint32_t i) { return ok(upto[from + i - o0]); });
@@ -754,10 +780,10 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
       };
       n2 = by_p ? first(kReach, share * n1.sum, n1.n, p_lo, p_hi) : n1;
       chosen = first(kPass, u * n2.sum, n2.n, d_lo, d_hi);
-      if (t == 0) s.fill = fits;
+      if (t == 0) s.fits = fits;
     }
     __syncthreads();
-    many = !s.fill;
+    many = !s.fits;
   }
   if (many) {
     Found n1{0, total, s.c[BINS]};
