@@ -451,7 +451,7 @@ class BatchEngine:
             "logits": self.s_vocab * max_seq, "controls": 8 * max_seq, "history": self.s_hist * max_seq,
             "bias": 2 * self.MAX_BIASES * max_seq, "mask": self.s_mask * max_seq,
             "axes": 4 * E.BATCH, "spans": 2 * E.BATCH, "slopes": c.n_head, "sampling": 8 * max_seq,
-            "drawn": 4 * max_seq, "sample": sample_size(max_seq, c.n_vocab)})
+            "drawn": 4 * max_seq, "sample": sample_size(max_seq, c.n_vocab) if self._draws() else 0})
         x = a.extra
         for _ in range(c.n_layer):
             self.pools.append(ctx.alloc_host(self.paged.bytes()))
@@ -471,8 +471,6 @@ class BatchEngine:
 
     @staticmethod
     def _check_shape(c: E.Config) -> None:
-        if c.n_vocab > SAMPLE_VOCAB:
-            raise ValueError(f"a vocabulary of {c.n_vocab} tokens: at most {SAMPLE_VOCAB}")
         if c.axes is not None and (len(c.axes) != c.head_dim // 2 or any(a not in (0, 1, 2, 3) for a in c.axes)):
             raise ValueError(f"axes: one of 0 to 3 for each of {c.head_dim // 2} pairs")
         if c.score_cap != 0 and not MIN_CAP <= c.score_cap <= MAX_CAP:
@@ -481,6 +479,9 @@ class BatchEngine:
             raise ValueError(f"windows: a number of positions for each of {c.n_layer} layers (0: all)")
         if c.slopes is not None and (len(c.slopes) != c.n_head or not (np.abs(c.slopes) <= 2**16).all()):
             raise ValueError(f"slopes: a number of 2^16 at most for each of {c.n_head} heads")
+
+    def _draws(self) -> bool:
+        return self.c.n_vocab <= SAMPLE_VOCAB
 
     def window(self, layer: int) -> int:
         return self.c.windows[layer] if self.c.windows is not None else 0
@@ -830,8 +831,10 @@ class BatchEngine:
 
     def sample(self, tokens: dict, draws: dict, prompt=()) -> Drawn:
         """step(), but the tokens that come next, each drawn as its sequence's sampling has it from the logits after
-        its controls, by its random number draws[sequence], an integer of 32 bits: the same number draws the same
-        token, whatever else is in the batch."""
+        its controls, by its random number draws[sequence], an integer of 32 bits: from the same logits the same
+        number draws the same token, whatever else is in the batch."""
+        if not self._draws():
+            raise ValueError(f"tokens are drawn from a vocabulary of {SAMPLE_VOCAB} at most, not of {self.c.n_vocab}")
         if set(draws) != set(tokens):
             raise ValueError("draws: a random number for each sequence of this step")
         draws = {q: int(d) for q, d in draws.items()}

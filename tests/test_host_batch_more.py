@@ -226,9 +226,20 @@ def test_configs_that_no_kernel_serves():
     base = dict(n_embd=256, n_head=2, n_head_kv=1, n_vocab=1000, n_layer=2)
     for bad in (dict(axes=(0,) * 63), dict(axes=(4,) * 64), dict(axes=(-1,) * 64), dict(score_cap=-1.0), dict(score_cap=1e6),
                 dict(score_cap=float("nan")), dict(windows=(1,)), dict(windows=(1, -1)), dict(slopes=(1.0,)),
-                dict(slopes=(1.0, float("nan"))), dict(n_vocab=(1 << 20) + 1)):
+                dict(slopes=(1.0, float("nan")))):
         with pytest.raises(ValueError):
             B.BatchEngine(_Context(), {}, E.Config(**(base | bad)), 64, 8)
+
+
+def test_vocabularies_that_no_draw_takes(make, monkeypatch):  # noqa: F811
+    """They are decoded as any other; only drawing is refused."""
+    monkeypatch.setattr(B, "SAMPLE_VOCAB", 999)
+    eng, _ = make()
+    a = eng.open()
+    eng.step({a: 900})
+    with pytest.raises(ValueError):
+        eng.sample({a: 1}, {a: 2})
+    assert eng.length(a) == 1
 
 
 def test_rope_axes_table():
