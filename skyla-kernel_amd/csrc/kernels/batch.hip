@@ -115,6 +115,17 @@ SK_DEV Range row_range(const uint32_t *ctl, uint32_t rows_off, uint32_t row, uin
 // the longest of the rows (0: ctl[5] alone; layers of one step may have windows of their own).  No row attends to a
 // part of it: a row takes it with share != 0 and len >= P if it attends to all of it, lo <= S.  Its own pages serve
 // [lo, S), its lead, in n_lead parts (without lead parts lo must be S), and those from P on.
+// The bodies are attention_paged's, with these masks, scores and runs, so that what bounds them is the same.  Own runs of
+// rows that are one prompt's go together (16 query rows a workgroup for 2 to 8 as elsewhere): a chunk's 128 rows would
+// else read their common positions once each (73 -> 57 us a chunk behind a window of 4096 of 12000 positions).  A window
+// leaves out tiles before they are read: a pass of that chunk takes, with windows of 64 / 512 / 4096 / none, 33 / 43 / 62 /
+// 105 us.
+// Measured (MI355X, + merge): 8 rows of up to 100 own positions, capped, 8.0 us; 32 rows with a window of 1024, f16 keys
+// and 8-bit values, 27.5 + 4.2 (97 MB, 3.5 TB/s); 128 rows of 32 heads over 16384 shared and 300 own positions of 8 key
+// heads, capped, f16, 105 + 11.3 (products 0.76 PFLOP/s in two f16 parts); the chunk above 41.4 + 10.5; 100 rows of
+// documents to 4000 positions of 4 key heads, sloped, 8 bits, 34.5 + 8.3 (a partial's row each: 19 MB there and back).
+// What shaping costs a pass of those 128 rows (f16 / f16 keys, 8-bit values / 8 bits): scores as they are 122 / 146 / 157
+// us, sloped 130 / 151 / 162, capped 130 / 150 / 170, both 147 / 170 / 191: vector instructions beside the products.
 struct ShapedRange : Range {  // tail: [start, len), len the end hi
   uint32_t lo, at;            // lead: [lo, S) of a member; the position i
 };
@@ -169,11 +180,20 @@ SK_DEV bool rows_together(const uint32_t *ctl, uint32_t rows_off, uint32_t row, 
   }
   return one && most != 0 && most - least <= 256;
 }
-SK_DEV bool rows_together(const uint32_t *ctl, uint32_t rows_off, uint32_t row, uint32_t n_rows, uint32_t n_grid, uint32_t T) {
-  return T == 16  ? rows_together<16>(ctl, rows_off, row, n_rows, n_grid)
-         : T == 8 ? rows_together<8>(ctl, rows_off, row, n_rows, n_grid)
-         : T == 4 ? rows_together<4>(ctl, rows_off, row, n_rows, n_grid)
-                  : rows_together<2>(ctl, rows_off, row, n_rows, n_grid);
+// The same for a T that is known when the kernel runs, by whole waves, lane l with row l % T (the merge's: with each T
+// unrolled as above a launch of 100 rows took 8.8 us for 8.3).
+SK_DEV bool rows_together(const uint32_t *ctl, uint32_t rows_off, uint32_t row, uint32_t n_rows, uint32_t n_grid,
+                          uint32_t T) {
+  const uint32_t r = row / T * T + (threadIdx.x & (T - 1));
+  const uint2 w = *(const uint2 *)(ctl + rows_off + 4 * min(r, n_grid - 1));
+  const bool live = r < n_rows && w.y != 0;
+  const uint64_t m = __ballot(live);
+  const uint32_t seq = __builtin_amdgcn_readlane(w.x, m ? (uint32_t)__builtin_ctzll(m) : 0);
+  const bool one = m && !__ballot(live && w.x != seq);
+  uint32_t least = live ? w.y : ~0u, most = live ? w.y : 0;
+  for (uint32_t d = T / 2; d >= 1; d >>= 1)
+    least = min(least, (uint32_t)__shfl_xor(least, d, 64)), most = max(most, (uint32_t)__shfl_xor(most, d, 64));
+  return __builtin_amdgcn_readfirstlane(one && most - least <= 256);
 }
 // The positions of row row's own run, its tail or its lead, and of the run that it is part of.  (Whole waves: lane l
 // looks at row l % T of the rows that may go together.)
@@ -182,7 +202,8 @@ struct OwnRun {
   uint32_t seq, lane_lo, lane_hi, lane_at;  // row l % T's, in lane l
 };
 template <typename P>
-SK_DEV OwnRun own_run(const uint32_t *ctl, const P &p, uint32_t row, uint32_t n_rows, uint32_t T, bool together, uint32_t shared, bool lead) {
+SK_DEV OwnRun own_run(const uint32_t *ctl, const P &p, uint32_t row, uint32_t n_rows, uint32_t T, bool together,
+                      uint32_t shared, bool lead) {
   uint32_t lo = 0, hi = 0, seq = 0, at = 0;
   auto look = [&](uint32_t i) {
     const ShapedRange r = shaped_range(ctl, p, i, shared);
@@ -211,7 +232,8 @@ SK_DEV OwnRun own_run(const uint32_t *ctl, const P &p, uint32_t row, uint32_t n_
 template <typename P>
 SK_DEV float slope_of(const uint32_t *ctl, const P &p, uint32_t head) {
   if (p.slopes_off == ~0u) return 0.0f;
-  return __builtin_amdgcn_fmed3f(__builtin_bit_cast(float, ctl[p.slopes_off + head]), -0x1p16f, 0x1p16f) * 1.44269504088896340736f;
+  const float slope = __builtin_bit_cast(float, ctl[p.slopes_off + head]);
+  return __builtin_amdgcn_fmed3f(slope, -0x1p16f, 0x1p16f) * 1.44269504088896340736f;
 }
 // a row's range, whichever kernel's
 template <typename P>
@@ -287,7 +309,9 @@ SK_DEV void store_row(f16 *kv, int8_t *kv8, uint32_t cache, uint32_t scales, uin
 // kv_append_axes turns by positions of several axes (time, height, width of images and video): row r has four words
 // at axes_off + 4 r, and pair d's angle is the sum over the axes a < n_axes <= 4 of word a times the frequency
 // at rope_off + 64 a + d, formed in 64 bits.  A pair that one axis turns has its frequency at that axis and 0 at
-// the others, so any layout of sections is the table's.
+// the others, so any layout of sections is the table's.  A row's four words come with a load beside its others, and the
+// sum is four f64 products a lane: 1 row 2.8 us, 37 rows in 8 bits 4.4, 2048 rows of 48 heads, f16 keys and 8-bit values,
+// 42 (where a launch before left the caches written; the smallest 23), bound as kv_append is.
 template <int K8, int V8, int PASSES, int AXES>
 SK_DEV void append_body(const float *w, float *a, const uint32_t *ctl, f16 *kv, int8_t *kv8, const AppendPush &p,
                         uint32_t axes_off = 0, uint32_t n_axes = 0) {
@@ -429,7 +453,8 @@ SK_DEV float to_scalar(float v) {
 }
 SK_DEV Cap cap_of(float cap) {
   const float c = cap * 1.44269504088896340736f, inv = 1.0f / c, k = inv * inv;
-  Cap x{c, inv, 0.5f * c, {0.9999999869f, -0.3333306939f * k, 0.1332477932f * k * k, -0.0529860752f * k * k * k, 0.0171350065f * k * k * k * k}};
+  Cap x{c, inv, 0.5f * c, {0.9999999869f, -0.3333306939f * k, 0.1332477932f * k * k, -0.0529860752f * k * k * k,
+                           0.0171350065f * k * k * k * k}};
   x.c = to_scalar(x.c), x.inv = to_scalar(x.inv), x.edge = to_scalar(x.edge);
 #pragma unroll
   for (int i = 0; i < 5; i++) x.p[i] = to_scalar(x.p[i]);
@@ -595,7 +620,10 @@ SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
   if constexpr (SHAPED<P>) {
     all_lo = my_lo, all_hi = my_hi;
 #pragma unroll
-    for (int d = 8; d >= 1; d >>= 1) all_lo = max(all_lo, (uint32_t)__shfl_xor(all_lo, d, 64)), all_hi = min(all_hi, (uint32_t)__shfl_xor(all_hi, d, 64));
+    for (int d = 8; d >= 1; d >>= 1) {
+      all_lo = max(all_lo, (uint32_t)__shfl_xor(all_lo, d, 64));
+      all_hi = min(all_hi, (uint32_t)__shfl_xor(all_hi, d, 64));
+    }
     all_lo = __builtin_amdgcn_readfirstlane(all_lo), all_hi = __builtin_amdgcn_readfirstlane(all_hi);
   }
   const float unit = SHAPED<P> ? 1.0f : inv;  // of the scores as they are weighed
@@ -709,7 +737,8 @@ SK_DEV void wave_run(float *a, const uint32_t *ctl, const f16 *kv, const int8_t 
     const float cm = (float)E_SHIFT - (m > -INFINITY ? m : 0.0f);
     f16x8 ph, pl;
 #pragma unroll
-    for (int n = 0; n < 4; n++) weigh(sc[n >> 1][2 * (n & 1)], sc[n >> 1][2 * (n & 1) + 1], unit, unit, cm, l, ph, pl, 2 * n);
+    for (int n = 0; n < 4; n++)
+      weigh(sc[n >> 1][2 * (n & 1)], sc[n >> 1][2 * (n & 1) + 1], unit, unit, cm, l, ph, pl, 2 * n);
     f16x2 sv[V8 ? 4 : 1];
     if constexpr (V8) {
       const int up = 4 - ve + WINDOW<9> * window;
@@ -1315,7 +1344,8 @@ SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_
   const bool own = w >= n_first;
   uint32_t i0;  // query rows i0 + [0, n_live) of the key head: row i / N_REP, head i % N_REP
   Split sp;
-  [[maybe_unused]] uint32_t slot = 0, tile0 = 0, n_own_rows = N_REP;  // of an own run's partial; of the rows that may go together
+  // of an own run: its partial, the first of the rows that may go together, the query rows that do
+  [[maybe_unused]] uint32_t slot = 0, tile0 = 0, n_own_rows = N_REP;
   [[maybe_unused]] OwnRun run;
   if (!own) {
     if (shared == 0 || (SHAPED<P> && n_rows == 0)) return;
@@ -1429,7 +1459,8 @@ SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_
       *(float2 *)result(i, d) = make_float2(x / l, y / l);
     } else {
       float *out = a + p.part_off +
-                   ((i / N_REP * p.n_kv * N_REP + kvh * N_REP + i % N_REP) * slots + (SHAPED<P> && own ? slot : (own ? p.n_shared : 0) + part)) * PART;
+                   ((i / N_REP * p.n_kv * N_REP + kvh * N_REP + i % N_REP) * slots +
+                    (SHAPED<P> && own ? slot : (own ? p.n_shared : 0) + part)) * PART;
       *(float2 *)(out + 2 + 2 * d) = make_float2(x, y);
       if (d == 0) *(float2 *)out = make_float2(m, l);
     }

@@ -10,7 +10,6 @@
 //   n1  the tokens whose w >= min_p (0: all), at most top_k of them (0: all), at least one
 //   n2  the first n with C(n) >= top_p C(n1) (n1 where top_p is 1 or more)
 //   the token is the first with C(n) > (draw + 1/2) 2^-32 C(n2); kept = n2, logprob = ln(w / C(n2))
-// (What a draw reads of the histograms reaches no memory outside the row, whatever they hold.)
 // T = 0 (or below 0, or no number) takes the first of the order.  Logits of -inf or NaN have no weight and
 // no place; +inf counts as the type's largest value.  A row without tokens gets {~0, 0, -inf, 0}.
 //
@@ -18,7 +17,11 @@
 // t = x 8 log2(e) / T, one rint(t) each, in which a weight is 2^((t - rint(t)) / 8) of its bin's middle's.
 // A bin's count and sum of weights are integers (36 bits after the point: a weight is off by 8e-12 of itself at
 // most), the same in any order, and only the tokens of the bins in which a border lies (min_p's or top_k's,
-// top_p's, the draw's) are looked at one by one.
+// top_p's, the draw's) are looked at one by one.  No order of a whole row is ever made: a row is read once, by many
+// workgroups, and a draw reads an eighth of that (of 152k tokens 78 KB of bins) and what little lies around the borders.
+//
+// Measured (MI355X, 151936 tokens, both kernels): 1 row 6.2 + 10.7 us, 16 rows at their temperature alone 10.8 + 15.1,
+// 48 masked rows 16.6 + 10.8, 128 rows of wide nuclei 31.8 + 21.8.  A replay of two empty launches takes 14.7.
 #include "common.h"
 
 namespace {
@@ -121,6 +124,10 @@ SK_DEV float wave_max(float v) {
 }  // namespace
 
 // A workgroup's CHUNK tokens of a row: their bins below its own largest value, and the tokens in the bins' order.
+// 128 rows of 151936 tokens (78 MB read, 47 written) take 31.8 us: 41 vector instructions a token (10 us of the 32 went
+// with the moves of the series' constants), 57% of the cycles' issue, and the atomics' and lists' LDS banks (8 us) beside
+// them.  Chunks of 16384 (1024 threads, 61 registers) took 85 us for 78 then, 8 or 16 tokens on their way at once 83 and
+// 79, a workgroup that goes on to a second chunk with its loads ahead 101 (171 registers).
 extern "C" __global__ __launch_bounds__(THREADS) void logits_sample(float *a, const uint32_t *ctl, SamplePush p) {
 #pragma clang fp contract(off)
   constexpr uint32_t WAVES = THREADS / 64;
@@ -205,7 +212,8 @@ extern "C" __global__ __launch_bounds__(THREADS) void logits_sample(float *a, co
       const uint32_t i = (uint32_t)__builtin_ctz(far);
       const double s = scaled(x[4 * (t + THREADS * (i / 4)) + i % 4], c), g = __builtin_rint(s);
       // what is 2^-37 of the last bin's middle's or less adds nothing
-      if (first - g < BINS + 8 * 37) atomicAdd(&bin[BINS - 1], (unsigned long long)far_weight(series_, s - g, first - g));
+      if (first - g < BINS + 8 * 37)
+        atomicAdd(&bin[BINS - 1], (unsigned long long)far_weight(series_, s - g, first - g));
     }
   }
   __syncthreads();
@@ -249,8 +257,8 @@ constexpr uint32_t RUNS = 512;     // 3 * CHUNKS and more, a power of two
 constexpr uint32_t ID_BITS = 20;   // of a token's id
 constexpr uint32_t DIGITS = 2048;  // buckets of the search that takes any number of them
 
-// Where a row's borders lie: of bin b1 some tokens stay (BINS: all of all bins), as min_p has it if that is bm, as top_k
-// if bk; n2 ends in bins [p_lo, p_hi] and the draw falls into [d_lo, d_hi].
+// Where a row's borders lie: of bin b1 some tokens stay (BINS: all of all bins), as min_p has it if that is bm, as
+// top_k if bk; n2 ends in bins [p_lo, p_hi] and the draw falls into [d_lo, d_hi].
 struct Borders {
   double least;  // min_p's t
   uint32_t k, bm, bk, b1, p_lo, p_hi, d_lo, d_hi;
@@ -281,7 +289,7 @@ struct DrawShared {
   uint32_t counts[DRAW_WAVES];
   unsigned long long below;
   Borders at;
-  uint2 runs[RUNS];       // of the chunks' lists the tokens in each run of bins: where from, less its own place; its end here
+  uint2 runs[RUNS];       // of a chunk's list the tokens in a run of bins: where from, less their place here; their end
   uint32_t fits, found[2];
 };
 
@@ -299,10 +307,13 @@ SK_DEV uint32_t bin_of(const Row &r, double t) {
   const double d = r.edge - __builtin_rint(t);
   return d < BINS - 1 ? (uint32_t)(int)d : BINS - 1;
 }
-SK_DEV uint64_t fixed_weight(const Series &k, const Row &r, double t) { return fixed_weight_at(k, t, r.edge - __builtin_rint(t)); }
+SK_DEV uint64_t fixed_weight(const Series &k, const Row &r, double t) {
+  return fixed_weight_at(k, t, r.edge - __builtin_rint(t));
+}
 // a sum of a bin's weights
 SK_DEV double sum_of(uint64_t fixed, double edge) { return (double)fixed * 0x1p-36 * edge; }
-constexpr double UP = 1.0442737824274138, DOWN = 0.9576032806985737;  // 2^(1/16), 2^(-1/16): a weight of its bin's middle's
+// 2^(1/16), 2^(-1/16): a weight's bounds in its bin's middle's
+constexpr double UP = 1.0442737824274138, DOWN = 0.9576032806985737;
 
 // Every value of the row that may lie in [least, most) by its t, among them all that do: f(place, t).
 template <typename F>
@@ -468,7 +479,14 @@ SK_DEV uint32_t first_of(uint32_t n, F ok) {
 
 }  // namespace
 
-// A workgroup's row: its chunks' bins added up, the bins with the borders, and the tokens in these.
+// A workgroup's row: its chunks' bins added up, the bins with the borders, and the tokens in these.  What it reads of the
+// partials reaches no memory outside the row, whatever they hold.
+// Of a row of 151936 tokens whose borders' bins hold 6 / 1050 / 6000 tokens (23 / 38 / 50 thousand cycles): the partials'
+// heads 2400, their bins 6700, scans 1500, borders 3100 to 3700, the gather 4300 / 12200 / 21900 (two dependent loads a
+// token, from memory), buckets and order 150 / 2700 / 4600, the borders among them 4400 / 9000 / 11000.  Bound by chains
+// of loads and barriers of the one workgroup that a row has.  Against all values put in order, as before (27.8 us for 128
+// rows), ordering the three borders' buckets alone took 26.1, and the gather's values spread evenly over the workgroup,
+// not by their chunks, 21.8; a count of places by waves, or the same loads behind branches, changed nothing.
 extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, const uint32_t *ctl, DrawPush p) {
 #pragma clang fp contract(off)
   __shared__ DrawShared s;
@@ -572,7 +590,8 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
       }
       if (b1 == 0) lo = fmax(lo, DOWN * LESS);  // the largest stays
     }
-    const uint32_t b_last = min(b1, first_bin(s.n, [&](uint32_t n) { return n >= total; }));  // where n1 lies, or past it
+    // where n1 lies, or past it
+    const uint32_t b_last = min(b1, first_bin(s.n, [&](uint32_t n) { return n >= total; }));
     uint32_t p_lo = b_last, p_hi = b_last;  // where n2 lies
     if (by_p) {
       lo *= share * LESS, hi *= share * MORE;
@@ -587,8 +606,8 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
   }
   __syncthreads();
   const double least = s.at.least;
-  const uint32_t k = s.at.k, bm = s.at.bm, bk = s.at.bk, b1 = s.at.b1, p_lo = s.at.p_lo, p_hi = s.at.p_hi, d_lo = s.at.d_lo,
-                 d_hi = s.at.d_hi;
+  const uint32_t k = s.at.k, bm = s.at.bm, bk = s.at.bk, b1 = s.at.b1, p_lo = s.at.p_lo, p_hi = s.at.p_hi;
+  const uint32_t d_lo = s.at.d_lo, d_hi = s.at.d_hi;
   // up to three runs of bins [f, e], each below the one before (one that is not there: f = ~0)
   uint32_t f0 = d_lo, e0 = d_hi, f1 = ~0u, e1 = 0, f2 = ~0u, e2 = 0;
   if (by_p) {
@@ -629,7 +648,8 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
       if (which < runs) {
         const uint32_t f = which == 0 ? f0 : which == 1 && f1 != ~0u ? f1 : f2;
         const uint32_t e = which == 0 ? e0 : which == 1 && f1 != ~0u ? e1 : e2, down = s.down[i];
-        if (down <= e) run = make_uint2(f > down ? s.ends[i][f - down - 1] : 0, min((uint32_t)s.ends[i][e - down], CHUNK));
+        if (down <= e)
+          run = make_uint2(f > down ? s.ends[i][f - down - 1] : 0, min((uint32_t)s.ends[i][e - down], CHUNK));
       }
       uint32_t all;
       const uint32_t end = block_scan(run.y - run.x, s.counts, all);
@@ -723,7 +743,8 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
           for (uint32_t i = 0; i < m; i++) rank += s.place[1][o0 + i] < v;
           sorted[rank] = v;
         }
-        const uint32_t span = q / per, b = span >= span2 ? f2 + span - span2 : span >= span1 ? f1 + span - span1 : f0 + span;
+        const uint32_t span = q / per;
+        const uint32_t b = span >= span2 ? f2 + span - span2 : span >= span1 ? f1 + span - span1 : f0 + span;
         uint64_t before = sum_before(q) - sum_before(span * per);
         for (uint32_t j0 = 0; j0 < m; j0 += 64) {
           const uint32_t j = j0 + t;
@@ -738,7 +759,9 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
       };
       // the token at place i of the order here (within a run of bins places and ranks go together), if it lies in order
       auto found_at = [&](uint32_t i) {
-        const uint32_t rank = i >= at2 && f2 != ~0u ? s.n[f2] + i - at2 : i >= at1 && f1 != ~0u ? s.n[f1] + i - at1 : s.n[f0] + i;
+        const uint32_t rank = i >= at2 && f2 != ~0u   ? s.n[f2] + i - at2
+                              : i >= at1 && f1 != ~0u ? s.n[f1] + i - at1
+                                                      : s.n[f0] + i;
         const uint32_t j = min(i - o0, RANKED - 1);
         return Found{sorted[j], rank + 1, upto[j]};
       };
@@ -802,6 +825,7 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
   }
   if (t == 0) {
     const double y = (scaled(value_at(chosen.place), r.c) - r.edge) * 0.125 * 0.69314718055994530942 - log(n2.sum);
-    *(uint4 *)out = make_uint4((uint32_t)chosen.place & ((1u << ID_BITS) - 1), n2.n, __builtin_bit_cast(uint32_t, n2.n == 1 ? 0.0f : (float)y), 0);
+    const uint32_t id = (uint32_t)chosen.place & ((1u << ID_BITS) - 1);
+    *(uint4 *)out = make_uint4(id, n2.n, __builtin_bit_cast(uint32_t, n2.n == 1 ? 0.0f : (float)y), 0);
   }
 }
