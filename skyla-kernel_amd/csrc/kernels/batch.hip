@@ -121,9 +121,9 @@ SK_DEV Range row_range(const uint32_t *ctl, uint32_t rows_off, uint32_t row, uin
 // leaves out tiles before they are read: a pass of that chunk takes, with windows of 64 / 512 / 4096 / none, 33 / 43 / 62 /
 // 105 us.
 // Measured (MI355X, + merge): 8 rows of up to 100 own positions, capped, 8.0 us; 32 rows with a window of 1024, f16 keys
-// and 8-bit values, 27.5 + 4.2 (97 MB, 3.5 TB/s); 128 rows of 32 heads over 16384 shared and 300 own positions of 8 key
-// heads, capped, f16, 105 + 11.3 (products 0.76 PFLOP/s in two f16 parts); the chunk above 41.4 + 10.5; 100 rows of
-// documents to 4000 positions of 4 key heads, sloped, 8 bits, 34.5 + 8.3 (a partial's row each: 19 MB there and back).
+// and 8-bit values, 27.5 + 4.3 (97 MB, 3.5 TB/s); 128 rows of 32 heads over 16384 shared and 300 own positions of 8 key
+// heads, capped, f16, 105 + 11.5 (products 0.72 PFLOP/s in two f16 parts); the chunk above 41.8 + 9.6; 100 rows of
+// documents to 4000 positions of 4 key heads, sloped, 8 bits, 34.5 + 7.6 (partials of 20 MB written and read).
 // What shaping costs a pass of those 128 rows (f16 / f16 keys, 8-bit values / 8 bits): scores as they are 122 / 146 / 157
 // us, sloped 130 / 151 / 162, capped 130 / 150 / 170, both 147 / 170 / 191: vector instructions beside the products.
 struct ShapedRange : Range {  // tail: [start, len), len the end hi
@@ -181,7 +181,7 @@ SK_DEV bool rows_together(const uint32_t *ctl, uint32_t rows_off, uint32_t row, 
   return one && most != 0 && most - least <= 256;
 }
 // The same for a T that is known when the kernel runs, by whole waves, lane l with row l % T (the merge's: with each T
-// unrolled as above a launch of 100 rows took 8.8 us for 8.3).
+// unrolled as above a launch of 100 rows took 8.8 us for 8.4).
 SK_DEV bool rows_together(const uint32_t *ctl, uint32_t rows_off, uint32_t row, uint32_t n_rows, uint32_t n_grid,
                           uint32_t T) {
   const uint32_t r = row / T * T + (threadIdx.x & (T - 1));
@@ -1526,27 +1526,38 @@ PAGED_REP(1, 1)
 template <uint32_t W, typename P>
 SK_DEV void paged_merge(float *a, const uint32_t *ctl, const P &p, uint32_t h, uint32_t row, uint32_t wave,
                         uint32_t lane) {
-  const uint32_t shared = shared_end(ctl, p);
-  const auto r = range_of(ctl, p, row, shared);
   uint32_t ns, no, nl = 0;  // live partials: the shared run's, the row's own, its lead's
   uint32_t o0 = p.n_shared, l0 = 0;  // the first of the latter two
   if constexpr (SHAPED<P>) {
-    const uint32_t n_rows = min(ctl[2], gridDim.y);  // the attention's
-    const bool together = rows_together(ctl, p.rows_off, row, n_rows, gridDim.y, 16 / p.rep);
-    // the parts of [x.all_lo, x.all_hi) with some of [x.lo, x.hi)
-    auto parts_of = [&](bool lead, uint32_t n_parts, uint32_t &at) {
-      const OwnRun x = own_run(ctl, p, row, n_rows, 16 / p.rep, together, shared, lead);
-      if (x.lo >= x.hi) return 0u;
-      const Split sp = split_of(x.all_lo, x.all_hi, n_parts);
-      const uint32_t k = min((x.lo - sp.base) / TILE / sp.per, n_parts - 1);
-      at += k;
-      return min((x.hi - 1 - sp.base) / TILE / sp.per, n_parts - 1) - k + 1;
-    };
-    ns = r.member ? live_parts(split_of(shared_first(ctl, p, shared), shared, p.n_shared)) : 0;
-    no = parts_of(false, p.n_own, o0);
-    l0 = p.n_shared + p.n_own;
-    if (p.n_lead) nl = parts_of(true, p.n_lead, l0);
+    // by the first wave for all of the workgroup's heads (500 vector instructions: by each wave a launch of 100 rows and 12
+    // partials took 8.4 us for 7.6, of 128 rows and 10 10.4 for 9.6)
+    __shared__ uint32_t of_row[5];
+    if (threadIdx.x < 64) {
+      const uint32_t shared = shared_end(ctl, p);
+      const auto r = range_of(ctl, p, row, shared);
+      const uint32_t n_rows = min(ctl[2], gridDim.y);  // the attention's
+      const bool together = rows_together(ctl, p.rows_off, row, n_rows, gridDim.y, 16 / p.rep);
+      // the parts of [x.all_lo, x.all_hi) with some of [x.lo, x.hi)
+      auto parts_of = [&](bool lead, uint32_t n_parts, uint32_t &at) {
+        const OwnRun x = own_run(ctl, p, row, n_rows, 16 / p.rep, together, shared, lead);
+        if (x.lo >= x.hi) return 0u;
+        const Split sp = split_of(x.all_lo, x.all_hi, n_parts);
+        const uint32_t k = min((x.lo - sp.base) / TILE / sp.per, n_parts - 1);
+        at += k;
+        return min((x.hi - 1 - sp.base) / TILE / sp.per, n_parts - 1) - k + 1;
+      };
+      ns = r.member ? live_parts(split_of(shared_first(ctl, p, shared), shared, p.n_shared)) : 0;
+      no = parts_of(false, p.n_own, o0);
+      l0 = p.n_shared + p.n_own;
+      if (p.n_lead) nl = parts_of(true, p.n_lead, l0);
+      if (lane == 0) of_row[0] = ns, of_row[1] = no, of_row[2] = nl, of_row[3] = o0, of_row[4] = l0;
+    }
+    __syncthreads();
+    ns = of_row[0], no = of_row[1], nl = of_row[2], o0 = of_row[3], l0 = of_row[4];
+    if (h >= p.n_head) return;
   } else {
+    const uint32_t shared = shared_end(ctl, p);
+    const auto r = range_of(ctl, p, row, shared);
     ns = r.member ? live_parts(split_of(0, shared, p.n_shared)) : 0;
     no = live_parts(split_of(r.start, r.len, p.n_own));
   }
@@ -1610,7 +1621,7 @@ extern "C" __global__ __launch_bounds__(512) void attention_paged_merge_8__128(f
 extern "C" __global__ __launch_bounds__(256) void attention_paged_shaped_merge__128(float *a, const uint32_t *ctl,
                                                                                     ShapedMergePush p) {
   const uint32_t h = blockIdx.x * 4 + (threadIdx.x >> 6), row = blockIdx.y;
-  if (row < ctl[2] && h < p.n_head) paged_merge<1>(a, ctl, p, h, row, 0, threadIdx.x & 63);
+  if (row < ctl[2]) paged_merge<1>(a, ctl, p, h, row, 0, threadIdx.x & 63);
 }
 extern "C" __global__ __launch_bounds__(512) void attention_paged_shaped_merge_8__128(float *a, const uint32_t *ctl,
                                                                                       ShapedMergePush p) {
