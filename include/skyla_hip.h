@@ -88,8 +88,9 @@ int skyla_hip_buffer_copy(skyla_hip_buffer *dst, uint64_t dst_off, const skyla_h
 /* Context::create_pipeline_sets(shader, n_buffers, push_size, spec, n_sets).
  * `name` is the reference shader name (matvec_q4k, matvec_q6k, matvec_q8_0, matmul,
  * moe_logits, moe_route, moe_sort, moe_combine, silu_mul, to_half, bandwidth), or one of a
- * served batch's, which the reference lacks: kv_append, attention_paged,
- * attention_paged_merge, logits_adjust.  Their push words and grid are checked against the
+ * served batch's, which the reference lacks: kv_append, kv_append_axes, attention_paged,
+ * attention_paged_merge, attention_paged_shaped, attention_paged_shaped_merge,
+ * logits_adjust, logits_sample, logits_sample_draw.  Their push words and grid are checked against the
  * bound buffers when they are dispatched (SKYLA_HIP_E_ARG).  The
  * kernel is the gfx950 instantiation for `spec`; an unknown (name, spec) fails with
  * SKYLA_HIP_E_NO_KERNEL, as a shader that does not compile fails pipeline creation.
