@@ -158,8 +158,16 @@ class ShapedParts(NamedTuple):
 
 def shaped_splits(rows: int, n_kv: int, rep: int, shared: int, own: int, lead: int = 0) -> ShapedParts:
     """Parts for a shared run of `shared` positions, at most `own` of a row's own and `lead` of those
-    before the run."""
+    before the run.
+
+    Where nothing is shared one part saves the merge.  It is taken from 256 rows x key heads on, and below for up
+    to 8 positions for each of these.  A pass of 8 key heads, f16, us in one part / the best of two and more: 8
+    rows of 512 / 1024 / 2048 positions 22.0 / 23.5, 27.7 / 25.8, 36.8 / 30.1; 16 rows 23.7 / 26.1, 28.0 / 31.3,
+    39.3 / 39.0; 24 rows 24.1 / 31.4, 30.7 / 37.7, 51.2 / 52.7; 32 rows 25.9 / 32.1, 34.0 / 40.4, 60.6 / 67.3, of
+    4096 99.9 / 113; 48 rows of 4096 168 / 157."""
     parts = splits(rows, n_kv, rep, shared, own)
+    if shared == 0 and (n_kv * rows >= 256 or own <= 8 * n_kv * rows):
+        parts = Parts(0, 1)
     n_lead = max(1, min(-(-512 // (n_kv * rows)), -(-lead // 256), 128)) if lead and shared else 0
     return ShapedParts(*parts, n_lead)
 
