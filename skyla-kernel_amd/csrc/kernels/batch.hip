@@ -121,7 +121,7 @@ SK_DEV Range row_range(const uint32_t *ctl, uint32_t rows_off, uint32_t row, uin
 // leaves out tiles before they are read: a pass of that chunk takes, with windows of 64 / 512 / 4096 / none, 33 / 43 / 62 /
 // 105 us.
 // Measured (MI355X, + merge): 8 rows of up to 100 own positions, capped, 8.0 us; 32 rows with a window of 1024, f16 keys
-// and 8-bit values, 27.5 + 4.3 (97 MB, 3.5 TB/s); 128 rows of 32 heads over 16384 shared and 300 own positions of 8 key
+// and 8-bit values, 27.8, no merge (97 MB, 3.5 TB/s); 128 rows of 32 heads over 16384 shared and 300 own positions of 8 key
 // heads, capped, f16, 105 + 11.5 (products 0.72 PFLOP/s in two f16 parts); the chunk above 41.8 + 9.6; 100 rows of
 // documents to 4000 positions of 4 key heads, sloped, 8 bits, 34.5 + 7.6 (partials of 20 MB written and read).
 // What shaping costs a pass of those 128 rows (f16 / f16 keys, 8-bit values / 8 bits): scores as they are 122 / 146 / 157

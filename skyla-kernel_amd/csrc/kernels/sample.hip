@@ -20,8 +20,8 @@
 // top_p's, the draw's) are looked at one by one.  No order of a whole row is ever made: a row is read once, by many
 // workgroups, and a draw reads an eighth of that (of 152k tokens 78 KB of bins) and what little lies around the borders.
 //
-// Measured (MI355X, 151936 tokens, both kernels): 1 row 6.2 + 10.7 us, 16 rows at their temperature alone 10.8 + 15.1,
-// 48 masked rows 16.6 + 10.8, 128 rows of wide nuclei 31.8 + 21.8.  A replay of two empty launches takes 14.7.
+// Measured (MI355X, 151936 tokens, both kernels): 1 row 6.2 + 10.6 us, 16 rows at their temperature alone 10.2 to 11 + 14.9,
+// 48 masked rows 16.6 + 10.6, 128 rows of wide nuclei 31.9 + 22.  A replay of two empty launches takes 14.7.
 #include "common.h"
 
 namespace {
@@ -293,6 +293,12 @@ struct DrawShared {
   uint32_t fits, found[2];
 };
 
+// What lies `bytes` past an address that is the same for all lanes: an offset of 32 bits a lane is one register and no
+// sum (a draw is bound by what one compute unit issues).
+template <typename T>
+SK_DEV T past(const void *base, uint32_t bytes) {
+  return *(const T *)((const char *)base + bytes);
+}
 template <uint32_t U>
 struct Count {
   static constexpr uint32_t value = U;
@@ -481,12 +487,13 @@ SK_DEV uint32_t first_of(uint32_t n, F ok) {
 
 // A workgroup's row: its chunks' bins added up, the bins with the borders, and the tokens in these.  What it reads of the
 // partials reaches no memory outside the row, whatever they hold.
-// Of a row of 151936 tokens whose borders' bins hold 6 / 1050 / 6000 tokens (23 / 38 / 50 thousand cycles): the partials'
-// heads 2400, their bins 6700, scans 1500, borders 3100 to 3700, the gather 4300 / 12200 / 21900 (two dependent loads a
-// token, from memory), buckets and order 150 / 2700 / 4600, the borders among them 4400 / 9000 / 11000.  Bound by chains
-// of loads and barriers of the one workgroup that a row has.  Against all values put in order, as before (27.8 us for 128
+// Of a row of 151936 tokens whose borders' bins hold 6 / 1050 / 6000 tokens (22 / 37 / 50 thousand cycles): the partials'
+// heads 2400, their bins 5900, scans 1600, borders 3100 to 3700, the gather 4300 / 12000 / 22000 (two dependent loads a
+// token, from memory), buckets and order 150 / 2700 / 4500, the borders among them 4200 / 8900 / 10400.  Bound by chains
+// of loads and barriers and by the issue of the one workgroup that a row has.  Against all values put in order, as before (27.8 us for 128
 // rows), ordering the three borders' buckets alone took 26.1, and the gather's values spread evenly over the workgroup,
-// not by their chunks, 21.8; a count of places by waves, or the same loads behind branches, changed nothing.
+// not by their chunks, 21.8 to 22.1; a count of places by waves, or the same loads behind branches, changed nothing, the bins on
+// their way beside the heads, through LDS, cost 1 us.
 extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, const uint32_t *ctl, DrawPush p) {
 #pragma clang fp contract(off)
   __shared__ DrawShared s;
@@ -522,21 +529,21 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
 
   // the row's bins: thread t has bin t % BINS of every other chunk
   {
-    const uint32_t b = t % BINS;
+    const uint32_t b = t % BINS, first = __builtin_amdgcn_readfirstlane(t / BINS);  // (waves of one chunk each)
     uint32_t n = 0;  // tokens that end with it
-    uint64_t sum = 0;
+    uint64_t sum = 0, below = 0;
     constexpr uint32_t U = 10, STEP = DRAW / BINS;  // chunks whose loads are in flight
-    for (uint32_t i0 = t / BINS; i0 < n_chunks; i0 += U * STEP) {
+    for (uint32_t i0 = first; i0 < n_chunks; i0 += U * STEP) {
       uint64_t w[U], low[U];
-      uint32_t downs[U];
+      uint32_t downs[U], deep = 0;
 #pragma unroll
       for (uint32_t j = 0; j < U; j++) {
         const uint32_t i = min(i0 + j * STEP, n_chunks - 1);
-        const uint64_t *bins = (const uint64_t *)(parts + (size_t)i * PART + HEAD);
-        downs[j] = i0 + j * STEP < n_chunks ? s.down[i] : ~0u;
-        w[j] = bins[b >= downs[j] ? b - downs[j] : 0];
+        const void *bins = parts + (size_t)i * PART + HEAD;
+        downs[j] = i0 + j * STEP < n_chunks ? __builtin_amdgcn_readfirstlane(s.down[i]) : ~0u;
+        w[j] = past<uint64_t>(bins, b >= downs[j] ? 8 * (b - downs[j]) : 0);
         // the chunk's bin b, if it lies in the row's last
-        low[j] = downs[j] != ~0u && b + downs[j] >= BINS - 1 ? bins[b] : 0;
+        low[j] = downs[j] != ~0u && b + downs[j] >= BINS - 1 ? past<uint64_t>(bins, 8 * b) : 0;
       }
 #pragma unroll
       for (uint32_t j = 0; j < U; j++) {
@@ -548,12 +555,16 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
           s.ends[i][b - downs[j]] = end;
         }
         if (b == BINS - 1) n += (uint32_t)(low[j] >> COUNT_AT);  // how many the chunk has
-        if (low[j] & SUM) {  // in weights of the last bin's middle
-          const double by = exp2(((double)(BINS - 1) - (double)b - (r.edge - s.first[i])) * 0.125);
-          atomicAdd(&s.below, (unsigned long long)__builtin_rint((double)(low[j] & SUM) * by));
-        }
+        if (low[j] & SUM) deep |= 1u << j;
+      }
+      for (; deep; deep &= deep - 1) {  // in weights of the last bin's middle (read again: few rows reach so deep)
+        const uint32_t i = i0 + (uint32_t)__builtin_ctz(deep) * STEP;
+        const uint64_t low = ((const uint64_t *)(parts + (size_t)i * PART + HEAD))[b];
+        const double by = exp2(((double)(BINS - 1) - (double)b - (r.edge - s.first[i])) * 0.125);
+        below += (uint64_t)__builtin_rint((double)(low & SUM) * by);
       }
     }
+    if (below) atomicAdd(&s.below, (unsigned long long)below);
     if (t >= BINS) s.half_sum[b] = sum, s.half_n[b] = n;
     __syncthreads();
     double c = 0.0, c_all;
@@ -670,12 +681,12 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
         for (uint32_t u = 0; u < U; u++) j[u] += s.runs[j[u] + h - 1].y <= min(t + DRAW * u, n - 1) ? h : 0;
 #pragma unroll
       for (uint32_t u = 0; u < U; u++) {
-        const uint32_t i = j[u] % n_chunks;
-        const uint16_t *ids = (const uint16_t *)(parts + (size_t)i * PART + HEAD + 2 * BINS);
-        id[u] = min(i * CHUNK + ids[min(s.runs[j[u]].x + min(t + DRAW * u, n - 1), CHUNK - 1)], r.n_vocab - 1);
+        const uint32_t i = j[u] < n_chunks ? j[u] : j[u] < 2 * n_chunks ? j[u] - n_chunks : j[u] - 2 * n_chunks;
+        const uint32_t at = min(s.runs[j[u]].x + min(t + DRAW * u, n - 1), CHUNK - 1);
+        id[u] = past<uint16_t>(parts + HEAD + 2 * BINS, min(i, n_chunks - 1) * (PART * 4) + 2 * at) + i * CHUNK;
       }
 #pragma unroll
-      for (uint32_t u = 0; u < U; u++) x[u] = r.x[id[u]];
+      for (uint32_t u = 0; u < U; u++) id[u] = min(id[u], r.n_vocab - 1), x[u] = past<float>(r.x, 4 * id[u]);
 #pragma unroll
       for (uint32_t u = 0; u < U; u++) {
         if (t + DRAW * u >= n) break;
