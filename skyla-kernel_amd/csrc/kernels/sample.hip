@@ -263,9 +263,16 @@ struct Borders {
   double least;  // min_p's t
   uint32_t k, bm, bk, b1, p_lo, p_hi, d_lo, d_hi;
 };
+// The tokens of up to three runs of bins, as the chunks list them: run w of chunk i is run w n_chunks + i of all.  Bin f
+// of them, f0 and on, f1 and on (~0: none) and f2, is span 0 and on, span1 and on, span2, each of `per` buckets.
+struct Lists {
+  uint32_t f0, f1, f2, span1, span2, per, n_chunks, half, n;
+};
 struct DrawShared {
   union {
-    uint64_t place[2][MOST];  // as they came, then those of one bucket in order and behind them C there; by buckets
+    // few: as they came, then those of one bucket in order and behind them C there; by buckets.  More: those of one
+    // bucket in order, C there; as they came, and how many end with a bucket.
+    uint64_t place[2][MOST];
     struct {
       unsigned long long sum[DIGITS];
       uint32_t count[DIGITS];
@@ -274,7 +281,7 @@ struct DrawShared {
   };
   union {
     uint64_t half_sum[BINS];
-    uint32_t next[DRAW];  // a bucket's next free place
+    uint32_t next[DRAW];  // a bucket's next free place, or how many it has
   };
   uint32_t half_n[BINS];
   float largest[CHUNKS];
@@ -290,7 +297,8 @@ struct DrawShared {
   unsigned long long below;
   Borders at;
   uint2 runs[RUNS];       // of a chunk's list the tokens in a run of bins: where from, less their place here; their end
-  uint32_t fits, found[2];
+  Lists lists;
+  uint32_t fits, fill, found[2];
 };
 
 // What lies `bytes` past an address that is the same for all lanes: an offset of 32 bits a lane is one register and no
@@ -483,6 +491,73 @@ SK_DEV uint32_t first_of(uint32_t n, F ok) {
   return hi;
 }
 
+SK_DEV uint32_t bucket_of(const Row &r, const Lists &l, double v) {
+  const double g = __builtin_rint(v), f = 0.5 - (v - g);
+  const uint32_t b = (uint32_t)(int)(r.edge - g);
+  const uint32_t i = b >= l.f2 ? l.span2 + b - l.f2 : b >= l.f1 ? l.span1 + b - l.f1 : b - l.f0;
+  return min(i * l.per + min((uint32_t)(int)(f * (double)l.per), l.per - 1), DRAW - 1);
+}
+// The lists' tokens base + t + DRAW u of thread t, all of them on their way at once: f(number, logit, id).
+template <uint32_t U, typename F>
+SK_DEV void each_listed(const DrawShared &s, const Row &r, const float *parts, const Lists &l, uint32_t base, F f) {
+  uint32_t id[U], j[U];
+  float x[U];
+  auto number = [&](uint32_t u) { return base + threadIdx.x + DRAW * u; };
+#pragma unroll
+  for (uint32_t u = 0; u < U; u++) j[u] = 0;
+  for (uint32_t h = l.half; h; h /= 2)  // the first run that ends behind it
+#pragma unroll
+    for (uint32_t u = 0; u < U; u++) j[u] += s.runs[j[u] + h - 1].y <= min(number(u), l.n - 1) ? h : 0;
+#pragma unroll
+  for (uint32_t u = 0; u < U; u++) {
+    const uint32_t i = j[u] < l.n_chunks ? j[u] : j[u] < 2 * l.n_chunks ? j[u] - l.n_chunks : j[u] - 2 * l.n_chunks;
+    const uint32_t at = min(s.runs[j[u]].x + min(number(u), l.n - 1), CHUNK - 1);
+    id[u] = past<uint16_t>(parts + HEAD + 2 * BINS, min(i, l.n_chunks - 1) * (PART * 4) + 2 * at) + i * CHUNK;
+  }
+#pragma unroll
+  for (uint32_t u = 0; u < U; u++) id[u] = min(id[u], r.n_vocab - 1), x[u] = past<float>(r.x, 4 * id[u]);
+#pragma unroll
+  for (uint32_t u = 0; u < U; u++) {
+    if (number(u) >= l.n) break;
+    f(number(u), x[u], id[u]);
+  }
+}
+// More tokens than LDS takes: how many each bucket has and their sums, up to each
+__device__ __attribute__((noinline)) void tally(DrawShared &s, const Row r, const float *parts) {
+  const Lists l = s.lists;
+  const Series series_ = series();
+  const uint32_t t = threadIdx.x;
+  s.next[t] = 0;
+  __syncthreads();
+  for (uint32_t base = 0; base < l.n; base += MOST)
+    each_listed<MOST / DRAW>(s, r, parts, l, base, [&](uint32_t, float x, uint32_t) {
+      const double v = scaled(x, r.c);
+      const uint32_t b = bucket_of(r, l, v);
+      atomicAdd(&s.bucket[b], (unsigned long long)fixed_weight(series_, r, v));
+      atomicAdd(&s.next[b], 1u);
+    });
+  __syncthreads();
+  uint64_t sum;
+  uint32_t count;
+  s.bucket[t] = block_scan((uint64_t)s.bucket[t], s.words, sum);
+  ((uint32_t *)s.place[1])[2 * RANKED + t] = block_scan(s.next[t], s.counts, count);
+  __syncthreads();
+}
+// and the tokens of bucket q, RANKED at most
+__device__ __attribute__((noinline)) void collect(DrawShared &s, const Row r, const float *parts, uint32_t q) {
+  const Lists l = s.lists;
+  __syncthreads();
+  if (threadIdx.x == 0) s.fill = 0;
+  __syncthreads();
+  for (uint32_t base = 0; base < l.n; base += MOST)
+    each_listed<MOST / DRAW>(s, r, parts, l, base, [&](uint32_t, float x, uint32_t id) {
+      if (bucket_of(r, l, scaled(x, r.c)) != q) return;
+      const uint32_t to = atomicAdd(&s.fill, 1u);
+      if (to < RANKED) s.place[1][to] = place(x, id);
+    });
+  __syncthreads();
+}
+
 }  // namespace
 
 // A workgroup's row: its chunks' bins added up, the bins with the borders, and the tokens in these.  What it reads of the
@@ -641,16 +716,12 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
   span2 = n_spans, at2 = n;
   if (f2 != ~0u) n_spans++, n += s.n[e2 + 1] - s.n[f2], deepest = e2;
   Found n2, chosen;
-  bool many = n_spans > SPANS || n > MOST || deepest == BINS - 1;
+  bool many = n_spans > SPANS || deepest == BINS - 1;
   if (!many) {
-    // ---- few: from the chunks' lists into LDS, in buckets by t
+    // ---- few: from the chunks' lists into LDS, in buckets by t; more: sums of the buckets, then those with borders
+    const bool few = n <= MOST;
     const uint32_t per = DRAW / n_spans;
     const float per_inverse = 1.0f / (float)per;
-    auto bucket_of = [&](double v) {
-      const double g = __builtin_rint(v), f = 0.5 - (v - g);
-      const uint32_t b = (uint32_t)(int)(r.edge - g), i = b >= f2 ? span2 + b - f2 : b >= f1 ? span1 + b - f1 : b - f0;
-      return min(i * per + min((uint32_t)(int)(f * (double)per), per - 1), DRAW - 1);
-    };
     const uint32_t runs = 1 + (f1 != ~0u) + (f2 != ~0u);
     const Series series_ = series();
     {
@@ -669,40 +740,25 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
     __syncthreads();
     uint32_t half = 1;
     while (2 * half < n_chunks * runs) half *= 2;
-    // thread t has the values t + DRAW u, all of them on their way at once
-    auto gather = [&](auto u_) {
-      constexpr uint32_t U = decltype(u_)::value;
-      uint32_t id[U], j[U];
-      float x[U];
-#pragma unroll
-      for (uint32_t u = 0; u < U; u++) j[u] = 0;
-      for (uint32_t h = half; h; h /= 2)  // the first run that ends behind it
-#pragma unroll
-        for (uint32_t u = 0; u < U; u++) j[u] += s.runs[j[u] + h - 1].y <= min(t + DRAW * u, n - 1) ? h : 0;
-#pragma unroll
-      for (uint32_t u = 0; u < U; u++) {
-        const uint32_t i = j[u] < n_chunks ? j[u] : j[u] < 2 * n_chunks ? j[u] - n_chunks : j[u] - 2 * n_chunks;
-        const uint32_t at = min(s.runs[j[u]].x + min(t + DRAW * u, n - 1), CHUNK - 1);
-        id[u] = past<uint16_t>(parts + HEAD + 2 * BINS, min(i, n_chunks - 1) * (PART * 4) + 2 * at) + i * CHUNK;
-      }
-#pragma unroll
-      for (uint32_t u = 0; u < U; u++) id[u] = min(id[u], r.n_vocab - 1), x[u] = past<float>(r.x, 4 * id[u]);
-#pragma unroll
-      for (uint32_t u = 0; u < U; u++) {
-        if (t + DRAW * u >= n) break;
-        // (with the bucket above the id: it goes by the value, so that the order is the same)
-        const double v = scaled(x[u], r.c);
-        const uint32_t b = n > 64 ? bucket_of(v) : 0;
-        s.place[0][t + DRAW * u] = place(x[u], id[u] | b << ID_BITS);
-        if (n > 64) atomicAdd(&s.bucket[b], (unsigned long long)fixed_weight(series_, r, v) + (1ull << COUNT_AT));
-      }
+    const Lists lists{f0, f1, f2, span1, span2, per, n_chunks, half, n};
+    auto take = [&](uint32_t i, float x, uint32_t id) {
+      // (with the bucket above the id: it goes by the value, so that the order is the same)
+      const double v = scaled(x, r.c);
+      const uint32_t b = n > 64 ? bucket_of(r, lists, v) : 0;
+      s.place[0][i] = place(x, id | b << ID_BITS);
+      if (n > 64) atomicAdd(&s.bucket[b], (unsigned long long)fixed_weight(series_, r, v) + (1ull << COUNT_AT));
     };
-    if (n <= DRAW)
-      gather(Count<1>());
-    else
-      gather(Count<MOST / DRAW>());
+    if (n <= DRAW) {
+      each_listed<1>(s, r, parts, lists, 0, take);
+    } else if (few) {
+      each_listed<MOST / DRAW>(s, r, parts, lists, 0, take);
+    } else {
+      if (t == 0) s.lists = lists;
+      __syncthreads();
+      tally(s, r, parts);
+    }
     __syncthreads();
-    if (n > 64) {
+    if (n > 64 && few) {
       uint64_t all;
       const uint64_t mine = s.bucket[t], end = block_scan(mine, s.words, all);
       s.bucket[t] = end;
@@ -714,7 +770,8 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
       }
       __syncthreads();
     }
-    if (t < 64) {  // the first wave alone
+    if (t < 64 || !few) {  // the first wave alone, or every wave the same
+      const uint32_t lane = t & 63;
       uint32_t o0 = 0, m = n;  // of the order here, the places whose tokens lie in order
       uint64_t *sorted = s.place[0];
       double *upto = (double *)(s.place[0] + RANKED);
@@ -724,8 +781,11 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
         return b >= f2 ? at2 + s.n[b] - s.n[f2] : b >= f1 ? at1 + s.n[b] - s.n[f1] : s.n[b] - s.n[f0];
       };
       auto span_of = [&](uint32_t b) { return b >= f2 ? span2 + b - f2 : b >= f1 ? span1 + b - f1 : b - f0; };
-      auto count_to = [&](uint32_t q) { return (uint32_t)(s.bucket[q] >> COUNT_AT); };  // with bucket q
-      auto sum_to = [&](uint32_t q) { return s.bucket[q] & SUM; };
+      // with bucket q
+      auto count_to = [&](uint32_t q) {
+        return few ? (uint32_t)(s.bucket[q] >> COUNT_AT) : ((const uint32_t *)s.place[1])[2 * RANKED + q];
+      };
+      auto sum_to = [&](uint32_t q) { return few ? s.bucket[q] & SUM : s.bucket[q]; };
       auto sum_before = [&](uint32_t q) { return q ? sum_to(q - 1) : 0; };
       if (n <= 64) {  // all of them
         const uint64_t v = t < n ? s.place[0][t] : ~0ull;
@@ -747,18 +807,20 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
         if (m && i0 == o0) return;
         fits = fits && size <= RANKED;  // (if not, nothing found from here on is used)
         o0 = i0, m = size <= RANKED ? size : 0;
-        for (uint32_t j = t; j < m; j += 64) {
-          const uint64_t v = s.place[1][o0 + j];
+        if (!few && m) collect(s, r, parts, q);
+        const uint64_t *of = s.place[1] + (few ? o0 : 0);
+        for (uint32_t j = lane; j < m; j += 64) {
+          const uint64_t v = of[j];
           uint32_t rank = 0;
 #pragma unroll 4
-          for (uint32_t i = 0; i < m; i++) rank += s.place[1][o0 + i] < v;
+          for (uint32_t i = 0; i < m; i++) rank += of[i] < v;
           sorted[rank] = v;
         }
         const uint32_t span = q / per;
         const uint32_t b = span >= span2 ? f2 + span - span2 : span >= span1 ? f1 + span - span1 : f0 + span;
         uint64_t before = sum_before(q) - sum_before(span * per);
         for (uint32_t j0 = 0; j0 < m; j0 += 64) {
-          const uint32_t j = j0 + t;
+          const uint32_t j = j0 + lane;
           const uint64_t sum = before + wave_scan(j < m ? weight_of(sorted[j]) : 0);
           if (j < m) upto[j] = s.c[b] + sum_of(sum, s.edge[b]);
           before = __shfl(sum, 63);
@@ -783,7 +845,7 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
         uint32_t some = s.n[b1 + 1] - s.n[b1];
         if (b1 == bk) some = k - s.n[b1];
         if (b1 == bm) {  // (what lies in the buckets before `least`'s is larger, in those behind it smaller)
-          if (n > 64) order(bucket_of(least));
+          if (n > 64) order(bucket_of(r, lists, least));
           const uint32_t at = max(o0, i0) - i0;
           some = min(some, at + first_of(o0 + m - max(o0, i0), [&](uint32_t i) {
             return scaled(value_at(sorted[i + max(o0, i0) - o0]), r.c) < least;

@@ -199,6 +199,17 @@ def test_settings_outside_the_usual(ctx, settings):
         rows.free()
 
 
+@pytest.mark.parametrize("v", [30000, 151936, 1 << 20])
+@pytest.mark.parametrize("T", [2.0, 5.0, 40.0])
+def test_borders_among_thousands(ctx, v, T):
+    """So even that a bin has more tokens than are taken at once, of values all their own and of few."""
+    g = np.random.default_rng(v + int(T))
+    x = (g.standard_normal((6, v)) * 2.5).astype(np.float32)
+    x[4:] = np.round(x[4:] * 4) / 4
+    for p, m, k in ((1.0, 0.0, 0), (0.95, 0.0, 0), (0.9, 0.0, v // 3), (0.8, 0.02, 0), (0.5, 0.1, v // 2)):
+        _check(ctx, x, [(T, p, m, k, int(d)) for d in g.integers(0, 2**32, 6)])
+
+
 def test_many_rows_again_and_again(ctx):
     """A full batch of the benchmark's vocabulary, replayed: the same tokens each time."""
     g = np.random.default_rng(1)
