@@ -18,10 +18,14 @@
 // A bin's count and sum of weights are integers (36 bits after the point: a weight is off by 8e-12 of itself at
 // most), the same in any order, and only the tokens of the bins in which a border lies (min_p's or top_k's,
 // top_p's, the draw's) are looked at one by one.  No order of a whole row is ever made: a row is read once, by many
-// workgroups, and a draw reads an eighth of that (of 152k tokens 78 KB of bins) and what little lies around the borders.
+// workgroups, and a draw reads an eighth of that (of 152k tokens 78 KB of bins) and what lies around the borders: up to
+// 8192 tokens, which it takes into LDS, of more the sums of 1024 buckets and the tokens of the buckets with a border.
+// Only borders in the last bin, or in a bucket of more than 512 tokens (equal logits), cost passes over the row.
 //
-// Measured (MI355X, 151936 tokens, both kernels): 1 row 6.2 + 10.6 us, 16 rows at their temperature alone 10.2 to 11 + 14.9,
-// 48 masked rows 16.6 + 10.6, 128 rows of wide nuclei 31.9 + 22.  A replay of two empty launches takes 14.7.
+// Measured (MI355X, 151936 tokens, both kernels): 1 row 6.2 + 10.6 us, 16 rows at their temperature alone 10.2 to 11 +
+// 14.9, 48 masked rows 16.6 + 10.6, 128 rows of wide nuclei 31.9 + 22.  A replay of two empty launches takes 14.7.
+// Logits of N(0, 2.5^2) at temperature 0.7 / 2 / 5 with top_p 0.95, 1 row 34 / 38 / 39 us on the device, 128 rows 60 / 95
+// / 114; top_k 50000 and top_p 0.9 at 5 80 and 143.
 #include "common.h"
 
 namespace {
@@ -394,6 +398,20 @@ SK_DEV T block_scan(T v, T *waves, T &total) {  // inclusive, over DRAW threads;
   return before + v;
 }
 
+// A token of weight w and value `value` into word b of sums and counts; of a wave that has one value and one word, all
+// its tokens at once (equal logits would else wait for one another: 1 row of them 2500 -> 740 us).
+SK_DEV void count_in(unsigned long long *sums, uint32_t *counts, uint32_t b, uint32_t value, uint64_t w) {
+  const bool other = b != __builtin_amdgcn_readfirstlane(b) || value != __builtin_amdgcn_readfirstlane(value);
+  uint32_t n = 1;
+  if (!__ballot(other)) {
+    const uint64_t all = __ballot(true);
+    if ((threadIdx.x & 63) != (uint32_t)__builtin_ctzll(all)) return;
+    n = (uint32_t)__builtin_popcountll(all);
+  }
+  atomicAdd(&sums[b], (unsigned long long)(w * n));
+  atomicAdd(&counts[b], n);
+}
+
 // A token of the order: its place, how many tokens end with it and their sum.
 struct Found {
   uint64_t place;
@@ -427,8 +445,7 @@ __device__ __attribute__((noinline)) Found search(DrawShared &s, const Row r, Wa
     each_value_of(r, b, [&](uint64_t place, double v) {
       if (above < 64 && place >> above != f.place >> above) return;
       const uint32_t d = (uint32_t)(place >> at[k]) & (DIGITS - 1);
-      atomicAdd(&s.digit.sum[d], (unsigned long long)fixed_weight(series_, r, v));
-      atomicAdd(&s.digit.count[d], 1u);
+      count_in(s.digit.sum, s.digit.count, d, (uint32_t)(place >> 32), fixed_weight(series_, r, v));
     });
     __syncthreads();
     // two digits a thread
@@ -532,9 +549,7 @@ __device__ __attribute__((noinline)) void tally(DrawShared &s, const Row r, cons
   for (uint32_t base = 0; base < l.n; base += MOST)
     each_listed<MOST / DRAW>(s, r, parts, l, base, [&](uint32_t, float x, uint32_t) {
       const double v = scaled(x, r.c);
-      const uint32_t b = bucket_of(r, l, v);
-      atomicAdd(&s.bucket[b], (unsigned long long)fixed_weight(series_, r, v));
-      atomicAdd(&s.next[b], 1u);
+      count_in(s.bucket, s.next, bucket_of(r, l, v), __builtin_bit_cast(uint32_t, x), fixed_weight(series_, r, v));
     });
   __syncthreads();
   uint64_t sum;
@@ -565,10 +580,10 @@ __device__ __attribute__((noinline)) void collect(DrawShared &s, const Row r, co
 // Of a row of 151936 tokens whose borders' bins hold 6 / 1050 / 6000 tokens (22 / 37 / 50 thousand cycles): the partials'
 // heads 2400, their bins 5900, scans 1600, borders 3100 to 3700, the gather 4300 / 12000 / 22000 (two dependent loads a
 // token, from memory), buckets and order 150 / 2700 / 4500, the borders among them 4200 / 8900 / 10400.  Bound by chains
-// of loads and barriers and by the issue of the one workgroup that a row has.  Against all values put in order, as before (27.8 us for 128
-// rows), ordering the three borders' buckets alone took 26.1, and the gather's values spread evenly over the workgroup,
-// not by their chunks, 21.8 to 22.1; a count of places by waves, or the same loads behind branches, changed nothing, the bins on
-// their way beside the heads, through LDS, cost 1 us.
+// of loads and barriers and by the issue of the one workgroup that a row has.  Against all values put in order, as before
+// (27.8 us for 128 rows), ordering the three borders' buckets alone took 26.1, and the gather's values spread evenly over
+// the workgroup, not by their chunks, 22; a count of places by waves, or the same loads behind branches, changed
+// nothing, and the bins on their way beside the heads, through LDS, cost 1 us.
 extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, const uint32_t *ctl, DrawPush p) {
 #pragma clang fp contract(off)
   __shared__ DrawShared s;
