@@ -498,7 +498,7 @@ template <typename F>
 SK_DEV uint32_t first_of(uint32_t n, F ok) {
   uint32_t lo = 0, hi = n;  // none before lo does, hi does
   while (lo < hi) {
-    const uint32_t step = (hi - lo + 63) / 64, i = lo + (threadIdx.x & 63) * step + step - 1;
+    const uint32_t step = (hi - lo - 1) / 64 + 1, i = lo + (threadIdx.x & 63) * step + step - 1;
     const uint64_t m = __ballot(i >= hi || ok(i));
     if (!m) return hi;
     const uint32_t k = (uint32_t)__builtin_ctzll(m);
@@ -730,6 +730,7 @@ extern "C" __global__ __launch_bounds__(DRAW) void logits_sample_draw(float *a, 
   if (f1 != ~0u) n_spans += e1 - f1 + 1, n += s.n[e1 + 1] - s.n[f1], deepest = e1;
   span2 = n_spans, at2 = n;
   if (f2 != ~0u) n_spans++, n += s.n[e2 + 1] - s.n[f2], deepest = e2;
+  n = min(n, r.n_vocab);  // (as it is, of this row's partials)
   Found n2, chosen;
   bool many = n_spans > SPANS || deepest == BINS - 1;
   if (!many) {
