@@ -49,7 +49,13 @@ constexpr uint64_t SUM = (1ull << COUNT_AT) - 1;
 // What both kernels take a logit for, to the same bits.
 SK_DEV bool has_weight(float x) { return x > -INFINITY; }  // (not NaN)
 SK_DEV double scale_of(float T) { return 11.541560327111707 / (T > 0.0f ? (double)T : 1.0); }  // 8 log2(e) / T
-SK_DEV double scaled(float x, double c) { return (double)fminf(x, 3.402823466e38f) * c; }
+SK_DEV float finite(float x) { return fminf(x, 3.402823466e38f); }
+SK_DEV double scaled(float x, double c) { return (double)finite(x) * c; }
+SK_DEV uint32_t saturated(double x) {  // (as the instruction converts: past the largest the largest, NaN 0)
+  uint32_t y;
+  asm("v_cvt_i32_f64 %0, %1" : "=v"(y) : "v"(x));
+  return y;
+}
 // 2^(f / 8) for |f| <= 1/2 in units of 2^-36, as the low bits of the double behind 2^52: 1 + the polynomial of degree 5
 // nearest to the rest (4e-13 of it at most).  The constants are scalar registers: known as constants they would be moved
 // into vector ones for each use.
@@ -179,6 +185,10 @@ extern "C" __global__ __launch_bounds__(THREADS) void logits_sample(float *a, co
     }
     return;
   }
+  if (top == INFINITY) {
+#pragma unroll
+    for (uint32_t i = 0; i < EACH; i++) v[i / 4][i % 4] = finite(v[i / 4][i % 4]);
+  }
   const Series series_ = series();
   uint32_t at[EACH];  // a token's bin (BINS and above: none), and its place among those of the bin
   uint32_t far = 0;   // one bit each: below the last bin, as most of a row are where T is low
@@ -190,9 +200,9 @@ extern "C" __global__ __launch_bounds__(THREADS) void logits_sample(float *a, co
 #pragma unroll
     for (uint32_t j = 0; j < U; j++) {
       const float y = v[(i0 + j) / 4][(i0 + j) % 4];
-      const double s = scaled(y, c), g = __builtin_rint(s);
+      const double s = (double)y * c, g = __builtin_rint(s);
       word[j] = fixed_weight(series_, s - g) + (1ull << COUNT_AT);
-      b[j] = (uint32_t)(int)fmin(first - g, 2.0 * BINS);
+      b[j] = saturated(first - g);
       far |= has_weight(y) && b[j] >= BINS ? 1u << (i0 + j) : 0;
       b[j] = has_weight(y) && b[j] < BINS ? b[j] : BINS + lane;
     }
