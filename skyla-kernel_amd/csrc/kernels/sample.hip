@@ -22,8 +22,8 @@
 // 8192 tokens, which it takes into LDS, of more the sums of 1024 buckets and the tokens of the buckets with a border.
 // Only borders in the last bin, or in a bucket of more than 512 tokens (equal logits), cost passes over the row.
 //
-// Measured (MI355X, 151936 tokens, both kernels): 1 row 6.2 + 10.6 us, 16 rows at their temperature alone 10.2 to 11 +
-// 14.9, 48 masked rows 16.6 + 10.6, 128 rows of wide nuclei 31.9 + 22.  A replay of two empty launches takes 14.7.
+// Measured (MI355X, 151936 tokens, both kernels): 1 row 6.0 + 10.6 us, 16 rows at their temperature alone 9.5 to 11 +
+// 15, 48 masked rows 15.7 + 10.6, 128 rows of wide nuclei 30.4 + 22.  A replay of two empty launches takes 14.7.
 // Logits of N(0, 2.5^2) at temperature 0.7 / 2 / 5 with top_p 0.95, 1 row 34 / 38 / 39 us on the device, 128 rows 60 / 95
 // / 114; top_k 50000 and top_p 0.9 at 5 80 and 143.
 #include "common.h"
@@ -134,9 +134,9 @@ SK_DEV float wave_max(float v) {
 }  // namespace
 
 // A workgroup's CHUNK tokens of a row: their bins below its own largest value, and the tokens in the bins' order.
-// 128 rows of 151936 tokens (78 MB read, 47 written) take 31.8 us: 41 vector instructions a token (10 us of the 32 went
-// with the moves of the series' constants), 57% of the cycles' issue, and the atomics' and lists' LDS banks (8 us) beside
-// them.  Chunks of 16384 (1024 threads, 61 registers) took 85 us for 78 then, 8 or 16 tokens on their way at once 83 and
+// 128 rows of 151936 tokens (78 MB read, 47 written) take 30.4 us: 38 vector instructions a token, half the cycles' issue
+// (41, with clamps of every logit, took 32; with moves of the series' constants 42), and the atomics' and lists' LDS banks
+// (8 us) beside them; 2 fewer, the far tokens told by wave, changed nothing.  Chunks of 16384 (1024 threads, 61 registers) took 85 us for 78 then, 8 or 16 tokens on their way at once 83 and
 // 79, a workgroup that goes on to a second chunk with its loads ahead 101 (171 registers).
 extern "C" __global__ __launch_bounds__(THREADS) void logits_sample(float *a, const uint32_t *ctl, SamplePush p) {
 #pragma clang fp contract(off)
