@@ -134,10 +134,11 @@ SK_DEV float wave_max(float v) {
 }  // namespace
 
 // A workgroup's CHUNK tokens of a row: their bins below its own largest value, and the tokens in the bins' order.
-// 128 rows of 151936 tokens (78 MB read, 47 written) take 30.4 us: 38 vector instructions a token, half the cycles' issue
-// (41, with clamps of every logit, took 32; with moves of the series' constants 42), and the atomics' and lists' LDS banks
-// (8 us) beside them; 2 fewer, the far tokens told by wave, changed nothing.  Chunks of 16384 (1024 threads, 61 registers) took 85 us for 78 then, 8 or 16 tokens on their way at once 83 and
-// 79, a workgroup that goes on to a second chunk with its loads ahead 101 (171 registers).
+// 128 rows of 151936 tokens (78 MB read, 47 written) take 30.4 us: 38 vector instructions a token, half the cycles'
+// issue (41, with clamps of every logit, took 32; with moves of the series' constants 42), and the atomics' and lists'
+// LDS banks (8 us) beside them; 2 fewer, the far tokens told by wave, changed nothing.  Chunks of 16384 (1024 threads, 61
+// registers) took 85 us for 78 then, 8 or 16 tokens on their way at once 83 and 79, a workgroup that goes on to a second
+// chunk with its loads ahead 101 (171 registers).
 extern "C" __global__ __launch_bounds__(THREADS) void logits_sample(float *a, const uint32_t *ctl, SamplePush p) {
 #pragma clang fp contract(off)
   constexpr uint32_t WAVES = THREADS / 64;
