@@ -184,6 +184,29 @@ def test_images_in_a_prompt(ctx, precision):
         eng.free()
 
 
+@pytest.mark.parametrize("n", [1, 2, 130])
+def test_frames_behind_a_document(ctx, n):
+    """Vectors at positions of axes, of any number, that see from a document's start on, in a model with a window."""
+    c = _config(axes=tuple(i % 3 if i < 60 else 0 for i in range(64)), windows=(40, 0, 100))
+    g = np.random.default_rng(n)
+    tensors = synth.qwen3("test-frames", c, "q8_0", "random")
+    eng, m = _both(ctx, c, tensors, P.F16_KEYS_Q8_VALUES)
+    try:
+        s, text = eng.open(), _tokens(g, c, 70)
+        rows = (m.w["token_embd.weight"][_tokens(g, c, n)] * g.uniform(0.5, 2, (n, 1))).astype(np.float32)
+        at = np.stack([70 + np.arange(n) // 64, 70 + np.arange(n) % 64 // 8, 70 + np.arange(n) % 8], 1)
+        eng.extend(s, text)
+        m.extend(text)
+        eng.extend(s, [1] * n, axes=at, vectors=rows, since=66)
+        for i in range(0, n, 128):
+            k = slice(i, i + 128)
+            m.extend([1] * len(at[k]), axes=np.concatenate([at, at[:, :1]], 1)[k], vectors=rows[k], since=66)
+        for t in _tokens(g, c, 3):
+            assert rel_l2(eng.step({s: t})[0], m.extend([t])[0]) < BAR
+    finally:
+        eng.free()
+
+
 def test_one_axis_as_none(ctx):
     """A model whose axes are all the first, served as text: the logits of the model without them, to the bit."""
     g = np.random.default_rng(2)
