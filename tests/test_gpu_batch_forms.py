@@ -1,9 +1,11 @@
 """The served batch's newer operators (kernels/batch.hip, kernels/sample.hip) by every way there is to run
 them: as a recording's launches, as its graph while what it reads changes, and one dispatch at a time."""
+import threading
+
 import numpy as np
 import pytest
 
-from skyla_hip.abi import SkylaHipError
+from skyla_hip.abi import Context, SkylaHipError
 from test_gpu_batch import P, _Direct
 from test_gpu_batch_axes import Axes
 from test_gpu_batch_shaped import Shaped
@@ -115,3 +117,34 @@ def test_sample_as_a_graph(ctx):
             many.free()
     finally:
         rows.free()
+
+
+def test_two_contexts_at_once(ctx):
+    """A draw and an attention on streams of their own, from two threads: each as alone."""
+    g = np.random.default_rng(6)
+    other = Context.new(0)
+    rows = Rows(ctx, (g.standard_normal((40, 50000)) * 2).astype(np.float32), _some(g, 40))
+    b = Shaped(other, P["f16"], 2, 4, 32, [400, 333, 256, 257], cap=30.0, window=300, shares=[256] * 4, shared=256)
+    try:
+        b.prepare()
+        b.check()
+        alone, failed = b.rows_of(b.out, b.sq, b.sq, b.grid).copy(), []
+
+        def attend():
+            try:
+                for _ in range(20):
+                    b.attend()
+                    assert np.array_equal(b.rows_of(b.out, b.sq, b.sq, b.grid), alone)
+            except BaseException as e:  # (a thread's own goes nowhere)
+                failed.append(e)
+        t = threading.Thread(target=attend)
+        t.start()
+        try:
+            rows.check(times=10)
+        finally:
+            t.join()
+        assert not failed, failed
+    finally:
+        b.free()
+        rows.free()
+        other.free()
