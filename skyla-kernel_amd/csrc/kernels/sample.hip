@@ -49,7 +49,7 @@ constexpr uint64_t SUM = (1ull << COUNT_AT) - 1;
 // What both kernels take a logit for, to the same bits.
 SK_DEV bool has_weight(float x) { return x > -INFINITY; }  // (not NaN)
 SK_DEV double scale_of(float T) { return 11.541560327111707 / (T > 0.0f ? (double)T : 1.0); }  // 8 log2(e) / T
-SK_DEV float finite(float x) { return fminf(x, 3.402823466e38f); }
+SK_DEV float finite(float x) { return fminf(x, 3.402823466e38f); }  // of one with a weight
 SK_DEV double scaled(float x, double c) { return (double)finite(x) * c; }
 SK_DEV uint32_t saturated(double x) {  // (as the instruction converts: past the largest the largest, NaN 0)
   uint32_t y;
@@ -186,9 +186,10 @@ extern "C" __global__ __launch_bounds__(THREADS) void logits_sample(float *a, co
     }
     return;
   }
-  if (top == INFINITY) {
+  if (top == INFINITY) {  // (+inf alone: a minimum would make a number of NaN)
 #pragma unroll
-    for (uint32_t i = 0; i < EACH; i++) v[i / 4][i % 4] = finite(v[i / 4][i % 4]);
+    for (uint32_t i = 0; i < EACH; i++)
+      if (v[i / 4][i % 4] == INFINITY) v[i / 4][i % 4] = 3.402823466e38f;
   }
   const Series series_ = series();
   uint32_t at[EACH];  // a token's bin (BINS and above: none), and its place among those of the bin

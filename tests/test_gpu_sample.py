@@ -232,3 +232,22 @@ def test_refusals(ctx):
     finally:
         kernels.free()
         arena.free()
+
+
+@pytest.mark.parametrize("v", [5, 9000, 40000])
+@pytest.mark.parametrize("T", [0.0, 0.7, 30.0])
+def test_nan_beside_infinity(ctx, v, T):
+    """NaN has no place where a chunk's largest is +inf either: before it and behind it, in its chunk and in others,
+    most of a row, and beside more +inf than are put in order."""
+    g = np.random.default_rng(v)
+    x = (g.standard_normal((7, v)) * 2).astype(np.float32)
+    x[0, 0], x[0, 1] = np.nan, np.inf
+    x[1, 0], x[1, v - 1] = np.nan, np.inf
+    x[2, 0], x[2, v - 1] = np.inf, np.nan
+    x[3], x[3, v // 2] = np.nan, np.inf
+    x[4, g.random(v) < 0.5], x[4, [1, v - 2]] = np.nan, np.inf
+    x[5] = np.where(np.arange(v) % 3 == 0, np.nan, np.inf)
+    x[6] = np.where(np.arange(v) % 3 == 0, np.nan, np.where(np.arange(v) % 3 == 1, -np.inf, x[6]))
+    x[6, v // 2] = np.inf
+    for s in ((1.0, 0.0, 0), (0.9, 0.05, 20), (1.0, 0.0, 3)):
+        _check(ctx, x, [(T, *s, int(d)) for d in g.integers(0, 2**32, 7)])
