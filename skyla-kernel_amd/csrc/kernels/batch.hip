@@ -1392,8 +1392,8 @@ SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_
     return a + p.o_off + i / N_REP * p.o_stride + (kvh * N_REP + i % N_REP) * HD + 2 * j;
   };
   if (part * sp.per >= sp.tiles) {
-    if (slots == 1 && hi == 0)  // a row without positions
-      for (uint32_t j = t; j < N_REP * 64; j += 256) *(float2 *)result(i0 + j / 64, j % 64) = make_float2(0.0f, 0.0f);
+    if (slots == 1 && hi == 0)  // a row without positions, or all that go together
+      for (uint32_t j = t; j < n_live * 64; j += 256) *(float2 *)result(i0 + j / 64, j % 64) = make_float2(0.0f, 0.0f);
     return;
   }
   // Each row's [lo, hi) of the run (shaped): rows that go together may see parts of it.

@@ -345,6 +345,31 @@ def test_rows_that_go_together_or_not(ctx, rows):
                    until=np.where(np.arange(rows) % 3 == 1, lens.max(), 0))
 
 
+@pytest.mark.parametrize("heads", [(2, 1), (2, 2), (1, 4), (1, 8)])
+@pytest.mark.parametrize("parts", [(0, 1, False, 0), (0, 3, False, 0)])
+@pytest.mark.parametrize("lens", ["all", "one", "first idle"])
+def test_rows_that_go_together_and_see_nothing(ctx, heads, parts, lens):
+    """Tiles of one sequence's rows, and what is left of one, whose masks leave nothing, one live row among idle
+    ones, rows that name no sequence: zeros in all of them, whatever the output held."""
+    T = 16 // heads[1]
+    n = 2 * T + T // 2
+    ends = 40 + np.arange(n)
+    if lens == "one":
+        ends[np.arange(n) % T != T // 2] = 0
+    elif lens == "first idle":
+        ends[::T] = 0
+    for begin in (ends + 3, np.where(np.arange(n) // T == 1, 5, ends + 3)):  # all, all but the second tile
+        _check(ctx, P["f16k_q8v"], *heads, 16, ends, seqs=np.zeros(n, int), parts=parts, begin=begin, grid=n + 3)
+    b = Shaped(ctx, P["f16"], *heads, 16, ends, seqs=np.zeros(n, int), parts=parts, grid=n + 3)
+    try:
+        b.prepare()
+        b.arena.as_u32()[b.at.rows: b.at.rows + 4 * n: 4] = 3  # no such sequence
+        b.lens = b.ends = np.zeros(n, int)
+        b.check()
+    finally:
+        b.free()
+
+
 def test_refusals(ctx):
     b = Shaped(ctx, P["f16"], 2, 2, 16, [50, 40])
     try:
