@@ -160,13 +160,13 @@ SK_DEV ShapedRange shaped_range(const uint32_t *ctl, const P &p, uint32_t row, u
   r.start = r.member ? shared : r.lo;
   return r;
 }
-// Whether the T rows from row / T * T on go together: those with a token are of one sequence and at most 256
-// positions apart, as a prompt's are.  Their own runs (tails, and leads) are then one, cut into parts as one, with each
+// Whether the T rows from row / T * T on go together: those with a token are of one sequence that there is, and at most
+// 256 positions apart, as a prompt's are.  Their own runs (tails, and leads) are then one, cut into parts as one, with each
 // row's mask.  (The words through the scalar cache: nothing writes them while the kernel runs.)
 typedef const __attribute__((address_space(4))) uint32_t ConstWord;
 template <uint32_t T>
-SK_DEV bool rows_together(const uint32_t *ctl, uint32_t rows_off, uint32_t row, uint32_t n_rows, uint32_t n_grid) {
-  if constexpr (T == 1) return false;
+SK_DEV bool rows_together(const uint32_t *ctl, uint32_t rows_off, uint32_t row, uint32_t n_rows, uint32_t n_grid,
+                          uint32_t n_seq) {
   ConstWord *w = (ConstWord *)(uintptr_t)(ctl + rows_off);
   uint32_t seq = ~0u, least = ~0u, most = 0;
   bool one = true;
@@ -174,7 +174,7 @@ SK_DEV bool rows_together(const uint32_t *ctl, uint32_t rows_off, uint32_t row, 
   for (uint32_t i = 0; i < T; i++) {
     // (the grid's rows, so that the loads wait for no control word)
     const uint32_t r = row / T * T + i, of = w[4 * min(r, n_grid - 1)], len = w[4 * min(r, n_grid - 1) + 1];
-    const bool live = r < n_rows && len != 0;
+    const bool live = r < n_rows && len != 0 && of < n_seq;  // (so that no live one is of ~0)
     one = one && (!live || seq == ~0u || of == seq);
     seq = live ? of : seq, least = live ? min(least, len) : least, most = live ? max(most, len) : most;
   }
@@ -183,10 +183,10 @@ SK_DEV bool rows_together(const uint32_t *ctl, uint32_t rows_off, uint32_t row, 
 // The same for a T that is known when the kernel runs, by whole waves, lane l with row l % T (the merge's: with each T
 // unrolled as above a launch of 100 rows took 8.8 us for 8.4).
 SK_DEV bool rows_together(const uint32_t *ctl, uint32_t rows_off, uint32_t row, uint32_t n_rows, uint32_t n_grid,
-                          uint32_t T) {
+                          uint32_t n_seq, uint32_t T) {
   const uint32_t r = row / T * T + (threadIdx.x & (T - 1));
   const uint2 w = *(const uint2 *)(ctl + rows_off + 4 * min(r, n_grid - 1));
-  const bool live = r < n_rows && w.y != 0;
+  const bool live = r < n_rows && w.y != 0 && w.x < n_seq;
   const uint64_t m = __ballot(live);
   const uint32_t seq = __builtin_amdgcn_readlane(w.x, m ? (uint32_t)__builtin_ctzll(m) : 0);
   const bool one = m && !__ballot(live && w.x != seq);
@@ -1370,7 +1370,7 @@ SK_DEV void paged_body(float *a, const uint32_t *ctl, const f16 *kv, const int8_
       constexpr uint32_t T = 16 / N_REP;
       const uint32_t tiles = (n_grid + T - 1) / T;
       row = row % tiles * T + row / tiles;
-      const bool together = rows_together<T>(ctl, p.rows_off, row, n_rows, n_grid), lead = part >= p.n_own;
+      const bool together = rows_together<T>(ctl, p.rows_off, row, n_rows, n_grid, p.n_seq), lead = part >= p.n_own;
       tile0 = row / T * T;
       if (row >= n_rows || (together && row != tile0)) return;
       run = own_run(ctl, p, row, n_rows, T, together, shared, lead);
@@ -1536,7 +1536,7 @@ SK_DEV void paged_merge(float *a, const uint32_t *ctl, const P &p, uint32_t h, u
       const uint32_t shared = shared_end(ctl, p);
       const auto r = range_of(ctl, p, row, shared);
       const uint32_t n_rows = min(ctl[2], gridDim.y);  // the attention's
-      const bool together = rows_together(ctl, p.rows_off, row, n_rows, gridDim.y, 16 / p.rep);
+      const bool together = rows_together(ctl, p.rows_off, row, n_rows, gridDim.y, p.n_seq, 16 / p.rep);
       // the parts of [x.all_lo, x.all_hi) with some of [x.lo, x.hi)
       auto parts_of = [&](bool lead, uint32_t n_parts, uint32_t &at) {
         const OwnRun x = own_run(ctl, p, row, n_rows, 16 / p.rep, together, shared, lead);

@@ -370,6 +370,25 @@ def test_rows_that_go_together_and_see_nothing(ctx, heads, parts, lens):
         b.free()
 
 
+@pytest.mark.parametrize("heads", [(2, 1), (2, 2), (1, 4), (1, 8)])
+@pytest.mark.parametrize("word", [0xFFFFFFFF, 0xFFFFFFFE, 1])
+@pytest.mark.parametrize("at", ["first", "last", "first of all"])
+def test_rows_of_no_sequence_among_ones_that_go_together(ctx, heads, word, at):
+    """The attention and its merge cut the others' positions the same, whichever rows of a tile name no sequence."""
+    T = 16 // heads[1]
+    n = 2 * T + T // 2
+    b = Shaped(ctx, P["f16k_q8v"], *heads, 16, 300 + 9 * np.arange(n) % 100, seqs=np.zeros(n, int), window=90,
+               parts=(0, 5, False, 0), until=np.where(np.arange(n) % 3 == 1, 400, 0))
+    try:
+        b.prepare()
+        bad = {"first": slice(0, n, T), "last": slice(T - 1, n, T), "first of all": slice(0, 1)}[at]
+        b.arena.as_u32()[b.at.rows: b.at.rows + 4 * n].reshape(n, 4)[bad, 0] = word
+        b.lens[bad] = 0  # (as the result has them; the words keep their lengths)
+        b.check()
+    finally:
+        b.free()
+
+
 def test_refusals(ctx):
     b = Shaped(ctx, P["f16"], 2, 2, 16, [50, 40])
     try:
