@@ -247,3 +247,15 @@ def test_rope_axes_table():
     t = E.rope_axes_table(c)
     assert t.shape == (3, 64) and (t.sum(0) == E.rope_frequencies(c)).all() and ((t != 0).sum(0) == 1).all()
     assert (t[1, 1], t[2, 1]) == (E.rope_frequencies(c)[1], 0)
+
+
+@pytest.mark.parametrize("rows,n_kv,own,more", [(8, 8, 512, 2), (8, 8, 513, 3), (5, 8, 320, 2), (5, 8, 321, 2), (31, 8, 1984, 3),
+                                                (31, 8, 1985, 3), (32, 8, 1985, 2), (32, 8, 100000, 2), (255, 1, 2041, 3),
+                                                (256, 1, 2041, 2)])
+def test_one_part_of_rows_that_share_nothing(rows, n_kv, own, more):
+    """Where splits has `more`, one from 256 rows x key heads on, and below for 8 positions for each of these; with a
+    shared run always splits'."""
+    assert B.splits(rows, n_kv, 4, 0, own) == (0, more, False)
+    one = rows * n_kv >= 256 or own <= 8 * rows * n_kv
+    assert B.shaped_splits(rows, n_kv, 4, 0, own) == (0, 1 if one else more, False, 0)
+    assert B.shaped_splits(rows, n_kv, 4, 1000, own)[:3] == B.splits(rows, n_kv, 4, 1000, own)
