@@ -439,6 +439,7 @@ class BatchEngine:
                          for _, p in self._shaped_parts(r, shared, own, lead)))
                    for r in self._buckets(E.BATCH) for shared in [0, *self._buckets(max_ctx)]
                    for own in self._buckets(max_ctx))
+        part = max(part, sample_size(max_seq, c.n_vocab) if self._draws() else 0)
         self.weights = self.arena = self.batch = self.logits = None
         self.pools, self.recordings = [], {}
         try:
@@ -459,12 +460,13 @@ class BatchEngine:
             "logits": self.s_vocab * max_seq, "controls": 8 * max_seq, "history": self.s_hist * max_seq,
             "bias": 2 * self.MAX_BIASES * max_seq, "mask": self.s_mask * max_seq,
             "axes": 4 * E.BATCH, "spans": 2 * E.BATCH, "slopes": c.n_head, "sampling": 8 * max_seq,
-            "drawn": 4 * max_seq, "sample": sample_size(max_seq, c.n_vocab) if self._draws() else 0})
+            "drawn": 4 * max_seq})
         x = a.extra
         for _ in range(c.n_layer):
             self.pools.append(ctx.alloc_host(self.paged.bytes()))
         self.at = BatchRegions(rows=x["rows"], table=x["table"], part=x["part"], axes=x["axes"], spans=x["spans"])
-        self.sample_at = SampleRegions(controls=x["sampling"], out=x["drawn"], part=x["sample"])
+        # (a step's draws come when its attention's partials have been merged, and lie in their place)
+        self.sample_at = SampleRegions(controls=x["sampling"], out=x["drawn"], part=x["part"])
         self.slopes = None
         if c.slopes is not None:
             self.slopes = x["slopes"]

@@ -259,3 +259,18 @@ def test_one_part_of_rows_that_share_nothing(rows, n_kv, own, more):
     one = rows * n_kv >= 256 or own <= 8 * rows * n_kv
     assert B.shaped_splits(rows, n_kv, 4, 0, own) == (0, 1 if one else more, False, 0)
     assert B.shaped_splits(rows, n_kv, 4, 1000, own)[:3] == B.splits(rows, n_kv, 4, 1000, own)
+
+
+def test_draws_take_the_attentions_partials(make, monkeypatch):  # noqa: F811
+    """An engine's arena holds what is larger of the two, not both."""
+    eng, _ = make()
+    x, sample = eng.arena.extra, B.sample_size(eng.max_seq, eng.c.n_vocab)
+    part = max(B.shaped_part_size(r, eng.c.n_head, p) for r in eng._buckets(E.BATCH)
+               for shared in [0, *eng._buckets(eng.max_ctx)] for own in eng._buckets(eng.max_ctx)
+               for lead in (False, True) for _, p in eng._shaped_parts(r, shared, own, lead))
+    assert eng.sample_at.part == eng.at.part == x["part"]
+    assert x["logits"] - x["part"] == -(-max(part, sample) // 64) * 64
+    monkeypatch.setattr(B, "SAMPLE_VOCAB", eng.c.n_vocab - 1)
+    plain, _ = make()
+    assert plain.arena.extra["logits"] - plain.arena.extra["part"] == -(-part // 64) * 64
+    assert eng.arena.size - plain.arena.size == max(0, -(-sample // 64) * 64 - -(-part // 64) * 64)
