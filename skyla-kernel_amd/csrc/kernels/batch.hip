@@ -118,14 +118,15 @@ SK_DEV Range row_range(const uint32_t *ctl, uint32_t rows_off, uint32_t row, uin
 // The bodies are attention_paged's, with these masks, scores and runs, so that what bounds them is the same.  Own runs of
 // rows that are one prompt's go together (16 query rows a workgroup for 2 to 8 as elsewhere): a chunk's 128 rows would
 // else read their common positions once each (73 -> 57 us a chunk behind a window of 4096 of 12000 positions).  A window
-// leaves out tiles before they are read: a pass of that chunk takes, with windows of 64 / 512 / 4096 / none, 33 / 43 / 62 /
-// 105 us.
+// leaves out tiles before they are read: a pass of that chunk takes, with windows of 64 / 512 / 4096 / none, 32 / 41 / 61 /
+// 106 us one by one (57 of 4096 among others).
 // Measured (MI355X, + merge): 8 rows of up to 100 own positions, capped, 8.0 us; 32 rows with a window of 1024, f16 keys
 // and 8-bit values, 27.8, no merge (97 MB, 3.5 TB/s); 128 rows of 32 heads over 16384 shared and 300 own positions of 8 key
-// heads, capped, f16, 105 + 11.5 (products 0.72 PFLOP/s in two f16 parts); the chunk above 41.8 + 9.6; 100 rows of
+// heads, capped, f16, 105 to 111 + 12 (products 0.68 to 0.72 PFLOP/s in two f16 parts); the chunk above 41.8 + 9.6; 100 rows of
 // documents to 4000 positions of 4 key heads, sloped, 8 bits, 34.5 + 7.6 (partials of 20 MB written and read).
-// What shaping costs a pass of those 128 rows (f16 / f16 keys, 8-bit values / 8 bits): scores as they are 122 / 146 / 157
-// us, sloped 130 / 151 / 162, capped 130 / 150 / 170, both 147 / 170 / 191: vector instructions beside the products.
+// What shaping costs a pass of those 128 rows (f16 / f16 keys, 8-bit values / 8 bits): scores as they are 122 / 148 / 156
+// us, sloped 125 / 152 / 163, capped 134 / 152 / 174, both 150 / 171 / 191, one by one: vector instructions beside the
+// products.
 struct ShapedRange : Range {  // tail: [start, len), len the end hi
   uint32_t lo, at;            // lead: [lo, S) of a member; the position i
 };

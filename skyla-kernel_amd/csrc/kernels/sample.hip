@@ -17,15 +17,23 @@
 // t = x 8 log2(e) / T, one rint(t) each, in which a weight is 2^((t - rint(t)) / 8) of its bin's middle's.
 // A bin's count and sum of weights are integers (36 bits after the point: a weight is off by 8e-12 of itself at
 // most), the same in any order, and only the tokens of the bins in which a border lies (min_p's or top_k's,
-// top_p's, the draw's) are looked at one by one.  No order of a whole row is ever made: a row is read once, by many
-// workgroups, and a draw reads an eighth of that (of 152k tokens 78 KB of bins) and what lies around the borders: up to
-// 8192 tokens, which it takes into LDS, of more the sums of 1024 buckets and the tokens of the buckets with a border.
-// Only borders in the last bin, or in a bucket of more than 512 tokens (equal logits), cost passes over the row.
+// top_p's, the draw's) are looked at one by one.  The last bin holds whatever is 44 temperatures or more below the
+// largest: there a weight is off by 2^-37 of the bin's middle's, and again where a chunk's bin is taken into the row's,
+// and is nothing from 26 temperatures further down.  All of them are less than 2^-43 of a row, which no top_p below 1
+// (2^-24) and no draw (2^-33) tells from the whole; min_p's border goes by t and top_k's by the count.
+// No order of a whole row is ever made: a row is read once, by many workgroups, and a draw reads an eighth of that (of
+// 152k tokens 78 KB of bins) and what lies around the borders: up to 8192 tokens, which it takes into LDS, of more the
+// sums of 1024 buckets and the tokens of the buckets with a border.  Only borders in the last bin, or in a bucket of
+// more than 512 tokens (equal logits), cost passes over the row, five for each border.
 //
 // Measured (MI355X, 151936 tokens, both kernels): 1 row 6.0 + 10.6 us, 16 rows at their temperature alone 9.5 to 11 +
-// 15, 48 masked rows 15.7 + 10.6, 128 rows of wide nuclei 30.4 + 22.  A replay of two empty launches takes 14.7.
-// Logits of N(0, 2.5^2) at temperature 0.7 / 2 / 5 with top_p 0.95, 1 row 34 / 38 / 39 us on the device, 128 rows 60 / 95
-// / 114; top_k 50000 and top_p 0.9 at 5 80 and 143.
+// 15, 48 masked rows 15.7 + 10.6, 128 rows of wide nuclei 30.4 + 23.  A replay of two empty launches takes 14.7.
+// Logits of N(0, 2.5^2) at temperature 0.7 / 2 / 5 with top_p 0.95, 1 row 34 / 38 / 39 us on the device, 128 rows 60 /
+// 95 / 114; top_k 50000 and top_p 0.9 at 5 80 and 143.
+// Low temperatures cost more.  Tokens 44 to 70 temperatures below their chunk's largest are weighed one by one into one
+// bin: at 0.3 / 0.2 / 0.1 / 0.05 / 0.02 logits_sample takes 25 / 41 / 27 / 17 / 14 us for 1 row, 74 / 195 / 112 / 70 / 57
+// for 128.  And where a top_k's last token lies 44 temperatures down, the search for it takes the draw from 17 to 380
+// us (top_k 50: 1 row at 0.05, the slowest of 128 at 0.1).
 #include "common.h"
 
 namespace {

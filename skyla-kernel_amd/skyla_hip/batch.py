@@ -164,7 +164,8 @@ def shaped_splits(rows: int, n_kv: int, rep: int, shared: int, own: int, lead: i
     to 8 positions for each of these.  A pass of 8 key heads, f16, us in one part / the best of two and more: 8
     rows of 512 / 1024 / 2048 positions 22.0 / 23.5, 27.7 / 25.8, 36.8 / 30.1; 16 rows 23.7 / 26.1, 28.0 / 31.3,
     39.3 / 39.0; 24 rows 24.1 / 31.4, 30.7 / 37.7, 51.2 / 52.7; 32 rows 25.9 / 32.1, 34.0 / 40.4, 60.6 / 67.3, of
-    4096 99.9 / 113; 48 rows of 4096 168 / 157."""
+    4096 99.9 / 113; 48 rows of 4096 168 / 157.  Rows are taken to be about as long: one of 16000 among 31 of 200 takes
+    168 in its one part, 49 in 16, and 37 alone."""
     parts = splits(rows, n_kv, rep, shared, own)
     if shared == 0 and (n_kv * rows >= 256 or own <= 8 * n_kv * rows):
         parts = Parts(0, 1)
@@ -764,7 +765,7 @@ class BatchEngine:
         image's patches or a video's have them; without, they follow one another as text, which goes on behind the
         largest so far.  vectors: rows of n_embd numbers in place of the tokens' own (an image's; the tokens then
         are what the history says of them).  since: the first position that the tokens attend to, as where a document
-        of its own begins.  together: the tokens, BATCH at most, attend to one another, later ones too."""
+        of its own begins (these tokens alone: what is generated behind them attends to all).  together: the tokens, BATCH at most, attend to one another, later ones too."""
         s, tokens = self._get(seq), self._check(tokens)
         n_all = len(tokens)
         if axes is not None:
